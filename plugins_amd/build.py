@@ -41,12 +41,14 @@ SOURCES = [
     *[("exl3_rate_gemm.hip", f"exl3_rate_gemm_k{k}", DEVICE_FLAGS + [f"-DEXL3_INST_K={k}"])
       for k in range(9)],
     ("decoder_ops.hip", "decoder_ops", DEVICE_FLAGS),
+    ("paged_ops.hip", "paged_ops", DEVICE_FLAGS),
     ("exl3_noalloc.hip", "exl3_noalloc", DEVICE_FLAGS),
     ("exl3_host.cpp", "exl3_host", HOST_FLAGS),
     ("exl3_json.cpp", "exl3_json", HOST_FLAGS),
     ("exl3_codebooks.cpp", "exl3_codebooks", HOST_FLAGS),
     ("exl3_dense.cpp", "exl3_dense", HOST_FLAGS),
     ("exl3_pack.cpp", "exl3_pack", HOST_FLAGS),
+    ("paged_book.cpp", "paged_book", HOST_FLAGS),
     ("exl3_selfcheck.cpp", "exl3_selfcheck", HOST_FLAGS),
 ]
 

@@ -1,0 +1,553 @@
+"""The operators over a paged KV cache on the GPU, against their formulas in 64
+bits (tests/_paged.py derives the bounds)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from plugins_amd import exl3 as X  # noqa: E402
+from plugins_amd import paged as P  # noqa: E402
+from tests import _paged as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def batch(counts, lens, dtype, kv, group, dim, page, seed, extra=3, layers=1, max_pages=None):
+    """Host tensors of a step: pools of random values, NaN wherever no sequence
+    has a key, a random table, cu, q."""
+    g = torch.Generator().manual_seed(seed)
+    table, pages = R.random_table(counts, lens, page, extra, g, max_pages)
+    shape = (layers, pages, kv, page, dim)
+    k, v = torch.randn(shape, generator=g).to(dtype), torch.randn(shape, generator=g).to(dtype)
+    mine = torch.zeros(pages, page, dtype=torch.bool)
+    for s, (n, c) in enumerate(zip(counts, lens)):
+        pg, row = R.slots(table, s, page, n + c)
+        mine[pg, row] = True
+    hole = ~mine[None, :, None, :, None]
+    k, v = k.masked_fill(hole, math.nan), v.masked_fill(hole, math.nan)
+    cu = [0]
+    for n in counts:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1], kv * group, dim, generator=g).to(dtype)
+    return g, k, v, table, cu, q
+
+
+def attended(k, v, table, counts, lens, q, mask, rows=None, **kw):
+    cache = P.PagedCache.over(k.to(DEV), v.to(DEV), table.to(DEV))
+    rows = rows or P.Rows.of(counts, lens, DEV)
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device=DEV)
+    got = P.attend(cache, kw.pop("layer", 0), rows, q.to(DEV), out,
+                   mask=None if mask is None else mask.to(DEV), **kw)
+    torch.cuda.synchronize()
+    assert got is out
+    return out.cpu()
+
+
+def near(got, want, tol, what):
+    off = (got.double() - want).abs()
+    assert not torch.isnan(off).any(), what
+    worst = float((off - tol).max())
+    assert worst <= 0, (what, worst, float((off / tol.clamp(min=1e-300)).max()))
+
+
+CASES = [
+    # counts, lens, kv, group, dim, page
+    ([1], [0], 1, 1, 64, 16),
+    ([1], [1], 2, 4, 128, 16),
+    ([1], [2047], 2, 4, 128, 64),
+    ([1, 1, 1], [15, 16, 17], 2, 3, 64, 16),
+    ([5, 0, 3, 1], [31, 200, 0, 64], 2, 4, 128, 32),
+    ([17, 64, 2], [100, 3, 1000], 1, 8, 128, 16),
+    ([70, 1, 33], [0, 513, 250], 2, 5, 64, 64),
+    ([129], [300], 1, 2, 128, 256),
+    ([40], [90], 1, 7, 64, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts,lens,kv,group,dim,page", CASES)
+@pytest.mark.parametrize("tree", [False, True])
+def test_attend(counts, lens, kv, group, dim, page, dtype, tree):
+    g, k, v, table, cu, q = batch(counts, lens, dtype, kv, group, dim, page, 11 + sum(counts))
+    parents = [R.random_tree(n, g) if n else [] for n in counts]
+    seen = [R.ancestors(p) if tree else [list(range(i + 1)) for i in range(len(p))] for p in parents]
+    mask = R.masks([js for s in seen for js in s], -(-max(counts) // 64)) if tree else None
+    scale = 1 / math.sqrt(dim)
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, page, group, scale)
+    got = attended(k, v, table, counts, lens, q, mask)
+    near(got, want, tol, "attend")
+    # again, bit for bit
+    assert torch.equal(got, attended(k, v, table, counts, lens, q, mask))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attend_free_masks_and_empty_rows(dtype):
+    """Masks that are no tree's: rows that see none of the rows, not even
+    themselves; behind an empty context such a row is zeros."""
+    counts, lens = [6, 70, 4], [0, 40, 0]
+    g, k, v, table, cu, q = batch(counts, lens, dtype, 2, 4, 128, 16, 5)
+    seen = [[[j for j in range(n) if torch.rand(1, generator=g) < 0.4] for _ in range(n)]
+            for n in counts]
+    seen[0][2], seen[2] = [], [[] for _ in range(4)]
+    mask = R.masks([js for s in seen for js in s], 3)  # a word more than is needed
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, 16, 4, 0.3)
+    got = attended(k, v, table, counts, lens, q, mask, scale=0.3)
+    near(got, want, tol, "free masks")
+    assert not got[2].any() and not got[cu[2]:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("n,group", [(3, 4), (40, 4)])
+def test_attend_keeps_what_is_masked_out(dtype, what, n, group):
+    """A drafted row whose key and value overflowed: the rows that see it are
+    NaN or infinite, the others as if it were not there."""
+    counts, lens, page = [n, 2], [37, 50], 16
+    g, k, v, table, cu, q = batch(counts, lens, dtype, 2, group, 128, page, 6)
+    parents = [[-1] + [max(0, i - 2) for i in range(1, n)], [-1, 0]]
+    seen = [R.ancestors(p) for p in parents]
+    mask = R.masks([js for s in seen for js in s], 1)
+    pg, row = R.slots(table, 0, page, 37 + n)
+    for pool in (k, v):
+        pool[0, pg[37 + 1], :, row[37 + 1]] = what
+    bad = [i for i in range(n) if 1 in seen[0][i]]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, page, group, 1 / math.sqrt(128))
+    got = attended(k, v, table, counts, lens, q, mask)
+    fine = [t for t in range(n + 2) if t not in bad]
+    near(got[fine], want[fine], tol[fine], "masked out")
+    assert not torch.isfinite(got[bad].float()).all(-1).any()
+    # without a mask: the rows before it
+    seen = [[list(range(i + 1)) for i in range(m)] for m in counts]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, page, group, 1 / math.sqrt(128))
+    got = attended(k, v, table, counts, lens, q, None)
+    fine = [0, n, n + 1]
+    near(got[fine], want[fine], tol[fine], "masked out, in a line")
+    assert not torch.isfinite(got[1:n].float()).all(-1).any()
+
+
+def test_attend_large_scores_and_an_infinite_key():
+    """Scores of thousands (f32 exponents far apart), and a context whose one
+    key is -inf against positive queries: weight 0."""
+    counts, lens = [2], [100]
+    g, k, v, table, cu, q = batch(counts, lens, torch.float16, 1, 4, 64, 16, 7)
+    q = q.abs() * 30
+    k = k * 30
+    pg, row = R.slots(table, 0, 16, 102)
+    k[0, pg[5], :, row[5]] = -math.inf
+    seen = [[[0], [0, 1]]]
+    k2 = k.clone()
+    k2[0, pg[5], :, row[5]] = -60.0
+    want, tol = R.attention(q, k2, v, table, cu, lens, seen, 16, 4, 0.125)
+    got = attended(k, v, table, counts, lens, q, None, scale=0.125)
+    # es of these scores: the bound's own, from |q k|
+    assert torch.isfinite(got.float()).all()
+    near(got, want, tol, "large scores")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attend_many_small_weights(dtype):
+    """One key far above 20000 others whose weights only count together: each is
+    about 2^-21 of the largest, where f16 alone would hold one bit of it."""
+    n_ctx = 20000
+    counts, lens = [1], [n_ctx]
+    g, k, v, table, cu, q = batch(counts, lens, dtype, 1, 1, 64, 256, 8)
+    v = v.abs()
+    q = torch.ones_like(q)
+    k = torch.zeros_like(k)
+    pg, row = R.slots(table, 0, 256, n_ctx + 1)
+    k[0, pg[123], :, row[123]] = 14.5 / 64
+    v[0, pg[123], :, row[123]] = 0
+    want, tol = R.attention(q, k, v, table, cu, lens, [[[0]]], 256, 1, 1.0)
+    near(attended(k, v, table, counts, lens, q, None, scale=1.0), want, tol, "small weights")
+
+
+def test_attend_strides_and_rows_behind():
+    """q inside a fused q+k+v matrix, an output with wider rows, and rows of the
+    tensors behind the last sequence: left as they were."""
+    counts, lens, kv, group, dim, page = [3, 9], [40, 7], 2, 4, 128, 16
+    g, k, v, table, cu, q = batch(counts, lens, torch.float16, kv, group, dim, page, 9)
+    total, extra = 12, 5
+    width = kv * group * dim
+    fused = torch.randn(total + extra, width + 2 * kv * dim, generator=g).half()
+    fused[:total, :width] = q.view(total, width)
+    rows = P.Rows(torch.tensor(cu, dtype=torch.int32, device=DEV),
+                  torch.tensor(lens, dtype=torch.int32, device=DEV), total + extra, 9)
+    out = torch.full((total + extra, width + 64), 5.0, dtype=torch.float16, device=DEV)
+    cache = P.PagedCache.over(k.to(DEV), v.to(DEV), table.to(DEV))
+    P.attend(cache, 0, rows, fused.to(DEV)[:, :width], out[:, :width])
+    seen = [[list(range(i + 1)) for i in range(n)] for n in counts]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, page, group, 1 / math.sqrt(dim))
+    near(out[:total, :width].cpu().view(total, -1, dim), want, tol, "strides")
+    assert bool((out[:, width:] == 5.0).all()) and bool((out[total:] == 5.0).all())
+
+
+def test_attend_bad_pages_and_lengths_are_nan():
+    """A sequence whose table names no page, whose length is negative or does not
+    fit its table is NaN; the others are what they are alone."""
+    counts, lens = [2, 2, 2, 2, 2], [30, 30, 30, 30, 30]
+    g, k, v, table, cu, q = batch(counts, lens, torch.float16, 1, 4, 64, 16, 10)
+    seen = [[[0], [0, 1]]] * 5
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, 16, 4, 0.125)
+    bad = table.clone()
+    bad[1, 1] = -1
+    bad[2, 0] = k.shape[1]
+    rows = P.Rows.of(counts, [30, 30, 30, -1, 100], DEV)
+    got = attended(k, v, bad, counts, lens, q, None, rows=rows)
+    assert torch.isnan(got[2:]).all()
+    near(got[:2], want[:2], tol[:2], "beside bad ones")
+
+
+def test_attend_beyond_32_bits():
+    """Pages whose bytes and elements lie past 2^32 of a layer."""
+    kv, page, dim, group = 8, 256, 128, 1
+    per = kv * page * dim
+    pages = (1 << 32) // per + 9
+    free = torch.cuda.mem_get_info()[0]
+    if free < 4 * 2 * per * pages:
+        pytest.skip("not enough memory")
+    k = torch.empty(2, pages, kv, page, dim, dtype=torch.float16, device=DEV)
+    v = torch.empty_like(k)
+    g = torch.Generator().manual_seed(12)
+    small_k = torch.randn(2, 3, kv, page, dim, generator=g).half()
+    small_v = torch.randn(2, 3, kv, page, dim, generator=g).half()
+    at = [pages - 1, pages - 5, pages - 3]
+    for x, p in enumerate(at):
+        k[:, p], v[:, p] = small_k[:, x].to(DEV), small_v[:, x].to(DEV)
+    cache = P.PagedCache.over(k, v, torch.tensor([at], dtype=torch.int32, device=DEV))
+    counts, lens = [2], [600]
+    q = torch.randn(2, kv, dim, generator=g).half()
+    rows = P.Rows.of(counts, lens, DEV)
+    got = P.attend(cache, 1, rows, q.to(DEV)).cpu().view(2, kv, dim)
+    tab = torch.tensor([[0, 1, 2]], dtype=torch.int32)
+    want, tol = R.attention(q, small_k, small_v, tab, [0, 2], lens, [[[0], [0, 1]]], page, 1,
+                            1 / math.sqrt(dim), layer=1)
+    near(got, want, tol, "far pages")
+    # append, commit and copies there
+    pos, slot, mask = P.plan(cache, rows, torch.tensor([-1, 0], dtype=torch.int32, device=DEV))
+    assert slot.tolist() == [at[2] * page + 88, at[2] * page + 89]
+    new = torch.randn(2, kv * dim, generator=g).half().to(DEV)
+    P.qkv_append(cache, 1, q.to(DEV), new, new, None, None, torch.zeros_like(pos), slot,
+                 q.to(DEV))
+    torch.cuda.synchronize()
+    assert torch.equal(v[1, at[2], :, 88:90], new.view(2, kv, dim).transpose(0, 1))
+    assert torch.equal(k[1, at[2], :, 88:90], new.view(2, kv, dim).transpose(0, 1))
+    P.copy_pages(cache, [at[2]], [pages - 8])
+    torch.cuda.synchronize()
+    assert torch.equal(v[:, pages - 8], v[:, at[2]])
+
+
+def test_attend_other_stream_and_graph():
+    """A call on another stream than the current one; captured, with lengths,
+    table and q changed between the replays; two graphs over the same rows."""
+    counts, lens = [3, 20], [500, 70]
+    g, k, v, table, cu, q = batch(counts, lens, torch.bfloat16, 2, 4, 128, 32, 13, max_pages=40)
+    want0 = attended(k, v, table, counts, lens, q, None)
+    cache = P.PagedCache.over(k.to(DEV), v.to(DEV), table.to(DEV))
+    rows = P.Rows.of(counts, lens, DEV)
+    qd = q.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    out = P.attend(cache, 0, rows, qd, stream=side)
+    side.synchronize()
+    assert torch.equal(out.cpu().view(q.shape), want0)
+    outs, graphs = [], []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side, capture_error_mode="thread_local"):
+            outs.append(P.attend(cache, 0, rows, qd))
+        graphs.append(gr)
+    for turn in range(3):
+        new = [500 - 100 * turn, 70 - 30 * turn]
+        rows.len.copy_(torch.tensor(new, dtype=torch.int32))
+        qd.copy_((q * (1 + turn)).to(DEV))
+        want = attended(k, v, table, counts, new, q * (1 + turn), None)
+        for gr, out in zip(graphs, outs):
+            out.fill_(3.0)
+            gr.replay()
+        eager = P.attend(cache, 0, rows, qd)
+        torch.cuda.synchronize()
+        for out in (*outs, eager):
+            assert torch.equal(out.cpu().view(q.shape), want), turn
+
+
+@pytest.mark.parametrize("heads", [1, 5])
+def test_attend_many_sequences(heads):
+    """More sequences than a wave has lanes, most without rows; the context's
+    keys differ widely."""
+    g = torch.Generator().manual_seed(14)
+    counts = [int(torch.randint(0, 3, (1,), generator=g)) for _ in range(150)]
+    lens = [int(torch.randint(0, 90, (1,), generator=g)) for _ in range(150)]
+    lens[70], counts[70], counts[149] = 3000, 2, 2
+    g, k, v, table, cu, q = batch(counts, lens, torch.float16, 1, heads, 64, 16, 15)
+    seen = [[list(range(i + 1)) for i in range(n)] for n in counts]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, 16, heads, 0.125)
+    near(attended(k, v, table, counts, lens, q, None), want, tol, "many sequences")
+
+
+# ------------------------------------------------------------------ tree plan
+
+@pytest.mark.parametrize("counts,lens,page", [
+    ([1], [0], 16), ([60], [2048], 64), ([64, 65, 0, 1, 130], [0, 5, 9, 300, 31], 16),
+    ([1024], [100], 256), ([3] * 200, list(range(200)), 16)])
+def test_tree_plan(counts, lens, page):
+    g = torch.Generator().manual_seed(sum(counts))
+    table, pages = R.random_table(counts, lens, page, 2, g)
+    k = torch.empty(1, pages, 1, page, 64, dtype=torch.float16, device=DEV)
+    cache = P.PagedCache.over(k, k.clone(), table.to(DEV))
+    rows = P.Rows.of(counts, lens, DEV)
+    trees = [R.random_tree(n, g) if n else [] for n in counts]
+    if counts[0] >= 60:  # a line, several roots, parents that are no parents
+        trees[0] = [-1] + list(range(counts[0] - 1))
+        trees[-1] = [-1 if i % 3 == 0 else i - 1 for i in range(counts[-1])]
+        trees[0][7], trees[0][9], trees[0][11] = 7, 1000000, -5
+    flat = [p for t in trees for p in t]
+    anc = [a for t in trees for a in R.ancestors(t)]
+    for words in (-(-max(counts) // 64), -(-max(counts) // 64) + 2):
+        pos = torch.full((len(flat),), -9, dtype=torch.int32, device=DEV)
+        slot, mask = pos.clone(), torch.full((len(flat), words), -9, dtype=torch.int64, device=DEV)
+        P.tree_plan(cache, rows, torch.tensor(flat, dtype=torch.int32, device=DEV), pos, slot, mask)
+        torch.cuda.synchronize()
+        assert torch.equal(mask.cpu(), R.masks(anc, words))
+        t = 0
+        for s, n in enumerate(counts):
+            for i in range(n):
+                assert pos[t].item() == lens[s] + len(anc[t]) - 1 if t < 300 else True
+                t += 1
+        want = torch.cat([(R.slots(table, s, page, lens[s] + n)[0] * page
+                           + R.slots(table, s, page, lens[s] + n)[1])[lens[s]:]
+                          for s, n in enumerate(counts)])
+        assert torch.equal(slot.cpu().long(), want)
+        depth = torch.tensor([len(a) - 1 for a in anc])
+        base = torch.cat([torch.full((n,), c) for n, c in zip(counts, lens)])
+        assert torch.equal(pos.cpu().long(), base + depth)
+    # rows in a line: no parent
+    pos, slot, mask = P.plan(cache, rows)
+    assert mask is None and torch.equal(slot.cpu().long(), want)
+    line = torch.cat([torch.arange(c, c + n) for n, c in zip(counts, lens)])
+    assert torch.equal(pos.cpu().long(), line)
+    mask = torch.empty(len(flat), words, dtype=torch.int64, device=DEV)
+    P.tree_plan(cache, rows, None, pos, slot, mask)
+    torch.cuda.synchronize()
+    assert torch.equal(mask.cpu(), R.masks([list(range(i + 1)) for n in counts for i in range(n)],
+                                           words))
+
+
+def test_tree_plan_of_rows_and_keys_that_do_not_fit():
+    """Rows behind the last sequence, rows past max_rows, a length that does not
+    fit its table, a page that is none: slot -1."""
+    page, k = 16, torch.empty(1, 6, 1, 16, 64, dtype=torch.float16, device=DEV)
+    table = torch.tensor([[0, 1], [2, -1], [3, 9], [4, 5]], dtype=torch.int32, device=DEV)
+    cache = P.PagedCache.over(k, k.clone(), table)
+    cu = torch.tensor([0, 4, 7, 9, 11], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([5, 14, 15, 31], dtype=torch.int32, device=DEV)
+    rows = P.Rows(cu, lens, 13, 3)
+    pos, slot, mask = P.plan(cache, rows, torch.full((13,), -1, dtype=torch.int32, device=DEV))
+    assert slot.tolist() == [5, 6, 7, -1, 46, 47, -1, 63, -1, -1, -1, -1, -1]
+    assert pos[:3].tolist() == [5, 5, 5] and pos[4:7].tolist() == [14, 14, 14]
+    assert mask[:, 0].tolist() == [1, 2, 4, 0, 1, 2, 4, 1, 2, 1, 2, 0, 0]
+
+
+# --------------------------------------------------- norms, rotation and append
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,kv,group,dim,page,norms", [
+    (1, 8, 4, 128, 64, True), (7, 1, 1, 64, 16, True), (37, 2, 5, 64, 32, False),
+    (130, 2, 4, 128, 256, True), (600, 1, 3, 128, 16, True)])
+def test_qkv_append(rows, kv, group, dim, page, norms, dtype):
+    g = torch.Generator().manual_seed(rows)
+    pages = -(-rows // page) + 3
+    fused = (3 * torch.randn(rows, (group + 2) * kv * dim, generator=g)).to(dtype)
+    wq, wk = group * kv * dim, kv * dim
+    qn = (1 + 0.1 * torch.randn(dim, generator=g)).to(dtype) if norms else None
+    kn = (1 + 0.1 * torch.randn(dim, generator=g)).to(dtype) if norms else None
+    # positions from the first to the far end of the type
+    pos = torch.randint(0, 1 << 20, (rows,), generator=g, dtype=torch.int32)
+    pos[0] = 0
+    pos[-1] = 2 ** 31 - 1 if rows > 1 else 12345
+    slot = torch.randperm(pages * page, generator=g)[:rows].int()
+    dead = rows // 3 if rows > 2 else None
+    if dead is not None:
+        slot[dead] = -1
+    old = torch.randn(2, pages, kv, page, dim, generator=g).to(dtype)
+    k, v = old.to(DEV), (old + 1).to(DEV)
+    cache = P.PagedCache.over(k, v, torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+    fd = fused.to(DEV)
+    out = torch.full((rows, wq), 9.0, dtype=dtype, device=DEV)
+    dv = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    P.qkv_append(cache, 1, fd[:, :wq], fd[:, wq:wq + wk], fd[:, wq + wk:], dv(qn), dv(kn), pos.to(DEV),
+                 slot.to(DEV), out, 1e-6, 1e6)
+    torch.cuda.synchronize()
+    live = [t for t in range(rows) if t != dead]
+    want, tol = R.rotated(fused[:, :wq].reshape(rows, -1, dim), qn, pos, 1e-6, 1e6)
+    near(out.cpu().view(rows, -1, dim)[live], want[live], tol[live], "q")
+    if dead is not None:
+        assert bool((out[dead] == 9.0).all())
+    want, tol = R.rotated(fused[:, wq:wq + wk].reshape(rows, kv, dim), kn, pos, 1e-6, 1e6)
+    kc, vc = k.cpu(), v.cpu()
+    at = slot.long()[live]
+    near(kc[1, at // page, :, at % page], want[live], tol[live], "k")
+    assert torch.equal(vc[1, at // page, :, at % page],
+                       fused[:, wq + wk:].reshape(rows, kv, dim)[live])
+    # every other key and value, and the other layer, as they were
+    keep = torch.ones(pages, page, dtype=torch.bool)
+    keep[at // page, at % page] = False
+    for pool, was in ((kc, old), (vc, (old + 1).to(dtype))):
+        assert torch.equal(pool[0], was[0])
+        assert torch.equal(pool[1].transpose(1, 2)[keep], was[1].transpose(1, 2)[keep])
+    # in place, the same bits
+    P.qkv_append(cache, 1, fd[:, :wq], fd[:, wq:wq + wk], fd[:, wq + wk:], dv(qn), dv(kn), pos.to(DEV),
+                 slot.to(DEV), fd[:, :wq], 1e-6, 1e6)
+    torch.cuda.synchronize()
+    assert torch.equal(fd[:, :wq][live], out[live])
+    if dead is not None:
+        assert torch.equal(fd[dead, :wq].cpu(), fused[dead, :wq])
+
+
+# --------------------------------------------------------------------- commit
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts,lens,kv,dim,page,layers,most", [
+    ([1], [0], 1, 64, 16, 1, 1), ([8], [13], 2, 128, 16, 3, 8), ([24, 0, 1, 64], [7, 5, 30, 100], 8, 128, 64, 2, 64),
+    ([130, 40], [60, 15], 3, 64, 16, 2, 40), ([300], [5], 8, 128, 32, 1, 300)])
+def test_commit(counts, lens, kv, dim, page, layers, most, dtype):
+    g = torch.Generator().manual_seed(sum(counts))
+    table, pages = R.random_table(counts, lens, page, 2, g)
+    shape = (layers, pages, kv, page, dim)
+    k, v = torch.randn(shape, generator=g).to(dtype), torch.randn(shape, generator=g).to(dtype)
+    trees, ids, target = [], [], []
+    for n in counts:
+        t = R.random_tree(n, g) if n else []
+        if n > 100:  # deep: most rows follow the one before or the one before that
+            t = [-1] + [max(0, i - 1 - int(torch.randint(0, 2, (1,), generator=g)))
+                        for i in range(1, n)]
+        trees.append(t)
+        # few tokens: siblings of one token and long accepted paths are common
+        ids.append([int(x) for x in torch.randint(0, 2, (n,), generator=g)])
+        target.append([int(x) for x in torch.randint(0, 2, (n,), generator=g)])
+        for j in range(1, n):
+            if torch.rand(1, generator=g) < 0.6:
+                target[-1][t[j]] = ids[-1][j]
+    cu = [0]
+    for n in counts:
+        cu.append(cu[-1] + n)
+    flat = lambda x: torch.tensor([y for z in x for y in z], dtype=torch.int32, device=DEV)  # noqa: E731
+    kd, vd = k.to(DEV), v.to(DEV)
+    cache = P.PagedCache.over(kd, vd, table.to(DEV))
+    rows = P.Rows.of(counts, lens, DEV)
+    S = len(counts)
+    path = torch.full((S, most), -7, dtype=torch.int32, device=DEV)
+    count, nxt, new = (torch.full((S,), -7, dtype=torch.int32, device=DEV) for _ in range(3))
+    P.commit(cache, rows, flat(trees), flat(ids), flat(target), path, count, nxt, new)
+    torch.cuda.synchronize()
+    longest = 0
+    for s, n in enumerate(counts):
+        way, after = R.walk(trees[s], ids[s], target[s], most)
+        longest = max(longest, len(way))
+        assert path[s].tolist() == way + [-1] * (most - len(way))
+        assert (count[s].item(), nxt[s].item(), new[s].item()) == (len(way), after, lens[s] + len(way))
+        pg, row = R.slots(table, s, page, lens[s] + n)
+        src = [lens[s] + i for i in way]
+        dst = list(range(lens[s], lens[s] + len(way)))
+        for pool in (k, v):
+            pool[:, pg[dst], :, row[dst]] = pool[:, pg[src], :, row[src]].clone()
+    assert longest > 1 or max(counts) <= 8
+    assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+
+
+def test_commit_of_lines_and_bad_sequences():
+    """Without parents the rows are a line; a sequence that does not fit its
+    table accepts nothing; a page that is none moves nothing."""
+    page = 16
+    g = torch.Generator().manual_seed(3)
+    k = torch.randn(1, 4, 1, page, 64, generator=g).half()
+    table = torch.tensor([[0, 1], [2, -1], [3, -1]], dtype=torch.int32, device=DEV)
+    kd = k.to(DEV)
+    cache = P.PagedCache.over(kd, kd.clone(), table)
+    rows = P.Rows.of([4, 4, 4], [10, 30, 14], DEV)
+    ids = torch.tensor([5, 6, 7, 8] * 3, dtype=torch.int32, device=DEV)
+    target = torch.tensor([6, 7, 0, 0, 6, 7, 8, 9, 6, 7, 8, 9], dtype=torch.int32, device=DEV)
+    path = torch.empty(3, 3, dtype=torch.int32, device=DEV)
+    count, nxt, new = (torch.empty(3, dtype=torch.int32, device=DEV) for _ in range(3))
+    P.commit(cache, rows, None, ids, target, path, count, nxt, new)
+    torch.cuda.synchronize()
+    assert path.tolist() == [[0, 1, 2], [-1, -1, -1], [0, 1, 2]]
+    assert count.tolist() == [3, 0, 3] and nxt.tolist() == [0, -1, 8] and new.tolist() == [13, 30, 17]
+    assert torch.equal(kd.cpu(), k)
+
+
+# ----------------------------------------------------------------------- pages
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("count,pages,layers,kv,page,dim", [
+    (1, 3, 2, 1, 16, 64), (5, 20, 3, 3, 16, 128), (300, 700, 1, 2, 16, 64), (2, 6, 4, 8, 64, 128)])
+def test_copy_pages(count, pages, layers, kv, page, dim, dtype):
+    g = torch.Generator().manual_seed(count)
+    k, v = (torch.randn(layers, pages, kv, page, dim, generator=g).to(dtype) for _ in range(2))
+    order = torch.randperm(pages, generator=g).tolist()
+    dst, rest = order[:count], order[count:]
+    src = [rest[i % len(rest)] for i in range(count)]  # a page may be read twice
+    kd, vd = k.to(DEV), v.to(DEV)
+    cache = P.PagedCache.over(kd, vd, torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+    P.copy_pages(cache, src, dst)
+    torch.cuda.synchronize()
+    for pool, got in ((k, kd), (v, vd)):
+        pool[:, dst] = pool[:, src]
+        assert torch.equal(got.cpu(), pool)
+
+
+def test_forks_and_compaction_keep_every_sequence():
+    """Sequences that fork, write, roll back and go: each reads its own keys
+    throughout, and after the pool is compacted."""
+    cache = P.PagedCache(layers=2, pages=24, kv_heads=2, seqs=4, max_pages=8, page=16, head_dim=64,
+                         device=DEV)
+    g = torch.Generator().manual_seed(1)
+    text = {}  # what each sequence holds: values [keys, layers, kv, dim]
+
+    def write(seq, start, n):
+        cache.reserve(seq, start, start + n)
+        rows = P.Rows.of([n], [start], DEV)
+        at = P.Rows.of([0] * seq + [n], [0] * seq + [start], DEV)
+        pos, slot, _ = P.plan(cache, at)
+        new = torch.randn(n, 2, 2, 64, generator=g).half()
+        for layer in range(2):
+            x = new[:, layer].reshape(n, 128).to(DEV)
+            P.qkv_append(cache, layer, x, x, x, None, None, pos, slot, x.clone())
+        text[seq] = torch.cat([text.get(seq, new[:0])[:start], new])
+        assert rows.rows == n
+
+    def check():
+        torch.cuda.synchronize()
+        table = cache.table.cpu()
+        assert torch.equal(table, torch.from_numpy(cache.book.table()))
+        for seq, want in text.items():
+            pg, row = R.slots(table, seq, 16, len(want))
+            got = cache.v.cpu()[:, pg, :, row].view(len(want), 2, 2, 64)
+            assert torch.equal(got, want), seq
+
+    write(0, 0, 40)
+    for a, b, keys in ((0, 1, 40), (0, 2, 17)):
+        cache.fork(a, b, keys)
+        text[b] = text[a][:keys]
+    check()
+    write(1, 40, 3)   # into a page that 0 holds too: copied first
+    write(2, 17, 30)
+    check()
+    write(0, 35, 20)  # rolled back and written again
+    check()
+    cache.fork(1, 3, 43)
+    text[3] = text[1]
+    cache.trim(1, 20)
+    text[1] = text[1][:20]
+    write(1, 20, 9)
+    check()
+    cache.trim(0, 0)
+    del text[0]
+    assert cache.compact() > 0
+    check()
+    used = {int(p) for p in cache.table.flatten() if p >= 0}
+    assert used == set(range(len(used)))
+    assert cache.compact() == 0
+    write(0, 0, 33)
+    check()

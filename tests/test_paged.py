@@ -1,0 +1,260 @@
+"""The paged KV cache without a GPU: the header's symbols, the book of pages
+against a plain restatement, and the refusals, which launch nothing."""
+import ctypes
+import os
+import random
+import re
+
+import pytest
+
+from plugins_amd import exl3 as X
+from plugins_amd import paged as P
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_paged_header_symbols_are_exported():
+    text = open(os.path.join(ROOT, "include", "exl3_paged.h")).read()
+    declared = set(re.findall(r"\b(exl3p_[a-z_0-9]+)\s*\(", text))
+    L = X.lib()
+    for name in sorted(declared):
+        assert hasattr(L, name), name
+    assert declared == set(P._SIGS), declared ^ set(P._SIGS)
+
+
+# ------------------------------------------------------------------ the book
+
+class PlainBook:
+    """The book with lists of pages and a set of free ones."""
+
+    def __init__(self, pages, page, seqs, max_pages):
+        self.page, self.max_pages, self.free = page, max_pages, set(range(pages))
+        self.has = [[] for _ in range(seqs)]
+
+    def holders(self, p):
+        return sum(p in h for h in self.has)
+
+    def take(self):
+        p = min(self.free)
+        self.free.remove(p)
+        return p
+
+    def reserve(self, seq, start, stop):
+        need, h = -(-stop // self.page), list(self.has[seq])
+        if need > self.max_pages:
+            return None
+        first = start // self.page if stop > start else need
+        redo = [i for i in range(first, min(need, len(h))) if self.holders(h[i]) > 1]
+        if len(redo) + max(0, need - len(h)) > len(self.free):
+            return None
+        src, dst = [], []
+        for i in redo:
+            p = self.take()
+            if i * self.page < start:
+                src.append(h[i])
+                dst.append(p)
+            h[i] = p
+        while len(h) < need:
+            h.append(self.take())
+        self.has[seq] = h
+        return src, dst
+
+    def fork(self, src, dst, keys):
+        n = -(-keys // self.page)
+        if src == dst or self.has[dst] or n > len(self.has[src]):
+            return None
+        self.has[dst] = self.has[src][:n]
+        return True
+
+    def trim(self, seq, keys):
+        n = -(-keys // self.page)
+        gone, self.has[seq] = self.has[seq][n:], self.has[seq][:n]
+        self.free |= {p for p in gone if self.holders(p) == 0}
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_book_against_a_plain_one(seed):
+    rng = random.Random(seed)
+    pages, page, seqs, most = rng.randint(5, 40), rng.choice([16, 64]), rng.randint(2, 6), rng.randint(2, 12)
+    a, b = P.Book(pages, page, seqs, most), PlainBook(pages, page, seqs, most)
+    for _ in range(400):
+        do, s = rng.choice(["reserve", "reserve", "fork", "trim", "compact"]), rng.randrange(seqs)
+        if do == "reserve":
+            stop = rng.randint(0, most * page + page)
+            start = rng.randint(0, stop)
+            want = b.reserve(s, start, stop)
+            if want is None:
+                with pytest.raises(X.Exl3Error) as e:
+                    a.reserve(s, start, stop)
+                assert e.value.code == X.TOO_LARGE
+            else:
+                assert a.reserve(s, start, stop) == want
+        elif do == "fork":
+            t, keys = rng.randrange(seqs), rng.randint(0, most * page)
+            if b.fork(s, t, keys) is None:
+                with pytest.raises(X.Exl3Error):
+                    a.fork(s, t, keys)
+            else:
+                a.fork(s, t, keys)
+        elif do == "trim":
+            keys = rng.randint(0, most * page)
+            a.trim(s, keys)
+            b.trim(s, keys)
+        elif rng.random() < 0.3:
+            room = rng.choice([None, 0, 1, 3])
+            src, dst = a.compact(room)
+            assert not set(src) & set(dst) and len(set(dst)) == len(dst)
+            used = sorted({p for h in b.has for p in h})
+            if room is None:
+                assert set(used) - set(src) | set(dst) == set(range(len(used)))
+            to = dict(zip(src, dst))
+            b.has = [[to.get(p, p) for p in h] for h in b.has]
+            b.free = set(range(pages)) - {p for h in b.has for p in h}
+        t = a.table()
+        for s2, h in enumerate(b.has):
+            assert t[s2].tolist() == h + [-1] * (most - len(h))
+            assert a.held(s2) == len(h)
+        assert a.free_pages() == len(b.free)
+        for p in range(pages):
+            assert a.shared(p) == b.holders(p)
+
+
+def test_book_refuses():
+    for bad in ((0, 16, 1, 1), (1, 15, 1, 1), (1, 8, 1, 1), (1, 512, 1, 1), (1, 48, 1, 1),
+                (1, 16, 0, 1), (1, 16, 1, 0)):
+        with pytest.raises(X.Exl3Error, match="PagedBookShape"):
+            P.Book(*bad)
+    with pytest.raises(X.Exl3Error) as e:
+        P.Book(1 << 27, 16, 1, 1)
+    assert e.value.code == X.TOO_LARGE
+    b = P.Book(4, 16, 2, 3)
+    for call in (lambda: b.reserve(2, 0, 1), lambda: b.reserve(-1, 0, 1), lambda: b.reserve(0, 5, 4),
+                 lambda: b.reserve(0, -1, 4), lambda: b.fork(0, 0, 0), lambda: b.fork(0, 2, 0),
+                 lambda: b.fork(0, 1, 1), lambda: b.fork(0, 1, -1), lambda: b.trim(2, 0),
+                 lambda: b.trim(0, -1)):
+        with pytest.raises(X.Exl3Error):
+            call()
+    assert b.free_pages() == 4 and b.held(5) == -1 and b.shared(4) == -1
+    # no room for the pair: nothing happens
+    b.reserve(0, 0, 20)
+    b.fork(0, 1, 20)
+    n = ctypes.c_int32(5)
+    v = P.paged_lib().exl3p_book_reserve(b._b, 1, 20, 21, None, None, 0, ctypes.byref(n))
+    assert v.code == X.TOO_LARGE and n.value == 0 and b.table().tolist() == [[0, 1, -1], [0, 1, -1]]
+
+
+# ------------------------------------------------------------------- refusals
+
+def desc(**kw):
+    """A cache whose arrays are addresses that nothing reads."""
+    f = dict(size=ctypes.sizeof(P.CacheDesc), dtype=X.DT_F16, k=4096, v=8192, layers=2, pages=8,
+             kv_heads=2, page=16, dim=128, seqs=3, max_pages=4, table=64)
+    f.update(kw)
+    return P.CacheDesc(**f)
+
+
+def step(**kw):
+    f = dict(size=ctypes.sizeof(P.RowsDesc), seqs=2, rows=6, max_rows=4, cu=64, len=64)
+    f.update(kw)
+    return P.RowsDesc(**f)
+
+
+def entries(c, r, **kw):
+    """Every operator's entry on these, with arguments that nothing reads; kw
+    replaces some of them."""
+    L, A = P.paged_lib(), dict(parent=64, pos=64, slot=64, mask=64, words=1, layer=0, heads=8,
+                               q=4096, qs=1024, kn=None, eps=1e-6, theta=1e4, out=4096, os=1024,
+                               ks=256, scale=1.0, scratch=4096, bytes=1 << 40, ids=64, target=64,
+                               path=64, most=4, count=64, new_len=128, src=(0,), dst=(1,), n=None,
+                               rows=6)
+    A.update(kw)
+    c, r = ctypes.byref(c), ctypes.byref(r)
+    arr = lambda x: (ctypes.c_int32 * max(1, len(x)))(*x)  # noqa: E731
+    return {
+        "plan": lambda: L.exl3p_tree_plan(c, r, A["parent"], A["pos"], A["slot"], A["mask"],
+                                          A["words"], None),
+        "append": lambda: L.exl3p_qkv_append(c, A["layer"], A["rows"], A["heads"], A["q"], A["qs"],
+                                             A["q"], A["ks"], A["q"], A["ks"], None, A["kn"],
+                                             A["pos"], A["slot"], A["out"], A["os"], A["eps"],
+                                             A["theta"], None),
+        "attend": lambda: L.exl3p_attend(c, A["layer"], r, A["heads"], A["q"], A["qs"], A["mask"],
+                                         A["words"], A["scale"], A["out"], A["os"], A["scratch"],
+                                         A["bytes"], None),
+        "commit": lambda: L.exl3p_commit(c, r, A["parent"], A["ids"], A["target"], A["path"],
+                                         A["most"], A["count"], A["count"], A["new_len"], None),
+        "copy": lambda: L.exl3p_copy_pages(c, arr(A["src"]), arr(A["dst"]),
+                                           len(A["src"]) if A["n"] is None else A["n"], None),
+    }
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(size=8), "another version"), (dict(dtype=X.DT_F32), "PagedCacheDtype"),
+    (dict(k=None), "missing"), (dict(v=None), "missing"), (dict(table=None), "missing"),
+    (dict(k=4100), "Alignment"), (dict(dim=96), "PagedCacheDim"), (dict(dim=256), "PagedCacheDim"),
+    (dict(page=8), "PagedCachePage"), (dict(page=48), "PagedCachePage"),
+    (dict(page=512), "PagedCachePage"), (dict(pages=0), "PagedCacheShape"),
+    (dict(layers=-1), "PagedCacheShape"), (dict(pages=1 << 27), "2\\^31"),
+    (dict(max_pages=1 << 27), "2\\^31"), (dict(kv_heads=65536), "65535")])
+def test_caches_that_are_refused(kw, why):
+    for name, call in entries(desc(**kw), step()).items():
+        v = call()
+        assert v.code != X.OK and re.search(why, v.reason), (name, v)
+    assert P.paged_lib().exl3p_attend_scratch_bytes(ctypes.byref(desc(**kw)), ctypes.byref(step()), 8) == 0
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(size=1), "another version"), (dict(seqs=-1), "PagedRows"), (dict(seqs=4), "more sequences"),
+    (dict(rows=-1), "PagedRows"), (dict(max_rows=7), "PagedRows"), (dict(max_rows=-1), "PagedRows"),
+    (dict(cu=None), "missing"), (dict(len=None), "missing")])
+def test_rows_that_are_refused(kw, why):
+    e = entries(desc(), step(**kw))
+    for name in ("plan", "attend", "commit"):
+        v = e[name]()
+        assert v.code != X.OK and re.search(why, v.reason), (name, v)
+
+
+@pytest.mark.parametrize("names,kw,why", [
+    (("plan", "attend"), dict(mask=None), "PagedMask"), (("plan", "attend"), dict(words=0), "PagedMask"),
+    (("plan", "attend"), dict(words=-1), "PagedMask"),
+    (("plan", "append"), dict(pos=None), "missing"), (("plan", "append"), dict(slot=None), "missing"),
+    (("append", "attend"), dict(layer=2), "PagedLayer"), (("append", "attend"), dict(layer=-1), "PagedLayer"),
+    (("append", "attend"), dict(heads=7), "PagedHeads"), (("append", "attend"), dict(heads=0), "PagedHeads"),
+    (("append", "attend"), dict(q=None), "missing"), (("append", "attend"), dict(q=4104), "Alignment"),
+    (("append", "attend"), dict(qs=1020), "Alignment"), (("append", "attend"), dict(qs=1016), "overlap"),
+    (("append", "attend"), dict(out=None), "missing"), (("append", "attend"), dict(os=512), "overlap"),
+    (("append",), dict(ks=128), "overlap"), (("append",), dict(theta=0.0), "PagedTheta"),
+    (("append",), dict(theta=float("nan")), "PagedTheta"),
+    (("append",), dict(theta=float("inf")), "PagedTheta"),
+    (("append",), dict(kn=68), "Alignment"), (("append",), dict(rows=-1), "PagedRows"),
+    (("attend",), dict(scratch=None), "PagedScratch"), (("attend",), dict(scratch=4100), "PagedScratch"),
+    (("attend",), dict(bytes=100), "PagedScratch"),
+    (("commit",), dict(most=0), "PagedPath"), (("commit",), dict(path=None), "missing"),
+    (("commit",), dict(ids=None), "missing"), (("commit",), dict(target=None), "missing"),
+    (("commit",), dict(new_len=64), "over len"), (("commit",), dict(count=None), "missing"),
+    (("copy",), dict(n=-1), "below 0"), (("copy",), dict(src=(8,)), "outside"),
+    (("copy",), dict(dst=(-1,)), "outside"), (("copy",), dict(src=(0, 1), dst=(2, 2)), "twice"),
+    (("copy",), dict(src=(0, 1), dst=(1, 2)), "both"), (("copy",), dict(src=(3,), dst=(3,)), "both"),
+    (("copy",), dict(src=tuple([0] * 9), dst=tuple(range(9))), "twice")])
+def test_calls_that_are_refused(names, kw, why):
+    e = entries(desc(), step(), **kw)
+    for name in names:
+        v = e[name]()
+        assert v.code != X.OK and re.search(why, v.reason), (name, v)
+
+
+def test_masks_and_trees_too_large_are_refused():
+    big = step(rows=5000, max_rows=1025)
+    e = entries(desc(), big, words=17)
+    assert "1024" in e["plan"]().reason and "1024" in e["commit"]().reason
+    for name in ("plan", "attend"):
+        assert "PagedMask" in entries(desc(), big, words=16)[name]().reason
+
+
+def test_nothing_to_do_is_no_refusal():
+    """No rows, no sequences, no pages: accepted before any launch."""
+    none = step(rows=0, max_rows=0)
+    e = entries(desc(), none, words=0, mask=None, rows=0, src=(), dst=())
+    for name in ("plan", "append", "attend", "copy"):
+        assert e[name]().code == X.OK, name
+    e = entries(desc(), step(seqs=0), words=1)
+    assert e["attend"]().code == X.OK and e["commit"]().code == X.OK
