@@ -96,6 +96,21 @@ __device__ __forceinline__ float xor_lanes(float v, int m) {
   return bits<float>((lane & 32) ? r[0] : r[1]);
 }
 
+// 16 bytes per lane from global memory (base + voff) straight into LDS at
+// address lds + 16 * lane.  M0 carries the LDS address (the compiler uses
+// M0 for nothing in these kernels); an LDS DMA that reads M0 right after it
+// is written needs wait states between them (the compiler's hazard check
+// does not see into asm), hence the s_nop.  vmcnt counts the load until its
+// bytes are in LDS.
+__device__ __forceinline__ void lds_dma16(const void *base, uint32_t voff, uint32_t lds) {
+  // M0 is not named as clobbered: the AMDGPU backend reserves it and ignores
+  // (with a warning) such a clobber; no other instruction in the kernels that
+  // call this reads M0 (their gfx950 code sets it only here).
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds),
+               "v"(voff), "s"(base)
+               : "memory");
+}
+
 // One Hadamard butterfly step with the partner's value p: the lower lane of
 // the pair (sg = +1) forms v + p, the upper (sg = -1) p - v.  sg * v is exact,
 // so the fused form rounds once, exactly as the add or the subtraction does.

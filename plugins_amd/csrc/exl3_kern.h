@@ -1414,21 +1414,6 @@ constexpr int GW_A0 = 2 * GW_BBUF;            // the A buffers follow the two B 
 constexpr int GW_LDS_BYTES = GW_A0 + 3 * GW_ABUF;  // 132 KiB
 static_assert(64 * GM_FLD * 4 <= GW_A0, "finish exchange reaches the A buffers");
 
-// 16 bytes per lane from global memory (base + voff) straight into LDS at
-// address lds + 16 * lane.  M0 carries the LDS address (the compiler uses
-// M0 for nothing in these kernels); an LDS DMA that reads M0 right after it
-// is written needs wait states between them (the compiler's hazard check
-// does not see into asm), hence the s_nop.  vmcnt counts the load until its
-// bytes are in LDS.
-__device__ __forceinline__ void lds_dma16(const void *base, uint32_t voff, uint32_t lds) {
-  // M0 is not named as clobbered: the AMDGPU backend reserves it and ignores
-  // (with a warning) such a clobber; no other instruction in the kernels that
-  // call this reads M0 (their gfx950 code sets it only here).
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds),
-               "v"(voff), "s"(base)
-               : "memory");
-}
-
 // The MFMA waves' main loop.  ax[kk]: byte address of the wave's A fragment
 // kk in A buffer 0 (row block i adds 4 KiB, buffer a adds a * GW_ABUF);
 // brd: half index of its B fragment 0 in B buffer 0; voff[u]: its

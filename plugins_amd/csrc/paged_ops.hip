@@ -16,6 +16,11 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -24,24 +29,42 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // and the power of two that softmax weights are scaled by (exponents below).
 struct F16 {
   typedef _Float16 T;
+  typedef half2_t T2;
   typedef half8 V8;
   static constexpr uint32_t EXP = 0x7C00u;
-  // weights of 2^15 and less: one 2^-40 as large as the row's largest is still
-  // not lost to f16's smallest number (2^-24)
-  static constexpr float LIFT = 15.0f;
+  // weights of 2^(11 + SLACK) and less: one 2^-35 as large as the row's largest
+  // is still not lost to f16's smallest number (2^-24)
+  static constexpr float LIFT = 11.0f;
   static __device__ __forceinline__ f32x4 mma(V8 a, V8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mma(V8 a, V8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  // c plus both elements
+  static __device__ __forceinline__ float add2(uint32_t v, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, v), half2_t{1, 1}, c, false);
   }
 };
 struct BF16 {
   typedef __bf16 T;
+  typedef bf16x2 T2;
   typedef bf16x8 V8;
   static constexpr uint32_t EXP = 0x7F80u;
   static constexpr float LIFT = 0.0f;  // f32's exponents
   static __device__ __forceinline__ f32x4 mma(V8 a, V8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x16 mma(V8 a, V8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add2(uint32_t v, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), bf16x2{1, 1}, c, false);
+  }
 };
+// A row's reference for its weights follows its running maximum only in steps of
+// more than SLACK (powers of two): what has been summed is rarely scaled again.
+constexpr float SLACK = 4.0f;
 
 template <typename E>
 __device__ __forceinline__ float to_f32(uint32_t bits) {
@@ -53,7 +76,7 @@ __device__ __forceinline__ uint32_t from_f32(float f) {
 }
 template <typename E>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return from_f32<E>(a) | (from_f32<E>(b) << 16);
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), typename E::T2));
 }
 
 // What the kernels need of a cache and of a step's rows.
@@ -277,7 +300,8 @@ __device__ __forceinline__ int keys_of_item(const Step &st, const Split &sl, int
   return max(sl.least, (int)fmin(per, (double)(1 << 24)) * 64);
 }
 
-// Item (ITEM) or tile (otherwise) number x among the sequences' ones.
+// Item (ITEM) number x among the sequences' ones, or tile number x among those
+// that are split.
 template <bool ITEM>
 __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64_t room, int x) {
   const int lane = threadIdx.x & 63;
@@ -295,7 +319,7 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
       ns = (int)(((int64_t)sp.len + sp.n + chunk - 1) / chunk);
     }
     // inclusive sums over the lanes
-    int it = nt * ns, ti = nt;
+    int it = nt * ns, ti = ns > 1 ? nt : 0;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
       const int a = __shfl_up(it, m, 64), b = __shfl_up(ti, m, 64);
@@ -313,14 +337,16 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
       // the last tile first: a prompt's last rows see the most keys
       const int u = ITEM ? (x - before) / ns : nt - 1 - (x - tbefore);
       const int tile = ITEM ? nt - 1 - u : x - tbefore;
-      w.s = s_;
-      w.sp = sp;
-      w.r0 = tile * sl.tile;
-      w.first = before + (nt - 1 - tile) * ns;
-      w.splits = ns;
       const int j = ITEM ? (x - before) % ns : 0;
-      w.k0 = j * chunk;
-      w.k1 = min(w.k0 + chunk, sp.len + sp.n);
+      // the same in all lanes: said so, for addresses and branches in scalars
+      auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+      w.s = one(s_);
+      w.sp = Span{one(sp.row), one(sp.n), one(sp.len), (bool)one(sp.bad)};
+      w.r0 = one(tile * sl.tile);
+      w.first = one(before + (nt - 1 - tile) * ns);
+      w.splits = one(ns);
+      w.k0 = one(j * chunk);
+      w.k1 = one(min(j * chunk + chunk, sp.len + sp.n));
       return w;
     }
     items += __shfl(it, 63, 64);
@@ -337,21 +363,77 @@ struct AttnArgs {
   int64_t qs;
   const uint64_t *mask;
   int words;
-  float scale;  // times log2(e): weights are powers of two
+  float scale;    // |scale| log2(e): weights are powers of two
+  uint32_t flip;  // 0x80008000 where the scale is negative: q's sign bits
   uint16_t *out;
   int64_t os;
   float *part;  // [items * kv][tile][D] sums, then [items * kv][tile][2] (max, sum)
   int slots;    // items * kv that part holds
 };
 
-// Bit `node` of a row's mask; without masks a row sees the rows up to itself.
-__device__ __forceinline__ bool sees(const AttnArgs &a, const Span &sp, int i, int node) {
-  if (node >= sp.n) return false;
-  if (a.mask == nullptr) return node <= i;
-  return (a.mask[(size_t)(sp.row + i) * a.words + (node >> 6)] >> (node & 63)) & 1;
+// Which of keys kb .. kb + 63 (below `last`) row i of a sequence sees, a bit a
+// key: the context's, and of the rows those in its mask, or up to itself.
+__device__ __forceinline__ uint64_t seen64(const AttnArgs &a, const Span &sp, int i, int kb,
+                                           int last) {
+  const int lim = a.mask == nullptr ? min(last, sp.len + i + 1) : min(last, sp.len + sp.n);
+  if (lim <= kb) return 0;
+  uint64_t v = lim - kb >= 64 ? ~0ull : ~0ull >> (64 - (lim - kb));
+  if (a.mask != nullptr && lim > sp.len) {
+    const uint64_t *m = a.mask + (size_t)(sp.row + i) * a.words;
+    const int j = kb - sp.len;  // the first key's number among the rows
+    const uint64_t lo = j >= 0 && (j >> 6) < a.words ? m[j >> 6] >> (j & 63) : 0;
+    const int next = j >= 0 ? (j >> 6) + 1 : 0, by = j >= 0 ? 64 - (j & 63) : -j;
+    const uint64_t hi = by < 64 && next < a.words ? m[next] << by : 0;
+    v &= j >= 0 ? lo | hi : j > -64 ? hi | ~(~0ull << -j) : ~0ull;
+  }
+  return v;
 }
 
-constexpr int AW = 4;  // waves of an attention workgroup
+constexpr int AW = 4;      // waves of an attention workgroup
+constexpr int FEW = 16;    // pairs of a tile: one of attend_few's,
+constexpr int MANY = 128;  // one of attend_many's
+
+// A wave's softmax over the keys it has seen: the reference of each pair's
+// weights and the sum of them.
+struct Soft {
+  float ref, sum;
+};
+
+// The running maximum `hi` (already times the scale) of each lane's pair joins
+// its reference; the factor for what has been summed so far is 1 (false) unless
+// some pair of the wave outgrew its reference by more than SLACK.
+__device__ __forceinline__ bool outgrown(Soft &so, float hi, float &alpha) {
+  if (__ballot(hi > so.ref + SLACK) == 0) return false;
+  const float now = fmaxf(so.ref, hi);
+  alpha = __builtin_amdgcn_exp2f(so.ref - (now == -INFINITY ? 0.0f : now));
+  so.ref = now;
+  so.sum *= alpha;
+  return true;
+}
+
+// A new row's value that is infinite or NaN would reach, times a weight of zero,
+// the rows that do not see it.  Such elements are taken out of the products
+// (finite(): zero in their place), and added afterwards to the rows that see
+// them: they are so whatever their weight.
+template <typename E>
+__device__ __forceinline__ uint32_t finite(uint32_t two) {
+  if ((two & E::EXP) == E::EXP) two &= 0xFFFF0000u;
+  if (((two >> 16) & E::EXP) == E::EXP) two &= 0xFFFFu;
+  return two;
+}
+// element e of a pair of elements where it is not finite, else 0
+template <typename E>
+__device__ __forceinline__ float not_finite(uint32_t two, int e) {
+  const uint32_t one = e ? two >> 16 : two & 0xFFFFu;
+  return (one & E::EXP) == E::EXP ? to_f32<E>(one) : 0.0f;
+}
+// a key's value row, for the rare rows above (nullptr: no page)
+__device__ __forceinline__ const uint16_t *value_row(const Pool &p, int s, int head, int key, int D) {
+  const int sl = slot_of(p, s, key);
+  if (sl < 0) return nullptr;
+  const size_t row = (((size_t)(sl >> p.lp) * p.kv + head) << p.lp) + (sl & ((1 << p.lp) - 1));
+  return reinterpret_cast<const uint16_t *>(p.v) + row * D;
+}
 
 // 16 pairs a workgroup; its waves take 32 keys in turn and join at the end.
 // Scores are S^T = K q^T (rows keys, columns pairs), so a lane holds 8 keys'
@@ -359,79 +441,104 @@ constexpr int AW = 4;  // waves of an attention workgroup
 // P^T, wants its right operand if V's keys are taken in the same order: the
 // weights never leave their lane.
 template <typename E, int D>
-__global__ __launch_bounds__(64 * AW) void attend_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
   constexpr int KK = D / 32;  // products of 32 dims a score
   constexpr int VH = D / 16;  // dims a lane loads of a value
   typedef typename std::conditional<VH == 8, u32x4, u32x2>::type VV;
   typedef typename E::V8 V8;
-  __shared__ float so[AW][16][D + 4];
-  __shared__ float sm[AW][16], sl[AW][16];
+  __shared__ float so[AW][FEW][D + 4];
+  __shared__ float sm[AW][FEW], sl[AW][FEW];
   __shared__ int sbad;
   const int head = blockIdx.x % a.pool.kv, item = blockIdx.x / a.pool.kv;
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
-  Work w = find_work<true>(a.st, a.sl, room, item);
+  const Work w = find_work<true>(a.st, a.sl, room, item);
   if (w.s < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int G = a.sl.group, pairs = w.sp.n * G;
-  const int pair = w.r0 + col, i = min(pair, pairs - 1) / G;
-  const int hq = head * G + min(pair, pairs - 1) % G;
-  const bool direct = w.splits == 1;
+  const int pair = min(w.r0 + col, pairs - 1), i = pair / G, hq = head * G + pair % G;
   // no row of the tile sees past its last row's own key without masks
   int last = w.sp.bad ? w.k0 : w.k1;
-  if (a.mask == nullptr) last = min(last, w.sp.len + (min(w.r0 + 16, pairs) - 1) / G + 1);
-
+  if (a.mask == nullptr) last = min(last, w.sp.len + (min(w.r0 + FEW, pairs) - 1) / G + 1);
   if (threadIdx.x == 0) sbad = w.sp.bad;
   __syncthreads();
-  u32x4 qf[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk)
-    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.sp.row + i) * a.qs + hq * D + 32 * kk + 8 * g);
-
-  f32x4 acc[VH];
-#pragma unroll
-  for (int m = 0; m < VH; ++m) acc[m] = f32x4{0, 0, 0, 0};
-  float top = -INFINITY, sum = 0.0f;
-  bool bad = false;
 
   const int steps = last > w.k0 ? (last - w.k0 + 31) / 32 : 0;
   const int *trow = a.pool.table + (size_t)w.s * a.pool.max_pages;
+  const uint16_t *pk = reinterpret_cast<const uint16_t *>(a.pool.k) + col * D + 8 * g;
+  const uint16_t *pv = reinterpret_cast<const uint16_t *>(a.pool.v) + 4 * g * D + VH * col;
+  bool bad = false;
   u32x4 kf[2][KK];
   VV vf[8];
-  // where the two blocks of 16 keys of a step lie (elements from the layer's
-  // first); blocks behind the last key read the last key's block
+  uint32_t ids[2];
   size_t at[2];
+  // the pages of a step's two blocks of 16 keys; blocks behind the last key
+  // stand for the last key's
+  auto key_of = [&](int step, int t) {
+    return min(w.k0 + step * 32 + 16 * t, (last - 1) & ~15);
+  };
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) ids[t] = (uint32_t)trow[key_of(step, t) >> a.pool.lp];
+  };
+  // where the blocks lie (elements from the layer's first)
   auto locate = [&](int step) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int key = min(w.k0 + step * 32 + 16 * t, (last - 1) & ~15);
-      uint32_t page = (uint32_t)trow[key >> a.pool.lp];
+      uint32_t page = __builtin_amdgcn_readfirstlane(ids[t]);
       if (page >= (uint32_t)a.pool.pages) bad = true, page = 0;
-      at[t] = ((((size_t)page * a.pool.kv + head) << a.pool.lp) + (key & ((1 << a.pool.lp) - 1))) * D;
+      at[t] = ((((size_t)page * a.pool.kv + head) << a.pool.lp) +
+               (key_of(step, t) & ((1 << a.pool.lp) - 1))) * D;
     }
   };
-  auto load_k = [&]() {
+  auto load_k = [&] {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint16_t *p = reinterpret_cast<const uint16_t *>(a.pool.k) + at[t] + col * D + 8 * g;
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) kf[t][kk] = *reinterpret_cast<const u32x4 *>(p + 32 * kk);
-    }
+      for (int kk = 0; kk < KK; ++kk)
+        kf[t][kk] = *reinterpret_cast<const u32x4 *>(pk + at[t] + 32 * kk);
   };
-  auto load_v = [&]() {
+  auto load_v = [&] {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint16_t *p = reinterpret_cast<const uint16_t *>(a.pool.v) + at[t] + 4 * g * D + VH * col;
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) vf[4 * t + r] = *reinterpret_cast<const VV *>(p + r * D);
-    }
+      for (int r = 0; r < 4; ++r)
+        vf[4 * t + r] = *reinterpret_cast<const VV *>(pv + at[t] + r * D);
   };
 
-  for (int step = wave; step < steps; step += AW) {
-    const int kb = w.k0 + step * 32;
-    locate(step);
+  u32x4 qf[KK];
+  if (wave < steps) {
+    fetch(wave);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.sp.row + i) * a.qs + hq * D + 32 * kk + 8 * g);
+      qf[kk] = qf[kk] ^ a.flip;
+    }
+    locate(wave);
     load_k();
     load_v();
+    if (wave + AW < steps) fetch(wave + AW);
+  }
+  f32x4 acc[VH];
+#pragma unroll
+  for (int m = 0; m < VH; ++m) acc[m] = f32x4{0, 0, 0, 0};
+  Soft sf{-INFINITY, 0.0f};
+
+  auto products = [&](const VV(&vv)[8], const uint32_t(&pp)[4], f32x4(&o)[VH]) {
+    const V8 pb = __builtin_bit_cast(V8, u32x4{pp[0], pp[1], pp[2], pp[3]});
+#pragma unroll
+    for (int m = 0; m < VH; ++m) {
+      const uint32_t sel = m & 1 ? 0x07060302u : 0x05040100u;
+      u32x4 av;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        av[x] = __builtin_amdgcn_perm(vv[2 * x + 1][m >> 1], vv[2 * x][m >> 1], sel);
+      o[m] = E::mma(__builtin_bit_cast(V8, av), pb, o[m]);
+    }
+  };
+  auto turn = [&](int step, auto MORE) {
+    constexpr bool more = decltype(MORE)::value;
+    const int kb = w.k0 + step * 32;
     f32x4 s2[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -439,89 +546,80 @@ __global__ __launch_bounds__(64 * AW) void attend_kernel(AttnArgs a) {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
         s2[t] = E::mma(__builtin_bit_cast(V8, kf[t][kk]), __builtin_bit_cast(V8, qf[kk]), s2[t]);
-      s2[t] = s2[t] * a.scale;
+    }
+    if constexpr (more) {
+      locate(step + AW);
+      load_k();
+      fetch(min(step + 2 * AW, steps - 1));
     }
     const bool tail = kb + 32 > min(w.sp.len, last);
-    bool odd = false;  // a value among the new rows that is not finite
+    uint32_t seen = ~0u;
+    uint32_t odd = 0;  // keys among the new rows with a value that is not finite
     if (tail) {
+      seen = (uint32_t)seen64(a, w.sp, i, kb, last);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int key = kb + 16 * (e >> 2) + 4 * g + (e & 3);
-        const bool in = key < last && (key < w.sp.len || sees(a, w.sp, i, key - w.sp.len));
-        if (!in) s2[e >> 2][e & 3] = -INFINITY;
+        const int x = 16 * (e >> 2) + 4 * g + (e & 3);
+        if (!(seen >> x & 1)) s2[e >> 2][e & 3] = -INFINITY;
         // values behind the last key are nobody's
-        if (key >= last) vf[e] = VV{};
+        if (kb + x >= last) vf[e] = VV{};
+        bool bad_value = false;
+        if (kb + x >= w.sp.len) {
 #pragma unroll
-        for (int x = 0; x < VH / 2; ++x)
-          odd |= key >= w.sp.len && ((vf[e][x] & E::EXP) == E::EXP ||
-                                     (vf[e][x] >> 16 & E::EXP) == E::EXP);
+          for (int y = 0; y < VH / 2; ++y) {
+            const uint32_t f = finite<E>(vf[e][y]);
+            bad_value |= f != vf[e][y];
+            vf[e][y] = f;
+          }
+        }
+        const uint64_t lanes = __ballot(bad_value);
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (lanes >> (16 * z) & 0xFFFFu) odd |= 1u << (16 * (e >> 2) + 4 * z + (e & 3));
       }
     }
-    float hi = -INFINITY;
+    float hi = fmaxf(s2[0][0], s2[0][1]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) hi = fmaxf(hi, s2[e >> 2][e & 3]);
+    for (int e = 2; e < 8; ++e) hi = fmaxf(hi, s2[e >> 2][e & 3]);
     hi = fmaxf(hi, exl3::xor_lanes(hi, 16));
     hi = fmaxf(hi, exl3::xor_lanes(hi, 32));
-    const float now = fmaxf(top, hi);
-    const float ref = now == -INFINITY ? 0.0f : now;
-    const float alpha = __builtin_amdgcn_exp2f(top - ref);
-    top = now;
-    sum *= alpha;
+    float alpha;
+    if (outgrown(sf, hi * a.scale, alpha)) {
 #pragma unroll
-    for (int m = 0; m < VH; ++m) acc[m] = acc[m] * alpha;
+      for (int m = 0; m < VH; ++m) acc[m] = acc[m] * alpha;
+    }
+    const float by = E::LIFT - (sf.ref == -INFINITY ? 0.0f : sf.ref);
     uint32_t pw[4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const uint32_t b = pack2<E>(__builtin_amdgcn_exp2f(s2[e >> 2][e & 3] - ref + E::LIFT),
-                                  __builtin_amdgcn_exp2f(s2[e >> 2][(e & 3) + 1] - ref + E::LIFT));
-      pw[e >> 1] = b;
+      pw[e >> 1] = pack2<E>(__builtin_amdgcn_exp2f(fmaf(s2[e >> 2][e & 3], a.scale, by)),
+                            __builtin_amdgcn_exp2f(fmaf(s2[e >> 2][(e & 3) + 1], a.scale, by)));
       // the sum of the rounded weights: they add up to one after the division
-      sum += to_f32<E>(b) + to_f32<E>(b >> 16);
+      sf.sum = E::add2(pw[e >> 1], sf.sum);
     }
-    auto products = [&](const VV(&vv)[8], const uint32_t(&pp)[4], f32x4(&o)[VH]) {
-      const V8 pb = __builtin_bit_cast(V8, u32x4{pp[0], pp[1], pp[2], pp[3]});
+    products(vf, pw, acc);
+    for (; odd != 0; odd &= odd - 1) {
+      const int x = __builtin_ctz(odd);
+      const uint16_t *row = value_row(a.pool, w.s, head, kb + x, D);
+      if (row == nullptr || !(seen >> x & 1)) continue;
 #pragma unroll
-      for (int m = 0; m < VH; ++m) {
-        const uint32_t sel = m & 1 ? 0x07060302u : 0x05040100u;
-        u32x4 av;
+      for (int r = 0; r < 4; ++r) {
+        const VV b = *reinterpret_cast<const VV *>(row + VH * (4 * g + r));
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          av[x] = __builtin_amdgcn_perm(vv[2 * x + 1][m >> 1], vv[2 * x][m >> 1], sel);
-        o[m] = E::mma(__builtin_bit_cast(V8, av), pb, o[m]);
-      }
-    };
-    if (!tail || __ballot(odd) == 0) {
-      products(vf, pw, acc);
-    } else {
-      // a new row's value is infinite or NaN: a weight of zero would not keep
-      // it from the rows that do not see it, so key by key, and only the pairs
-      // that see the key take its product
-      for (int x = 0; x < 32; ++x) {
-        const int e = 4 * (x >> 4) + (x & 3);
-        const bool mine = g == ((x >> 2) & 3);
-        VV vx[8];
-        uint32_t px[4];
-#pragma unroll
-        for (int y = 0; y < 8; ++y) vx[y] = y == e && mine ? vf[y] : VV{};
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-          px[y] = y == e >> 1 && mine ? pw[y] & (e & 1 ? 0xFFFF0000u : 0xFFFFu) : 0;
-        f32x4 o[VH];
-#pragma unroll
-        for (int m = 0; m < VH; ++m) o[m] = acc[m];
-        products(vx, px, o);
-        const int key = kb + x;
-        const bool in = key < last && (key < w.sp.len || sees(a, w.sp, i, key - w.sp.len));
-#pragma unroll
-        for (int m = 0; m < VH; ++m)
-          if (in) acc[m] = o[m];
+        for (int m = 0; m < VH; ++m) acc[m][r] += not_finite<E>(b[m >> 1], m & 1);
       }
     }
-  }
+    if constexpr (more) load_v();
+  };
+  int step = wave;
+  for (; step + AW < steps; step += AW) turn(step, std::true_type{});
+  if (step < steps) turn(step, std::false_type{});
+
   if (bad) sbad = 1;
+  float sum = sf.sum;
   sum += exl3::xor_lanes(sum, 16);
   sum += exl3::xor_lanes(sum, 32);
-  if (g == 0) sm[wave][col] = top, sl[wave][col] = sum;
+  if (g == 0) sm[wave][col] = sf.ref, sl[wave][col] = sum;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -546,8 +644,8 @@ __global__ __launch_bounds__(64 * AW) void attend_kernel(AttnArgs a) {
   if (sbad) l = __builtin_nanf("");
   const int p = w.r0 + row;
   if (p >= pairs) return;
-  if (direct) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (w.splits == 1) {
+    const float inv = 1.0f / l;
     uint16_t *dst = a.out + (int64_t)(w.sp.row + p / G) * a.os + (head * G + p % G) * D + VH * c;
     VV b;
 #pragma unroll
@@ -555,45 +653,337 @@ __global__ __launch_bounds__(64 * AW) void attend_kernel(AttnArgs a) {
       b[m >> 1] = l == 0.0f ? 0u : pack2<E>(o[m] * inv, o[m + 1] * inv);
     *reinterpret_cast<VV *>(dst) = b;
   } else if ((int)blockIdx.x < a.slots) {
-    float *dst = a.part + ((size_t)blockIdx.x * 16 + row) * D + VH * c;
+    float *dst = a.part + ((size_t)blockIdx.x * FEW + row) * D + VH * c;
 #pragma unroll
     for (int m = 0; m < VH; m += 4)
       *reinterpret_cast<f32x4 *>(dst + m) = f32x4{o[m], o[m + 1], o[m + 2], o[m + 3]};
-    float *ml = a.part + (size_t)a.slots * 16 * D + ((size_t)blockIdx.x * 16 + row) * 2;
+    float *ml = a.part + (size_t)a.slots * FEW * D + ((size_t)blockIdx.x * FEW + row) * 2;
     if (c == 0) ml[0] = all, ml[1] = l;
   }
 }
 
-// The items of a tile joined: 16 lanes a pair.
+// A barrier that orders LDS alone: loads in flight stay so.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// 128 pairs a workgroup, 32 a wave; tiles of 64 keys and values pass through
+// LDS, two of them so that one is loaded while the other is used.  The products
+// are those of attend_few with 32 x 32 tiles: a lane holds 32 keys' scores of
+// one pair and feeds its weights to the second product as they are.  A row of
+// LDS holds a key's 16-byte pieces at places q ^ swz(row) (the lanes that load
+// choose their pieces so): 8 rows' pieces of one number lie in 8 bank groups,
+// and so do the 4 rows by 32 bytes that a transposing read takes of the values.
+template <typename E, int D>
+__global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
+  constexpr int KK = D / 16, ND = D / 32;
+  constexpr int ROW = D * 2;          // bytes of a key
+  constexpr int ARR = 64 * ROW;       // of a tile's keys, or values
+  constexpr int LOADS = 16 * ROW / 1024;  // a wave loads 16 keys, 1 KiB an instruction
+  constexpr int LR = 1024 / ROW;          // rows an instruction loads
+  typedef typename E::V8 V8;
+  __shared__ __align__(1024) char lds[4 * ARR];  // [buffer][keys, values]
+  __shared__ int sbad;
+  __shared__ uint32_t sodd[AW];  // rows of a tile whose values are not all finite
+  const int head = blockIdx.x % a.pool.kv, item = blockIdx.x / a.pool.kv;
+  const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
+  const Work w = find_work<true>(a.st, a.sl, room, item);
+  if (w.s < 0) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const int G = a.sl.group, pairs = w.sp.n * G;
+  const int r0 = w.r0 + 32 * wave;
+  const int pair = min(r0 + col, pairs - 1), i = pair / G, hq = head * G + pair % G;
+  // the last key that the workgroup's, and the wave's, rows see
+  int last = w.sp.bad ? w.k0 : w.k1, mine = last;
+  if (a.mask == nullptr) {
+    last = min(last, w.sp.len + (min(w.r0 + MANY, pairs) - 1) / G + 1);
+    mine = min(last, w.sp.len + (min(r0 + 32, pairs) - 1) / G + 1);
+  }
+  if (r0 >= pairs) mine = w.k0;
+  if (threadIdx.x == 0) sbad = w.sp.bad;
+
+  const int steps = last > w.k0 ? (last - w.k0 + 63) / 64 : 0;
+  const int *trow = a.pool.table + (size_t)w.s * a.pool.max_pages;
+  const uint32_t base = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
+  // a lane's pieces of a load: row LR u + lane / (64 / LR), place lane % (64 / LR)
+  uint32_t voff[LOADS];
+#pragma unroll
+  for (int u = 0; u < LOADS; ++u) {
+    const int row = LR * u + lane / (ROW / 16), place = lane % (ROW / 16);
+    const int swz = D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+    voff[u] = row * ROW + (place ^ swz) * 16;
+  }
+  bool bad = false;
+  auto key_of = [&](int step) { return min(w.k0 + step * 64 + 16 * wave, (last - 1) & ~15); };
+  uint32_t id = 0;
+  auto fetch = [&](int step) { id = (uint32_t)trow[key_of(step) >> a.pool.lp]; };
+  auto load = [&](int step) {
+    uint32_t page = __builtin_amdgcn_readfirstlane(id);
+    if (page >= (uint32_t)a.pool.pages) bad = true, page = 0;
+    const size_t at = ((((size_t)page * a.pool.kv + head) << a.pool.lp) +
+                       (key_of(step) & ((1 << a.pool.lp) - 1))) * ROW;
+    const uint32_t to = base + (step & 1) * 2 * ARR + 16 * wave * ROW;
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) exl3::lds_dma16(a.pool.k + at, voff[u], to + u * 1024);
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) exl3::lds_dma16(a.pool.v + at, voff[u], to + ARR + u * 1024);
+  };
+  if (steps > 0) {
+    fetch(0);
+    load(0);
+    if (steps > 1) fetch(1);
+  }
+  u32x4 qf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.sp.row + i) * a.qs + hq * D + 16 * kk + 8 * h);
+    qf[kk] = qf[kk] ^ a.flip;
+  }
+  // byte addresses in a tile: piece 2 kk + h of row `col`; the values' 4 keys by
+  // 4 dims of a transposing read (16 lanes: keys 4 h + 0 .. 3, dims 16 u + 0 .. 15)
+  const int ti = lane & 15, tu = (lane >> 4) & 1;
+  const int krow = D == 128 ? (lane & 7) : ((lane >> 1) & 3);
+  const int vrow = D == 128 ? ((4 * h + (ti >> 2)) & 7) : ((2 * h + (ti >> 3)) & 3);
+  // (the piece's number stands in bits that nothing else touches: one exclusive
+  // or a read, on an address the compiler may not spread over registers)
+  uint32_t ka = col * ROW + 32 * krow + 16 * h;
+  uint32_t va = (4 * h + (ti >> 2)) * ROW + 32 * (tu ^ vrow) + 16 * ((ti & 3) >> 1) + 8 * (ti & 1);
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+  Soft sf{-INFINITY, 0.0f};
+
+  auto turn = [&](int step, auto TAIL) {
+    constexpr bool tail = decltype(TAIL)::value;
+    const int kb = w.k0 + step * 64;
+    const char *tk = lds + (step & 1) * 2 * ARR;
+    const char *tv = tk + ARR;
+    asm volatile("" : "+v"(ka), "+v"(va));
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        s[b] = E::mma(*reinterpret_cast<const V8 *>(tk + (ka ^ (32 * kk)) + b * 32 * ROW),
+                      __builtin_bit_cast(V8, qf[kk]), s[b]);
+    }
+    // element r of block b: key 32 b + 8 (r / 4) + 4 h + r % 4
+    uint64_t seen = ~0ull;
+    if constexpr (tail) {
+      seen = seen64(a, w.sp, i, kb, last);
+      const uint64_t my = seen >> (4 * h);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((uint32_t)(my >> (32 * b)) >> (8 * (r >> 2) + (r & 3)) & 1)) s[b][r] = -INFINITY;
+    }
+    float hi = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) hi = fmaxf(hi, fmaxf(s[0][r], s[1][r]));
+    hi = fmaxf(hi, exl3::xor_lanes(hi, 32));
+    float alpha;
+    if (outgrown(sf, hi * a.scale, alpha)) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+    }
+    const float by = E::LIFT - (sf.ref == -INFINITY ? 0.0f : sf.ref);
+    u32x4 pw[4];  // of 16 keys each
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const uint32_t x = pack2<E>(__builtin_amdgcn_exp2f(fmaf(s[b][r], a.scale, by)),
+                                    __builtin_amdgcn_exp2f(fmaf(s[b][r + 1], a.scale, by)));
+        pw[2 * b + (r >> 3)][(r & 7) >> 1] = x;
+        sf.sum = E::add2(x, sf.sum);
+      }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        typedef __attribute__((address_space(3))) s16x4 *lptr;
+        s16x4 v[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          v[c] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lptr)(tv + (va ^ (64 * d)) + (16 * b + 8 * c) * ROW));
+        u32x4 av = {__builtin_bit_cast(u32x2, v[0])[0], __builtin_bit_cast(u32x2, v[0])[1],
+                    __builtin_bit_cast(u32x2, v[1])[0], __builtin_bit_cast(u32x2, v[1])[1]};
+        acc[d] = E::mma(__builtin_bit_cast(V8, av), __builtin_bit_cast(V8, pw[b]), acc[d]);
+      }
+    if constexpr (tail) {
+      for (int x16 = 0; x16 < 4; ++x16)
+        for (int odd = __builtin_amdgcn_readfirstlane(sodd[x16]); odd != 0; odd &= odd - 1) {
+          const int x = 16 * x16 + __builtin_ctz(odd);
+          const uint16_t *row = value_row(a.pool, w.s, head, kb + x, D);
+          if (row == nullptr || !(seen >> x & 1)) continue;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const u32x2 v = *reinterpret_cast<const u32x2 *>(row + 32 * d + 8 * y + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[d][4 * y + e] += not_finite<E>(v[e >> 1], e & 1);
+            }
+        }
+    }
+  };
+  // The wave's 16 rows of a tile's values that reaches behind the context:
+  // zeros behind the last key (nobody's), and in place of what is not finite.
+  auto mend = [&](int step) {
+    const int kb = w.k0 + step * 64 + 16 * wave;
+    char *tv = lds + (step & 1) * 2 * ARR + ARR + 16 * wave * ROW;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int key = kb + LR * u + lane / (ROW / 16);
+      u32x4 *p = reinterpret_cast<u32x4 *>(tv + u * 1024 + lane * 16);
+      bool bad_value = false;
+      if (key >= last) {
+        *p = u32x4{0, 0, 0, 0};
+      } else if (key >= w.sp.len) {
+        u32x4 v = *p;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const uint32_t f = finite<E>(v[y]);
+          bad_value |= f != v[y];
+          v[y] = f;
+        }
+        if (bad_value) *p = v;
+      }
+      const uint64_t lanes = __ballot(bad_value);
+#pragma unroll
+      for (int j = 0; j < LR; ++j)
+        if (lanes >> (j * (ROW / 16)) & ((1ull << (ROW / 16)) - 1)) odd |= 1u << (LR * u + j);
+    }
+    if (lane == 0) sodd[wave] = odd;
+  };
+  for (int step = 0; step < steps; ++step) {
+    // this wave's loads of the tile are in LDS, and so are, behind the barrier,
+    // the others'; all have read the tile before, whose buffer is loaded next
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (step + 1 < steps) {
+      load(step + 1);
+      if (step + 2 < steps) fetch(step + 2);
+    }
+    const int kb = w.k0 + step * 64;
+    if (kb + 64 > min(w.sp.len, last)) {
+      mend(step);
+      lds_barrier();
+    }
+    if (kb >= mine) continue;
+    if (kb + 64 > min(w.sp.len, mine))
+      turn(step, std::true_type{});
+    else
+      turn(step, std::false_type{});
+  }
+  __syncthreads();
+  if (bad) sbad = 1;
+  __syncthreads();
+  float l = sf.sum;
+  l += exl3::xor_lanes(l, 32);
+  if (sbad) l = __builtin_nanf("");
+  if (r0 + col >= pairs) return;
+  // a lane's dims: 32 d + 8 x + 4 h + 0 .. 3
+  if (w.splits == 1) {
+    const float inv = 1.0f / l;
+    uint16_t *dst = a.out + (int64_t)(w.sp.row + i) * a.os + hq * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        u32x2 b = {pack2<E>(acc[d][4 * x] * inv, acc[d][4 * x + 1] * inv),
+                   pack2<E>(acc[d][4 * x + 2] * inv, acc[d][4 * x + 3] * inv)};
+        if (l == 0.0f) b = u32x2{0, 0};
+        *reinterpret_cast<u32x2 *>(dst + 32 * d + 8 * x) = b;
+      }
+  } else if ((int)blockIdx.x < a.slots) {
+    const size_t row = (size_t)blockIdx.x * MANY + 32 * wave + col;
+    float *dst = a.part + row * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        *reinterpret_cast<f32x4 *>(dst + 32 * d + 8 * x) =
+            f32x4{acc[d][4 * x], acc[d][4 * x + 1], acc[d][4 * x + 2], acc[d][4 * x + 3]};
+    float *ml = a.part + (size_t)a.slots * MANY * D + row * 2;
+    if (h == 0) ml[0] = sf.ref, ml[1] = l;
+  }
+}
+
+// The items of a tile joined: 16 lanes a pair, 16 pairs a workgroup.  The wave's
+// lanes hold the items' references and sums, so the loop over the items has no
+// load that another waits for.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   constexpr int VH = D / 16;
   typedef typename std::conditional<VH == 8, u32x4, u32x2>::type VV;
-  const int head = blockIdx.x % a.pool.kv, tile = blockIdx.x / a.pool.kv;
+  const int parts = a.sl.tile / 16;
+  const int head = blockIdx.x % a.pool.kv, tile = blockIdx.x / a.pool.kv / parts;
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
   const Work w = find_work<false>(a.st, a.sl, room, tile);
-  if (w.s < 0 || w.splits == 1) return;
-  const int G = a.sl.group, row = threadIdx.x >> 4, c = threadIdx.x & 15;
+  if (w.s < 0) return;
+  const int G = a.sl.group, c = threadIdx.x & 15;
+  const int row = 16 * ((blockIdx.x / a.pool.kv) % parts) + (threadIdx.x >> 4);
   const int p = w.r0 + row;
   if (p >= w.sp.n * G) return;
-  const float *ml = a.part + (size_t)a.slots * 16 * D;
-  float all = -INFINITY;
-  for (int x = 0; x < w.splits; ++x) {
-    const int64_t slot = (int64_t)(w.first + x) * a.pool.kv + head;
-    if (slot < a.slots) all = fmaxf(all, ml[(slot * 16 + row) * 2]);
-  }
-  const float ref = all == -INFINITY ? 0.0f : all;
-  float o[VH], l = 0.0f;
+  const float *ml = a.part + (size_t)a.slots * a.sl.tile * D;
+  const int n = min(w.splits, a.slots / a.pool.kv - w.first);
+  float top = -INFINITY, o[VH], l = 0.0f;
 #pragma unroll
   for (int m = 0; m < VH; ++m) o[m] = 0.0f;
-  for (int x = 0; x < w.splits; ++x) {
-    const int64_t slot = (int64_t)(w.first + x) * a.pool.kv + head;
-    if (slot >= a.slots) continue;
-    const float f = __builtin_amdgcn_exp2f(ml[(slot * 16 + row) * 2] - ref);
-    l += f * ml[(slot * 16 + row) * 2 + 1];
-    const float *src = a.part + (slot * 16 + row) * D + VH * c;
+  for (int x0 = 0; x0 < n; x0 += 16) {
+    // 16 items a round, one a lane
+    float ref = -INFINITY, sum = 0.0f;
+    if (x0 + c < n) {
+      const size_t slot = (size_t)(w.first + x0 + c) * a.pool.kv + head;
+      const f32x2 v = *reinterpret_cast<const f32x2 *>(ml + (slot * a.sl.tile + row) * 2);
+      ref = v[0], sum = v[1];
+    }
+    float hi = ref;
 #pragma unroll
-    for (int m = 0; m < VH; ++m) o[m] += f * src[m];
+    for (int m = 1; m < 16; m <<= 1) hi = fmaxf(hi, __shfl_xor(hi, m, 16));
+    const float now = fmaxf(top, hi), to = now == -INFINITY ? 0.0f : now;
+    const float alpha = __builtin_amdgcn_exp2f(top - to), f = __builtin_amdgcn_exp2f(ref - to);
+    top = now;
+    float part = f * sum;
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) part += __shfl_xor(part, m, 16);
+    l = l * alpha + part;
+#pragma unroll
+    for (int m = 0; m < VH; ++m) o[m] *= alpha;
+    const int e = min(16, n - x0);
+    const float *src = a.part + (((size_t)(w.first + x0) * a.pool.kv + head) * a.sl.tile + row) * D + VH * c;
+    const size_t stride = (size_t)a.pool.kv * a.sl.tile * D;
+    for (int x = 0; x < e; x += 4) {
+      f32x4 y[4][VH / 4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int m = 0; m < VH / 4; ++m)
+          y[u][m] = *reinterpret_cast<const f32x4 *>(src + min(x + u, e - 1) * stride + 4 * m);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float fx = __shfl(f, min(x + u, 15), 16);
+        if (x + u < e) {
+#pragma unroll
+          for (int m = 0; m < VH; ++m) o[m] += fx * y[u][m >> 2][m & 3];
+        }
+      }
+    }
   }
   const float inv = 1.0f / l;
   uint16_t *dst = a.out + (int64_t)(w.sp.row + p / G) * a.os + (head * G + p % G) * D + VH * c;
@@ -784,11 +1174,11 @@ int device_cus() {
   return cached[dev];
 }
 
-Split split_of(const exl3p_cache *c, int32_t heads) {
+Split split_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads) {
   Split sl;
   sl.group = heads / c->kv_heads;
-  sl.tile = 16;
-  sl.least = 32 * AW;
+  sl.tile = (int64_t)r->max_rows * sl.group > FEW ? MANY : FEW;
+  sl.least = sl.tile == FEW ? 32 * AW : 256;
   const int n = (2 * device_cus() + c->kv_heads - 1) / c->kv_heads;
   sl.target = n > 1 ? n : 1;
   return sl;
@@ -800,6 +1190,12 @@ int64_t most_tiles(const exl3p_rows *r, const Split &sl) {
   return (int64_t)r->rows * sl.group / sl.tile + r->seqs;
 }
 int64_t most_items(const exl3p_rows *r, const Split &sl) { return most_tiles(r, sl) + sl.target; }
+// Tiles that are split: each has a whole item at least, and those are no more
+// than the target.
+int64_t most_split(const exl3p_rows *r, const Split &sl) {
+  const int64_t tiles = most_tiles(r, sl);
+  return tiles < sl.target ? tiles : sl.target;
+}
 
 template <typename F>
 exl3_verdict by_type(const exl3p_cache *c, F &&f) {
@@ -879,7 +1275,7 @@ size_t exl3p_attend_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int
   if (check_cache(c).code != EXL3_OK || check_rows(c, r).code != EXL3_OK ||
       check_heads(c, heads).code != EXL3_OK)
     return 0;
-  const Split sl = split_of(c, heads);
+  const Split sl = split_of(c, r, heads);
   return (size_t)most_items(r, sl) * c->kv_heads * sl.tile * (c->dim + 2) * sizeof(float);
 }
 
@@ -897,7 +1293,7 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   const int64_t wq = (int64_t)heads * c->dim;
   EXL3P_TRY(check_matrix(q, q_stride, wq));
   EXL3P_TRY(check_matrix(out, out_stride, wq));
-  const Split sl = split_of(c, heads);
+  const Split sl = split_of(c, r, heads);
   if ((int64_t)r->max_rows * sl.group > INT32_MAX / 2 || most_items(r, sl) * c->kv_heads > INT32_MAX / 16)
     return refuse(EXL3_TOO_LARGE, "PagedAttend: too many rows and heads for one call");
   if (scratch == nullptr || !aligned(scratch, 16) ||
@@ -906,16 +1302,23 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   AttnArgs a;
   a.pool = pool_of(c, layer), a.st = step_of(r), a.sl = sl;
   a.q = static_cast<const uint16_t *>(q), a.qs = q_stride, a.mask = mask, a.words = words;
-  a.scale = scale * 1.4426950408889634f;
+  // at least f32's smallest, so that a hidden key's -inf times it stays -inf
+  a.scale = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f);
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.out = static_cast<uint16_t *>(out), a.os = out_stride;
   a.part = static_cast<float *>(scratch);
   a.slots = (int)(most_items(r, sl) * c->kv_heads);
   const hipStream_t st = static_cast<hipStream_t>(s);
   return by_type(c, [&](auto e, auto d) {
-    hipLaunchKernelGGL((attend_kernel<decltype(e), d>), dim3((unsigned)a.slots), dim3(64 * AW), 0, st,
-                       a);
+    if (sl.tile == FEW)
+      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d>), dim3((unsigned)a.slots), dim3(64 * AW),
+                         0, st, a);
+    else
+      hipLaunchKernelGGL((attend_many_kernel<decltype(e), d>), dim3((unsigned)a.slots),
+                         dim3(64 * AW), 0, st, a);
     hipLaunchKernelGGL((attend_join_kernel<decltype(e), d>),
-                       dim3((unsigned)(most_tiles(r, sl) * c->kv_heads)), dim3(256), 0, st, a);
+                       dim3((unsigned)(most_split(r, sl) * c->kv_heads * (sl.tile / 16))), dim3(256),
+                       0, st, a);
   });
 }
 

@@ -48,7 +48,8 @@ def attention(q, kpool, vpool, table, cu, lens, seen, page, group, scale, layer=
       (dim + 4) 2^-24 * (sum |q k| scale), a weight by the factor e^es: 2 es A
       (es below 1/4, so e^es - 1 <= 1.2 es: 2.4);
       f32 powers, sums and divisions: (keys + 64) 2^-23 A;
-      weights below f16's smallest at 2^-40 of the row's largest: keys 2^-40 max|v|;
+      weights below f16's smallest, 2^-24 where the row's reference weighs 2^11 (half of
+        a step of 2^-24 is 2^-36 of it): keys 2^-36 max|v|;
       the output's own rounding: u |out|, or half of the type's smallest number.
     """
     dt = q.dtype
@@ -78,7 +79,7 @@ def attention(q, kpool, vpool, table, cu, lens, seen, page, group, scale, layer=
                 es = float((k.abs() @ x.abs()).max()) * abs(scale) * (dim + 4) * 2.0 ** -24
                 out[cu[s] + i, h] = o
                 tol[cu[s] + i, h] = (A * (2 * u + 2.4 * es + (len(at) + 64) * 2.0 ** -23)
-                                     + len(at) * 2.0 ** -40 * v.abs().amax(0) + u * o.abs() + tiny)
+                                     + len(at) * 2.0 ** -36 * v.abs().amax(0) + u * o.abs() + tiny)
     return out, tol
 
 
