@@ -267,90 +267,80 @@ struct Work {
 
 struct Split {
   int group;   // query heads a kv head
-  int tile;    // pairs a tile
+  int tile;    // pairs a tile, a power of two: log2 of it
   int target;  // items wanted, of a kv head
   int least;   // keys an item has at least
+  float per;   // a little over 64-key units of an item by units of all
 };
 
-__device__ __forceinline__ int wave_sum_i(int v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+__device__ __forceinline__ int tiles_of(const Span &sp, const Split &sl) {
+  return (int)((uint32_t)(sp.n * sl.group + (1 << sl.tile) - 1) >> sl.tile);
+}
+
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ int scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // 1, 2, 4, 8 lanes down a row
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // a row's last lane to the next
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // the second row's to both after
   return v;
 }
 
-__device__ __forceinline__ int tiles_of(const Span &sp, const Split &sl) {
-  return (int)(((int64_t)sp.n * sl.group + sl.tile - 1) / sl.tile);
-}
-// 64-key units of a sequence
-__device__ __forceinline__ int units_of(const Span &sp) { return (sp.len + sp.n + 63) >> 6; }
-
-// Keys of an item, from all sequences: the units of all tiles over the target.
-__device__ __forceinline__ int keys_of_item(const Step &st, const Split &sl, int64_t room) {
-  const int lane = threadIdx.x & 63;
-  // units up to 2^24 a sequence times its tiles: in double, exact and far from
-  // overflow
-  double units = 0.0;
-  for (int s = lane; s < st.seqs; s += 64) {
-    const Span sp = span_of(st, s, room);
-    units += (double)tiles_of(sp, sl) * units_of(sp);
-  }
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) units += __shfl_xor(units, m, 64);
-  const double per = ceil(units / (double)sl.target);
-  return max(sl.least, (int)fmin(per, (double)(1 << 24)) * 64);
-}
-
 // Item (ITEM) number x among the sequences' ones, or tile number x among those
-// that are split.
+// that are split.  Every workgroup finds its own: no plan on the device or the
+// host depends on the lengths, so a captured call follows them.  Items have
+// `chunk` keys: the 64-key units that all tiles cover over the items wanted,
+// plus what 32-bit sums may be short of, so items are never more than the
+// target and a tile's last ones.  (Lane exchanges by DPP and scalars: 1 us of a
+// launch less than through LDS, with 64-bit divisions.)
 template <bool ITEM>
 __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64_t room, int x) {
   const int lane = threadIdx.x & 63;
-  const int chunk = keys_of_item(st, sl, room);
+  Span sp{0, 0, 0, false};
+  float units = 0.0f;
+  for (int s = lane; s < st.seqs; s += 64) {
+    sp = span_of(st, s, room);
+    units += (float)tiles_of(sp, sl) * (float)((uint32_t)(sp.len + sp.n + 63) >> 6);
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) units += exl3::xor_lanes(units, m);
+  const uint32_t chunk = __builtin_amdgcn_readfirstlane(
+      max(sl.least, (int)fminf(ceilf(units * sl.per), (float)(1 << 23)) * 64));
   Work w;
   w.s = -1;
   int items = 0, tiles = 0;  // of the sequences before
   for (int s0 = 0; s0 < st.seqs; s0 += 64) {
     const int s = s0 + lane;
-    Span sp{0, 0, 0, false};
     int nt = 0, ns = 0;
     if (s < st.seqs) {
-      sp = span_of(st, s, room);
+      if (st.seqs > 64) sp = span_of(st, s, room);
       nt = tiles_of(sp, sl);
-      ns = (int)(((int64_t)sp.len + sp.n + chunk - 1) / chunk);
+      ns = (int)(((uint32_t)(sp.len + sp.n) + chunk - 1) / chunk);
     }
-    // inclusive sums over the lanes
-    int it = nt * ns, ti = ns > 1 ? nt : 0;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int a = __shfl_up(it, m, 64), b = __shfl_up(ti, m, 64);
-      if (lane >= m) it += a, ti += b;
-    }
-    const int mine = ITEM ? items + it : tiles + ti;
-    const uint64_t past = __ballot(mine > x);
+    const int mi = nt * ns, mt = ns > 1 ? nt : 0;
+    const int it = scan(mi), ti = scan(mt);
+    const uint64_t past = __ballot((ITEM ? items + it : tiles + ti) > x);
     if (past != 0) {
       const int l = __builtin_ctzll(past);
-      const int s_ = s0 + l;
-      sp = span_of(st, s_, room);
-      nt = __shfl(nt, l, 64), ns = __shfl(ns, l, 64);
-      const int before = items + __shfl(it, l, 64) - nt * ns;
-      const int tbefore = tiles + __shfl(ti, l, 64) - nt;
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      const int n_t = of(nt), n_s = of(ns);
+      const int before = items + of(it - mi);
       // the last tile first: a prompt's last rows see the most keys
-      const int u = ITEM ? (x - before) / ns : nt - 1 - (x - tbefore);
-      const int tile = ITEM ? nt - 1 - u : x - tbefore;
-      const int j = ITEM ? (x - before) % ns : 0;
-      // the same in all lanes: said so, for addresses and branches in scalars
-      auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-      w.s = one(s_);
-      w.sp = Span{one(sp.row), one(sp.n), one(sp.len), (bool)one(sp.bad)};
-      w.r0 = one(tile * sl.tile);
-      w.first = one(before + (nt - 1 - tile) * ns);
-      w.splits = one(ns);
-      w.k0 = one(j * chunk);
-      w.k1 = one(min(j * chunk + chunk, sp.len + sp.n));
+      const int u = ITEM ? (x - before) / n_s : n_t - 1 - (x - (tiles + of(ti - mt)));
+      const int j = ITEM ? (x - before) - u * n_s : 0;
+      w.s = s0 + l;
+      w.sp = Span{of(sp.row), of(sp.n), of(sp.len), (bool)of(sp.bad)};
+      w.r0 = (n_t - 1 - u) << sl.tile;
+      w.first = before + u * n_s;
+      w.splits = n_s;
+      w.k0 = j * (int)chunk;
+      w.k1 = min(w.k0 + (int)chunk, w.sp.len + w.sp.n);
       return w;
     }
-    items += __shfl(it, 63, 64);
-    tiles += __shfl(ti, 63, 64);
+    items += __builtin_amdgcn_readlane(it, 63);
+    tiles += __builtin_amdgcn_readlane(ti, 63);
   }
   return w;
 }
@@ -399,6 +389,12 @@ struct Soft {
   float ref, sum;
 };
 
+// The larger, NaN if either is: without the canonicalizing instructions that
+// fmaxf takes for each operand.
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+
 // The running maximum `hi` (already times the scale) of each lane's pair joins
 // its reference; the factor for what has been summed so far is 1 (false) unless
 // some pair of the wave outgrew its reference by more than SLACK.
@@ -435,6 +431,11 @@ __device__ __forceinline__ const uint16_t *value_row(const Pool &p, int s, int h
   return reinterpret_cast<const uint16_t *>(p.v) + row * D;
 }
 
+// Keys below this every row of the work's tile sees: its first row's.
+__device__ __forceinline__ int clear_of(const AttnArgs &a, const Work &w, int last) {
+  return min(last, a.mask == nullptr ? w.sp.len + w.r0 / a.sl.group + 1 : w.sp.len);
+}
+
 // 16 pairs a workgroup; its waves take 32 keys in turn and join at the end.
 // Scores are S^T = K q^T (rows keys, columns pairs), so a lane holds 8 keys'
 // scores of one pair, in just the places where the second product, O^T = V^T
@@ -460,6 +461,7 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
   // no row of the tile sees past its last row's own key without masks
   int last = w.sp.bad ? w.k0 : w.k1;
   if (a.mask == nullptr) last = min(last, w.sp.len + (min(w.r0 + FEW, pairs) - 1) / G + 1);
+  const int clear = clear_of(a, w, last);
   if (threadIdx.x == 0) sbad = w.sp.bad;
   __syncthreads();
 
@@ -552,7 +554,7 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
       load_k();
       fetch(min(step + 2 * AW, steps - 1));
     }
-    const bool tail = kb + 32 > min(w.sp.len, last);
+    const bool tail = kb + 32 > clear;
     uint32_t seen = ~0u;
     uint32_t odd = 0;  // keys among the new rows with a value that is not finite
     if (tail) {
@@ -578,11 +580,11 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
           if (lanes >> (16 * z) & 0xFFFFu) odd |= 1u << (16 * (e >> 2) + 4 * z + (e & 3));
       }
     }
-    float hi = fmaxf(s2[0][0], s2[0][1]);
+    float hi = larger(s2[0][0], s2[0][1]);
 #pragma unroll
-    for (int e = 2; e < 8; ++e) hi = fmaxf(hi, s2[e >> 2][e & 3]);
-    hi = fmaxf(hi, exl3::xor_lanes(hi, 16));
-    hi = fmaxf(hi, exl3::xor_lanes(hi, 32));
+    for (int e = 2; e < 8; ++e) hi = larger(hi, s2[e >> 2][e & 3]);
+    hi = larger(hi, exl3::xor_lanes(hi, 16));
+    hi = larger(hi, exl3::xor_lanes(hi, 32));
     float alpha;
     if (outgrown(sf, hi * a.scale, alpha)) {
 #pragma unroll
@@ -673,9 +675,10 @@ __device__ __forceinline__ void lds_barrier() {
 // LDS, two of them so that one is loaded while the other is used.  The products
 // are those of attend_few with 32 x 32 tiles: a lane holds 32 keys' scores of
 // one pair and feeds its weights to the second product as they are.  A row of
-// LDS holds a key's 16-byte pieces at places q ^ swz(row) (the lanes that load
-// choose their pieces so): 8 rows' pieces of one number lie in 8 bank groups,
-// and so do the 4 rows by 32 bytes that a transposing read takes of the values.
+// LDS holds a key's 16-byte pieces at places q ^ f(row) (the lanes that load
+// choose their pieces so): pieces of one number of 16 rows of keys lie in 16
+// places of the 64 banks, and so do the 4 rows by 64 bytes of values that 32
+// lanes of a transposing read take.
 template <typename E, int D>
 __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   constexpr int KK = D / 16, ND = D / 32;
@@ -703,6 +706,7 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
     mine = min(last, w.sp.len + (min(r0 + 32, pairs) - 1) / G + 1);
   }
   if (r0 >= pairs) mine = w.k0;
+  const int clear = clear_of(a, w, last);
   if (threadIdx.x == 0) sbad = w.sp.bad;
 
   const int steps = last > w.k0 ? (last - w.k0 + 63) / 64 : 0;
@@ -710,12 +714,12 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   const uint32_t base = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
   // a lane's pieces of a load: row LR u + lane / (64 / LR), place lane % (64 / LR)
-  uint32_t voff[LOADS];
+  uint32_t voff[2][LOADS];  // keys, values
 #pragma unroll
   for (int u = 0; u < LOADS; ++u) {
     const int row = LR * u + lane / (ROW / 16), place = lane % (ROW / 16);
-    const int swz = D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
-    voff[u] = row * ROW + (place ^ swz) * 16;
+    voff[0][u] = row * ROW + (place ^ (D == 128 ? row & 15 : (row >> 1) & 7)) * 16;
+    voff[1][u] = row * ROW + (place ^ (D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1))) * 16;
   }
   bool bad = false;
   auto key_of = [&](int step) { return min(w.k0 + step * 64 + 16 * wave, (last - 1) & ~15); };
@@ -728,9 +732,10 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
                        (key_of(step) & ((1 << a.pool.lp) - 1))) * ROW;
     const uint32_t to = base + (step & 1) * 2 * ARR + 16 * wave * ROW;
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) exl3::lds_dma16(a.pool.k + at, voff[u], to + u * 1024);
+    for (int u = 0; u < LOADS; ++u) exl3::lds_dma16(a.pool.k + at, voff[0][u], to + u * 1024);
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) exl3::lds_dma16(a.pool.v + at, voff[u], to + ARR + u * 1024);
+    for (int u = 0; u < LOADS; ++u)
+      exl3::lds_dma16(a.pool.v + at, voff[1][u], to + ARR + u * 1024);
   };
   if (steps > 0) {
     fetch(0);
@@ -746,13 +751,10 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   // byte addresses in a tile: piece 2 kk + h of row `col`; the values' 4 keys by
   // 4 dims of a transposing read (16 lanes: keys 4 h + 0 .. 3, dims 16 u + 0 .. 15)
   const int ti = lane & 15, tu = (lane >> 4) & 1;
-  const int krow = D == 128 ? (lane & 7) : ((lane >> 1) & 3);
-  const int vrow = D == 128 ? ((4 * h + (ti >> 2)) & 7) : ((2 * h + (ti >> 3)) & 3);
-  // (the piece's number stands in bits that nothing else touches: one exclusive
-  // or a read, on an address the compiler may not spread over registers)
-  uint32_t ka = col * ROW + 32 * krow + 16 * h;
-  uint32_t va = (4 * h + (ti >> 2)) * ROW + 32 * (tu ^ vrow) + 16 * ((ti & 3) >> 1) + 8 * (ti & 1);
-
+  // (a product's piece number only changes bits that an exclusive or reaches; the
+  // compiler may not spread the addresses over registers)
+  uint32_t ka = col * ROW + 16 * (h ^ (D == 128 ? col & 15 : (col >> 1) & 7));
+  uint32_t va = (4 * h + (ti >> 2)) * ROW + 64 * (D == 128 ? ti >> 2 : ti >> 3) + 32 * tu + 8 * (ti & 3);
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -787,10 +789,10 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
         for (int r = 0; r < 16; ++r)
           if (!((uint32_t)(my >> (32 * b)) >> (8 * (r >> 2) + (r & 3)) & 1)) s[b][r] = -INFINITY;
     }
-    float hi = fmaxf(s[0][0], s[1][0]);
+    float hi = larger(s[0][0], s[1][0]);
 #pragma unroll
-    for (int r = 1; r < 16; ++r) hi = fmaxf(hi, fmaxf(s[0][r], s[1][r]));
-    hi = fmaxf(hi, exl3::xor_lanes(hi, 32));
+    for (int r = 1; r < 16; ++r) hi = larger(larger(hi, s[0][r]), s[1][r]);
+    hi = larger(hi, exl3::xor_lanes(hi, 32));
     float alpha;
     if (outgrown(sf, hi * a.scale, alpha)) {
 #pragma unroll
@@ -871,24 +873,26 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
     }
     if (lane == 0) sodd[wave] = odd;
   };
-  for (int step = 0; step < steps; ++step) {
-    // this wave's loads of the tile are in LDS, and so are, behind the barrier,
-    // the others'; all have read the tile before, whose buffer is loaded next
+  // this wave's loads of the tile are in LDS, and so are, behind the barrier,
+  // the others'; all have read the tile before, whose buffer is loaded next
+  auto begin = [&](int step) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (step + 1 < steps) {
       load(step + 1);
       if (step + 2 < steps) fetch(step + 2);
     }
-    const int kb = w.k0 + step * 64;
-    if (kb + 64 > min(w.sp.len, last)) {
-      mend(step);
-      lds_barrier();
-    }
-    if (kb >= mine) continue;
-    if (kb + 64 > min(w.sp.len, mine))
-      turn(step, std::true_type{});
-    else
-      turn(step, std::false_type{});
+  };
+  const int whole = max(0, clear - w.k0) / 64;  // tiles that every row sees whole
+  int step = 0;
+  for (; step < whole; ++step) {
+    begin(step);
+    if (r0 < pairs) turn(step, std::false_type{});
+  }
+  for (; step < steps; ++step) {
+    begin(step);
+    mend(step);
+    lds_barrier();
+    if (w.k0 + step * 64 < mine) turn(step, std::true_type{});
   }
   __syncthreads();
   if (bad) sbad = 1;
@@ -931,7 +935,7 @@ template <typename E, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   constexpr int VH = D / 16;
   typedef typename std::conditional<VH == 8, u32x4, u32x2>::type VV;
-  const int parts = a.sl.tile / 16;
+  const int rows = 1 << a.sl.tile, parts = rows / 16;
   const int head = blockIdx.x % a.pool.kv, tile = blockIdx.x / a.pool.kv / parts;
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
   const Work w = find_work<false>(a.st, a.sl, room, tile);
@@ -940,7 +944,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   const int row = 16 * ((blockIdx.x / a.pool.kv) % parts) + (threadIdx.x >> 4);
   const int p = w.r0 + row;
   if (p >= w.sp.n * G) return;
-  const float *ml = a.part + (size_t)a.slots * a.sl.tile * D;
+  const float *ml = a.part + (size_t)a.slots * rows * D;
   const int n = min(w.splits, a.slots / a.pool.kv - w.first);
   float top = -INFINITY, o[VH], l = 0.0f;
 #pragma unroll
@@ -950,7 +954,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
     float ref = -INFINITY, sum = 0.0f;
     if (x0 + c < n) {
       const size_t slot = (size_t)(w.first + x0 + c) * a.pool.kv + head;
-      const f32x2 v = *reinterpret_cast<const f32x2 *>(ml + (slot * a.sl.tile + row) * 2);
+      const f32x2 v = *reinterpret_cast<const f32x2 *>(ml + (slot * rows + row) * 2);
       ref = v[0], sum = v[1];
     }
     float hi = ref;
@@ -966,8 +970,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int m = 0; m < VH; ++m) o[m] *= alpha;
     const int e = min(16, n - x0);
-    const float *src = a.part + (((size_t)(w.first + x0) * a.pool.kv + head) * a.sl.tile + row) * D + VH * c;
-    const size_t stride = (size_t)a.pool.kv * a.sl.tile * D;
+    const float *src = a.part + (((size_t)(w.first + x0) * a.pool.kv + head) * rows + row) * D + VH * c;
+    const size_t stride = (size_t)a.pool.kv * rows * D;
     for (int x = 0; x < e; x += 4) {
       f32x4 y[4][VH / 4];
 #pragma unroll
@@ -1121,6 +1125,7 @@ exl3_verdict check_rows(const exl3p_cache *c, const exl3p_rows *r) {
     return refuse(EXL3_FAILED, "PagedRows: no rows, or another version's");
   if (r->seqs < 0 || r->rows < 0 || r->max_rows < 0 || r->max_rows > r->rows)
     return refuse(EXL3_UNSUPPORTED, "PagedRows: sizes below 0, or more rows a sequence than rows");
+  if (r->seqs > 65535) return refuse(EXL3_TOO_LARGE, "PagedRows: over 65535 sequences");
   if (r->seqs > c->seqs) return refuse(EXL3_UNSUPPORTED, "PagedRows: more sequences than the cache's");
   if (r->cu == nullptr || r->len == nullptr)
     return refuse(EXL3_FAILED, "PagedRows: a missing array");
@@ -1177,17 +1182,20 @@ int device_cus() {
 Split split_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads) {
   Split sl;
   sl.group = heads / c->kv_heads;
-  sl.tile = (int64_t)r->max_rows * sl.group > FEW ? MANY : FEW;
-  sl.least = sl.tile == FEW ? 32 * AW : 256;
+  const bool few = (int64_t)r->max_rows * sl.group <= FEW;
+  sl.tile = log2_of(few ? FEW : MANY);
+  sl.least = few ? 32 * AW : 256;
   const int n = (2 * device_cus() + c->kv_heads - 1) / c->kv_heads;
   sl.target = n > 1 ? n : 1;
+  // 65535 sequences are 1024 sums a lane, each off by 2^-24 at most
+  sl.per = (1.0f + 0x1p-12f) / (float)sl.target;
   return sl;
 }
 
 // Tiles of a kv head that the rows can make, and items: a sequence's last tile
 // and a tile's last item may be short.
 int64_t most_tiles(const exl3p_rows *r, const Split &sl) {
-  return (int64_t)r->rows * sl.group / sl.tile + r->seqs;
+  return ((int64_t)r->rows * sl.group >> sl.tile) + r->seqs;
 }
 int64_t most_items(const exl3p_rows *r, const Split &sl) { return most_tiles(r, sl) + sl.target; }
 // Tiles that are split: each has a whole item at least, and those are no more
@@ -1276,7 +1284,7 @@ size_t exl3p_attend_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int
       check_heads(c, heads).code != EXL3_OK)
     return 0;
   const Split sl = split_of(c, r, heads);
-  return (size_t)most_items(r, sl) * c->kv_heads * sl.tile * (c->dim + 2) * sizeof(float);
+  return (size_t)most_items(r, sl) * c->kv_heads * ((size_t)1 << sl.tile) * (c->dim + 2) * sizeof(float);
 }
 
 exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
@@ -1310,14 +1318,14 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   a.slots = (int)(most_items(r, sl) * c->kv_heads);
   const hipStream_t st = static_cast<hipStream_t>(s);
   return by_type(c, [&](auto e, auto d) {
-    if (sl.tile == FEW)
+    if (sl.tile == log2_of(FEW))
       hipLaunchKernelGGL((attend_few_kernel<decltype(e), d>), dim3((unsigned)a.slots), dim3(64 * AW),
                          0, st, a);
     else
       hipLaunchKernelGGL((attend_many_kernel<decltype(e), d>), dim3((unsigned)a.slots),
                          dim3(64 * AW), 0, st, a);
     hipLaunchKernelGGL((attend_join_kernel<decltype(e), d>),
-                       dim3((unsigned)(most_split(r, sl) * c->kv_heads * (sl.tile / 16))), dim3(256),
+                       dim3((unsigned)(most_split(r, sl) * c->kv_heads << (sl.tile - 4))), dim3(256),
                        0, st, a);
   });
 }

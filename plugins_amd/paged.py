@@ -30,6 +30,15 @@ from . import exl3 as X
 
 TREE_MAX = 1024  # EXL3P_TREE_MAX
 
+_torch = None  # the module, from the first cache or rows on
+
+
+def _t():
+    global _torch
+    if _torch is None:
+        _torch = X._torch()
+    return _torch
+
 
 class CacheDesc(Structure):
     """exl3p_cache"""
@@ -143,7 +152,7 @@ class PagedCache:
 
     def __init__(self, layers: int, pages: int, kv_heads: int, seqs: int, max_pages: int,
                  page: int = 64, head_dim: int = 128, dtype=None, device="cuda"):
-        torch = X._torch()
+        torch = _t()
         book = Book(pages, page, seqs, max_pages)
         shape = (layers, pages, kv_heads, page, head_dim)
         dtype = torch.float16 if dtype is None else dtype
@@ -162,7 +171,9 @@ class PagedCache:
         return c
 
     def _over(self, k, v, table) -> None:
-        torch = X._torch()
+        torch = _t()
+        if k.device.type != "cuda":
+            raise ValueError("a cache lies on a GPU")
         if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype or table.dim() != 2:
             raise ValueError("k and v are alike, [layers][pages][kv heads][page][dim]; table has 2 dims")
         if table.dtype != torch.int32:
@@ -189,7 +200,7 @@ class PagedCache:
 
     def _sync(self, seq: int | None = None, stream=None) -> None:
         """The book's table, or a sequence's row of it, to the device."""
-        torch = X._torch()
+        torch = _t()
         t = torch.from_numpy(self._book().table())
         with _on(self, stream):
             if seq is None:
@@ -231,7 +242,7 @@ class Rows:
     `max_rows` of a sequence."""
 
     def __init__(self, cu, len, rows: int, max_rows: int):
-        torch = X._torch()
+        torch = _t()
         if cu.dtype != torch.int32 or len.dtype != torch.int32:
             raise TypeError("cu and len are int32")
         if cu.dim() != 1 or len.dim() != 1 or cu.numel() != len.numel() + 1 or cu.device != len.device:
@@ -240,7 +251,9 @@ class Rows:
             raise ValueError("cu and len are dense")
         self.cu, self.len = cu, len
         self.rows, self.max_rows, self.seqs = rows, max_rows, len.numel()
-        self.device = cu.device
+        if cu.device.type != "cuda":
+            raise ValueError("a step's rows lie on a GPU")
+        self.device, self.index = cu.device, cu.device.index
         self.desc = RowsDesc(ctypes.sizeof(RowsDesc), self.seqs, rows, max_rows, cu.data_ptr(),
                              len.data_ptr())
         self._ref = ctypes.addressof(self.desc)
@@ -248,7 +261,7 @@ class Rows:
     @classmethod
     def of(cls, counts, lens, device="cuda") -> "Rows":
         """Rows from host lists: counts[s] rows behind lens[s] cached keys."""
-        torch = X._torch()
+        torch = _t()
         if len(counts) != len(lens):
             raise ValueError("a count and a length for each sequence")
         cu = [0]
@@ -263,9 +276,9 @@ class _on:
     """The cache's device, and the stream given, as torch's current ones."""
 
     def __init__(self, cache, stream):
-        torch = X._torch()
+        torch = _t()
         self.held = []
-        if cache.index is not None and cache.index != torch.cuda.current_device():
+        if cache.index != torch.cuda.current_device():
             self.held.append(torch.cuda.device(cache.index))
         if stream is not None:
             self.held.append(torch.cuda.stream(stream))
@@ -281,50 +294,50 @@ class _on:
 
 def _matrix(t, what: str, cache, rows: int, width: int):
     """Base and row stride of a step's tensor [rows, ...] of `width` a row."""
-    if t.dtype != cache.dtype:
+    if t.dtype is not cache.dtype:
         raise TypeError(f"{what} is {t.dtype}, the cache {cache.dtype}")
-    if t.device != cache.device:
+    if t.get_device() != cache.index:
         raise ValueError(f"{what} is on {t.device}, the cache on {cache.device}")
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
-        ok = shape[0] == rows and shape[1] == width and (stride[1] == 1 or width <= 1)
+        ok = shape[1] == width and stride[1] == 1
     else:
-        ok = (len(shape) == 3 and shape[0] == rows and shape[1] * shape[2] == width and
+        ok = (len(shape) == 3 and shape[1] * shape[2] == width and
               shape[2] == cache.head_dim and stride[2] == 1 and
               (stride[1] == shape[2] or shape[1] == 1))
-    if not ok:
+    if not ok or shape[0] != rows:
         raise ValueError(f"{what}: [{rows}, {width}] (or heads apart), elements side by side, not "
                          f"{tuple(shape)} with strides {tuple(stride)}")
-    return t.data_ptr(), stride[0] if rows > 1 else max(width, 8)
+    return t.data_ptr(), stride[0] if rows > 1 else width
 
 
 def _ints(t, what: str, cache, n: int):
-    torch = X._torch()
-    if t.dtype != torch.int32:
+    if t.dtype is not _torch.int32:
         raise TypeError(f"{what} is int32")
-    if t.device != cache.device or not t.is_contiguous() or t.numel() != n:
+    if t.get_device() != cache.index or not t.is_contiguous() or t.numel() != n:
         raise ValueError(f"{what}: {n} dense elements on {cache.device}")
     return t.data_ptr()
 
 
 def _stream(cache, stream):
-    torch = X._torch()
-    return (stream if stream is not None else torch.cuda.current_stream(cache.device)).cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # torch.cuda.current_stream(device).cuda_stream without the Stream object (2 us)
+    return _torch._C._cuda_getCurrentRawStream(cache.index)
 
 
 def _call(cache, fn, what, *args):
-    torch = X._torch()
-    if cache.index is None or cache.index == torch.cuda.current_device():
+    if cache.index == _torch.cuda.current_device():
         v = fn(*args)
     else:
-        with torch.cuda.device(cache.index):
+        with _torch.cuda.device(cache.index):
             v = fn(*args)
     if v.code != X.OK:
         raise X.Exl3Error(v, what)
 
 
 def _of(cache, rows) -> None:
-    if rows.device != cache.device:
+    if rows.index != cache.index:
         raise ValueError(f"the rows are on {rows.device}, the cache on {cache.device}")
 
 
@@ -332,13 +345,17 @@ def _mask(mask, cache, rows):
     """Address and words of ancestor masks int64 [rows, words]."""
     if mask is None:
         return None, 0
-    torch = X._torch()
-    if mask.dtype not in (torch.int64, getattr(torch, "uint64", torch.int64)):
+    if mask.dtype is not _torch.int64:
         raise TypeError("a mask is int64")
-    if mask.dim() != 2 or mask.shape[0] != rows.rows or not mask.is_contiguous() or \
-            mask.device != cache.device:
+    shape = mask.shape
+    if len(shape) != 2 or shape[0] != rows.rows or not mask.is_contiguous() or \
+            mask.get_device() != cache.index:
         raise ValueError(f"a mask is dense [{rows.rows}, words] on {cache.device}")
-    return mask.data_ptr(), mask.shape[1]
+    return mask.data_ptr(), shape[1]
+
+
+def _heads(q, cache) -> int:
+    return q.shape[1] if q.dim() == 3 else q.shape[1] // cache.head_dim
 
 
 # ------------------------------------------------------------------ operators
@@ -356,7 +373,7 @@ def tree_plan(cache, rows, parent, pos, slot, mask=None, stream=None) -> None:
 def plan(cache, rows, parent=None, stream=None):
     """tree_plan into new tensors: pos, slot, mask (None without a parent: rows
     in a line see those before them)."""
-    torch = X._torch()
+    torch = _torch
     with _on(cache, stream):
         pos = torch.empty(rows.rows, dtype=torch.int32, device=cache.device)
         slot = torch.empty_like(pos)
@@ -371,14 +388,14 @@ def qkv_append(cache, layer: int, q, k, v, q_norm, k_norm, pos, slot, q_out, eps
     """exl3p_qkv_append: q [rows, heads * dim] normalized and rotated to q_out,
     k and v into the layer's pages.  q_norm, k_norm [dim], or None: no norm."""
     n, dim = q.shape[0], cache.head_dim
-    heads = math.prod(q.shape[1:]) // dim
+    heads = _heads(q, cache)
     qp, qs = _matrix(q, "q", cache, n, heads * dim)
     kp, ks = _matrix(k, "k", cache, n, cache.kv_heads * dim)
     vp, vs = _matrix(v, "v", cache, n, cache.kv_heads * dim)
     op, os_ = _matrix(q_out, "q_out", cache, n, heads * dim)
     norms = []
     for w in (q_norm, k_norm):
-        if w is not None and (w.dtype != cache.dtype or w.device != cache.device or
+        if w is not None and (w.dtype is not cache.dtype or w.get_device() != cache.index or
                               w.shape != (dim,) or not w.is_contiguous()):
             raise ValueError(f"a norm's weights are [{dim}], of the cache's type and device")
         norms.append(None if w is None else w.data_ptr())
@@ -393,11 +410,11 @@ def attend(cache, layer: int, rows, q, out=None, mask=None, scale: float | None 
     cache's keys and, by their masks, the rows'.  scratch: a byte tensor of at
     least attend_scratch_bytes() that no overlapping call uses (None: taken from
     torch's allocator for this call)."""
-    torch = X._torch()
+    torch = _torch
     _of(cache, rows)
     L = paged_lib()
     n, dim = rows.rows, cache.head_dim
-    heads = math.prod(q.shape[1:]) // dim
+    heads = _heads(q, cache)
     if out is None:
         with _on(cache, stream):
             out = torch.empty(n, heads * dim, dtype=cache.dtype, device=cache.device)
@@ -411,7 +428,7 @@ def attend(cache, layer: int, rows, q, out=None, mask=None, scale: float | None 
         else:
             with _on(cache, stream):
                 scratch = torch.empty(need, dtype=torch.uint8, device=cache.device)
-    elif scratch.device != cache.device or not scratch.is_contiguous():
+    elif scratch.get_device() != cache.index or not scratch.is_contiguous():
         raise ValueError(f"scratch is dense, on {cache.device}")
     _call(cache, L.exl3p_attend, "attend", cache._ref, layer, rows._ref, heads, qp, qs, mp, words,
           1.0 / math.sqrt(dim) if scale is None else scale, op, os_, scratch.data_ptr(),
