@@ -380,8 +380,8 @@ __device__ __forceinline__ uint64_t seen64(const AttnArgs &a, const Span &sp, in
 }
 
 constexpr int AW = 4;      // waves of an attention workgroup
-constexpr int FEW = 16;    // pairs of a tile: one of attend_few's,
-constexpr int MANY = 128;  // one of attend_many's
+constexpr int FEW = 32;    // the most pairs of a tile of attend_few (16 or 32),
+constexpr int MANY = 128;  // a tile of attend_many's
 
 // A wave's softmax over the keys it has seen: the reference of each pair's
 // weights and the sum of them.
@@ -436,19 +436,20 @@ __device__ __forceinline__ int clear_of(const AttnArgs &a, const Work &w, int la
   return min(last, a.mask == nullptr ? w.sp.len + w.r0 / a.sl.group + 1 : w.sp.len);
 }
 
-// 16 pairs a workgroup; its waves take 32 keys in turn and join at the end.
+// 16 NT pairs a workgroup; its waves take 32 keys in turn and join at the end.
 // Scores are S^T = K q^T (rows keys, columns pairs), so a lane holds 8 keys'
 // scores of one pair, in just the places where the second product, O^T = V^T
 // P^T, wants its right operand if V's keys are taken in the same order: the
 // weights never leave their lane.
-template <typename E, int D>
+template <typename E, int D, int NT>
 __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
   constexpr int KK = D / 32;  // products of 32 dims a score
   constexpr int VH = D / 16;  // dims a lane loads of a value
+  constexpr int ROWS = 16 * NT;
   typedef typename std::conditional<VH == 8, u32x4, u32x2>::type VV;
   typedef typename E::V8 V8;
-  __shared__ float so[AW][FEW][D + 4];
-  __shared__ float sm[AW][FEW], sl[AW][FEW];
+  __shared__ float so[AW][16][D + 4];
+  __shared__ float sm[AW][16], sl[AW][16];
   __shared__ int sbad;
   const int head = blockIdx.x % a.pool.kv, item = blockIdx.x / a.pool.kv;
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
@@ -457,13 +458,11 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int G = a.sl.group, pairs = w.sp.n * G;
-  const int pair = min(w.r0 + col, pairs - 1), i = pair / G, hq = head * G + pair % G;
   // no row of the tile sees past its last row's own key without masks
   int last = w.sp.bad ? w.k0 : w.k1;
-  if (a.mask == nullptr) last = min(last, w.sp.len + (min(w.r0 + FEW, pairs) - 1) / G + 1);
+  if (a.mask == nullptr) last = min(last, w.sp.len + (min(w.r0 + ROWS, pairs) - 1) / G + 1);
   const int clear = clear_of(a, w, last);
   if (threadIdx.x == 0) sbad = w.sp.bad;
-  __syncthreads();
 
   const int steps = last > w.k0 ? (last - w.k0 + 31) / 32 : 0;
   const int *trow = a.pool.table + (size_t)w.s * a.pool.max_pages;
@@ -508,61 +507,65 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
         vf[4 * t + r] = *reinterpret_cast<const VV *>(pv + at[t] + r * D);
   };
 
-  u32x4 qf[KK];
-  if (wave < steps) {
-    fetch(wave);
+  u32x4 qf[NT][KK];
+  int row_of[NT];  // a lane's pairs' rows of the sequence
+  if (wave < steps) fetch(wave);
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.sp.row + i) * a.qs + hq * D + 32 * kk + 8 * g);
-      qf[kk] = qf[kk] ^ a.flip;
-    }
+  for (int n = 0; n < NT; ++n) {
+    const int pair = min(w.r0 + 16 * n + col, pairs - 1);
+    row_of[n] = pair / G;
+    const uint16_t *src = a.q + (w.sp.row + row_of[n]) * a.qs +
+                          (head * G + pair - row_of[n] * G) * D + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      qf[n][kk] = *reinterpret_cast<const u32x4 *>(src + 32 * kk) ^ a.flip;
+  }
+  if (wave < steps) {
     locate(wave);
     load_k();
     load_v();
     if (wave + AW < steps) fetch(wave + AW);
   }
-  f32x4 acc[VH];
+  f32x4 acc[NT][VH];
+  Soft sf[NT];
 #pragma unroll
-  for (int m = 0; m < VH; ++m) acc[m] = f32x4{0, 0, 0, 0};
-  Soft sf{-INFINITY, 0.0f};
+  for (int n = 0; n < NT; ++n) {
+    sf[n] = Soft{-INFINITY, 0.0f};
+#pragma unroll
+    for (int m = 0; m < VH; ++m) acc[n][m] = f32x4{0, 0, 0, 0};
+  }
 
-  auto products = [&](const VV(&vv)[8], const uint32_t(&pp)[4], f32x4(&o)[VH]) {
-    const V8 pb = __builtin_bit_cast(V8, u32x4{pp[0], pp[1], pp[2], pp[3]});
-#pragma unroll
-    for (int m = 0; m < VH; ++m) {
-      const uint32_t sel = m & 1 ? 0x07060302u : 0x05040100u;
-      u32x4 av;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        av[x] = __builtin_amdgcn_perm(vv[2 * x + 1][m >> 1], vv[2 * x][m >> 1], sel);
-      o[m] = E::mma(__builtin_bit_cast(V8, av), pb, o[m]);
-    }
-  };
   auto turn = [&](int step, auto MORE) {
     constexpr bool more = decltype(MORE)::value;
     const int kb = w.k0 + step * 32;
-    f32x4 s2[2];
+    f32x4 s2[NT][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s2[t] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        s2[t] = E::mma(__builtin_bit_cast(V8, kf[t][kk]), __builtin_bit_cast(V8, qf[kk]), s2[t]);
-    }
+      for (int n = 0; n < NT; ++n) {
+        s2[n][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          s2[n][t] = E::mma(__builtin_bit_cast(V8, kf[t][kk]), __builtin_bit_cast(V8, qf[n][kk]),
+                            s2[n][t]);
+      }
     if constexpr (more) {
       locate(step + AW);
       load_k();
       fetch(min(step + 2 * AW, steps - 1));
     }
     const bool tail = kb + 32 > clear;
-    uint32_t seen = ~0u;
+    uint32_t seen[NT];
     uint32_t odd = 0;  // keys among the new rows with a value that is not finite
     if (tail) {
-      seen = (uint32_t)seen64(a, w.sp, i, kb, last);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) seen[n] = (uint32_t)seen64(a, w.sp, row_of[n], kb, last);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int x = 16 * (e >> 2) + 4 * g + (e & 3);
-        if (!(seen >> x & 1)) s2[e >> 2][e & 3] = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          if (!(seen[n] >> x & 1)) s2[n][e >> 2][e & 3] = -INFINITY;
         // values behind the last key are nobody's
         if (kb + x >= last) vf[e] = VV{};
         bool bad_value = false;
@@ -580,35 +583,54 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
           if (lanes >> (16 * z) & 0xFFFFu) odd |= 1u << (16 * (e >> 2) + 4 * z + (e & 3));
       }
     }
-    float hi = larger(s2[0][0], s2[0][1]);
+    u32x4 pw[NT];
 #pragma unroll
-    for (int e = 2; e < 8; ++e) hi = larger(hi, s2[e >> 2][e & 3]);
-    hi = larger(hi, exl3::xor_lanes(hi, 16));
-    hi = larger(hi, exl3::xor_lanes(hi, 32));
-    float alpha;
-    if (outgrown(sf, hi * a.scale, alpha)) {
+    for (int n = 0; n < NT; ++n) {
+      float hi = larger(s2[n][0][0], s2[n][0][1]);
 #pragma unroll
-      for (int m = 0; m < VH; ++m) acc[m] = acc[m] * alpha;
+      for (int e = 2; e < 8; ++e) hi = larger(hi, s2[n][e >> 2][e & 3]);
+      hi = larger(hi, exl3::xor_lanes(hi, 16));
+      hi = larger(hi, exl3::xor_lanes(hi, 32));
+      float alpha;
+      if (outgrown(sf[n], hi * a.scale, alpha)) {
+#pragma unroll
+        for (int m = 0; m < VH; ++m) acc[n][m] = acc[n][m] * alpha;
+      }
+      const float by = E::LIFT - (sf[n].ref == -INFINITY ? 0.0f : sf[n].ref);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float(&x)[2] = {fmaf(s2[n][e >> 2][e & 3], a.scale, by),
+                              fmaf(s2[n][e >> 2][(e & 3) + 1], a.scale, by)};
+        pw[n][e >> 1] = pack2<E>(__builtin_amdgcn_exp2f(x[0]), __builtin_amdgcn_exp2f(x[1]));
+        // the sum of the rounded weights: they add up to one after the division
+        sf[n].sum = E::add2(pw[n][e >> 1], sf[n].sum);
+      }
     }
-    const float by = E::LIFT - (sf.ref == -INFINITY ? 0.0f : sf.ref);
-    uint32_t pw[4];
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      pw[e >> 1] = pack2<E>(__builtin_amdgcn_exp2f(fmaf(s2[e >> 2][e & 3], a.scale, by)),
-                            __builtin_amdgcn_exp2f(fmaf(s2[e >> 2][(e & 3) + 1], a.scale, by)));
-      // the sum of the rounded weights: they add up to one after the division
-      sf.sum = E::add2(pw[e >> 1], sf.sum);
+    for (int m = 0; m < VH; ++m) {
+      const uint32_t sel = m & 1 ? 0x07060302u : 0x05040100u;
+      u32x4 av;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        av[x] = __builtin_amdgcn_perm(vf[2 * x + 1][m >> 1], vf[2 * x][m >> 1], sel);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        acc[n][m] = E::mma(__builtin_bit_cast(V8, av), __builtin_bit_cast(V8, pw[n]), acc[n][m]);
     }
-    products(vf, pw, acc);
     for (; odd != 0; odd &= odd - 1) {
       const int x = __builtin_ctz(odd);
       const uint16_t *row = value_row(a.pool, w.s, head, kb + x, D);
-      if (row == nullptr || !(seen >> x & 1)) continue;
+      if (row == nullptr) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const VV b = *reinterpret_cast<const VV *>(row + VH * (4 * g + r));
 #pragma unroll
-        for (int m = 0; m < VH; ++m) acc[m][r] += not_finite<E>(b[m >> 1], m & 1);
+        for (int m = 0; m < VH; ++m) {
+          const float v = not_finite<E>(b[m >> 1], m & 1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            if (seen[n] >> x & 1) acc[n][m][r] += v;
+        }
       }
     }
     if constexpr (more) load_v();
@@ -617,50 +639,56 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
   for (; step + AW < steps; step += AW) turn(step, std::true_type{});
   if (step < steps) turn(step, std::false_type{});
 
-  if (bad) sbad = 1;
-  float sum = sf.sum;
-  sum += exl3::xor_lanes(sum, 16);
-  sum += exl3::xor_lanes(sum, 32);
-  if (g == 0) sm[wave][col] = sf.ref, sl[wave][col] = sum;
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int m = 0; m < VH; ++m) so[wave][col][VH * (4 * g + r) + m] = acc[m][r];
   __syncthreads();
-  // 16 lanes a pair, D / 16 dims each
+  if (bad) sbad = 1;
+  // the waves' sums join, 16 pairs at a time: 16 lanes a pair, D / 16 dims each
   const int row = threadIdx.x >> 4, c = threadIdx.x & 15;
-  float all = -INFINITY;
 #pragma unroll
-  for (int x = 0; x < AW; ++x) all = fmaxf(all, sm[x][row]);
-  const float ref = all == -INFINITY ? 0.0f : all;
-  float o[VH], l = 0.0f;
+  for (int n = 0; n < NT; ++n) {
+    if (n > 0) __syncthreads();
+    float sum = sf[n].sum;
+    sum += exl3::xor_lanes(sum, 16);
+    sum += exl3::xor_lanes(sum, 32);
+    if (g == 0) sm[wave][col] = sf[n].ref, sl[wave][col] = sum;
 #pragma unroll
-  for (int m = 0; m < VH; ++m) o[m] = 0.0f;
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-  for (int x = 0; x < AW; ++x) {
-    const float f = __builtin_amdgcn_exp2f(sm[x][row] - ref);
-    l += f * sl[x][row];
+      for (int m = 0; m < VH; ++m) so[wave][col][VH * (4 * g + r) + m] = acc[n][m][r];
+    __syncthreads();
+    float all = -INFINITY;
 #pragma unroll
-    for (int m = 0; m < VH; ++m) o[m] += f * so[x][row][VH * c + m];
-  }
-  if (sbad) l = __builtin_nanf("");
-  const int p = w.r0 + row;
-  if (p >= pairs) return;
-  if (w.splits == 1) {
-    const float inv = 1.0f / l;
-    uint16_t *dst = a.out + (int64_t)(w.sp.row + p / G) * a.os + (head * G + p % G) * D + VH * c;
-    VV b;
+    for (int x = 0; x < AW; ++x) all = fmaxf(all, sm[x][row]);
+    const float ref = all == -INFINITY ? 0.0f : all;
+    float o[VH], l = 0.0f;
 #pragma unroll
-    for (int m = 0; m < VH; m += 2)
-      b[m >> 1] = l == 0.0f ? 0u : pack2<E>(o[m] * inv, o[m + 1] * inv);
-    *reinterpret_cast<VV *>(dst) = b;
-  } else if ((int)blockIdx.x < a.slots) {
-    float *dst = a.part + ((size_t)blockIdx.x * FEW + row) * D + VH * c;
+    for (int m = 0; m < VH; ++m) o[m] = 0.0f;
 #pragma unroll
-    for (int m = 0; m < VH; m += 4)
-      *reinterpret_cast<f32x4 *>(dst + m) = f32x4{o[m], o[m + 1], o[m + 2], o[m + 3]};
-    float *ml = a.part + (size_t)a.slots * FEW * D + ((size_t)blockIdx.x * FEW + row) * 2;
-    if (c == 0) ml[0] = all, ml[1] = l;
+    for (int x = 0; x < AW; ++x) {
+      const float f = __builtin_amdgcn_exp2f(sm[x][row] - ref);
+      l += f * sl[x][row];
+#pragma unroll
+      for (int m = 0; m < VH; ++m) o[m] += f * so[x][row][VH * c + m];
+    }
+    if (sbad) l = __builtin_nanf("");
+    const int p = w.r0 + 16 * n + row;
+    if (p >= pairs) continue;
+    if (w.splits == 1) {
+      const float inv = 1.0f / l;
+      uint16_t *dst = a.out + (int64_t)(w.sp.row + p / G) * a.os + (head * G + p % G) * D + VH * c;
+      VV b;
+#pragma unroll
+      for (int m = 0; m < VH; m += 2)
+        b[m >> 1] = l == 0.0f ? 0u : pack2<E>(o[m] * inv, o[m + 1] * inv);
+      *reinterpret_cast<VV *>(dst) = b;
+    } else if ((int)blockIdx.x < a.slots) {
+      const size_t to = (size_t)blockIdx.x * ROWS + 16 * n + row;
+      float *dst = a.part + to * D + VH * c;
+#pragma unroll
+      for (int m = 0; m < VH; m += 4)
+        *reinterpret_cast<f32x4 *>(dst + m) = f32x4{o[m], o[m + 1], o[m + 2], o[m + 3]};
+      float *ml = a.part + (size_t)a.slots * ROWS * D + to * 2;
+      if (c == 0) ml[0] = all, ml[1] = l;
+    }
   }
 }
 
@@ -972,15 +1000,15 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
     const int e = min(16, n - x0);
     const float *src = a.part + (((size_t)(w.first + x0) * a.pool.kv + head) * rows + row) * D + VH * c;
     const size_t stride = (size_t)a.pool.kv * rows * D;
-    for (int x = 0; x < e; x += 4) {
-      f32x4 y[4][VH / 4];
+    for (int x = 0; x < e; x += 8) {
+      f32x4 y[8][VH / 4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 8; ++u)
 #pragma unroll
         for (int m = 0; m < VH / 4; ++m)
           y[u][m] = *reinterpret_cast<const f32x4 *>(src + min(x + u, e - 1) * stride + 4 * m);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 8; ++u) {
         const float fx = __shfl(f, min(x + u, 15), 16);
         if (x + u < e) {
 #pragma unroll
@@ -1179,24 +1207,34 @@ int device_cus() {
   return cached[dev];
 }
 
+// Tiles of a kv head that the rows can make: a sequence's last one may be short.
+int64_t most_tiles(const exl3p_rows *r, const Split &sl) {
+  return ((int64_t)r->rows * sl.group >> sl.tile) + r->seqs;
+}
+
+// The tile by the most pairs that a sequence has, and how many items the keys
+// are split into: n workgroups of a kv head fill the CUs with two each.  With
+// few tiles of few pairs as many items as stay within one round (a tile's last
+// item comes on top: 4 contexts of up to 65536, 6 tiles, 140 us against 168 in n
+// items and 150 in 2 n); with more tiles than half a round, 4 n, for sequences
+// of unlike lengths (128 of up to 4096 keys: 203 us, 215 in n).  128-pair tiles
+// take n: their joins cost more (a tree of 60 rows over 32768 keys 60 us, 82 in
+// 2 n; prompts of 2048 rows 247 against 355 in 4 n; 16 trees 81, 78 in 1.5 n).
 Split split_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads) {
   Split sl;
   sl.group = heads / c->kv_heads;
-  const bool few = (int64_t)r->max_rows * sl.group <= FEW;
-  sl.tile = log2_of(few ? FEW : MANY);
-  sl.least = few ? 32 * AW : 256;
+  const int64_t pairs = (int64_t)r->max_rows * sl.group;
+  sl.tile = log2_of(pairs <= 16 ? 16 : pairs <= FEW ? FEW : MANY);
+  sl.least = pairs <= FEW ? 32 * AW : 256;
   const int n = (2 * device_cus() + c->kv_heads - 1) / c->kv_heads;
-  sl.target = n > 1 ? n : 1;
+  const int64_t room = n - most_tiles(r, sl);
+  sl.target = pairs > FEW ? n : room > n / 2 ? (int)room : 4 * n;
   // 65535 sequences are 1024 sums a lane, each off by 2^-24 at most
   sl.per = (1.0f + 0x1p-12f) / (float)sl.target;
   return sl;
 }
 
-// Tiles of a kv head that the rows can make, and items: a sequence's last tile
-// and a tile's last item may be short.
-int64_t most_tiles(const exl3p_rows *r, const Split &sl) {
-  return ((int64_t)r->rows * sl.group >> sl.tile) + r->seqs;
-}
+// Items of a kv head: a tile's last one may be short.
 int64_t most_items(const exl3p_rows *r, const Split &sl) { return most_tiles(r, sl) + sl.target; }
 // Tiles that are split: each has a whole item at least, and those are no more
 // than the target.
@@ -1318,9 +1356,12 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   a.slots = (int)(most_items(r, sl) * c->kv_heads);
   const hipStream_t st = static_cast<hipStream_t>(s);
   return by_type(c, [&](auto e, auto d) {
-    if (sl.tile == log2_of(FEW))
-      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d>), dim3((unsigned)a.slots), dim3(64 * AW),
-                         0, st, a);
+    if (sl.tile == 4)
+      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d, 1>), dim3((unsigned)a.slots),
+                         dim3(64 * AW), 0, st, a);
+    else if (sl.tile == 5)
+      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d, 2>), dim3((unsigned)a.slots),
+                         dim3(64 * AW), 0, st, a);
     else
       hipLaunchKernelGGL((attend_many_kernel<decltype(e), d>), dim3((unsigned)a.slots),
                          dim3(64 * AW), 0, st, a);
