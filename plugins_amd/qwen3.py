@@ -289,3 +289,63 @@ class Qwen3Decoder:
         linears([self.lm_head.weight], self.h, outs=[self.logits], norm_w=self.final_norm,
                 nssq=self.ssq, eps=c.eps, stream=stream)
         return self.logits
+
+
+class PagedDecoder:
+    """A Qwen3Decoder's weights over a paged cache (plugins_amd.paged): one pass
+    takes any rows of any sequences -- prompts, single tokens, trees of drafted
+    tokens -- and `verify` keeps what the model's own tokens accept.
+
+    The reference's counterpart is its drafter and verify step on MLX
+    (turboexl3_qwen38/src/spec/drafter.zig); its verify rows take the decode
+    chain of the quant table, as these linears do up to 16 rows."""
+
+    def __init__(self, model: Qwen3Decoder, seqs: int, pages: int, max_pages: int, page: int = 64):
+        from . import paged as P
+        self.P, self.m, self.cfg, self.torch = P, model, model.cfg, model.torch
+        c = model.cfg
+        self.cache = P.PagedCache(c.layers, pages, c.kv_heads, seqs, max_pages, page, HEAD_DIM,
+                                  self.torch.float16, model.embed_table.device)
+
+    def forward(self, rows, ids, parent=None, only=None, stream=None):
+        """Logits [rows, vocab] of the step's rows (of the rows numbered by `only`,
+        int64, if given), whose keys and values go into the cache behind each
+        sequence's `rows.len`; the pages are there (cache.reserve).  ids int32
+        [rows]; parent: the trees (None: each sequence's rows in a line)."""
+        torch, P, m, c, cache = self.torch, self.P, self.m, self.cfg, self.cache
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.forward(rows, ids, parent, only)
+        T = rows.rows
+        f16 = {"dtype": torch.float16, "device": ids.device}
+        h = torch.empty(T, c.hidden, dtype=torch.float32, device=ids.device)
+        x, att = torch.empty(T, c.hidden, **f16), torch.empty(T, c.q_dim, **f16)
+        pos, slot, mask = P.plan(cache, rows, parent)
+        embed(ids, m.embed_table, h)
+        add = None
+        for li, L in enumerate(m.layers):
+            add_rmsnorm(h, add, L["in_norm"], x, c.eps)
+            q, k, v = X.matmul_shared([L["q"].weight, L["k"].weight, L["v"].weight], x)
+            P.qkv_append(cache, li, q, k, v, L["q_norm"], L["k_norm"], pos, slot, q, c.eps, c.theta)
+            P.attend(cache, li, rows, q, att, mask)
+            add_rmsnorm(h, X.matmul(L["o"].weight, att), L["post_norm"], x, c.eps)
+            add = X.swiglu(L["gate"].weight, L["up"].weight, L["down"].weight, x)
+        add_rmsnorm(h, add, m.final_norm, x, c.eps)
+        return X.matmul(m.lm_head.weight, x if only is None else x[only])
+
+    def verify(self, rows, ids, parent=None, most: int | None = None, stream=None):
+        """One greedy verification: the rows' logits, then the walk down each
+        sequence's tree by the model's own tokens (row 0 is a token that is certain
+        already).  Returns path, count, next and new_len (int32 on the device);
+        the cache holds each sequence's first new_len keys, and the pages behind
+        them are the caller's to trim once the lengths are on the host."""
+        torch, P = self.torch, self.P
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.verify(rows, ids, parent, most)
+        target = self.forward(rows, ids, parent).float().argmax(-1).int()
+        i32 = {"dtype": torch.int32, "device": ids.device}
+        path = torch.empty(rows.seqs, most or max(1, rows.max_rows), **i32)
+        count, after, new_len = (torch.empty(rows.seqs, **i32) for _ in range(3))
+        P.commit(self.cache, rows, parent, ids, target, path, count, after, new_len)
+        return path, count, after, new_len
