@@ -1031,7 +1031,11 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
 // tree itself: the lowest fitting child of every row by an LDS minimum (the
 // same whatever the order), then one link a step.  path ascends and path[j] >=
 // j, so what row j's move overwrites no later row still reads; within a round
-// all rows are read before any is written.
+// all rows are read before any is written.  A round holds MOVES rows of a head a
+// thread group, so a usual path is one round: its time is a chain of loads
+// (tree, table, rows), not bytes.
+constexpr int MOVES = 4;
+
 __global__ __launch_bounds__(256) void commit_kernel(
     Pool pool, Step st, size_t layer_bytes, int row_bytes, const int32_t *__restrict__ parent,
     const int32_t *__restrict__ ids, const int32_t *__restrict__ target, int32_t *__restrict__ path,
@@ -1072,28 +1076,37 @@ __global__ __launch_bounds__(256) void commit_kernel(
       new_len[s] = (sp.bad ? st.len[s] : sp.len) + c;
     }
   }
+  // slots of the rows that move, where child and said were: -1 for the others
+  for (int j = threadIdx.x; j < c; j += 256) {
+    const int from = way[j] != j ? slot_of(pool, s, sp.len + way[j]) : -1;
+    const int to = from >= 0 ? slot_of(pool, s, sp.len + j) : -1;
+    child[j] = to >= 0 ? from : -1;
+    said[j] = to;
+  }
+  __syncthreads();
   char *data = (blockIdx.y & 1 ? pool.v : pool.k) + (size_t)(blockIdx.y >> 1) * layer_bytes;
   const int lanes = row_bytes / 16;  // of a row of one head
-  const int per = 256 / lanes;       // rows of one head a round
+  const int per = 256 / lanes;       // rows of one head at once
   const int x = threadIdx.x % lanes, y = threadIdx.x / lanes;
-  const int todo = c * pool.kv;
-  for (int b = 0; b < todo; b += per) {
-    const int j = (b + y) / pool.kv, h = (b + y) % pool.kv;
-    u32x4 val{};
-    size_t to = 0;
-    bool go = false;
-    if (b + y < todo && way[j] != j) {
-      const int from = slot_of(pool, s, sp.len + way[j]), dst = slot_of(pool, s, sp.len + j);
-      if (from >= 0 && dst >= 0) {
-        const int m = (1 << pool.lp) - 1;
+  const int todo = c * pool.kv, m = (1 << pool.lp) - 1;
+  for (int b = 0; b < todo; b += MOVES * per) {
+    u32x4 val[MOVES];
+    char *to[MOVES];
+#pragma unroll
+    for (int u = 0; u < MOVES; ++u) {
+      const int e = b + u * per + y, j = min(e, todo - 1) / pool.kv, h = e % pool.kv;
+      const int from = e < todo ? child[j] : -1, dst = said[j];
+      to[u] = nullptr;
+      if (from >= 0) {
         const size_t src = (((size_t)(from >> pool.lp) * pool.kv + h) << pool.lp) + (from & m);
-        to = ((((size_t)(dst >> pool.lp) * pool.kv + h) << pool.lp) + (dst & m)) * row_bytes + 16 * x;
-        val = *reinterpret_cast<const u32x4 *>(data + src * row_bytes + 16 * x);
-        go = true;
+        val[u] = *reinterpret_cast<const u32x4 *>(data + src * row_bytes + 16 * x);
+        to[u] = data + ((((size_t)(dst >> pool.lp) * pool.kv + h) << pool.lp) + (dst & m)) * row_bytes + 16 * x;
       }
     }
     __syncthreads();
-    if (go) *reinterpret_cast<u32x4 *>(data + to) = val;
+#pragma unroll
+    for (int u = 0; u < MOVES; ++u)
+      if (to[u] != nullptr) *reinterpret_cast<u32x4 *>(to[u]) = val[u];
   }
 }
 
