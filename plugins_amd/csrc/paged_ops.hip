@@ -265,12 +265,15 @@ struct Work {
   Span sp;
 };
 
+// How keys are split into items, by what the host knows; the lengths decide on
+// the device.  A tile (pairs of a row and a query head) has items of equal length.
 struct Split {
-  int group;   // query heads a kv head
-  int tile;    // pairs a tile, a power of two: log2 of it
-  int target;  // items wanted, of a kv head
-  int least;   // keys an item has at least
-  float per;   // a little over 64-key units of an item by units of all
+  int group;    // query heads a kv head
+  int tile;     // pairs a tile, a power of two: log2 of it
+  int least;    // 64-key units that an item has at least
+  float round;  // items of a kv head that fill the CUs once
+  float few;    // up to so many tiles, a round less the tiles is the target,
+  float most;   // else so many items
 };
 
 __device__ __forceinline__ int tiles_of(const Span &sp, const Split &sl) {
@@ -290,34 +293,47 @@ __device__ __forceinline__ int scan(int v) {
 
 // Item (ITEM) number x among the sequences' ones, or tile number x among those
 // that are split.  Every workgroup finds its own: no plan on the device or the
-// host depends on the lengths, so a captured call follows them.  Items have
-// `chunk` keys: the 64-key units that all tiles cover over the items wanted,
-// plus what 32-bit sums may be short of, so items are never more than the
-// target and a tile's last ones.  (Lane exchanges by DPP and scalars: 1 us of a
-// launch less than through LDS, with 64-bit divisions.)
+// host depends on the lengths, so a captured call follows them.  A tile of u
+// units has ceil(u / c) items, c the units of all tiles over the target, plus
+// what 32-bit sums may be short of: items are never more than target + tiles.
+// (Lane exchanges by DPP and scalars: 1 us of a launch less than through LDS,
+// with 64-bit divisions.)
 template <bool ITEM>
 __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64_t room, int x) {
   const int lane = threadIdx.x & 63;
   Span sp{0, 0, 0, false};
-  float units = 0.0f;
+  float units = 0.0f, all = 0.0f;
+  auto units_of = [](const Span &v) { return (uint32_t)(v.len + v.n + 63) >> 6; };
   for (int s = lane; s < st.seqs; s += 64) {
     sp = span_of(st, s, room);
-    units += (float)tiles_of(sp, sl) * (float)((uint32_t)(sp.len + sp.n + 63) >> 6);
+    const float t = (float)tiles_of(sp, sl);
+    units += t * (float)units_of(sp);
+    all += t;
   }
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) units += exl3::xor_lanes(units, m);
+  for (int m = 1; m < 64; m <<= 1) {
+    units += exl3::xor_lanes(units, m);
+    all += exl3::xor_lanes(all, m);
+  }
+  // 65535 sequences are 1024 sums a lane, each off by 2^-24 at most
+  const float target = all <= sl.few ? sl.round - all : sl.most;
   const uint32_t chunk = __builtin_amdgcn_readfirstlane(
-      max(sl.least, (int)fminf(ceilf(units * sl.per), (float)(1 << 23)) * 64));
+      max(sl.least, (int)fminf(ceilf(units * (1.0f + 0x1p-12f) / target), (float)(1 << 25))));
   Work w;
   w.s = -1;
   int items = 0, tiles = 0;  // of the sequences before
   for (int s0 = 0; s0 < st.seqs; s0 += 64) {
     const int s = s0 + lane;
     int nt = 0, ns = 0;
+    uint32_t each = 1;
     if (s < st.seqs) {
       if (st.seqs > 64) sp = span_of(st, s, room);
       nt = tiles_of(sp, sl);
-      ns = (int)(((uint32_t)(sp.len + sp.n) + chunk - 1) / chunk);
+      const uint32_t u = units_of(sp);
+      if (nt > 0) {
+        ns = (int)((u + chunk - 1) / chunk);
+        each = (u + ns - 1) / ns;  // the last items may be empty
+      }
     }
     const int mi = nt * ns, mt = ns > 1 ? nt : 0;
     const int it = scan(mi), ti = scan(mt);
@@ -325,7 +341,7 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
     if (past != 0) {
       const int l = __builtin_ctzll(past);
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      const int n_t = of(nt), n_s = of(ns);
+      const int n_t = of(nt), n_s = of(ns), keys = of((int)each) * 64;
       const int before = items + of(it - mi);
       // the last tile first: a prompt's last rows see the most keys
       const int u = ITEM ? (x - before) / n_s : n_t - 1 - (x - (tiles + of(ti - mt)));
@@ -335,8 +351,9 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
       w.r0 = (n_t - 1 - u) << sl.tile;
       w.first = before + u * n_s;
       w.splits = n_s;
-      w.k0 = j * (int)chunk;
-      w.k1 = min(w.k0 + (int)chunk, w.sp.len + w.sp.n);
+      const uint32_t end = w.sp.len + w.sp.n, from = (uint32_t)j * (uint32_t)keys;
+      w.k0 = (int)min(from, end);
+      w.k1 = (int)min(from + keys, end);
       return w;
     }
     items += __builtin_amdgcn_readlane(it, 63);
@@ -1225,35 +1242,34 @@ int64_t most_tiles(const exl3p_rows *r, const Split &sl) {
   return ((int64_t)r->rows * sl.group >> sl.tile) + r->seqs;
 }
 
-// The tile by the most pairs that a sequence has, and how many items the keys
-// are split into: n workgroups of a kv head fill the CUs with two each.  With
-// few tiles of few pairs as many items as stay within one round (a tile's last
-// item comes on top: 4 contexts of up to 65536, 6 tiles, 140 us against 168 in n
-// items and 150 in 2 n); with more tiles than half a round, 4 n, for sequences
-// of unlike lengths (128 of up to 4096 keys: 203 us, 215 in n).  128-pair tiles
-// take n: their joins cost more (a tree of 60 rows over 32768 keys 60 us, 82 in
-// 2 n; prompts of 2048 rows 247 against 355 in 4 n; 16 trees 81, 78 in 1.5 n).
+// The tile by the most pairs that a sequence has, and how many items its keys are
+// split into; n workgroups of a kv head fill the CUs with two each.  With few
+// tiles one round holds all items (n less the tiles, since a tile's items are
+// rounded up); with more, items are several rounds, for sequences of unlike
+// lengths: 4 n of few pairs, 1.5 n of 128, whose joins cost more.
 Split split_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads) {
   Split sl;
   sl.group = heads / c->kv_heads;
   const int64_t pairs = (int64_t)r->max_rows * sl.group;
   sl.tile = log2_of(pairs <= 16 ? 16 : pairs <= FEW ? FEW : MANY);
-  sl.least = pairs <= FEW ? 32 * AW : 256;
+  sl.least = pairs <= FEW ? 32 * AW / 64 : 4;
   const int n = (2 * device_cus() + c->kv_heads - 1) / c->kv_heads;
-  const int64_t room = n - most_tiles(r, sl);
-  sl.target = pairs > FEW ? n : room > n / 2 ? (int)room : 4 * n;
-  // 65535 sequences are 1024 sums a lane, each off by 2^-24 at most
-  sl.per = (1.0f + 0x1p-12f) / (float)sl.target;
+  sl.round = (float)n;
+  sl.few = (float)(pairs <= FEW ? n / 2 : 3 * n / 8);
+  sl.most = (float)(pairs <= FEW ? 4 * n : n + n / 2);
   return sl;
 }
 
-// Items of a kv head: a tile's last one may be short.
-int64_t most_items(const exl3p_rows *r, const Split &sl) { return most_tiles(r, sl) + sl.target; }
-// Tiles that are split: each has a whole item at least, and those are no more
-// than the target.
+// Items of a kv head, and tiles that are split (each has more units than an item
+// has at most, so they are fewer than the target).
+int64_t most_items(const exl3p_rows *r, const Split &sl) {
+  const int64_t tiles = most_tiles(r, sl);
+  return (float)tiles <= sl.few ? (int64_t)sl.round : tiles + (int64_t)sl.most;
+}
 int64_t most_split(const exl3p_rows *r, const Split &sl) {
   const int64_t tiles = most_tiles(r, sl);
-  return tiles < sl.target ? tiles : sl.target;
+  const int64_t target = (float)tiles <= sl.few ? (int64_t)sl.round : (int64_t)sl.most;
+  return tiles < target ? tiles : target;
 }
 
 template <typename F>

@@ -63,6 +63,12 @@ CASES = [
     ([70, 1, 33], [0, 513, 250], 2, 5, 64, 64),
     ([129], [300], 1, 2, 128, 256),
     ([40], [90], 1, 7, 64, 128),
+    ([7, 8, 0, 2], [0, 777, 5, 90], 2, 4, 128, 64),
+    ([9, 4], [63, 1500], 3, 3, 64, 16),
+    ([20, 9, 16], [130, 0, 2500], 2, 4, 128, 32),
+    ([33], [64], 5, 2, 64, 64),
+    ([60], [5000], 1, 4, 128, 64),
+    ([1, 1], [4095, 4096], 8, 1, 128, 256),
 ]
 
 
