@@ -262,7 +262,19 @@ struct Work {
   int k0, k1;
   int first;   // the tile's first work item
   int splits;  // items of the tile
+  int index;   // of the tile among those that are split
+  int total;   // of those, where asked for
   Span sp;
+};
+
+// What the join needs of a split tile, left for it in the scratch by the tile's
+// first item; the number of them stands before the first.
+struct Joint {
+  int row;     // the sequence's first row
+  int pairs;   // of the sequence
+  int r0;
+  int first, splits;
+  int pad[3];
 };
 
 // How keys are split into items, by what the host knows; the lengths decide on
@@ -291,14 +303,12 @@ __device__ __forceinline__ int scan(int v) {
   return v;
 }
 
-// Item (ITEM) number x among the sequences' ones, or tile number x among those
-// that are split.  Every workgroup finds its own: no plan on the device or the
+// Item number x among the sequences' ones.  Every workgroup finds its own: no plan on the device or the
 // host depends on the lengths, so a captured call follows them.  A tile of u
 // units has ceil(u / c) items, c the units of all tiles over the target, plus
 // what 32-bit sums may be short of: items are never more than target + tiles.
 // (Lane exchanges by DPP and scalars: 1 us of a launch less than through LDS,
 // with 64-bit divisions.)
-template <bool ITEM>
 __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64_t room, int x) {
   const int lane = threadIdx.x & 63;
   Span sp{0, 0, 0, false};
@@ -337,28 +347,29 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
     }
     const int mi = nt * ns, mt = ns > 1 ? nt : 0;
     const int it = scan(mi), ti = scan(mt);
-    const uint64_t past = __ballot((ITEM ? items + it : tiles + ti) > x);
-    if (past != 0) {
+    const uint64_t past = __ballot(items + it > x);
+    if (w.s < 0 && past != 0) {
       const int l = __builtin_ctzll(past);
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       const int n_t = of(nt), n_s = of(ns), keys = of((int)each) * 64;
       const int before = items + of(it - mi);
       // the last tile first: a prompt's last rows see the most keys
-      const int u = ITEM ? (x - before) / n_s : n_t - 1 - (x - (tiles + of(ti - mt)));
-      const int j = ITEM ? (x - before) - u * n_s : 0;
+      const int u = (x - before) / n_s, j = (x - before) - u * n_s;
       w.s = s0 + l;
       w.sp = Span{of(sp.row), of(sp.n), of(sp.len), (bool)of(sp.bad)};
       w.r0 = (n_t - 1 - u) << sl.tile;
       w.first = before + u * n_s;
       w.splits = n_s;
+      w.index = tiles + of(ti - mt) + u;
       const uint32_t end = w.sp.len + w.sp.n, from = (uint32_t)j * (uint32_t)keys;
       w.k0 = (int)min(from, end);
       w.k1 = (int)min(from + keys, end);
-      return w;
+      if (x > 0) return w;  // the first item looks at all sequences
     }
     items += __builtin_amdgcn_readlane(it, 63);
     tiles += __builtin_amdgcn_readlane(ti, 63);
   }
+  w.total = tiles;
   return w;
 }
 
@@ -374,9 +385,18 @@ struct AttnArgs {
   uint32_t flip;  // 0x80008000 where the scale is negative: q's sign bits
   uint16_t *out;
   int64_t os;
-  float *part;  // [items * kv][tile][D] sums, then [items * kv][tile][2] (max, sum)
-  int slots;    // items * kv that part holds
+  Joint *joint;  // [0].row: how many; [1 + i]: the split tiles
+  float *part;   // [items * kv][tile][D] sums, then [items * kv][tile][2] (max, sum)
+  int slots;     // items * kv that part holds
 };
+
+// The scratch's head, from the workgroups that find it.
+__device__ __forceinline__ void leave_joint(const AttnArgs &a, const Work &w, int item) {
+  if (blockIdx.x % a.pool.kv != 0 || threadIdx.x != 0) return;
+  if (item == 0) a.joint[0].row = w.total;
+  if (w.s >= 0 && w.splits > 1 && item == w.first)
+    a.joint[1 + w.index] = Joint{w.sp.row, w.sp.n * a.sl.group, w.r0, w.first, w.splits, {}};
+}
 
 // Which of keys kb .. kb + 63 (below `last`) row i of a sequence sees, a bit a
 // key: the context's, and of the rows those in its mask, or up to itself.
@@ -459,7 +479,7 @@ __device__ __forceinline__ int clear_of(const AttnArgs &a, const Work &w, int la
 // P^T, wants its right operand if V's keys are taken in the same order: the
 // weights never leave their lane.
 template <typename E, int D, int NT>
-__global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * AW, NT == 1 ? 3 : 2) void attend_few_kernel(AttnArgs a) {
   constexpr int KK = D / 32;  // products of 32 dims a score
   constexpr int VH = D / 16;  // dims a lane loads of a value
   constexpr int ROWS = 16 * NT;
@@ -470,7 +490,8 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_few_kernel(AttnArgs a) {
   __shared__ int sbad;
   const int head = blockIdx.x % a.pool.kv, item = blockIdx.x / a.pool.kv;
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
-  const Work w = find_work<true>(a.st, a.sl, room, item);
+  const Work w = find_work(a.st, a.sl, room, item);
+  leave_joint(a, w, item);
   if (w.s < 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -737,7 +758,8 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   __shared__ uint32_t sodd[AW];  // rows of a tile whose values are not all finite
   const int head = blockIdx.x % a.pool.kv, item = blockIdx.x / a.pool.kv;
   const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
-  const Work w = find_work<true>(a.st, a.sl, room, item);
+  const Work w = find_work(a.st, a.sl, room, item);
+  leave_joint(a, w, item);
   if (w.s < 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
@@ -973,8 +995,8 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   }
 }
 
-// The items of a tile joined: 16 lanes a pair, 16 pairs a workgroup.  The wave's
-// lanes hold the items' references and sums, so the loop over the items has no
+// The items of a tile joined: 16 lanes a pair, 16 pairs a workgroup.  A group's
+// lanes hold 16 items' references and sums, so the loop over the items has no
 // load that another waits for.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
@@ -982,13 +1004,12 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   typedef typename std::conditional<VH == 8, u32x4, u32x2>::type VV;
   const int rows = 1 << a.sl.tile, parts = rows / 16;
   const int head = blockIdx.x % a.pool.kv, tile = blockIdx.x / a.pool.kv / parts;
-  const int64_t room = (int64_t)a.pool.max_pages << a.pool.lp;
-  const Work w = find_work<false>(a.st, a.sl, room, tile);
-  if (w.s < 0) return;
+  const Joint w = a.joint[1 + tile];
+  if (tile >= a.joint[0].row) return;
   const int G = a.sl.group, c = threadIdx.x & 15;
   const int row = 16 * ((blockIdx.x / a.pool.kv) % parts) + (threadIdx.x >> 4);
   const int p = w.r0 + row;
-  if (p >= w.sp.n * G) return;
+  if (p >= w.pairs) return;
   const float *ml = a.part + (size_t)a.slots * rows * D;
   const int n = min(w.splits, a.slots / a.pool.kv - w.first);
   float top = -INFINITY, o[VH], l = 0.0f;
@@ -1035,7 +1056,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
     }
   }
   const float inv = 1.0f / l;
-  uint16_t *dst = a.out + (int64_t)(w.sp.row + p / G) * a.os + (head * G + p % G) * D + VH * c;
+  uint16_t *dst = a.out + (int64_t)(w.row + p / G) * a.os + (head * G + p % G) * D + VH * c;
   VV b;
 #pragma unroll
   for (int m = 0; m < VH; m += 2) b[m >> 1] = l == 0.0f ? 0u : pack2<E>(o[m] * inv, o[m + 1] * inv);
@@ -1351,7 +1372,8 @@ size_t exl3p_attend_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int
       check_heads(c, heads).code != EXL3_OK)
     return 0;
   const Split sl = split_of(c, r, heads);
-  return (size_t)most_items(r, sl) * c->kv_heads * ((size_t)1 << sl.tile) * (c->dim + 2) * sizeof(float);
+  return (size_t)(1 + most_split(r, sl)) * sizeof(Joint) +
+         (size_t)most_items(r, sl) * c->kv_heads * ((size_t)1 << sl.tile) * (c->dim + 2) * sizeof(float);
 }
 
 exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
@@ -1381,7 +1403,8 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   a.scale = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f);
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.out = static_cast<uint16_t *>(out), a.os = out_stride;
-  a.part = static_cast<float *>(scratch);
+  a.joint = static_cast<Joint *>(scratch);
+  a.part = reinterpret_cast<float *>(a.joint + 1 + most_split(r, sl));
   a.slots = (int)(most_items(r, sl) * c->kv_heads);
   const hipStream_t st = static_cast<hipStream_t>(s);
   return by_type(c, [&](auto e, auto d) {

@@ -278,6 +278,41 @@ def test_attend_other_stream_and_graph():
             assert torch.equal(out.cpu().view(q.shape), want), turn
 
 
+@pytest.mark.parametrize("n,group", [(1, 4), (6, 5)])
+def test_attend_split_calls_repeat(n, group):
+    """Split tiles of few pairs, joined from the scratch: two hundred calls in a
+    row on scratch that holds garbage or an earlier call's, and replays of one
+    captured call, all bit for bit."""
+    counts, lens = [n, 1, n], [3000, 700, 9000]
+    g, k, v, table, cu, q = batch(counts, lens, torch.float16, 2, group, 64, 64, 19)
+    seen = [[list(range(i + 1)) for i in range(m)] for m in counts]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, 64, group, 0.125)
+    cache = P.PagedCache.over(k.to(DEV), v.to(DEV), table.to(DEV))
+    rows, qd = P.Rows.of(counts, lens, DEV), q.to(DEV)
+    first = P.attend(cache, 0, rows, qd).clone()
+    near(first.cpu().view(q.shape), want, tol, "split")
+    scratch = torch.full((P.attend_scratch_bytes(cache, rows, 2 * group),), 255, dtype=torch.uint8,
+                         device=DEV)
+    out = torch.empty_like(first)
+    wrong = torch.zeros((), dtype=torch.int64, device=DEV)
+    for i in range(200):
+        out.fill_(3.0)
+        P.attend(cache, 0, rows, qd, out, scratch=scratch)
+        wrong += (out != first).sum()
+        if i % 50 == 0:
+            scratch.random_(0, 256)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side, capture_error_mode="thread_local"):
+        P.attend(cache, 0, rows, qd, out, scratch=scratch)
+    for i in range(200):
+        out.fill_(3.0)
+        gr.replay()
+        wrong += (out != first).sum()
+    assert wrong.item() == 0
+
+
 @pytest.mark.parametrize("heads", [1, 5])
 def test_attend_many_sequences(heads):
     """More sequences than a wave has lanes, most without rows; the context's
