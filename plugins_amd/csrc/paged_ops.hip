@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void qkv_append_kernel(
     const double x = (double)p * rates.turns[4 * c + e];
     sincospif(2.0f * (float)(x - floor(x)), &si[e], &co[e]);
   }
-  for (int h0 = wave * HW; h0 < heads; h0 += 4 * HW) {
+  for (int h0 = (blockIdx.y * 4 + wave) * HW; h0 < heads; h0 += gridDim.y * 4 * HW) {
     const int h = h0 + sub;
     if (h >= heads) break;  // the last heads of the row; no lane exchange follows for the others
     const bool isq = h < nq, isv = h >= nq + pool.kv;
@@ -327,8 +327,12 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
   }
   // 65535 sequences are 1024 sums a lane, each off by 2^-24 at most
   const float target = all <= sl.few ? sl.round - all : sl.most;
+  // a tile's first 16 items may be short; more of them are 8 units at least, since
+  // the join's time goes with their number (one token, 8192 keys: 15.1 us, 17.8 in
+  // 64 items of 2 units)
+  const float least = fminf(8.0f, floorf(units * 0.0625f * __builtin_amdgcn_rcpf(fmaxf(all, 1.0f))));
   const uint32_t chunk = __builtin_amdgcn_readfirstlane(
-      max(sl.least, (int)fminf(ceilf(units * (1.0f + 0x1p-12f) / target), (float)(1 << 25))));
+      max(sl.least, (int)fminf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / target), least), (float)(1 << 25))));
   Work w;
   w.s = -1;
   int items = 0, tiles = 0;  // of the sequences before
@@ -995,30 +999,40 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   }
 }
 
-// The items of a tile joined: 16 lanes a pair, 16 pairs a workgroup.  A group's
-// lanes hold 16 items' references and sums, so the loop over the items has no
-// load that another waits for.
+// The items of a tile joined, 16 pairs a workgroup, 16 lanes a group of threads.
+// Where the tile has fewer pairs (one token's query heads), several groups take a
+// share of a pair's items each.  A group's lanes hold 16 items' references and
+// sums, so the loop over the items has no load that another waits for.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
   constexpr int VH = D / 16;
   typedef typename std::conditional<VH == 8, u32x4, u32x2>::type VV;
+  __shared__ float so[16][D];
+  __shared__ float sm[16][2];
   const int rows = 1 << a.sl.tile, parts = rows / 16;
   const int head = blockIdx.x % a.pool.kv, tile = blockIdx.x / a.pool.kv / parts;
   const Joint w = a.joint[1 + tile];
   if (tile >= a.joint[0].row) return;
-  const int G = a.sl.group, c = threadIdx.x & 15;
-  const int row = 16 * ((blockIdx.x / a.pool.kv) % parts) + (threadIdx.x >> 4);
-  const int p = w.r0 + row;
-  if (p >= w.pairs) return;
-  const float *ml = a.part + (size_t)a.slots * rows * D;
+  const int row0 = 16 * ((blockIdx.x / a.pool.kv) % parts);
+  const int left = w.pairs - w.r0 - row0;
+  if (left <= 0) return;
   const int n = min(w.splits, a.slots / a.pool.kv - w.first);
+  // log2 of the pairs' groups (shares for more than 8 items, what a group has in
+  // flight at once); a group's pair and its share of the items
+  const int lp = left >= 16 || n <= 8 ? 4 : left > 1 ? 32 - __builtin_clz(left - 1) : 0;
+  const int G = a.sl.group, c = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const int row = row0 + (group & ((1 << lp) - 1)), share = group >> lp;
+  const int p = w.r0 + row;
+  const float *ml = a.part + (size_t)a.slots * rows * D;
+  const int each = (n + (16 >> lp) - 1) >> (4 - lp);
+  const int begin = min(n, share * each), end = p < w.pairs ? min(n, begin + each) : begin;
   float top = -INFINITY, o[VH], l = 0.0f;
 #pragma unroll
   for (int m = 0; m < VH; ++m) o[m] = 0.0f;
-  for (int x0 = 0; x0 < n; x0 += 16) {
+  for (int x0 = begin; x0 < end; x0 += 16) {
     // 16 items a round, one a lane
     float ref = -INFINITY, sum = 0.0f;
-    if (x0 + c < n) {
+    if (x0 + c < end) {
       const size_t slot = (size_t)(w.first + x0 + c) * a.pool.kv + head;
       const f32x2 v = *reinterpret_cast<const f32x2 *>(ml + (slot * rows + row) * 2);
       ref = v[0], sum = v[1];
@@ -1035,7 +1049,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
     l = l * alpha + part;
 #pragma unroll
     for (int m = 0; m < VH; ++m) o[m] *= alpha;
-    const int e = min(16, n - x0);
+    const int e = min(16, end - x0);
     const float *src = a.part + (((size_t)(w.first + x0) * a.pool.kv + head) * rows + row) * D + VH * c;
     const size_t stride = (size_t)a.pool.kv * rows * D;
     for (int x = 0; x < e; x += 8) {
@@ -1055,6 +1069,27 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
       }
     }
   }
+  if (lp < 4) {  // the shares, in their order
+#pragma unroll
+    for (int m = 0; m < VH; ++m) so[group][VH * c + m] = o[m];
+    if (c == 0) sm[group][0] = top, sm[group][1] = l;
+    __syncthreads();
+    if (share > 0) return;
+    float all = top;
+    for (int x = 1; x < 16 >> lp; ++x) all = fmaxf(all, sm[(x << lp) + group][0]);
+    const float ref = all == -INFINITY ? 0.0f : all;
+    l = 0.0f;
+#pragma unroll
+    for (int m = 0; m < VH; ++m) o[m] = 0.0f;
+    for (int x = 0; x < 16 >> lp; ++x) {
+      const int from = (x << lp) + group;
+      const float f = __builtin_amdgcn_exp2f(sm[from][0] - ref);
+      l += f * sm[from][1];
+#pragma unroll
+      for (int m = 0; m < VH; ++m) o[m] += f * so[from][VH * c + m];
+    }
+  }
+  if (p >= w.pairs) return;
   const float inv = 1.0f / l;
   uint16_t *dst = a.out + (int64_t)(w.row + p / G) * a.os + (head * G + p % G) * D + VH * c;
   VV b;
@@ -1357,8 +1392,13 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
   const double ratio = pow(theta, -2.0 / c->dim);
   double turn = 1.0 / 6.283185307179586476925287;
   for (int i = 0; i < c->dim / 2; ++i, turn *= ratio) rates.turns[i] = turn;
+  // A wave's angles serve all heads that it takes: one workgroup a row, or, where
+  // rows are few, as many as the heads fill (8 rows 4.7 -> 3.4 us, 256 5.2 -> 4.3;
+  // 1500 rows 10.7 with one, 12.2 with all).
+  const int all = (heads + 2 * c->kv_heads) * c->dim / 512;  // waves of a row's heads
+  const int y = rows < 512 ? (all + 3) / 4 : 1;
   return by_type(c, [&](auto e, auto d) {
-    hipLaunchKernelGGL((qkv_append_kernel<decltype(e), d>), dim3(rows), dim3(256), 0,
+    hipLaunchKernelGGL((qkv_append_kernel<decltype(e), d>), dim3(rows, y > 1 ? y : 1), dim3(256), 0,
                        static_cast<hipStream_t>(s), pool_of(c, layer), rows, heads,
                        static_cast<const uint16_t *>(q), q_stride, static_cast<const uint16_t *>(k),
                        k_stride, static_cast<const uint16_t *>(v), v_stride,

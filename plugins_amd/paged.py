@@ -31,12 +31,17 @@ from . import exl3 as X
 TREE_MAX = 1024  # EXL3P_TREE_MAX
 
 _torch = None  # the module, from the first cache or rows on
+_int32 = _device = _raw_stream = None
 
 
 def _t():
-    global _torch
+    global _torch, _int32, _device, _raw_stream
     if _torch is None:
         _torch = X._torch()
+        _int32 = _torch.int32
+        # torch.cuda.current_device() and current_stream(i).cuda_stream without what
+        # surrounds them (0.2 and 2 us a call)
+        _device, _raw_stream = _torch._C._cuda_getDevice, _torch._C._cuda_getCurrentRawStream
     return _torch
 
 
@@ -312,22 +317,21 @@ def _matrix(t, what: str, cache, rows: int, width: int):
 
 
 def _ints(t, what: str, cache, n: int):
-    if t.dtype is not _torch.int32:
+    if t.dtype is _int32 and t.numel() == n and t.get_device() == cache.index and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not _int32:
         raise TypeError(f"{what} is int32")
-    if t.get_device() != cache.index or not t.is_contiguous() or t.numel() != n:
-        raise ValueError(f"{what}: {n} dense elements on {cache.device}")
-    return t.data_ptr()
+    raise ValueError(f"{what}: {n} dense elements on {cache.device}")
 
 
 def _stream(cache, stream):
     if stream is not None:
         return stream.cuda_stream
-    # torch.cuda.current_stream(device).cuda_stream without the Stream object (2 us)
-    return _torch._C._cuda_getCurrentRawStream(cache.index)
+    return _raw_stream(cache.index)
 
 
 def _call(cache, fn, what, *args):
-    if cache.index == _torch.cuda.current_device():
+    if cache.index == _device():
         v = fn(*args)
     else:
         with _torch.cuda.device(cache.index):
@@ -396,7 +400,7 @@ def qkv_append(cache, layer: int, q, k, v, q_norm, k_norm, pos, slot, q_out, eps
     norms = []
     for w in (q_norm, k_norm):
         if w is not None and (w.dtype is not cache.dtype or w.get_device() != cache.index or
-                              w.shape != (dim,) or not w.is_contiguous()):
+                              w.numel() != dim or not w.is_contiguous()):
             raise ValueError(f"a norm's weights are [{dim}], of the cache's type and device")
         norms.append(None if w is None else w.data_ptr())
     _call(cache, paged_lib().exl3p_qkv_append, "qkv_append", cache._ref, layer, n, heads, qp, qs, kp,
