@@ -19,8 +19,9 @@
  *   exl3p_book_*      which pages are whose: host bookkeeping, no device work
  *
  * Device pointers unless said otherwise; every entry records its work on the
- * stream, allocates nothing, synchronizes nothing and may be captured into a
- * graph.  Refusals are named (exl3_verdict) and launch nothing.  What only the
+ * stream (of the current device), allocates nothing, synchronizes nothing and may
+ * be captured into a graph: what is on the device -- lengths, table, tokens -- is
+ * read when the work runs.  Refusals are named (exl3_verdict) and launch nothing.  What only the
  * device can see is checked by the kernels, which never leave the arrays:
  *  - a sequence whose len is negative, or whose len + rows pass max_pages *
  *    page, has slots of -1 and attends to NaN; exl3p_commit gives it count 0;
@@ -44,7 +45,7 @@ extern "C" {
 
 /* A cache.  k, v on a 16-byte boundary; dtype EXL3_DT_F16 or EXL3_DT_BF16 (of
  * q, k, v, the norm weights and the output too); page a power of two from 16
- * to 256; dim 64 or 128; pages * page and max_pages * page below 2^31. */
+ * to 256; dim 64 or 128; pages * page below 2^31, max_pages * page up to 2^30. */
 typedef struct exl3p_cache {
   uint32_t size; /* sizeof(exl3p_cache) */
   int32_t dtype;
@@ -95,7 +96,7 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
 /* out[t] = softmax(q[t] k^T * scale) v over what row t sees: the sequence's
  * first len keys and, of its rows, those in its mask (mask NULL: rows 0 .. i).
  * heads is a multiple of the cache's kv_heads, query head h reads kv head
- * h / (heads / kv_heads).  A row that sees nothing is zeros; what a row does
+ * h / (heads / kv_heads).  scale is finite.  A row that sees nothing is zeros; what a row does
  * not see cannot touch it, NaN or not.  scratch: exl3p_attend_scratch_bytes(),
  * written and read within the call (calls that may overlap need their own).
  * The sums' order goes by the sizes and lengths alone: results repeat. */
@@ -111,9 +112,9 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
  * path [seqs][max_path] (indices among the sequence's rows, -1 behind them),
  * count [seqs], next [seqs] = target of the last accepted row (-1 for a
  * sequence without rows), new_len = len + count.  The accepted rows' keys and
- * values move to key numbers len, len + 1, ... in every layer.  new_len may be
- * len itself only if nothing else on the device reads it meanwhile: it may not
- * alias r->len.  parent NULL: a chain. */
+ * values move to key numbers len, len + 1, ... in every layer.  new_len is not
+ * r->len (other workgroups read that meanwhile).  parent NULL: a chain.  At most
+ * EXL3P_TREE_MAX rows of a sequence. */
 exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32_t *parent,
                           const int32_t *ids, const int32_t *target, int32_t *path,
                           int32_t max_path, int32_t *count, int32_t *next, int32_t *new_len,
@@ -132,11 +133,11 @@ typedef struct exl3p_book exl3p_book;
 exl3p_book *exl3p_book_open(int32_t pages, int32_t page, int32_t seqs, int32_t max_pages,
                             exl3_verdict *why); /* NULL: *why says why */
 void exl3p_book_close(exl3p_book *b);
-/* Pages for keys up to `to` of a sequence, and keys from .. to - 1 writable:
- * those of their pages that others hold too are replaced by pages of its own,
- * and *pairs (at most `room`) pairs src[], dst[] say what exl3p_copy_pages has
- * to copy before the keys are written (a replaced page that holds no key below
- * `from` needs no copy and gives no pair).  All or nothing: too_large where
+/* Pages for keys up to `to` of a sequence, and keys from .. to - 1 writable (what
+ * the sequence holds from `from` on is given up): those of their pages that
+ * others hold too are replaced by pages of its own, and *pairs (0 or 1, at most
+ * `room`) pairs src[], dst[] say what exl3p_copy_pages has to copy before the
+ * keys are written: the page that holds earlier keys too.  All or nothing: too_large where
  * pages, table or room do not suffice. */
 exl3_verdict exl3p_book_reserve(exl3p_book *b, int32_t seq, int32_t from, int32_t to, int32_t *src,
                                 int32_t *dst, int32_t room, int32_t *pairs);

@@ -50,8 +50,8 @@ exl3p_book *exl3p_book_open(int32_t pages, int32_t page, int32_t seqs, int32_t m
                                     "power of two from 16 to 256");
     return nullptr;
   }
-  if ((int64_t)pages * page > INT32_MAX || (int64_t)max_pages * page > INT32_MAX) {
-    *why = refuse(EXL3_TOO_LARGE, "PagedBookShape: 2^31 keys or more");
+  if ((int64_t)pages * page > INT32_MAX || (int64_t)max_pages * page > 1 << 30) {
+    *why = refuse(EXL3_TOO_LARGE, "PagedBookShape: 2^31 keys or more, or over 2^30 of a sequence");
     return nullptr;
   }
   try {

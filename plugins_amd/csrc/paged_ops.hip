@@ -128,8 +128,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void tree_plan_kernel(
   const int s = blockIdx.x;
   const int64_t room = (int64_t)pool.max_pages << pool.lp;
   if (s == st.seqs) {
-    const int from = min(max(st.cu[st.seqs], 0), st.rows);
-    for (int t = from + threadIdx.x; t < st.rows; t += PLAN_THREADS) {
+    const int from = min(max(st.cu[st.seqs], 0), st.rows), first = st.cu[0];
+    for (int t = threadIdx.x; t < st.rows; t += PLAN_THREADS) {
+      if (t >= first && t < from) continue;
       pos[t] = 0;
       slot[t] = -1;
       for (int w = 0; w < words; ++w) mask[(size_t)t * words + w] = 0;
@@ -186,11 +187,11 @@ struct Rates {
 // turns together lies in one lane.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void qkv_append_kernel(
-    Pool pool, int rows, int nq, const uint16_t *__restrict__ q, int64_t qs,
+    Pool pool, int rows, int nq, const uint16_t *q, int64_t qs,
     const uint16_t *__restrict__ k, int64_t ks, const uint16_t *__restrict__ v, int64_t vs,
     const uint16_t *__restrict__ qn, const uint16_t *__restrict__ kn,
-    const int32_t *__restrict__ pos, const int32_t *__restrict__ slot, uint16_t *__restrict__ qo,
-    int64_t os, float eps, Rates rates) {
+    const int32_t *__restrict__ pos, const int32_t *__restrict__ slot, uint16_t *qo, int64_t os,
+    float eps, Rates rates) {
   constexpr int LH = D / 8, HW = 64 / LH;  // lanes a head, heads a wave
   const int t = blockIdx.x;
   const int sl = slot[t];
@@ -390,6 +391,7 @@ struct AttnArgs {
   uint16_t *out;
   int64_t os;
   Joint *joint;  // [0].row: how many; [1 + i]: the split tiles
+  int joints;    // that joint holds
   float *part;   // [items * kv][tile][D] sums, then [items * kv][tile][2] (max, sum)
   int slots;     // items * kv that part holds
 };
@@ -397,8 +399,8 @@ struct AttnArgs {
 // The scratch's head, from the workgroups that find it.
 __device__ __forceinline__ void leave_joint(const AttnArgs &a, const Work &w, int item) {
   if (blockIdx.x % a.pool.kv != 0 || threadIdx.x != 0) return;
-  if (item == 0) a.joint[0].row = w.total;
-  if (w.s >= 0 && w.splits > 1 && item == w.first)
+  if (item == 0) a.joint[0].row = min(w.total, a.joints);
+  if (w.s >= 0 && w.splits > 1 && item == w.first && w.index < a.joints)
     a.joint[1 + w.index] = Joint{w.sp.row, w.sp.n * a.sl.group, w.r0, w.first, w.splits, {}};
 }
 
@@ -1227,8 +1229,8 @@ exl3_verdict check_cache(const exl3p_cache *c) {
     return refuse(EXL3_UNSUPPORTED, "PagedCachePage: a power of two from 16 to 256");
   if (c->layers <= 0 || c->pages <= 0 || c->kv_heads <= 0 || c->seqs <= 0 || c->max_pages <= 0)
     return refuse(EXL3_UNSUPPORTED, "PagedCacheShape: sizes above 0");
-  if ((int64_t)c->pages * c->page > INT32_MAX || (int64_t)c->max_pages * c->page > INT32_MAX)
-    return refuse(EXL3_TOO_LARGE, "PagedCacheShape: 2^31 keys or more");
+  if ((int64_t)c->pages * c->page > INT32_MAX || (int64_t)c->max_pages * c->page > 1 << 30)
+    return refuse(EXL3_TOO_LARGE, "PagedCacheShape: 2^31 keys or more, or over 2^30 of a sequence");
   if (c->kv_heads > 65535 || c->layers > 32767)
     return refuse(EXL3_TOO_LARGE, "PagedCacheShape: over 65535 kv heads or 32767 layers");
   return OK;
@@ -1426,6 +1428,7 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   EXL3P_TRY(check_heads(c, heads));
   if (words < 0 || (mask == nullptr) != (words == 0) || (mask != nullptr && (int64_t)words * 64 < r->max_rows))
     return refuse(EXL3_UNSUPPORTED, "PagedMask: 64 * words below the rows of a sequence");
+  if (!(fabsf(scale) < INFINITY)) return refuse(EXL3_UNSUPPORTED, "PagedScale: finite");
   if (r->rows == 0 || r->seqs == 0 || r->max_rows == 0) return OK;
   const int64_t wq = (int64_t)heads * c->dim;
   EXL3P_TRY(check_matrix(q, q_stride, wq));
@@ -1443,7 +1446,7 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   a.scale = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f);
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.out = static_cast<uint16_t *>(out), a.os = out_stride;
-  a.joint = static_cast<Joint *>(scratch);
+  a.joint = static_cast<Joint *>(scratch), a.joints = (int)most_split(r, sl);
   a.part = reinterpret_cast<float *>(a.joint + 1 + most_split(r, sl));
   a.slots = (int)(most_items(r, sl) * c->kv_heads);
   const hipStream_t st = static_cast<hipStream_t>(s);

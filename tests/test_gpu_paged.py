@@ -153,19 +153,22 @@ def test_attend_large_scores_and_an_infinite_key():
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_attend_many_small_weights(dtype):
+@pytest.mark.parametrize("rows,gap", [(1, 14.5), (1, 18.5), (40, 14.5), (40, 18.5)])
+def test_attend_many_small_weights(dtype, rows, gap):
     """One key far above 20000 others whose weights only count together: each is
-    about 2^-21 of the largest, where f16 alone would hold one bit of it."""
+    about 2^-21 of the largest, where f16 alone would hold a few bits of it, or
+    2^-27, where the kernel's weights are f16's subnormal numbers."""
     n_ctx = 20000
-    counts, lens = [1], [n_ctx]
+    counts, lens = [rows], [n_ctx]
     g, k, v, table, cu, q = batch(counts, lens, dtype, 1, 1, 64, 256, 8)
     v = v.abs()
     q = torch.ones_like(q)
     k = torch.zeros_like(k)
-    pg, row = R.slots(table, 0, 256, n_ctx + 1)
-    k[0, pg[123], :, row[123]] = 14.5 / 64
+    pg, row = R.slots(table, 0, 256, n_ctx + rows)
+    k[0, pg[123], :, row[123]] = gap / 64
     v[0, pg[123], :, row[123]] = 0
-    want, tol = R.attention(q, k, v, table, cu, lens, [[[0]]], 256, 1, 1.0)
+    seen = [[list(range(i + 1)) for i in range(rows)]]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, 256, 1, 1.0)
     near(attended(k, v, table, counts, lens, q, None, scale=1.0), want, tol, "small weights")
 
 
@@ -373,6 +376,17 @@ def test_tree_plan(counts, lens, page):
     torch.cuda.synchronize()
     assert torch.equal(mask.cpu(), R.masks([list(range(i + 1)) for n in counts for i in range(n)],
                                            words))
+
+
+def test_tree_plan_of_a_first_sequence_that_starts_late():
+    """Rows before cu[0] are no sequence's."""
+    k = torch.empty(1, 2, 1, 16, 64, dtype=torch.float16, device=DEV)
+    cache = P.PagedCache.over(k, k.clone(), torch.tensor([[1]], dtype=torch.int32, device=DEV))
+    rows = P.Rows(torch.tensor([2, 4], dtype=torch.int32, device=DEV),
+                  torch.tensor([3], dtype=torch.int32, device=DEV), 5, 2)
+    pos, slot, mask = P.plan(cache, rows, torch.tensor([7, 7, -1, 0, 7], dtype=torch.int32, device=DEV))
+    assert slot.tolist() == [-1, -1, 19, 20, -1] and pos[2:4].tolist() == [3, 4]
+    assert mask[:, 0].tolist() == [0, 0, 1, 3, 0]
 
 
 def test_tree_plan_of_rows_and_keys_that_do_not_fit():

@@ -194,7 +194,7 @@ def entries(c, r, **kw):
     (dict(page=8), "PagedCachePage"), (dict(page=48), "PagedCachePage"),
     (dict(page=512), "PagedCachePage"), (dict(pages=0), "PagedCacheShape"),
     (dict(layers=-1), "PagedCacheShape"), (dict(pages=1 << 27), "2\\^31"),
-    (dict(max_pages=1 << 27), "2\\^31"), (dict(kv_heads=65536), "65535")])
+    (dict(max_pages=(1 << 26) + 1), "2\\^30"), (dict(kv_heads=65536), "65535")])
 def test_caches_that_are_refused(kw, why):
     for name, call in entries(desc(**kw), step()).items():
         v = call()
@@ -203,7 +203,7 @@ def test_caches_that_are_refused(kw, why):
 
 
 @pytest.mark.parametrize("kw,why", [
-    (dict(size=1), "another version"), (dict(seqs=-1), "PagedRows"), (dict(seqs=4), "more sequences"),
+    (dict(size=1), "another version"), (dict(seqs=-1), "PagedRows"), (dict(seqs=65536), "65535"), (dict(seqs=4), "more sequences"),
     (dict(rows=-1), "PagedRows"), (dict(max_rows=7), "PagedRows"), (dict(max_rows=-1), "PagedRows"),
     (dict(cu=None), "missing"), (dict(len=None), "missing")])
 def test_rows_that_are_refused(kw, why):
@@ -228,6 +228,8 @@ def test_rows_that_are_refused(kw, why):
     (("append",), dict(kn=68), "Alignment"), (("append",), dict(rows=-1), "PagedRows"),
     (("attend",), dict(scratch=None), "PagedScratch"), (("attend",), dict(scratch=4100), "PagedScratch"),
     (("attend",), dict(bytes=100), "PagedScratch"),
+    (("attend",), dict(scale=float("nan")), "PagedScale"),
+    (("attend",), dict(scale=float("-inf")), "PagedScale"),
     (("commit",), dict(most=0), "PagedPath"), (("commit",), dict(path=None), "missing"),
     (("commit",), dict(ids=None), "missing"), (("commit",), dict(target=None), "missing"),
     (("commit",), dict(new_len=64), "over len"), (("commit",), dict(count=None), "missing"),

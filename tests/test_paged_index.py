@@ -1,0 +1,96 @@
+"""The split of a paged attention's keys into work items, restated on the CPU
+(plugins_amd/csrc/paged_ops.hip: split_of, find_work): every key of every tile
+is in one item, items and split tiles stay within what the host sized the launch
+and the scratch for, whatever the lengths -- in the kernel's own 32-bit sums."""
+import random
+
+import numpy as np
+import pytest
+
+F = np.float32
+CUS = 256
+
+
+def split_of(kv, group, rows, seqs, max_rows):
+    pairs = max_rows * group
+    tile = 4 if pairs <= 16 else 5 if pairs <= 32 else 7
+    n = (2 * CUS + kv - 1) // kv
+    few = n // 2 if pairs <= 32 else 3 * n // 8
+    most = 4 * n if pairs <= 32 else n + n // 2
+    tiles = ((rows * group) >> tile) + seqs
+    return dict(group=group, tile=tile, least=2 if pairs <= 32 else 4, round=n, few=few, most=most,
+                items=n if tiles <= few else tiles + most,
+                split=min(tiles, n if tiles <= few else most))
+
+
+def butterfly(lanes):
+    v = lanes.copy()
+    for m in (1, 2, 4, 8, 16, 32):
+        v = (v + v[np.arange(64) ^ m]).astype(F)
+    assert (v == v[0]).all()
+    return v[0]
+
+
+def items_of(sl, counts, lens):
+    """[(sequence, tile, k0, k1)], split tiles."""
+    units, tiles = np.zeros(64, F), np.zeros(64, F)
+    nt = [(n * sl["group"] + (1 << sl["tile"]) - 1) >> sl["tile"] for n in counts]
+    un = [(n + c + 63) >> 6 for n, c in zip(counts, lens)]
+    for s, (t, u) in enumerate(zip(nt, un)):
+        units[s % 64] = F(units[s % 64] + F(F(t) * F(u)))
+        tiles[s % 64] = F(tiles[s % 64] + F(t))
+    units, tiles = butterfly(units), butterfly(tiles)
+    target = F(sl["round"]) - tiles if tiles <= F(sl["few"]) else F(sl["most"])
+    assert target > 0
+    # the reciprocal is right to one unit in the last place either way: both ends
+    rcp = F(1) / max(tiles, F(1))
+    out = []
+    for r in (np.nextafter(rcp, F(0)), np.nextafter(rcp, F(2))):
+        least = min(F(8), np.floor(F(F(units * F(0.0625)) * r)))
+        chunk = max(sl["least"], int(min(max(np.ceil(F(F(units * F(1 + 2.0 ** -12)) / target)), least),
+                                         F(1 << 25))))
+        items, split = [], 0
+        for s, (t, u) in enumerate(zip(nt, un)):
+            if t == 0:
+                continue
+            ns = (u + chunk - 1) // chunk
+            each = (u + ns - 1) // ns
+            split += t if ns > 1 else 0
+            for x in range(t):
+                for j in range(ns):
+                    end = counts[s] + lens[s]
+                    items.append((s, t - 1 - x, min(j * each * 64, end), min((j + 1) * each * 64, end)))
+        out.append((items, split))
+    return out
+
+
+def check(kv, group, counts, lens):
+    sl = split_of(kv, group, sum(counts), len(counts), max(counts))
+    for items, split in items_of(sl, counts, lens):
+        assert len(items) <= sl["items"] and split <= sl["split"], (len(items), split, sl)
+        at = {}
+        for s, tile, k0, k1 in items:
+            assert at.get((s, tile), 0) == k0 <= k1 and k0 % 64 in (0, k0 if k0 == k1 else 0)
+            at[s, tile] = k1
+        for (s, tile), end in at.items():
+            assert end == counts[s] + lens[s]
+        assert len(at) == sum((n * group + (1 << sl["tile"]) - 1) >> sl["tile"] for n in counts)
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_items_cover_every_key_once_within_their_bounds(seed):
+    rng = random.Random(seed)
+    seqs = rng.choice([1, 1, 2, 5, 17, 63, 64, 65, 130, 500])
+    most = rng.choice([1, 1, 2, 4, 8, 33, 64, 300, 2000])
+    ctx = rng.choice([0, 1, 63, 100, 5000, 200000, 3000000])
+    counts = [rng.randint(0, most) for _ in range(seqs)]
+    counts[rng.randrange(seqs)] = most
+    lens = [rng.randint(0, ctx) if rng.random() < 0.8 else 0 for _ in range(seqs)]
+    check(rng.choice([1, 2, 3, 8, 16, 200, 600]), rng.choice([1, 2, 3, 4, 5, 8, 16]), counts, lens)
+
+
+def test_items_of_the_largest_batches():
+    check(8, 4, [1] * 60000, [7] * 60000)
+    check(1, 1, [1], [(1 << 30) - 1])
+    check(2, 4, [1 << 20], [(1 << 30) - (1 << 20)])
+    check(1, 8, [1] * 63 + [1024], [1 << 24] * 64)
