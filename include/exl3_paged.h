@@ -21,8 +21,9 @@
  * Device pointers unless said otherwise; every entry records its work on the
  * stream (of the current device), allocates nothing, synchronizes nothing and may
  * be captured into a graph: what is on the device -- lengths, table, tokens -- is
- * read when the work runs.  Refusals are named (exl3_verdict) and launch nothing.  What only the
- * device can see is checked by the kernels, which never leave the arrays:
+ * read when the work runs.  Refusals are named (exl3_verdict) and launch nothing.
+ * What only the device can see is checked by the kernels, which never leave the
+ * arrays:
  *  - a sequence whose len is negative, or whose len + rows pass max_pages *
  *    page, has slots of -1 and attends to NaN; exl3p_commit gives it count 0;
  *  - a page number outside [0, pages) among a sequence's keys likewise: slot -1,
@@ -60,10 +61,10 @@ typedef struct exl3p_cache {
 typedef struct exl3p_rows {
   uint32_t size; /* sizeof(exl3p_rows) */
   int32_t seqs;     /* at most the cache's */
-  int32_t rows;     /* rows of the step's tensors */
+  int32_t rows;     /* rows of the step's tensors, at most 2^30 */
   int32_t max_rows; /* no sequence has more */
   const int32_t *cu;  /* [seqs + 1] */
-  const int32_t *len; /* [seqs] */
+  const int32_t *len; /* [seqs]; may be NULL where seqs is 0 */
 } exl3p_rows;
 
 /* The most rows a sequence may have where a tree is given. */
@@ -85,7 +86,7 @@ exl3_verdict exl3p_tree_plan(const exl3p_cache *c, const exl3p_rows *r, const in
  * k's heads the same with k_norm into the cache's keys at slot[t]; v's copied
  * into its values.  One rounding, at the end.  q, k, v and q_out have row
  * strides (in elements, multiples of 8) and 16-byte bases; q_out may be q.  Two
- * rows of one slot: either's keys and values. */
+ * rows of one slot: either's keys and values.  Fewer than 2^24 rows a call. */
 exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows, int32_t heads,
                               const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                               const void *v, int64_t v_stride, const void *q_norm,
@@ -96,9 +97,10 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
 /* out[t] = softmax(q[t] k^T * scale) v over what row t sees: the sequence's
  * first len keys and, of its rows, those in its mask (mask NULL: rows 0 .. i).
  * heads is a multiple of the cache's kv_heads, query head h reads kv head
- * h / (heads / kv_heads).  scale is finite.  A row that sees nothing is zeros; what a row does
- * not see cannot touch it, NaN or not.  scratch: exl3p_attend_scratch_bytes(),
- * written and read within the call (calls that may overlap need their own).
+ * h / (heads / kv_heads).  scale, and scale times log2(e), are finite.  A row that
+ * sees nothing is zeros; what a row does not see cannot touch it, NaN or not.
+ * scratch: exl3p_attend_scratch_bytes() of the same device, written and read within
+ * the call (calls that may overlap need their own).
  * The sums' order goes by the sizes and lengths alone: results repeat. */
 size_t exl3p_attend_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int32_t heads);
 exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
@@ -112,9 +114,9 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
  * path [seqs][max_path] (indices among the sequence's rows, -1 behind them),
  * count [seqs], next [seqs] = target of the last accepted row (-1 for a
  * sequence without rows), new_len = len + count.  The accepted rows' keys and
- * values move to key numbers len, len + 1, ... in every layer.  new_len is not
- * r->len (other workgroups read that meanwhile).  parent NULL: a chain.  At most
- * EXL3P_TREE_MAX rows of a sequence. */
+ * values move to key numbers len, len + 1, ... in every layer.  No output lies over
+ * an input (several workgroups read them): new_len is not r->len, next not ids.
+ * parent NULL: a chain.  At most EXL3P_TREE_MAX rows of a sequence. */
 exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32_t *parent,
                           const int32_t *ids, const int32_t *target, int32_t *path,
                           int32_t max_path, int32_t *count, int32_t *next, int32_t *new_len,

@@ -5,6 +5,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <new>
 #include <type_traits>
 
@@ -69,10 +70,6 @@ constexpr float SLACK = 4.0f;
 template <typename E>
 __device__ __forceinline__ float to_f32(uint32_t bits) {
   return (float)__builtin_bit_cast(typename E::T, (uint16_t)bits);
-}
-template <typename E>
-__device__ __forceinline__ uint32_t from_f32(float f) {
-  return __builtin_bit_cast(uint16_t, (typename E::T)f);
 }
 template <typename E>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -319,9 +316,9 @@ __device__ __forceinline__ int scan(int v) {
   return v;
 }
 
-// Item number x among the sequences' ones.  Every workgroup finds its own: no plan on the device or the
-// host depends on the lengths, so a captured call follows them.  A tile of u
-// units has ceil(u / c) items, c the units of all tiles over the target, plus
+// Item number x among the sequences' ones.  Every workgroup finds its own: no
+// plan on the device or the host depends on the lengths, so a captured call
+// follows them.  A tile of u units has ceil(u / c) items, c the units of all tiles over the target, plus
 // what 32-bit sums may be short of: items are never more than target + tiles.
 // (Lane exchanges by DPP and scalars: 1 us of a launch less than through LDS,
 // with 64-bit divisions.)
@@ -1269,9 +1266,18 @@ exl3_verdict check_rows(const exl3p_cache *c, const exl3p_rows *r) {
   if (r->seqs < 0 || r->rows < 0 || r->max_rows < 0 || r->max_rows > r->rows)
     return refuse(EXL3_UNSUPPORTED, "PagedRows: sizes below 0, or more rows a sequence than rows");
   if (r->seqs > 65535) return refuse(EXL3_TOO_LARGE, "PagedRows: over 65535 sequences");
+  if (r->rows > 1 << 30) return refuse(EXL3_TOO_LARGE, "PagedRows: over 2^30 rows");
   if (r->seqs > c->seqs) return refuse(EXL3_UNSUPPORTED, "PagedRows: more sequences than the cache's");
-  if (r->cu == nullptr || r->len == nullptr)
+  if (r->cu == nullptr || (r->len == nullptr && r->seqs > 0))
     return refuse(EXL3_FAILED, "PagedRows: a missing array");
+  return OK;
+}
+
+exl3_verdict check_mask(const exl3p_rows *r, const void *mask, int32_t words) {
+  // (of no rows it may lie nowhere)
+  if (words < 0 || (r->rows > 0 && (mask == nullptr) != (words == 0)) ||
+      (mask != nullptr && (int64_t)words * 64 < r->max_rows))
+    return refuse(EXL3_UNSUPPORTED, "PagedMask: 64 * words below the rows of a sequence");
   return OK;
 }
 
@@ -1308,18 +1314,27 @@ exl3_verdict check_matrix(const void *p, int64_t stride, int64_t width) {
     if (v_.code != EXL3_OK) return v_;   \
   } while (0)
 
+// A grid's workgroups of 256 threads in one dimension: the launch counts threads
+// in 32 bits.
+constexpr int64_t GRID_MAX = ((int64_t)1 << 24) - 1;
+
+bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && x < y + nb && y < x + na;
+}
+
 // The device's compute units, read once per device.
 int device_cus() {
-  static int cached[64] = {0};
+  static std::atomic<int> cached[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cached[dev] == 0) {
-    int n = 0;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
     if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
       n = 256;
-    cached[dev] = n;
+    cached[dev].store(n, std::memory_order_relaxed);
   }
-  return cached[dev];
+  return n;
 }
 
 // Tiles of a kv head that the rows can make: a sequence's last one may be short.
@@ -1384,8 +1399,7 @@ exl3_verdict exl3p_tree_plan(const exl3p_cache *c, const exl3p_rows *r, const in
                              exl3_stream s) {
   EXL3P_TRY(check_cache(c));
   EXL3P_TRY(check_rows(c, r));
-  if (words < 0 || (mask == nullptr) != (words == 0) || (mask != nullptr && (int64_t)words * 64 < r->max_rows))
-    return refuse(EXL3_UNSUPPORTED, "PagedMask: 64 * words below the rows of a sequence");
+  EXL3P_TRY(check_mask(r, mask, words));
   if (parent != nullptr && r->max_rows > EXL3P_TREE_MAX)
     return refuse(EXL3_TOO_LARGE, "PagedTree: over 1024 rows of a sequence");
   if (r->rows == 0) return OK;
@@ -1406,6 +1420,7 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
   EXL3P_TRY(check_layer(c, layer));
   EXL3P_TRY(check_heads(c, heads));
   if (rows < 0) return refuse(EXL3_UNSUPPORTED, "PagedRows: sizes below 0");
+  if (rows > GRID_MAX) return refuse(EXL3_TOO_LARGE, "PagedRows: 2^24 rows or more in one call");
   if (!(theta > 0.0) || !(theta < INFINITY))
     return refuse(EXL3_UNSUPPORTED, "PagedTheta: a rotation's base is positive and finite");
   if (rows == 0) return OK;
@@ -1453,15 +1468,17 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   EXL3P_TRY(check_layer(c, layer));
   EXL3P_TRY(check_rows(c, r));
   EXL3P_TRY(check_heads(c, heads));
-  if (words < 0 || (mask == nullptr) != (words == 0) || (mask != nullptr && (int64_t)words * 64 < r->max_rows))
-    return refuse(EXL3_UNSUPPORTED, "PagedMask: 64 * words below the rows of a sequence");
-  if (!(fabsf(scale) < INFINITY)) return refuse(EXL3_UNSUPPORTED, "PagedScale: finite");
+  EXL3P_TRY(check_mask(r, mask, words));
+  if (!(fabsf(scale) * 1.4426950408889634f < INFINITY))
+    return refuse(EXL3_UNSUPPORTED, "PagedScale: finite, also times log2(e)");
   if (r->rows == 0 || r->seqs == 0 || r->max_rows == 0) return OK;
   const int64_t wq = (int64_t)heads * c->dim;
   EXL3P_TRY(check_matrix(q, q_stride, wq));
   EXL3P_TRY(check_matrix(out, out_stride, wq));
   const Split sl = split_of(c, r, heads);
-  if ((int64_t)r->max_rows * sl.group > INT32_MAX / 2 || most_items(r, sl) * c->kv_heads > INT32_MAX / 16)
+  if ((int64_t)r->max_rows * sl.group > INT32_MAX / 2 ||
+      most_items(r, sl) * c->kv_heads > GRID_MAX ||
+      most_split(r, sl) * c->kv_heads << (sl.tile - 4) > GRID_MAX)
     return refuse(EXL3_TOO_LARGE, "PagedAttend: too many rows and heads for one call");
   if (scratch == nullptr || !aligned(scratch, 16) ||
       scratch_bytes < exl3p_attend_scratch_bytes(c, r, heads))
@@ -1507,6 +1524,17 @@ exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32
       (r->rows > 0 && (ids == nullptr || target == nullptr)))
     return refuse(EXL3_FAILED, "PagedCommit: a missing array");
   if (new_len == r->len) return refuse(EXL3_UNSUPPORTED, "PagedCommit: new_len over len itself");
+  // every workgroup of a sequence walks its tree, whatever the others have written
+  const size_t w = sizeof(int32_t), n = (size_t)r->seqs * w, t = (size_t)r->rows * w;
+  const struct {
+    const void *p;
+    size_t n;
+  } in[] = {{r->cu, n + w}, {r->len, n}, {parent, t}, {ids, t}, {target, t}},
+    out[] = {{path, n * max_path}, {count, n}, {next, n}, {new_len, n}};
+  for (const auto &o : out)
+    for (const auto &i : in)
+      if (overlap(o.p, o.n, i.p, i.n))
+        return refuse(EXL3_UNSUPPORTED, "PagedCommit: an output over an input");
   hipLaunchKernelGGL(commit_kernel, dim3(r->seqs, 2 * c->layers), dim3(256), 0,
                      static_cast<hipStream_t>(s), pool_of(c, 0), step_of(r), layer_bytes(c),
                      c->dim * 2, parent, ids, target, path, max_path, count, next, new_len);

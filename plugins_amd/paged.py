@@ -96,18 +96,27 @@ def paged_lib():
     return _paged
 
 
+def _c_int(x: int) -> int:
+    """x, refused where a C int32 would hold another number (ctypes takes the low bits)."""
+    if not -(1 << 31) <= x < 1 << 31:
+        raise OverflowError(f"{x} is no 32-bit integer")
+    return x
+
+
 class Book:
     """exl3p_book: which pages are whose (host memory only)."""
 
     def __init__(self, pages: int, page: int, seqs: int, max_pages: int):
         v = X.Verdict()
         self.pages, self.page, self.seqs, self.max_pages = pages, page, seqs, max_pages
-        self._b = paged_lib().exl3p_book_open(pages, page, seqs, max_pages, ctypes.byref(v))
+        self._b = None
+        self._b = paged_lib().exl3p_book_open(*map(_c_int, (pages, page, seqs, max_pages)),
+                                              ctypes.byref(v))
         X.check(v, "book")
 
     def _pairs(self, fn, *args, room):
         src, dst, n = (c_int32 * max(1, room))(), (c_int32 * max(1, room))(), c_int32(0)
-        X.check(fn(self._b, *args, src, dst, room, ctypes.byref(n)), "book")
+        X.check(fn(self._b, *map(_c_int, args), src, dst, _c_int(room), ctypes.byref(n)), "book")
         return list(src[:n.value]), list(dst[:n.value])
 
     def reserve(self, seq: int, start: int, stop: int):
@@ -116,10 +125,10 @@ class Book:
         return self._pairs(paged_lib().exl3p_book_reserve, seq, start, stop, room=1)
 
     def fork(self, src: int, dst: int, keys: int) -> None:
-        X.check(paged_lib().exl3p_book_fork(self._b, src, dst, keys), "book")
+        X.check(paged_lib().exl3p_book_fork(self._b, *map(_c_int, (src, dst, keys))), "book")
 
     def trim(self, seq: int, keys: int) -> None:
-        X.check(paged_lib().exl3p_book_trim(self._b, seq, keys), "book")
+        X.check(paged_lib().exl3p_book_trim(self._b, _c_int(seq), _c_int(keys)), "book")
 
     def compact(self, room: int | None = None):
         return self._pairs(paged_lib().exl3p_book_compact,
@@ -353,7 +362,7 @@ def _mask(mask, cache, rows):
         raise TypeError("a mask is int64")
     shape = mask.shape
     if len(shape) != 2 or shape[0] != rows.rows or not mask.is_contiguous() or \
-            mask.get_device() != cache.index:
+            mask.get_device() != cache.index or (shape[1] == 0 and rows.max_rows > 0):
         raise ValueError(f"a mask is dense [{rows.rows}, words] on {cache.device}")
     return mask.data_ptr(), shape[1]
 
@@ -426,7 +435,7 @@ def attend(cache, layer: int, rows, q, out=None, mask=None, scale: float | None 
     op, os_ = _matrix(out, "out", cache, n, heads * dim)
     mp, words = _mask(mask, cache, rows)
     if scratch is None:
-        need = L.exl3p_attend_scratch_bytes(cache._ref, rows._ref, heads)
+        need = attend_scratch_bytes(cache, rows, heads)
         if stream is None:
             scratch = torch.empty(need, dtype=torch.uint8, device=cache.device)
         else:
@@ -441,7 +450,11 @@ def attend(cache, layer: int, rows, q, out=None, mask=None, scale: float | None 
 
 
 def attend_scratch_bytes(cache, rows, heads: int) -> int:
-    return paged_lib().exl3p_attend_scratch_bytes(cache._ref, rows._ref, heads)
+    """exl3p_attend_scratch_bytes on the cache's device."""
+    if cache.index == _device():
+        return paged_lib().exl3p_attend_scratch_bytes(cache._ref, rows._ref, heads)
+    with _torch.cuda.device(cache.index):
+        return paged_lib().exl3p_attend_scratch_bytes(cache._ref, rows._ref, heads)
 
 
 def commit(cache, rows, parent, ids, target, path, count, next, new_len, stream=None) -> None:
@@ -464,5 +477,6 @@ def copy_pages(cache, src, dst, stream=None) -> None:
     if len(dst) != n:
         raise ValueError("as many pages to write as to read")
     arr = c_int32 * max(1, n)
+    src, dst = map(_c_int, src), map(_c_int, dst)
     _call(cache, paged_lib().exl3p_copy_pages, "copy_pages", cache._ref, arr(*src), arr(*dst), n,
           _stream(cache, stream))

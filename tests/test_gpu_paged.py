@@ -606,3 +606,49 @@ def test_forks_and_compaction_keep_every_sequence():
     assert cache.compact() == 0
     write(0, 0, 33)
     check()
+
+
+# ------------------------------------------------- calls that take no usual form
+
+def test_steps_without_sequences():
+    """No sequence, with and without rows: padding gets slot -1, the others write
+    nothing."""
+    k = torch.zeros(1, 2, 1, 16, 64, dtype=torch.float16, device=DEV)
+    cache = P.PagedCache.over(k, k.clone(), torch.zeros(2, 1, dtype=torch.int32, device=DEV))
+    i32 = {"dtype": torch.int32, "device": DEV}
+    rows = P.Rows.of([], [], DEV)
+    pos, slot, mask = P.plan(cache, rows, torch.empty(0, **i32))
+    assert pos.numel() == slot.numel() == mask.numel() == 0
+    empty = torch.empty(0, **i32)
+    P.commit(cache, rows, None, empty, empty, torch.empty(0, 3, **i32), empty, empty, empty)
+    padded = P.Rows(torch.zeros(1, **i32), empty, 3, 0)
+    pos, slot, _ = P.plan(cache, padded)
+    assert pos.tolist() == [0] * 3 and slot.tolist() == [-1] * 3
+    q = torch.ones(3, 128, dtype=torch.float16, device=DEV)
+    out = torch.full_like(q, 7.0)
+    P.attend(cache, 0, padded, q, out)
+    P.qkv_append(cache, 0, q, q[:, :64], q[:, 64:], None, None, pos, slot, out)
+    torch.cuda.synchronize()
+    assert bool((out == 7.0).all()) and not k.any()
+
+
+def test_arguments_that_would_pass_for_others_are_refused():
+    """A mask without words is none, `next` does not overwrite the tree's ids, a
+    page number past 32 bits is not its low bits."""
+    k = torch.zeros(1, 2, 1, 16, 64, dtype=torch.float16, device=DEV)
+    cache = P.PagedCache.over(k, k.clone(), torch.zeros(2, 1, dtype=torch.int32, device=DEV))
+    rows = P.Rows.of([2, 2], [0, 3], DEV)
+    i32 = {"dtype": torch.int32, "device": DEV}
+    none = torch.empty(4, 0, dtype=torch.int64, device=DEV)
+    q = torch.ones(4, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(ValueError, match="mask"):
+        P.attend(cache, 0, rows, q, mask=none)
+    with pytest.raises(ValueError, match="mask"):
+        P.tree_plan(cache, rows, None, torch.empty(4, **i32), torch.empty(4, **i32), none)
+    ids = torch.ones(4, **i32)
+    path, (a, b, c) = torch.empty(2, 2, **i32), (torch.empty(2, **i32) for _ in range(3))
+    for kw in ((a, ids[:2], c), (ids[2:], b, c), (a, b, rows.cu[1:])):
+        with pytest.raises(X.Exl3Error, match="over an input"):
+            P.commit(cache, rows, None, ids, ids.clone(), path, *kw)
+    with pytest.raises(OverflowError):
+        P.copy_pages(cache, [1 << 32], [1])

@@ -260,3 +260,53 @@ def test_nothing_to_do_is_no_refusal():
         assert e[name]().code == X.OK, name
     e = entries(desc(), step(seqs=0), words=1)
     assert e["attend"]().code == X.OK and e["commit"]().code == X.OK
+
+
+@pytest.mark.parametrize("kw", [
+    dict(count=2 << 20), dict(count=(2 << 20) + 20), dict(count=3 << 20), dict(new_len=(1 << 20) + 4),
+    dict(new_len=64 + 8), dict(path=(4 << 20) - 4), dict(path=(4 << 20) + 20), dict(path=64 + 4)])
+def test_commit_refuses_outputs_over_inputs(kw):
+    """Several workgroups read a sequence's tree: `next` in place of ids, say,
+    would change it under them."""
+    far = dict(parent=1 << 20, ids=2 << 20, target=3 << 20, path=5 << 20, count=6 << 20,
+               new_len=7 << 20)
+    if kw.get("path", 0) >> 20:
+        far["parent"] = 4 << 20
+    far.update(kw)
+    v = entries(desc(), step(len=64 + 12), **far)["commit"]()
+    assert v.code == X.UNSUPPORTED and "over an input" in v.reason, v
+
+
+def test_calls_past_a_grid_are_refused():
+    """A launch counts threads in 32 bits: 2^24 workgroups of 256 are too many."""
+    e = entries(desc(), step(rows=(1 << 30) + 1, max_rows=0), rows=1 << 24)
+    for name, why in (("append", "2\\^24"), ("plan", "2\\^30"), ("attend", "2\\^30"),
+                      ("commit", "2\\^30")):
+        v = e[name]()
+        assert v.code == X.TOO_LARGE and re.search(why, v.reason), (name, v)
+    many = desc(kv_heads=65535, seqs=4)
+    for r in (step(rows=4096, max_rows=4), step(rows=32768, max_rows=256)):
+        e = entries(many, r, heads=65535, qs=65535 * 128, os=65535 * 128, words=4)
+        v = e["attend"]()
+        assert v.code == X.TOO_LARGE and "too many rows and heads" in v.reason, v
+
+
+def test_scales_past_32_bits_are_refused():
+    for scale in (3e38, -3e38):
+        assert "PagedScale" in entries(desc(), step(), scale=scale)["attend"]().reason
+
+
+def test_a_step_without_sequences_needs_no_lengths():
+    e = entries(desc(), step(seqs=0, rows=0, max_rows=0, len=None), words=0, mask=None)
+    for name in ("plan", "attend", "commit"):
+        assert e[name]().code == X.OK, name
+
+
+def test_the_book_takes_no_number_for_another():
+    b = P.Book(4, 16, 2, 3)
+    for call in (lambda: P.Book(1 << 32, 16, 1, 1), lambda: b.reserve(0, 0, (1 << 32) + 16),
+                 lambda: b.reserve(1 << 32, 0, 16), lambda: b.fork(0, (1 << 32) + 1, 0),
+                 lambda: b.trim(0, 1 << 32), lambda: b.trim(1 << 32, 0)):
+        with pytest.raises(OverflowError):
+            call()
+    assert b.free_pages() == 4 and b.held(0) == 0
