@@ -273,7 +273,8 @@ struct Work {
   int s;       // -1: nothing
   int r0;      // first pair
   int k0, k1;
-  int first;   // the tile's first work item
+  int first;   // the place of the tile's first item in the scratch
+  int place;   // of this one: items of a tile lie side by side
   int splits;  // items of the tile
   int index;   // of the tile among those that are split
   int total;   // of those, where asked for
@@ -295,10 +296,11 @@ struct Joint {
 struct Split {
   int group;    // query heads a kv head
   int tile;     // pairs a tile, a power of two: log2 of it
-  int least;    // 64-key units that an item has at least
-  float round;  // items of a kv head that fill the CUs once
+  int least;    // 64-key units that an item has at least; 4 behind `few`
+  float round;  // items of a kv head that fill the CUs once, two each
   float few;    // up to so many tiles, a round less the tiles is the target,
   float most;   // else so many items
+  float whole, more;  // no tile is split whose units are at most whole * all + more
 };
 
 __device__ __forceinline__ int tiles_of(const Span &sp, const Split &sl) {
@@ -318,34 +320,51 @@ __device__ __forceinline__ int scan(int v) {
 
 // Item number x among the sequences' ones.  Every workgroup finds its own: no
 // plan on the device or the host depends on the lengths, so a captured call
-// follows them.  A tile of u units has ceil(u / c) items, c the units of all tiles over the target, plus
-// what 32-bit sums may be short of: items are never more than target + tiles.
-// (Lane exchanges by DPP and scalars: 1 us of a launch less than through LDS,
-// with 64-bit divisions.)
+// follows them.  A tile of u units has ceil(u / c) items, c the units of all tiles
+// over the target, plus what 32-bit sums may be short of: items are never more
+// than target + tiles.  (Lane exchanges by DPP and scalars: 1 us of a launch less
+// than through LDS, with 64-bit divisions.)
 __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64_t room, int x) {
   const int lane = threadIdx.x & 63;
   Span sp{0, 0, 0, false};
-  float units = 0.0f, all = 0.0f;
+  float units = 0.0f, all = 0.0f, longest = 0.0f;
   auto units_of = [](const Span &v) { return (uint32_t)(v.len + v.n + 63) >> 6; };
   for (int s = lane; s < st.seqs; s += 64) {
     sp = span_of(st, s, room);
     const float t = (float)tiles_of(sp, sl);
     units += t * (float)units_of(sp);
     all += t;
+    longest = fmaxf(longest, t > 0.0f ? (float)units_of(sp) : 0.0f);
   }
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     units += exl3::xor_lanes(units, m);
     all += exl3::xor_lanes(all, m);
+    longest = fmaxf(longest, exl3::xor_lanes(longest, m));
   }
   // 65535 sequences are 1024 sums a lane, each off by 2^-24 at most
   const float target = all <= sl.few ? sl.round - all : sl.most;
-  // a tile's first 16 items may be short; more of them are 8 units at least, since
-  // the join's time goes with their number (one token, 8192 keys: 15.1 us, 17.8 in
-  // 64 items of 2 units)
-  const float least = fminf(8.0f, floorf(units * 0.0625f * __builtin_amdgcn_rcpf(fmaxf(all, 1.0f))));
+  // Items of up to 16 units are made so long that half a round holds them: a
+  // workgroup alone on a CU takes a unit in little more than half the time, and
+  // the join has half to read (64 rows behind 8000 keys 34.3 us -> 28.8, two single
+  // tokens of 5000 14.8 -> 12.5).  Else a tile's first 16 items may be short; more
+  // of them are 8 units at least, since the join's time goes with their number.
+  const float spare = floorf(0.5f * sl.round) - all;
+  const float half = ceilf(units * __builtin_amdgcn_rcpf(spare));
+  const float least =
+      fmaxf((float)(all <= sl.few ? sl.least : 4),
+            spare > 0.0f && half <= 16.0f
+                ? half
+                : fminf(8.0f, floorf(units * 0.0625f * __builtin_amdgcn_rcpf(fmaxf(all, 1.0f)))));
+  // Whole tiles where the longest of them ends soon after a full round would (its
+  // parts' way through memory and the join cost more): four prompts of up to 500
+  // rows 50.8 us -> 31.0, one of 2000 73.9 -> 58.3, 64 single rows over up to 500
+  // keys 22.6 -> 18.9.
+  const float chunk_of = longest <= sl.whole * units + sl.more
+                             ? (float)(1 << 25)
+                             : ceilf(units * (1.0f + 0x1p-12f) / target);
   const uint32_t chunk = __builtin_amdgcn_readfirstlane(
-      max(sl.least, (int)fminf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / target), least), (float)(1 << 25))));
+      (int)fminf(fmaxf(chunk_of, least), (float)(1 << 25)));
   Work w;
   w.s = -1;
   int items = 0, tiles = 0;  // of the sequences before
@@ -370,12 +389,16 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       const int n_t = of(nt), n_s = of(ns), keys = of((int)each) * 64;
       const int before = items + of(it - mi);
-      // the last tile first: a prompt's last rows see the most keys
-      const int u = (x - before) / n_s, j = (x - before) - u * n_s;
+      // Tiles that read the same keys side by side, the last tile first: a prompt's
+      // last rows see the most keys, and items behind a tile's last key come last
+      // (a tile's items side by side: 1000 rows of 2 kv heads 25.0 us against 24.0,
+      // four prompts of up to 300 rows over up to 4000 keys 62.8 against 60.5).
+      const int j = (x - before) / n_t, u = (x - before) - j * n_t;
       w.s = s0 + l;
       w.sp = Span{of(sp.row), of(sp.n), of(sp.len), (bool)of(sp.bad)};
       w.r0 = (n_t - 1 - u) << sl.tile;
       w.first = before + u * n_s;
+      w.place = w.first + j;
       w.splits = n_s;
       w.index = tiles + of(ti - mt) + u;
       const uint32_t end = w.sp.len + w.sp.n, from = (uint32_t)j * (uint32_t)keys;
@@ -412,7 +435,7 @@ struct AttnArgs {
 __device__ __forceinline__ void leave_joint(const AttnArgs &a, const Work &w, int item) {
   if (blockIdx.x % a.pool.kv != 0 || threadIdx.x != 0) return;
   if (item == 0) a.joint[0].row = min(w.total, a.joints);
-  if (w.s >= 0 && w.splits > 1 && item == w.first && w.index < a.joints)
+  if (w.s >= 0 && w.splits > 1 && w.place == w.first && w.index < a.joints)
     a.joint[1 + w.index] = Joint{w.sp.row, w.sp.n * a.sl.group, w.r0, w.first, w.splits, {}};
 }
 
@@ -1007,8 +1030,8 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
         if (l == 0.0f) b = u32x2{0, 0};
         *reinterpret_cast<u32x2 *>(dst + 32 * d + 8 * x) = b;
       }
-  } else if ((int)blockIdx.x < a.slots) {
-    const size_t row = (size_t)blockIdx.x * MANY + 32 * wave + col;
+  } else if (w.place * a.pool.kv + head < a.slots) {
+    const size_t row = ((size_t)w.place * a.pool.kv + head) * MANY + 32 * wave + col;
     float *dst = a.part + row * D + 4 * h;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -1346,7 +1369,11 @@ int64_t most_tiles(const exl3p_rows *r, const Split &sl) {
 // split into; n workgroups of a kv head fill the CUs with two each.  With few
 // tiles one round holds all items (n less the tiles, since a tile's items are
 // rounded up); with more, items are several rounds, for sequences of unlike
-// lengths: 4 n of few pairs, 1.5 n of 128, whose joins cost more.
+// lengths: 4 n of few pairs, 1.5 n of 128, whose joins cost more.  A tile stays
+// whole up to 0.9 or 1.4 times a workgroup's share of all units and some more (128
+// pairs 1 + 8 and 1.8 + 8 the same, 2.5 + 8 prompts of 300 over 4000 92 us -> 102;
+// few pairs 1.4 + 8 one row over 300 keys 10.1 -> 11.2, 128 over up to 4096 keys
+// 205 -> 215).
 Split split_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads) {
   Split sl;
   sl.group = heads / c->kv_heads;
@@ -1357,6 +1384,8 @@ Split split_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads) {
   sl.round = (float)n;
   sl.few = (float)(pairs <= FEW ? n / 2 : 3 * n / 8);
   sl.most = (float)(pairs <= FEW ? 4 * n : n + n / 2);
+  sl.whole = (pairs <= FEW ? 0.9f : 1.4f) / (float)n;
+  sl.more = pairs <= FEW ? 4.5f : 8.0f;
   return sl;
 }
 

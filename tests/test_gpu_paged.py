@@ -652,3 +652,20 @@ def test_arguments_that_would_pass_for_others_are_refused():
             P.commit(cache, rows, None, ids, ids.clone(), path, *kw)
     with pytest.raises(OverflowError):
         P.copy_pages(cache, [1 << 32], [1])
+
+
+@pytest.mark.parametrize("counts,lens,kv,splits", [
+    ([300, 1], [6000, 40], 1, 10),       # ten tiles, several items each, of unlike ends
+    ([200, 90, 31, 1, 160], [0, 70, 500, 3, 0], 8, 0),   # whole tiles, several a sequence
+    ([2] * 300, [40] * 299 + [700], 8, 1)])  # one of 300 is split
+def test_attend_items_of_several_tiles(counts, lens, kv, splits):
+    """Items of a sequence go by keys first, then tiles; their sums lie in the
+    scratch by tiles."""
+    from tests import test_paged_index as I
+    group = 4
+    sl = I.split_of(kv, group, sum(counts), len(counts), max(counts))
+    assert all(n == splits for _, n in I.items_of(sl, counts, lens))
+    g, k, v, table, cu, q = batch(counts, lens, torch.float16, kv, group, 64, 64, 23)
+    seen = [[list(range(i + 1)) for i in range(n)] for n in counts]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, 64, group, 0.125)
+    near(attended(k, v, table, counts, lens, q, None), want, tol, "items")

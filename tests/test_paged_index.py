@@ -19,6 +19,7 @@ def split_of(kv, group, rows, seqs, max_rows):
     most = 4 * n if pairs <= 32 else n + n // 2
     tiles = ((rows * group) >> tile) + seqs
     return dict(group=group, tile=tile, least=2 if pairs <= 32 else 4, round=n, few=few, most=most,
+                whole=F(F(0.9 if pairs <= 32 else 1.4) / F(n)), more=F(4.5 if pairs <= 32 else 8),
                 items=n if tiles <= few else tiles + most,
                 split=min(tiles, n if tiles <= few else most))
 
@@ -40,15 +41,22 @@ def items_of(sl, counts, lens):
         units[s % 64] = F(units[s % 64] + F(F(t) * F(u)))
         tiles[s % 64] = F(tiles[s % 64] + F(t))
     units, tiles = butterfly(units), butterfly(tiles)
-    target = F(sl["round"]) - tiles if tiles <= F(sl["few"]) else F(sl["most"])
+    few = tiles <= F(sl["few"])
+    target = F(sl["round"]) - tiles if few else F(sl["most"])
     assert target > 0
-    # the reciprocal is right to one unit in the last place either way: both ends
-    rcp = F(1) / max(tiles, F(1))
+    longest = max([u for t, u in zip(nt, un) if t > 0], default=0)
+    spare = F(np.floor(F(0.5) * F(sl["round"])) - tiles)
     out = []
-    for r in (np.nextafter(rcp, F(0)), np.nextafter(rcp, F(2))):
-        least = min(F(8), np.floor(F(F(units * F(0.0625)) * r)))
-        chunk = max(sl["least"], int(min(max(np.ceil(F(F(units * F(1 + 2.0 ** -12)) / target)), least),
-                                         F(1 << 25))))
+    # reciprocals are right to one unit in the last place either way: both ends
+    for to in (F(0), F(np.inf)):
+        r, rs = (np.nextafter(F(1) / x if x else F(np.inf), to) for x in (max(tiles, F(1)), spare))
+        half = np.ceil(F(units * rs)) if spare > 0 else F(0)
+        least = max(F(sl["least"] if few else 4),
+                    half if spare > 0 and half <= 16 else
+                    min(F(8), np.floor(F(F(units * F(0.0625)) * r))))
+        whole = F(longest) <= F(F(sl["whole"] * units) + sl["more"])
+        chunk = int(min(max(F(1 << 25) if whole else
+                            np.ceil(F(F(units * F(1 + 2.0 ** -12)) / target)), least), F(1 << 25)))
         items, split = [], 0
         for s, (t, u) in enumerate(zip(nt, un)):
             if t == 0:
@@ -56,10 +64,10 @@ def items_of(sl, counts, lens):
             ns = (u + chunk - 1) // chunk
             each = (u + ns - 1) // ns
             split += t if ns > 1 else 0
-            for x in range(t):
-                for j in range(ns):
-                    end = counts[s] + lens[s]
-                    items.append((s, t - 1 - x, min(j * each * 64, end), min((j + 1) * each * 64, end)))
+            end = counts[s] + lens[s]
+            for x in range(t * ns):
+                j, i = divmod(x, t)
+                items.append((s, t - 1 - i, min(j * each * 64, end), min((j + 1) * each * 64, end)))
         out.append((items, split))
     return out
 
