@@ -1075,7 +1075,20 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int m = 0; m < VH; ++m) o[m] = 0.0f;
   for (int x0 = begin; x0 < end; x0 += 16) {
-    // 16 items a round, one a lane
+    // 16 items a round, one a lane; the first 8 items' sums are on their way before
+    // the references are
+    const int e = min(16, end - x0);
+    const float *src = a.part + (((size_t)(w.first + x0) * a.pool.kv + head) * rows + row) * D + VH * c;
+    const size_t stride = (size_t)a.pool.kv * rows * D;
+    f32x4 y[8][VH / 4];
+    auto fetch = [&](int x) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int m = 0; m < VH / 4; ++m)
+          y[u][m] = *reinterpret_cast<const f32x4 *>(src + min(x + u, e - 1) * stride + 4 * m);
+    };
+    fetch(0);
     float ref = -INFINITY, sum = 0.0f;
     if (x0 + c < end) {
       const size_t slot = (size_t)(w.first + x0 + c) * a.pool.kv + head;
@@ -1094,16 +1107,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttnArgs a) {
     l = l * alpha + part;
 #pragma unroll
     for (int m = 0; m < VH; ++m) o[m] *= alpha;
-    const int e = min(16, end - x0);
-    const float *src = a.part + (((size_t)(w.first + x0) * a.pool.kv + head) * rows + row) * D + VH * c;
-    const size_t stride = (size_t)a.pool.kv * rows * D;
     for (int x = 0; x < e; x += 8) {
-      f32x4 y[8][VH / 4];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int m = 0; m < VH / 4; ++m)
-          y[u][m] = *reinterpret_cast<const f32x4 *>(src + min(x + u, e - 1) * stride + 4 * m);
+      if (x > 0) fetch(x);
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float fx = __shfl(f, min(x + u, 15), 16);
