@@ -317,6 +317,7 @@ class PagedDecoder:
             with torch.cuda.stream(stream):
                 return self.forward(rows, ids, parent, only)
         T = rows.rows
+        P._ints(ids, "ids", cache, T)  # embed reads as many as there are rows
         f16 = {"dtype": torch.float16, "device": ids.device}
         h = torch.empty(T, c.hidden, dtype=torch.float32, device=ids.device)
         x, att = torch.empty(T, c.hidden, **f16), torch.empty(T, c.q_dim, **f16)

@@ -310,3 +310,31 @@ def test_the_book_takes_no_number_for_another():
         with pytest.raises(OverflowError):
             call()
     assert b.free_pages() == 4 and b.held(0) == 0
+
+
+# ------------------------------------------------- the decoder over the cache
+
+def decoder_without_a_gpu():
+    """A PagedDecoder that has nothing to launch with: what forward refuses, it
+    refuses before that."""
+    import types
+    torch = pytest.importorskip("torch")
+    from plugins_amd import qwen3 as Q
+    P._t()
+    d = Q.PagedDecoder.__new__(Q.PagedDecoder)
+    d.P, d.torch, d.cfg, d.m = P, torch, Q.Qwen3Config(layers=0, vocab=16), None
+    d.cache = types.SimpleNamespace(index=-1, device="cpu", dtype=torch.float16)
+    return torch, d, types.SimpleNamespace(rows=4, seqs=1, max_rows=4, index=-1, device="cpu")
+
+
+@pytest.mark.parametrize("make,why", [
+    (lambda t: t.zeros(4, dtype=t.int64), TypeError), (lambda t: t.zeros(3, dtype=t.int32), ValueError),
+    (lambda t: t.zeros(5, dtype=t.int32), ValueError),
+    (lambda t: t.zeros(8, dtype=t.int32)[::2], ValueError)])
+def test_decoder_refuses_ids_that_are_not_one_a_row(make, why):
+    """The embedding reads `rows` 32-bit numbers from wherever ids begins: 64-bit
+    ones would be other tokens, fewer a read behind them."""
+    torch, d, rows = decoder_without_a_gpu()
+    for call in (d.forward, d.verify):
+        with pytest.raises(why, match="ids"):
+            call(rows, make(torch))
