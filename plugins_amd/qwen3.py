@@ -311,7 +311,9 @@ class PagedDecoder:
         """Logits [rows, vocab] of the step's rows (of the rows numbered by `only`,
         int64, if given), whose keys and values go into the cache behind each
         sequence's `rows.len`; the pages are there (cache.reserve).  ids int32
-        [rows]; parent: the trees (None: each sequence's rows in a line)."""
+        [rows], one outside the vocabulary (in rows that pad the step, say) taken
+        as the nearest in it; parent: the trees (None: each sequence's rows in a
+        line)."""
         torch, P, m, c, cache = self.torch, self.P, self.m, self.cfg, self.cache
         if stream is not None:
             with torch.cuda.stream(stream):
@@ -322,7 +324,7 @@ class PagedDecoder:
         h = torch.empty(T, c.hidden, dtype=torch.float32, device=ids.device)
         x, att = torch.empty(T, c.hidden, **f16), torch.empty(T, c.q_dim, **f16)
         pos, slot, mask = P.plan(cache, rows, parent)
-        embed(ids, m.embed_table, h)
+        embed(ids.clamp(0, c.vocab - 1), m.embed_table, h)
         add = None
         for li, L in enumerate(m.layers):
             add_rmsnorm(h, add, L["in_norm"], x, c.eps)

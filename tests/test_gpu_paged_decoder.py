@@ -162,3 +162,20 @@ def test_a_verified_step_in_a_graph(model):
         for a, b in zip(got, want):
             assert torch.equal(a, b), turn
         assert torch.equal(d.cache.k, after[0]) and torch.equal(d.cache.v, after[1])
+
+
+@pytest.mark.parametrize("fill", [-1, CFG.vocab, 2 ** 31 - 1, -2 ** 31])
+def test_padding_rows_may_hold_any_id(model, fill):
+    """Rows behind the last sequence, and a drafted row of a token that the
+    vocabulary has not: the embedding reads inside its table, and the other rows
+    are what they are beside ids of the vocabulary."""
+    got = []
+    for pad, odd in ((0, 0 if fill < 0 else CFG.vocab - 1), (fill, fill)):
+        d = paged(model)
+        d.cache.reserve(0, 0, 6)
+        rows = P.Rows(torch.tensor([0, 6], dtype=torch.int32, device=DEV),
+                      torch.tensor([0], dtype=torch.int32, device=DEV), 9, 6)
+        ids = torch.cat([tokens(6, 30), torch.full((3,), pad, dtype=torch.int32, device=DEV)])
+        ids[4] = odd
+        got.append(d.forward(rows, ids)[:6].clone())
+    assert torch.isfinite(got[0].float()).all() and torch.equal(*got)
