@@ -135,12 +135,17 @@ typedef struct exl3p_book exl3p_book;
 exl3p_book *exl3p_book_open(int32_t pages, int32_t page, int32_t seqs, int32_t max_pages,
                             exl3_verdict *why); /* NULL: *why says why */
 void exl3p_book_close(exl3p_book *b);
-/* Pages for keys up to `to` of a sequence, and keys from .. to - 1 writable (what
- * the sequence holds from `from` on is given up): those of their pages that
- * others hold too are replaced by pages of its own, and *pairs (0 or 1, at most
- * `room`) pairs src[], dst[] say what exl3p_copy_pages has to copy before the
- * keys are written: the page that holds earlier keys too.  All or nothing: too_large where
- * pages, table or room do not suffice. */
+/* Pages for keys up to `to` of a sequence, and keys from .. to - 1 writable:
+ * those of their pages that others hold too are replaced by pages of its own,
+ * and *pairs (0 or 1, at most `room`) pairs src[], dst[] say what
+ * exl3p_copy_pages has to copy before the keys are written: the page that holds
+ * earlier keys too.  A page replaced without a copy has lost what it held of the
+ * sequence, keys behind `to` in it among them.  Pages behind that of key to - 1
+ * stay the sequence's as they are, those that others hold too still shared: not
+ * writable, until a reserve that covers them, or exl3p_book_trim, which gives
+ * them back (after a fork, trim to `from` before rows are written again from
+ * there on).  All or nothing: too_large where pages, table or room do not
+ * suffice. */
 exl3_verdict exl3p_book_reserve(exl3p_book *b, int32_t seq, int32_t from, int32_t to, int32_t *src,
                                 int32_t *dst, int32_t room, int32_t *pairs);
 /* Sequence dst, which holds no page, shares src's pages of its first `keys` keys. */

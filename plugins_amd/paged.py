@@ -120,8 +120,9 @@ class Book:
         return list(src[:n.value]), list(dst[:n.value])
 
     def reserve(self, seq: int, start: int, stop: int):
-        """Pages for keys up to `stop`, keys start .. stop - 1 writable; the
-        pairs (src, dst) that have to be copied first."""
+        """Pages for keys up to `stop`, keys start .. stop - 1 writable (pages held
+        behind them stay, shared ones shared); the pairs (src, dst) that have to be
+        copied first."""
         return self._pairs(paged_lib().exl3p_book_reserve, seq, start, stop, room=1)
 
     def fork(self, src: int, dst: int, keys: int) -> None:
@@ -223,9 +224,10 @@ class PagedCache:
                 self.table[seq].copy_(t[seq])
 
     def reserve(self, seq: int, start: int, stop: int, stream=None) -> None:
-        """Pages for a sequence's keys up to `stop`, keys start .. stop - 1 (and
-        those behind) its own to write: shared pages among them are replaced, the
-        one that holds earlier keys too by a copy."""
+        """Pages for a sequence's keys up to `stop`, keys start .. stop - 1 its own
+        to write: shared pages among them are replaced, the one that holds earlier
+        keys too by a copy.  Pages behind them that the sequence holds stay as they
+        are, shared ones shared: trim(seq, start) first to be rid of them."""
         src, dst = self._book().reserve(seq, start, stop)
         if src:
             copy_pages(self, src, dst, stream)

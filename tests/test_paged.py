@@ -143,6 +143,33 @@ def test_book_refuses():
     assert v.code == X.TOO_LARGE and n.value == 0 and b.table().tolist() == [[0, 1, -1], [0, 1, -1]]
 
 
+def test_a_rollback_after_a_fork():
+    """A fork that goes back and writes again: only the pages of the keys that
+    reserve names are its own; those held behind them stay the other sequence's
+    too, until a reserve that covers them or a trim.  Header and mirror promise
+    no more."""
+    def forked():
+        b = P.Book(16, 16, 2, 5)
+        b.reserve(0, 0, 80)
+        b.fork(0, 1, 80)
+        return b
+
+    b = forked()
+    assert b.reserve(1, 5, 10) == ([0], [5])
+    assert b.table().tolist() == [[0, 1, 2, 3, 4], [5, 1, 2, 3, 4]]
+    assert [b.shared(p) for p in range(6)] == [1, 2, 2, 2, 2, 1] and b.held(1) == 5
+    assert b.reserve(1, 10, 40) == ([], [])  # page 5 is its own already
+    assert b.table()[1].tolist() == [5, 6, 7, 3, 4] and b.shared(3) == 2
+    b = forked()
+    b.trim(1, 5)
+    assert b.reserve(1, 5, 10) == ([0], [5])
+    assert b.held(1) == 1 and [b.shared(p) for p in range(5)] == [1] * 5
+    # what is written about it
+    text = " ".join(open(os.path.join(ROOT, "include", "exl3_paged.h")).read().split())
+    assert "given up" not in text and "and those behind" not in P.PagedCache.reserve.__doc__
+    assert all("shared" in d for d in (P.PagedCache.reserve.__doc__, P.Book.reserve.__doc__))
+
+
 # ------------------------------------------------------------------- refusals
 
 def desc(**kw):
