@@ -208,6 +208,12 @@ class PagedCache:
 
     # ---- the book, and what it asks of the device
 
+    # What the book has changed and the device does not have yet: pairs of pages to
+    # copy and the sequence (None: all) whose row of the table changed.  It stays
+    # where a copy failed, and is done before the book changes again: until then
+    # the device's table and the pages in it are those of before, whole.
+    _owed = None
+
     def _book(self) -> Book:
         if self.book is None:
             raise RuntimeError("a cache over given tensors has no book")
@@ -223,32 +229,46 @@ class PagedCache:
             else:
                 self.table[seq].copy_(t[seq])
 
+    def _settle(self, stream) -> Book:
+        """The book, with nothing owed to the device."""
+        book = self._book()
+        if self._owed is not None:
+            src, dst, seq = self._owed
+            if src:
+                copy_pages(self, src, dst, stream)
+            self._sync(seq, stream)
+            self._owed = None
+        return book
+
     def reserve(self, seq: int, start: int, stop: int, stream=None) -> None:
         """Pages for a sequence's keys up to `stop`, keys start .. stop - 1 its own
         to write: shared pages among them are replaced, the one that holds earlier
         keys too by a copy.  Pages behind them that the sequence holds stay as they
-        are, shared ones shared: trim(seq, start) first to be rid of them."""
-        src, dst = self._book().reserve(seq, start, stop)
-        if src:
-            copy_pages(self, src, dst, stream)
-        self._sync(seq, stream)
+        are, shared ones shared: trim(seq, start) first to be rid of them.
+
+        Here, in fork, trim and compact: where the copy to the device fails, the
+        book keeps the change, and the next of these calls copies first."""
+        self._owed = (*self._settle(stream).reserve(seq, start, stop), seq)
+        self._settle(stream)
 
     def fork(self, src: int, dst: int, keys: int, stream=None) -> None:
         """Sequence dst starts with src's first `keys` keys, their pages shared."""
-        self._book().fork(src, dst, keys)
-        self._sync(dst, stream)
+        self._settle(stream).fork(src, dst, keys)
+        self._owed = ([], [], dst)
+        self._settle(stream)
 
     def trim(self, seq: int, keys: int, stream=None) -> None:
         """Gives back the pages behind the sequence's first `keys` keys (0: all)."""
-        self._book().trim(seq, keys)
-        self._sync(seq, stream)
+        self._settle(stream).trim(seq, keys)
+        self._owed = ([], [], seq)
+        self._settle(stream)
 
     def compact(self, stream=None) -> int:
         """Moves the pages in use to the lowest numbers; how many moved."""
-        src, dst = self._book().compact()
+        src, dst = self._settle(stream).compact()
         if src:
-            copy_pages(self, src, dst, stream)
-            self._sync(None, stream)
+            self._owed = (src, dst, None)
+            self._settle(stream)
         return len(src)
 
 

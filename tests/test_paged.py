@@ -170,6 +170,67 @@ def test_a_rollback_after_a_fork():
     assert all("shared" in d for d in (P.PagedCache.reserve.__doc__, P.Book.reserve.__doc__))
 
 
+class HostCache(P.PagedCache):
+    """A cache whose device is lists: pages of the text they hold, the table, and
+    copies that fail when told to (some of a call's pairs done, as where one of
+    its launches fails)."""
+
+    def __init__(self, pages, seqs, monkeypatch):
+        self.book, self.data, self.fail = P.Book(pages, 16, seqs, 6), [None] * pages, 0
+        self.rows = self.book.table().tolist()
+        monkeypatch.setattr(P, "copy_pages", self.copied)
+
+    def copied(self, cache, src, dst, stream=None):
+        assert cache is self and not set(src) & set(dst)
+        for n, (a, b) in enumerate(zip(src, dst)):
+            if self.fail and n >= len(src) // 2:
+                raise RuntimeError("a launch failed")
+            self.data[b] = self.data[a]
+
+    def _sync(self, seq=None, stream=None):
+        if self.fail == 2:
+            raise RuntimeError("a copy failed")
+        t = self.book.table().tolist()
+        self.rows = t if seq is None else [t[s] if s == seq else r for s, r in enumerate(self.rows)]
+
+    def text(self, seq):
+        return [None if p < 0 else self.data[p] for p in self.rows[seq]]
+
+    def write(self, seq, what):
+        for p, w in zip(self.rows[seq], what):
+            self.data[p] = w
+
+
+@pytest.mark.parametrize("then", ["reserve", "fork", "trim", "compact"])
+@pytest.mark.parametrize("first", ["reserve", "compact", "trim", "fork"])
+def test_a_failed_copy_is_made_up_for(first, then, monkeypatch):
+    """The book has changed when a copy to the device fails.  Until the copy is
+    made the device keeps the table and pages of before; whatever is called next
+    makes it first."""
+    c = HostCache(12, 4, monkeypatch)
+    c.reserve(3, 0, 32)
+    c.reserve(0, 0, 40)
+    c.write(0, "abc")
+    c.fork(0, 1, 40)
+    c.trim(3, 0)  # pages 0 and 1 are free
+    before = [c.text(s) for s in range(4)]
+    c.fail = 2
+    with pytest.raises(RuntimeError):
+        {"reserve": lambda: c.reserve(1, 36, 50), "compact": c.compact,
+         "trim": lambda: c.trim(1, 0), "fork": lambda: c.fork(0, 2, 20)}[first]()
+    assert [c.text(s) for s in range(4)] == before
+    with pytest.raises(RuntimeError):  # and again: nothing more is given out
+        c.reserve(3, 0, 90)
+    assert [c.text(s) for s in range(4)] == before and c.book.held(3) == 0
+    c.fail = 0
+    {"reserve": lambda: c.reserve(3, 0, 16), "fork": lambda: c.fork(0, 3, 16),
+     "trim": lambda: c.trim(3, 0), "compact": c.compact}[then]()
+    assert c.rows == c.book.table().tolist()
+    assert c.text(0)[:3] == list("abc")
+    assert c.text(1)[:3] == ([None] * 3 if first == "trim" else list("abc"))
+    assert c.text(2)[:2] == (list("ab") if first == "fork" else [None] * 2)
+
+
 # ------------------------------------------------------------------- refusals
 
 def desc(**kw):
