@@ -81,8 +81,9 @@ exl3_verdict exl3p_tree_plan(const exl3p_cache *c, const exl3p_rows *r, const in
                              exl3_stream s);
 
 /* For each of `rows` rows with slot[t] >= 0: q's heads normalized (RMS over the
- * head, times q_norm[dim]; q_norm NULL: as they are), rotated at pos[t] (halves
- * i and i + dim / 2 by pos * theta^(-2 i / dim), the angle in 64 bits) to q_out;
+ * head and finite eps >= 0, times q_norm[dim]; q_norm NULL: as they are), rotated
+ * at pos[t] (halves i and i + dim / 2 by pos * theta^(-2 i / dim), the angle in 64
+ * bits) to q_out;
  * k's heads the same with k_norm into the cache's keys at slot[t]; v's copied
  * into its values.  One rounding, at the end.  q, k, v and q_out have row
  * strides (in elements, multiples of 8) and 16-byte bases; q_out may be q.  Two

@@ -1466,6 +1466,8 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
   if (pos == nullptr || slot == nullptr) return refuse(EXL3_FAILED, "PagedAppend: a missing array");
   if (!aligned(q_norm, 8) || !aligned(k_norm, 8))
     return refuse(EXL3_UNSUPPORTED, "PagedMatrixAlignment: norm weights on an 8-byte boundary");
+  if ((q_norm != nullptr || k_norm != nullptr) && !(eps >= 0.0f && eps < INFINITY))
+    return refuse(EXL3_UNSUPPORTED, "PagedEps: a norm's eps is finite and not below 0");
   Rates rates{};
   const double ratio = pow(theta, -2.0 / c->dim);
   double turn = 1.0 / 6.283185307179586476925287;

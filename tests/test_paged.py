@@ -384,6 +384,13 @@ def test_scales_past_32_bits_are_refused():
         assert "PagedScale" in entries(desc(), step(), scale=scale)["attend"]().reason
 
 
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf"), float("-inf")])
+def test_a_norm_refuses_an_eps_that_is_none(eps):
+    """Roots of numbers below 0, or of none."""
+    v = entries(desc(), step(), eps=eps, kn=64, q=1 << 24, out=1 << 25)["append"]()
+    assert v.code == X.UNSUPPORTED and "PagedEps" in v.reason, v
+
+
 def test_a_step_without_sequences_needs_no_lengths():
     e = entries(desc(), step(seqs=0, rows=0, max_rows=0, len=None), words=0, mask=None)
     for name in ("plan", "attend", "commit"):
