@@ -86,8 +86,11 @@ exl3_verdict exl3p_tree_plan(const exl3p_cache *c, const exl3p_rows *r, const in
  * bits) to q_out;
  * k's heads the same with k_norm into the cache's keys at slot[t]; v's copied
  * into its values.  One rounding, at the end.  q, k, v and q_out have row
- * strides (in elements, multiples of 8) and 16-byte bases; q_out may be q.  Two
- * rows of one slot: either's keys and values.  Fewer than 2^24 rows a call. */
+ * strides (in elements, multiples of 8) and 16-byte bases.  q_out may be q, rows
+ * of the same stride; apart from that what is written (q_out, the layer's pages)
+ * lies over nothing else that is read or written (slices of one matrix are fine).
+ * Two rows of one slot: its keys and values are pieces of either's.  Fewer than
+ * 2^24 rows a call. */
 exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows, int32_t heads,
                               const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                               const void *v, int64_t v_stride, const void *q_norm,

@@ -1351,6 +1351,48 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb) {
   return a != nullptr && b != nullptr && x < y + nb && y < x + na;
 }
 
+// Memory of a tensor: `rows` pieces of `width` bytes, `stride` apart (rows that
+// do not overlap one another).
+struct Span2D {
+  const void *p;
+  int64_t rows, width, stride;
+};
+Span2D array(const void *p, int64_t bytes) { return Span2D{p, bytes > 0, bytes, bytes}; }
+Span2D matrix(const void *p, int64_t stride, int64_t width, int64_t rows) {
+  return Span2D{p, rows, 2 * width, 2 * stride};
+}
+
+// Whether a byte lies in both: exact for slices of one matrix too, whose rows
+// interleave.
+bool meet(Span2D x, Span2D y) {
+  typedef __int128 wide;
+  if (x.p == nullptr || y.p == nullptr || x.rows <= 0 || y.rows <= 0) return false;
+  const wide d = (wide) reinterpret_cast<uintptr_t>(y.p) - reinterpret_cast<uintptr_t>(x.p);
+  auto end = [](const Span2D &v) { return (wide)(v.rows - 1) * v.stride + v.width; };
+  if (d >= end(x) || -d >= end(y)) return false;
+  // row i of x against the last row of y that begins before it ends
+  auto row = [&](int64_t i) {
+    const wide from = (wide)i * x.stride - d, last = from + x.width - 1;
+    if (last < 0) return false;
+    const wide j = last / y.stride < y.rows - 1 ? last / y.stride : y.rows - 1;
+    return j * y.stride + y.width > from;
+  };
+  if (x.rows > 1 && y.rows > 1 && x.stride == y.stride) {
+    // every row lies alike among the other's, but for where those begin and end:
+    // row i meets row i + k, k the number below or the one before it
+    wide k = x.width - 1 - d;
+    k = k >= 0 ? k / x.stride : -((-k + x.stride - 1) / x.stride);
+    for (int u = 0; u < 2; ++u, --k)
+      if (k > -x.rows && k < y.rows && d + k * x.stride < x.width && d + k * x.stride > -(wide)y.width)
+        return true;
+    return false;
+  }
+  if (x.rows > y.rows) return meet(y, x);
+  for (int64_t i = 0; i < x.rows; ++i)
+    if (row(i)) return true;
+  return false;
+}
+
 // The device's compute units, read once per device.
 int device_cus() {
   static std::atomic<int> cached[64];
@@ -1466,8 +1508,26 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
   if (pos == nullptr || slot == nullptr) return refuse(EXL3_FAILED, "PagedAppend: a missing array");
   if (!aligned(q_norm, 8) || !aligned(k_norm, 8))
     return refuse(EXL3_UNSUPPORTED, "PagedMatrixAlignment: norm weights on an 8-byte boundary");
+  // workgroups take rows and heads in any order: what one writes no other reads
+  const Span2D out = matrix(q_out, out_stride, wq, rows), in = matrix(q, q_stride, wq, rows);
+  const Span2D reads[] = {matrix(k, k_stride, wk, rows), matrix(v, v_stride, wk, rows),
+                          array(q_norm, c->dim * 2),     array(k_norm, c->dim * 2),
+                          array(pos, (int64_t)rows * 4), array(slot, (int64_t)rows * 4)};
+  const Pool pool = pool_of(c, layer);
+  const Span2D kv[] = {array(pool.k, layer_bytes(c)), array(pool.v, layer_bytes(c))};
+  if (!(q_out == q && (out_stride == q_stride || rows == 1)) && meet(out, in))
+    return refuse(EXL3_UNSUPPORTED, "PagedOverlap: q_out over q, and not q itself");
+  for (const Span2D &x : reads)
+    if (meet(out, x)) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: q_out over another input");
+  for (const Span2D &y : kv) {
+    if (meet(out, y) || meet(in, y))
+      return refuse(EXL3_UNSUPPORTED, "PagedOverlap: q or q_out over the layer's pages");
+    for (const Span2D &x : reads)
+      if (meet(x, y)) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: an input over the layer's pages");
+  }
   if ((q_norm != nullptr || k_norm != nullptr) && !(eps >= 0.0f && eps < INFINITY))
     return refuse(EXL3_UNSUPPORTED, "PagedEps: a norm's eps is finite and not below 0");
+  if (meet(kv[0], kv[1])) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: keys over values");
   Rates rates{};
   const double ratio = pow(theta, -2.0 / c->dim);
   double turn = 1.0 / 6.283185307179586476925287;

@@ -391,6 +391,75 @@ def test_a_norm_refuses_an_eps_that_is_none(eps):
     assert v.code == X.UNSUPPORTED and "PagedEps" in v.reason, v
 
 
+# ------------------------------------------------- memory that two tensors share
+
+def bytes_of(base, rows, width, stride):
+    """The bytes of a matrix, in units of 16 (all sizes here are multiples)."""
+    return {(base + r * stride + x) // 16 for r in range(rows) for x in range(0, width, 16)}
+
+
+def append_on(rows, heads, kv, q, qs, k, ks, v, vs, out, os_, **kw):
+    """The append of matrices at these addresses (strides in elements) of a cache
+    far from them.  Its eps is refused last, so nothing is ever launched."""
+    a = dict(rows=rows, layer=0, pos=1 << 40, slot=1 << 41, kn=1 << 42, qn=None, eps=-1.0)
+    a.update(kw)
+    c = ctypes.byref(desc(kv_heads=kv, dim=64, k=1 << 43, v=1 << 44))
+    return P.paged_lib().exl3p_qkv_append(c, a["layer"], rows, heads, q, qs, k, ks, v, vs, a["qn"],
+                                          a["kn"], a["pos"], a["slot"], out, os_, a["eps"], 1e4, None)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_append_refuses_what_lies_over_its_output(seed):
+    """Random matrices in a small space, slices of common rows and others: refused
+    just where q_out shares a byte with k, v or, unless it is q itself, q."""
+    rng = random.Random(seed)
+    seen = {True: 0, False: 0}
+    for _ in range(1500):
+        rows, kv, group = rng.choice([1, 1, 2, 3, 5, 9]), rng.choice([1, 2]), rng.choice([1, 2])
+        wide = {"q": 64 * kv * group, "k": 64 * kv, "v": 64 * kv, "out": 64 * kv * group}
+        common = rng.choice([256, 384, 512, 640, 1024])
+        at = {}
+        for x, w in wide.items():
+            stride = max(w, common if rng.random() < 0.7 else w + 8 * rng.randint(0, 40))
+            at[x] = (1 << 20) + 16 * rng.randint(0, rng.choice([100, 2000])), stride
+        if rng.random() < 0.3:
+            at["out"] = at["q"]
+        mem = {x: bytes_of(b, rows, 2 * wide[x], 2 * s) for x, (b, s) in at.items()}
+        same = at["out"][0] == at["q"][0] and (at["out"][1] == at["q"][1] or rows == 1)
+        want = bool(mem["out"] & (mem["k"] | mem["v"] | (set() if same else mem["q"])))
+        seen[want] += 1
+        v = append_on(rows, kv * group, kv, *at["q"], *at["k"], *at["v"], *at["out"])
+        assert v.code == X.UNSUPPORTED
+        assert ("PagedOverlap" if want else "PagedEps") in v.reason, (rows, at, v)
+    assert min(seen.values()) > 100
+
+
+@pytest.mark.parametrize("kw", [
+    dict(pos=1 << 20), dict(pos=(1 << 20) + 3 * 2048 + 1024 - 4), dict(slot=(1 << 20) + 64),
+    dict(kn=(1 << 20) + 8), dict(qn=(1 << 20) + 1024 * 2 + 8), dict(pos=(1 << 43) + 8),
+    dict(slot=(1 << 44) - 4), dict(qn=1 << 43), dict(q=1 << 43), dict(k=(1 << 44) + 4096),
+    dict(v=(1 << 43) - 16), dict(out=(1 << 44) + 16), dict(v=(1 << 44) + 8 * 2 * 16 * 64 * 2 - 16)])
+def test_append_refuses_what_lies_over_its_other_memory(kw):
+    """Positions, slots and weights under q_out; anything under the pages that the
+    layer's keys and values go to."""
+    a = dict(q=1 << 30, k=1 << 31, v=1 << 32, out=1 << 20)
+    args = dict(rows=4, heads=8, kv=2, qs=1024, ks=256, vs=256, os_=1024)
+    assert "PagedEps" in append_on(**a, **args).reason
+    for x in a:
+        if x in kw:
+            a[x] = kw.pop(x)
+    v = append_on(**a, **args, **kw)
+    assert v.code == X.UNSUPPORTED and "PagedOverlap" in v.reason, v
+
+
+def test_append_refuses_keys_over_values():
+    for v in (1 << 30, (1 << 30) + 8 * 2 * 16 * 64 * 2 - 16):  # the layer's last bytes
+        c = ctypes.byref(desc(dim=64, k=1 << 30, v=v))
+        v = P.paged_lib().exl3p_qkv_append(c, 0, 4, 8, 1 << 20, 512, 1 << 21, 256, 1 << 22, 256, None,
+                                           None, 64, 1 << 19, 1 << 23, 512, 0.0, 1e4, None)
+        assert v.code == X.UNSUPPORTED and "keys over values" in v.reason, v
+
+
 def test_a_step_without_sequences_needs_no_lengths():
     e = entries(desc(), step(seqs=0, rows=0, max_rows=0, len=None), words=0, mask=None)
     for name in ("plan", "attend", "commit"):
