@@ -75,7 +75,8 @@ typedef struct exl3p_rows {
  * i or an ancestor of i.  parent[t] is the index of a row's parent among its
  * sequence's rows, -1 for a root; one that does not lie before its row counts
  * as -1.  parent NULL: each row follows the one before it (a prompt).  mask may
- * be NULL (words then 0); words * 64 >= max_rows otherwise. */
+ * be NULL (words then 0); words * 64 >= max_rows otherwise.  No output lies over
+ * another, or over parent, cu, len or the table. */
 exl3_verdict exl3p_tree_plan(const exl3p_cache *c, const exl3p_rows *r, const int32_t *parent,
                              int32_t *pos, int32_t *slot, uint64_t *mask, int32_t words,
                              exl3_stream s);

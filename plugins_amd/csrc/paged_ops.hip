@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <new>
 #include <type_traits>
 
@@ -1393,6 +1394,19 @@ bool meet(Span2D x, Span2D y) {
   return false;
 }
 
+// What a call writes lies over nothing that it reads and over nothing else that it
+// writes: workgroups come in any order.
+exl3_verdict check_apart(std::initializer_list<Span2D> writes, std::initializer_list<Span2D> reads) {
+  for (auto w = writes.begin(); w != writes.end(); ++w) {
+    for (const Span2D &x : reads)
+      if (meet(*w, x)) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: an output over an input");
+    for (auto x = writes.begin(); x != w; ++x)
+      if (meet(*w, *x)) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: an output over another");
+  }
+  return OK;
+}
+Span2D table_of(const exl3p_cache *c) { return array(c->table, (int64_t)c->seqs * c->max_pages * 4); }
+
 // The device's compute units, read once per device.
 int device_cus() {
   static std::atomic<int> cached[64];
@@ -1480,6 +1494,10 @@ exl3_verdict exl3p_tree_plan(const exl3p_cache *c, const exl3p_rows *r, const in
     return refuse(EXL3_TOO_LARGE, "PagedTree: over 1024 rows of a sequence");
   if (r->rows == 0) return OK;
   if (pos == nullptr || slot == nullptr) return refuse(EXL3_FAILED, "PagedPlan: a missing array");
+  const int64_t n = (int64_t)r->rows * 4;
+  EXL3P_TRY(check_apart({array(pos, n), array(slot, n), array(mask, 2 * n * words)},
+                        {array(r->cu, 4 * ((int64_t)r->seqs + 1)), array(r->len, 4 * (int64_t)r->seqs),
+                         array(parent, n), table_of(c)}));
   hipLaunchKernelGGL(tree_plan_kernel, dim3(r->seqs + 1), dim3(PLAN_THREADS), 0,
                      static_cast<hipStream_t>(s), pool_of(c, 0), step_of(r), parent, pos, slot, mask,
                      words);

@@ -460,6 +460,18 @@ def test_append_refuses_keys_over_values():
         assert v.code == X.UNSUPPORTED and "keys over values" in v.reason, v
 
 
+@pytest.mark.parametrize("kw", [
+    dict(pos=1 << 20), dict(slot=(1 << 20) + 20), dict(mask=(1 << 20) - 40), dict(pos=(1 << 21) + 8),
+    dict(slot=(1 << 22) - 20), dict(mask=(1 << 22) - 40), dict(pos=(1 << 23) + 3 * 4 * 4 - 4),
+    dict(mask=1 << 23), dict(slot=1 << 24), dict(mask=(1 << 24) + 16), dict(mask=(1 << 25) + 16)])
+def test_plan_refuses_outputs_over_anything(kw):
+    """One workgroup's positions or slots over another's tree, lengths or pages."""
+    a = dict(parent=1 << 20, pos=1 << 24, slot=1 << 25, mask=1 << 26)
+    a.update(kw)
+    v = entries(desc(table=1 << 23), step(cu=1 << 21, len=1 << 22), **a)["plan"]()
+    assert v.code == X.UNSUPPORTED and "PagedOverlap" in v.reason, v
+
+
 def test_a_step_without_sequences_needs_no_lengths():
     e = entries(desc(), step(seqs=0, rows=0, max_rows=0, len=None), words=0, mask=None)
     for name in ("plan", "attend", "commit"):
