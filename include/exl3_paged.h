@@ -120,7 +120,8 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
  * count [seqs], next [seqs] = target of the last accepted row (-1 for a
  * sequence without rows), new_len = len + count.  The accepted rows' keys and
  * values move to key numbers len, len + 1, ... in every layer.  No output lies over
- * an input (several workgroups read them): new_len is not r->len, next not ids.
+ * an input (several workgroups read them: new_len is not r->len, next not ids, and
+ * none is in the table), over another output or over the cache.
  * parent NULL: a chain.  At most EXL3P_TREE_MAX rows of a sequence. */
 exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32_t *parent,
                           const int32_t *ids, const int32_t *target, int32_t *path,

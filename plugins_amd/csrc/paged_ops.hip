@@ -1347,11 +1347,6 @@ exl3_verdict check_matrix(const void *p, int64_t stride, int64_t width) {
 // in 32 bits.
 constexpr int64_t GRID_MAX = ((int64_t)1 << 24) - 1;
 
-bool overlap(const void *a, size_t na, const void *b, size_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return a != nullptr && b != nullptr && x < y + nb && y < x + na;
-}
-
 // Memory of a tensor: `rows` pieces of `width` bytes, `stride` apart (rows that
 // do not overlap one another).
 struct Span2D {
@@ -1397,12 +1392,12 @@ bool meet(Span2D x, Span2D y) {
 // What a call writes lies over nothing that it reads and over nothing else that it
 // writes: workgroups come in any order.
 exl3_verdict check_apart(std::initializer_list<Span2D> writes, std::initializer_list<Span2D> reads) {
-  for (auto w = writes.begin(); w != writes.end(); ++w) {
+  for (const Span2D &w : writes)
     for (const Span2D &x : reads)
-      if (meet(*w, x)) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: an output over an input");
+      if (meet(w, x)) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: an output over an input");
+  for (auto w = writes.begin(); w != writes.end(); ++w)
     for (auto x = writes.begin(); x != w; ++x)
       if (meet(*w, *x)) return refuse(EXL3_UNSUPPORTED, "PagedOverlap: an output over another");
-  }
   return OK;
 }
 Span2D table_of(const exl3p_cache *c) { return array(c->table, (int64_t)c->seqs * c->max_pages * 4); }
@@ -1639,16 +1634,12 @@ exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32
     return refuse(EXL3_FAILED, "PagedCommit: a missing array");
   if (new_len == r->len) return refuse(EXL3_UNSUPPORTED, "PagedCommit: new_len over len itself");
   // every workgroup of a sequence walks its tree, whatever the others have written
-  const size_t w = sizeof(int32_t), n = (size_t)r->seqs * w, t = (size_t)r->rows * w;
-  const struct {
-    const void *p;
-    size_t n;
-  } in[] = {{r->cu, n + w}, {r->len, n}, {parent, t}, {ids, t}, {target, t}},
-    out[] = {{path, n * max_path}, {count, n}, {next, n}, {new_len, n}};
-  for (const auto &o : out)
-    for (const auto &i : in)
-      if (overlap(o.p, o.n, i.p, i.n))
-        return refuse(EXL3_UNSUPPORTED, "PagedCommit: an output over an input");
+  const int64_t n = (int64_t)r->seqs * 4, t = (int64_t)r->rows * 4;
+  const int64_t pool = (int64_t)layer_bytes(c) * c->layers;
+  EXL3P_TRY(check_apart({array(path, n * max_path), array(count, n), array(next, n),
+                         array(new_len, n), array(c->k, pool), array(c->v, pool)},
+                        {array(r->cu, n + 4), array(r->len, n), array(parent, t), array(ids, t),
+                         array(target, t), table_of(c)}));
   hipLaunchKernelGGL(commit_kernel, dim3(r->seqs, 2 * c->layers), dim3(256), 0,
                      static_cast<hipStream_t>(s), pool_of(c, 0), step_of(r), layer_bytes(c),
                      c->dim * 2, parent, ids, target, path, max_path, count, next, new_len);

@@ -472,6 +472,34 @@ def test_plan_refuses_outputs_over_anything(kw):
     assert v.code == X.UNSUPPORTED and "PagedOverlap" in v.reason, v
 
 
+def commit_on(c, r, **kw):
+    a = dict(parent=1 << 20, ids=2 << 20, target=3 << 20, path=4 << 20, count=5 << 20, next=6 << 20,
+             new_len=7 << 20)
+    a.update(kw)
+    return P.paged_lib().exl3p_commit(ctypes.byref(c), ctypes.byref(r), a["parent"], a["ids"],
+                                      a["target"], a["path"], 4, a["count"], a["next"], a["new_len"],
+                                      None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(next=5 << 20), dict(next=(5 << 20) + 4), dict(count=(4 << 20) + 2 * 4 * 4 - 4),
+    dict(new_len=(4 << 20) - 4), dict(new_len=6 << 20), dict(path=(9 << 20) + 8), dict(count=9 << 20),
+    dict(next=(9 << 20) + 3 * 4 * 4 - 4), dict(new_len=(9 << 20) - 4), dict(path=1 << 30),
+    dict(count=(1 << 31) + 4096), dict(next=(1 << 30) - 4), dict(ids=1 << 30), dict(target=1 << 31)])
+def test_commit_refuses_outputs_over_outputs_table_and_cache(kw):
+    """`next` in place of count, an output in the table that other workgroups look
+    pages up in, anything in the memory that the rows move in."""
+    c = desc(table=9 << 20, k=1 << 30, v=1 << 31)
+    v = commit_on(c, step(cu=10 << 20, len=11 << 20), **kw)
+    assert v.code == X.UNSUPPORTED and "PagedOverlap" in v.reason, v
+
+
+def test_commit_refuses_keys_over_values():
+    c = desc(table=9 << 20, k=1 << 30, v=(1 << 30) + 2 * 8 * 2 * 16 * 128 * 2 - 16)
+    v = commit_on(c, step(cu=10 << 20, len=11 << 20))
+    assert v.code == X.UNSUPPORTED and "PagedOverlap" in v.reason, v
+
+
 def test_a_step_without_sequences_needs_no_lengths():
     e = entries(desc(), step(seqs=0, rows=0, max_rows=0, len=None), words=0, mask=None)
     for name in ("plan", "attend", "commit"):
