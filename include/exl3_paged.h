@@ -106,6 +106,8 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
  * sees nothing is zeros; what a row does not see cannot touch it, NaN or not.
  * scratch: exl3p_attend_scratch_bytes() of the same device, written and read within
  * the call (calls that may overlap need their own).
+ * out may be q, rows of the same stride; apart from that out and the scratch lie
+ * over nothing that is read, nor over each other.
  * The sums' order goes by the sizes and lengths alone: results repeat. */
 size_t exl3p_attend_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int32_t heads);
 exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,

@@ -1592,8 +1592,19 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   if (scratch == nullptr || !aligned(scratch, 16) ||
       scratch_bytes < exl3p_attend_scratch_bytes(c, r, heads))
     return refuse(EXL3_FAILED, "PagedScratch: below exl3p_attend_scratch_bytes, or not aligned");
+  // a workgroup reads its pairs' q before it writes their out, the join writes when
+  // all have read: out may be q
+  const Span2D to = matrix(out, out_stride, wq, r->rows), from = matrix(q, q_stride, wq, r->rows),
+               held = array(scratch, (int64_t)exl3p_attend_scratch_bytes(c, r, heads));
+  const Pool pool = pool_of(c, layer);
+  EXL3P_TRY(check_apart({to, held}, {array(pool.k, layer_bytes(c)), array(pool.v, layer_bytes(c)),
+                                     array(mask, 8 * (int64_t)r->rows * words),
+                                     array(r->cu, 4 * ((int64_t)r->seqs + 1)),
+                                     array(r->len, 4 * (int64_t)r->seqs), table_of(c)}));
+  if (meet(held, from) || (!(out == q && (out_stride == q_stride || r->rows == 1)) && meet(to, from)))
+    return refuse(EXL3_UNSUPPORTED, "PagedOverlap: scratch over q, or out over q and not q itself");
   AttnArgs a;
-  a.pool = pool_of(c, layer), a.st = step_of(r), a.sl = sl;
+  a.pool = pool, a.st = step_of(r), a.sl = sl;
   a.q = static_cast<const uint16_t *>(q), a.qs = q_stride, a.mask = mask, a.words = words;
   // at least f32's smallest, so that a hidden key's -inf times it stays -inf
   a.scale = fmaxf(fabsf(scale) * 1.4426950408889634f, 1.17549435e-38f);

@@ -442,7 +442,7 @@ def qkv_append(cache, layer: int, q, k, v, q_norm, k_norm, pos, slot, q_out, eps
 def attend(cache, layer: int, rows, q, out=None, mask=None, scale: float | None = None,
            scratch=None, stream=None):
     """exl3p_attend: out [rows, heads * dim] = softmax(q k^T scale) v over the
-    cache's keys and, by their masks, the rows'.  scratch: a byte tensor of at
+    cache's keys and, by their masks, the rows'.  out may be q.  scratch: a byte tensor of at
     least attend_scratch_bytes() that no overlapping call uses (None: taken from
     torch's allocator for this call)."""
     torch = _torch

@@ -669,3 +669,50 @@ def test_attend_items_of_several_tiles(counts, lens, kv, splits):
     seen = [[list(range(i + 1)) for i in range(n)] for n in counts]
     want, tol = R.attention(q, k, v, table, cu, lens, seen, 64, group, 0.125)
     near(attended(k, v, table, counts, lens, q, None), want, tol, "items")
+
+
+@pytest.mark.parametrize("counts,lens,group", [
+    ([1, 1], [40, 3000], 4), ([6], [3000], 4), ([40, 3], [0, 20], 4), ([33, 7], [4000, 9], 8)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attend_in_place(counts, lens, group, dtype):
+    """out in place of q: tiles of few pairs and of many, whole and split, the bits
+    of a call with an output of its own; so with q a slice of a wider matrix."""
+    g, k, v, table, cu, q = batch(counts, lens, dtype, 2, group, 128, 64, 31)
+    want = attended(k, v, table, counts, lens, q, None)
+    cache = P.PagedCache.over(k.to(DEV), v.to(DEV), table.to(DEV))
+    rows, width = P.Rows.of(counts, lens, DEV), 2 * group * 128
+    wide = torch.full((cu[-1], width + 128), 3.0, dtype=dtype, device=DEV)
+    wide[:, :width] = q.view(cu[-1], -1).to(DEV)
+    for x in (q.to(DEV), wide[:, :width]):
+        assert P.attend(cache, 0, rows, x, x) is x
+        assert torch.equal(x.cpu().view(q.shape), want)
+    assert bool((wide[:, width:] == 3.0).all())
+
+
+def test_operators_refuse_what_would_race():
+    """Through the mirror: an output over an input, unless it is q itself."""
+    k = torch.zeros(1, 8, 2, 16, 64, dtype=torch.float16, device=DEV)
+    cache = P.PagedCache.over(k, k.clone(), torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2))
+    i32 = {"dtype": torch.int32, "device": DEV}
+    numbers = torch.tensor([0, 2, 4, 0, 3, 0], **i32)  # cu, len and more
+    rows = P.Rows(numbers[:3], numbers[3:5], 4, 2)
+    fused = torch.ones(5, 512, dtype=torch.float16, device=DEV)
+    q, kk, vv = fused[:4, :256], fused[:4, 256:384], fused[:4, 384:]
+    parent = torch.tensor([-1, 0, -1, 0], **i32)
+    pos, slot, _ = P.plan(cache, rows)
+    for out in (fused[1:, :256], fused[:4, 128:384], fused[:4, 256:]):
+        with pytest.raises(X.Exl3Error, match="PagedOverlap"):
+            P.qkv_append(cache, 0, q, kk, vv, None, None, pos, slot, out)
+    for out in (fused[1:, :256], fused[:4, 128:384]):
+        with pytest.raises(X.Exl3Error, match="PagedOverlap"):
+            P.attend(cache, 0, rows, q, out)
+    for p, s in ((parent, slot), (pos, pos), (numbers[2:], slot), (pos, numbers[:4])):
+        with pytest.raises(X.Exl3Error, match="PagedOverlap"):
+            P.tree_plan(cache, rows, parent, p, s)
+    one, two = torch.empty(2, 2, **i32), torch.empty(2, **i32)
+    with pytest.raises(X.Exl3Error, match="PagedOverlap"):
+        P.commit(cache, rows, parent, pos, slot, one, two, two, torch.empty(2, **i32))
+    # rows beside each other in one matrix are apart
+    P.qkv_append(cache, 0, q, kk, vv, None, None, pos, slot, q)
+    P.attend(cache, 0, rows, q, fused[:4, 256:])
+    torch.cuda.synchronize()

@@ -500,6 +500,29 @@ def test_commit_refuses_keys_over_values():
     assert v.code == X.UNSUPPORTED and "PagedOverlap" in v.reason, v
 
 
+@pytest.mark.parametrize("kw", [
+    dict(out=(1 << 20) + 16), dict(out=(1 << 20) + 1024), dict(os=1032), dict(out=(1 << 20) - 5 * 2048 - 16),
+    dict(out=(1 << 24) + 2048), dict(out=(1 << 25) - 16), dict(out=1 << 27), dict(out=(1 << 28) - 64),
+    dict(out=1 << 29), dict(out=1 << 30), dict(out=(1 << 31) + 8 * 2 * 16 * 128 * 2 - 16),
+    dict(scratch=1 << 20), dict(scratch=(1 << 20) + 5 * 2048), dict(scratch=1 << 27),
+    dict(scratch=(1 << 28)), dict(scratch=1 << 29), dict(scratch=1 << 26), dict(scratch=1 << 30),
+    dict(scratch=(1 << 31) + 4096)])
+def test_attend_refuses_outputs_over_anything(kw):
+    """An output over q at another place or stride than q's own, output or scratch
+    over masks, lengths, table or the layer's pages, or over each other."""
+    c = desc(table=1 << 29, k=1 << 30, v=1 << 31)
+    r = step(cu=1 << 27, len=1 << 28)
+    need = P.paged_lib().exl3p_attend_scratch_bytes(ctypes.byref(c), ctypes.byref(r), 8)
+    a = dict(q=1 << 20, out=1 << 20, qs=1024, os=1024, mask=1 << 26, words=1, scratch=(1 << 25) - need,
+             bytes=need)
+    a["scratch"] &= ~15
+    if kw.get("out") == (1 << 24) + 2048:
+        a["mask"] = 1 << 24 | 4096
+    a.update(kw)
+    v = entries(c, r, **a)["attend"]()
+    assert v.code == X.UNSUPPORTED and "PagedOverlap" in v.reason, v
+
+
 def test_a_step_without_sequences_needs_no_lengths():
     e = entries(desc(), step(seqs=0, rows=0, max_rows=0, len=None), words=0, mask=None)
     for name in ("plan", "attend", "commit"):
