@@ -321,6 +321,10 @@ class PagedDecoder:
         T = rows.rows
         P._ints(ids, "ids", cache, T)  # embed reads as many as there are rows
         f16 = {"dtype": torch.float16, "device": ids.device}
+        if T == 0:
+            if only is not None and only.numel() > 0:
+                raise IndexError("only: the step has no rows")
+            return torch.empty(0, c.vocab, **f16)
         h = torch.empty(T, c.hidden, dtype=torch.float32, device=ids.device)
         x, att = torch.empty(T, c.hidden, **f16), torch.empty(T, c.q_dim, **f16)
         pos, slot, mask = P.plan(cache, rows, parent)

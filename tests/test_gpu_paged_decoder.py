@@ -179,3 +179,20 @@ def test_padding_rows_may_hold_any_id(model, fill):
         ids[4] = odd
         got.append(d.forward(rows, ids)[:6].clone())
     assert torch.isfinite(got[0].float()).all() and torch.equal(*got)
+
+
+@pytest.mark.parametrize("seqs", [0, 2])
+def test_steps_without_rows(model, seqs):
+    """Nothing drafted and nothing prompted: no logits, nothing accepted, lengths
+    as they were."""
+    d = paged(model)
+    rows, ids = P.Rows.of([0] * seqs, [5] * seqs, DEV), tokens(0, 1)
+    none = torch.empty(0, dtype=torch.int64, device=DEV)
+    for only in (None, none):
+        assert d.forward(rows, ids, only=only).shape == (0, CFG.vocab)
+    with pytest.raises(IndexError):
+        d.forward(rows, ids, only=torch.zeros(1, dtype=torch.int64, device=DEV))
+    path, count, after, new_len = d.verify(rows, ids, ids)
+    assert path.tolist() == [[-1]] * seqs and count.tolist() == [0] * seqs
+    assert after.tolist() == [-1] * seqs and new_len.tolist() == [5] * seqs
+    torch.cuda.synchronize()
