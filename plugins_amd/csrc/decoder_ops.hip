@@ -656,12 +656,16 @@ extern "C" {
 
 int exl3d_embed(const int32_t *ids, int B, const uint16_t *table, int H, float *h, float *ssq,
                 hipStream_t s) {
-  if (B <= 0 || H <= 0 || B > 65535) return hipErrorInvalidValue;
-  if (ssq != nullptr) {
-    if (H % 128 != 0) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(embed_ssq_kernel, dim3(H / 128, B), dim3(64), 0, s, ids, table, H, h, ssq);
-  } else {
-    hipLaunchKernelGGL(embed_kernel, dim3((H + 255) / 256, B), dim3(256), 0, s, ids, table, H, h);
+  if (B <= 0 || H <= 0 || (ssq != nullptr && H % 128 != 0)) return hipErrorInvalidValue;
+  // a row a workgroup in y, where a grid has 65535
+  for (int64_t b = 0; b < B; b += 65535) {
+    const unsigned n = B - b < 65535 ? (unsigned)(B - b) : 65535u;
+    if (ssq != nullptr)
+      hipLaunchKernelGGL(embed_ssq_kernel, dim3(H / 128, n), dim3(64), 0, s, ids + b, table, H,
+                         h + b * H, ssq + b * (H / 128));
+    else
+      hipLaunchKernelGGL(embed_kernel, dim3((H + 255) / 256, n), dim3(256), 0, s, ids + b, table, H,
+                         h + b * H);
   }
   return hipGetLastError();
 }

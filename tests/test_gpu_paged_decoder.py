@@ -196,3 +196,29 @@ def test_steps_without_rows(model, seqs):
     assert path.tolist() == [[-1]] * seqs and count.tolist() == [0] * seqs
     assert after.tolist() == [-1] * seqs and new_len.tolist() == [5] * seqs
     torch.cuda.synchronize()
+
+
+def test_more_rows_than_a_grid_has_in_one_dimension(model):
+    """Prompts of 65600 rows in one step: the embedding of every row, and the last
+    prompt's logits as of the same prompt alone (f16 roundings in other places)."""
+    n = [30000, 35000, 600]
+    ids = tokens(sum(n), 40)
+    h = torch.empty(sum(n), CFG.hidden, device=DEV)
+    Q.embed(ids, model.embed_table, h)
+    assert torch.equal(h, model.embed_table[ids.long()].float())
+    ssq = torch.empty(sum(n), CFG.hidden // 128, device=DEV)
+    h.zero_()
+    Q.embed(ids, model.embed_table, h, ssq)
+    assert torch.equal(h, model.embed_table[ids.long()].float())
+    # a sum of 128 squares in 32 bits, in any order: 128 roundings of it at most
+    want = h.double().view(sum(n), -1, 128).pow(2).sum(-1)
+    assert bool(((ssq.double() - want).abs() <= 128 * 2.0 ** -24 * want).all())
+    d = paged(model, 3, 262, 140, 256)
+    for s, m in enumerate(n):
+        d.cache.reserve(s, 0, m)
+    last = torch.arange(65000, 65600, device=DEV)
+    got = d.forward(P.Rows.of(n, [0] * 3, DEV), ids, only=last)
+    d.cache.trim(2, 0)
+    d.cache.reserve(2, 0, 600)
+    alone = d.forward(P.Rows.of([0, 0, 600], [0] * 3, DEV), ids[65000:])
+    assert rel(got, alone) < 1e-2
