@@ -67,6 +67,12 @@ struct BF16 {
 // A row's reference for its weights follows its running maximum only in steps of
 // more than SLACK (powers of two): what has been summed is rarely scaled again.
 constexpr float SLACK = 4.0f;
+// Up to a reference of FAR a weight's exponent is one multiply-add of score, scale
+// and (LIFT - reference).  Beyond, the product's rounding that the reference has
+// and the sum has not, and the sum's own, are whole powers of two (at 2^20 they
+// are 2^-4 of one): such a wave multiplies its scores first, and what is far is
+// not lifted.
+constexpr float FAR = 0x1p20f;
 
 template <typename E>
 __device__ __forceinline__ float to_f32(uint32_t bits) {
@@ -463,9 +469,13 @@ constexpr int FEW = 32;    // the most pairs of a tile of attend_few (16 or 32),
 constexpr int MANY = 128;  // a tile of attend_many's
 
 // A wave's softmax over the keys it has seen: the reference of each pair's
-// weights and the sum of them.
+// weights, the sum of them and their lift: 2^(score * scale + lift - reference).
 struct Soft {
-  float ref, sum;
+  float ref, sum, lift;
+  // from some pair's first far reference on: the wave's scores are multiplied by
+  // AttnArgs' scale before all else, and scale is 1
+  bool far;
+  float scale;
 };
 
 // The larger, NaN if either is: without the canonicalizing instructions that
@@ -474,14 +484,24 @@ __device__ __forceinline__ float larger(float a, float b) {
   return __builtin_elementwise_maximum(a, b);
 }
 
-// The running maximum `hi` (already times the scale) of each lane's pair joins
+// The running maximum `hi` (of scores times so.scale) of each lane's pair joins
 // its reference; the factor for what has been summed so far is 1 (false) unless
-// some pair of the wave outgrew its reference by more than SLACK.
-__device__ __forceinline__ bool outgrown(Soft &so, float hi, float &alpha) {
-  if (__ballot(hi > so.ref + SLACK) == 0) return false;
+// some pair of the wave outgrew its reference by more than SLACK.  turned: the
+// wave's first far reference (-inf, nothing seen, is none).
+template <typename E>
+__device__ __forceinline__ bool outgrown(Soft &so, float hi, float &alpha, bool &turned) {
+  turned = false;
+  if (__ballot(hi - so.ref > SLACK) == 0) return false;
   const float now = fmaxf(so.ref, hi);
   alpha = __builtin_amdgcn_exp2f(so.ref - (now == -INFINITY ? 0.0f : now));
   so.ref = now;
+  turned = !so.far && __ballot(fabsf(now) > FAR && now != -INFINITY) != 0;
+  if (turned) so.far = true, so.scale = 1.0f;
+  if (so.far && E::LIFT > 0.0f) {
+    const float to = fabsf(now) > FAR ? 0.0f : E::LIFT;
+    alpha *= __builtin_amdgcn_exp2f(to - so.lift);
+    so.lift = to;
+  }
   so.sum *= alpha;
   return true;
 }
@@ -613,7 +633,7 @@ __global__ __launch_bounds__(64 * AW, NT == 1 ? 3 : 2) void attend_few_kernel(At
   Soft sf[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    sf[n] = Soft{-INFINITY, 0.0f};
+    sf[n] = Soft{-INFINITY, 0.0f, E::LIFT, false, a.scale};
 #pragma unroll
     for (int m = 0; m < VH; ++m) acc[n][m] = f32x4{0, 0, 0, 0};
   }
@@ -669,21 +689,24 @@ __global__ __launch_bounds__(64 * AW, NT == 1 ? 3 : 2) void attend_few_kernel(At
     u32x4 pw[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      if (sf[n].far) s2[n][0] *= a.scale, s2[n][1] *= a.scale;
       float hi = larger(s2[n][0][0], s2[n][0][1]);
 #pragma unroll
       for (int e = 2; e < 8; ++e) hi = larger(hi, s2[n][e >> 2][e & 3]);
       hi = larger(hi, exl3::xor_lanes(hi, 16));
       hi = larger(hi, exl3::xor_lanes(hi, 32));
       float alpha;
-      if (outgrown(sf[n], hi * a.scale, alpha)) {
+      bool turned;
+      if (outgrown<E>(sf[n], hi * sf[n].scale, alpha, turned)) {
+        if (turned) s2[n][0] *= a.scale, s2[n][1] *= a.scale;
 #pragma unroll
         for (int m = 0; m < VH; ++m) acc[n][m] = acc[n][m] * alpha;
       }
-      const float by = E::LIFT - (sf[n].ref == -INFINITY ? 0.0f : sf[n].ref);
+      const float by = sf[n].lift - (sf[n].ref == -INFINITY ? 0.0f : sf[n].ref);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float(&x)[2] = {fmaf(s2[n][e >> 2][e & 3], a.scale, by),
-                              fmaf(s2[n][e >> 2][(e & 3) + 1], a.scale, by)};
+        const float(&x)[2] = {fmaf(s2[n][e >> 2][e & 3], sf[n].scale, by),
+                              fmaf(s2[n][e >> 2][(e & 3) + 1], sf[n].scale, by)};
         pw[n][e >> 1] = pack2<E>(__builtin_amdgcn_exp2f(x[0]), __builtin_amdgcn_exp2f(x[1]));
         // the sum of the rounded weights: they add up to one after the division
         sf[n].sum = E::add2(pw[n][e >> 1], sf[n].sum);
@@ -729,6 +752,12 @@ __global__ __launch_bounds__(64 * AW, NT == 1 ? 3 : 2) void attend_few_kernel(At
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (n > 0) __syncthreads();
+    if (sf[n].far) {  // lifted as all other sums are
+      const float by = __builtin_amdgcn_exp2f(E::LIFT - sf[n].lift);
+      sf[n].sum *= by;
+#pragma unroll
+      for (int m = 0; m < VH; ++m) acc[n][m] = acc[n][m] * by;
+    }
     float sum = sf[n].sum;
     sum += exl3::xor_lanes(sum, 16);
     sum += exl3::xor_lanes(sum, 32);
@@ -877,7 +906,7 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
-  Soft sf{-INFINITY, 0.0f};
+  Soft sf{-INFINITY, 0.0f, E::LIFT, false, a.scale};
 
   auto turn = [&](int step, auto TAIL) {
     constexpr bool tail = decltype(TAIL)::value;
@@ -906,25 +935,38 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
         for (int r = 0; r < 16; ++r)
           if (!((uint32_t)(my >> (32 * b)) >> (8 * (r >> 2) + (r & 3)) & 1)) s[b][r] = -INFINITY;
     }
+    if (sf.far) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] *= a.scale;
+    }
     float hi = larger(s[0][0], s[1][0]);
 #pragma unroll
     for (int r = 1; r < 16; ++r) hi = larger(larger(hi, s[0][r]), s[1][r]);
     hi = larger(hi, exl3::xor_lanes(hi, 32));
     float alpha;
-    if (outgrown(sf, hi * a.scale, alpha)) {
+    bool turned;
+    if (outgrown<E>(sf, hi * sf.scale, alpha, turned)) {
+      if (turned) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[b][r] *= a.scale;
+      }
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
     }
-    const float by = E::LIFT - (sf.ref == -INFINITY ? 0.0f : sf.ref);
+    const float by = sf.lift - (sf.ref == -INFINITY ? 0.0f : sf.ref);
     u32x4 pw[4];  // of 16 keys each
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
-        const uint32_t x = pack2<E>(__builtin_amdgcn_exp2f(fmaf(s[b][r], a.scale, by)),
-                                    __builtin_amdgcn_exp2f(fmaf(s[b][r + 1], a.scale, by)));
+        const uint32_t x = pack2<E>(__builtin_amdgcn_exp2f(fmaf(s[b][r], sf.scale, by)),
+                                    __builtin_amdgcn_exp2f(fmaf(s[b][r + 1], sf.scale, by)));
         pw[2 * b + (r >> 3)][(r & 7) >> 1] = x;
         sf.sum = E::add2(x, sf.sum);
       }
@@ -1014,6 +1056,14 @@ __global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
   __syncthreads();
   if (bad) sbad = 1;
   __syncthreads();
+  if (sf.far) {  // lifted as all other sums are
+    const float by = __builtin_amdgcn_exp2f(E::LIFT - sf.lift);
+    sf.sum *= by;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= by;
+  }
   float l = sf.sum;
   l += exl3::xor_lanes(l, 32);
   if (sbad) l = __builtin_nanf("");

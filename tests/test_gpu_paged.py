@@ -716,3 +716,56 @@ def test_operators_refuse_what_would_race():
     P.qkv_append(cache, 0, q, kk, vv, None, None, pos, slot, q)
     P.attend(cache, 0, rows, q, fused[:4, 256:])
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [2.0 ** 17, 3e7, 1e9, -1e9, 1e30, -1e30])
+@pytest.mark.parametrize("rows,ctx", [(1, 50), (1, 5000), (40, 50), (40, 5000)])
+def test_attend_scales_that_make_scores_huge(rows, ctx, scale, dtype):
+    """Scores far past 2^24, exact in 32 bits and apart by far more than their
+    roundings: a row is the value of its one largest key, or the mean of the two
+    that tie for it, and never NaN or zeros.  The tie lies in two places of the
+    context, so in two waves and, where it is long, two items."""
+    page, dim, group = 16, 64, 4
+    g, k, v, table, cu, q = batch([rows], [ctx], dtype, 2, group, dim, page, 51)
+    q = torch.ones_like(q)
+    pg, at = R.slots(table, 0, page, ctx + rows)
+    # scores m / 16 of whole m, 64 products of 2^-10 m each
+    m = torch.randint(-100, 100, (ctx + rows,), generator=g)
+    top = 120 if scale > 0 else -120
+    one, two = ctx // 3, ctx - 9
+    m[one] = m[two] = top
+    k[0, pg, :, at] = (m.double() / 1024).to(dtype)[:, None, None].expand(-1, 2, dim)
+    got = attended(k, v, table, [rows], [ctx], q, None, scale=scale)
+    # equal weights of exactly 1: the sum of two values and its half round once, in
+    # 32 bits, before the output's rounding
+    want = (v[0, pg[one], :, at[one]].float() + v[0, pg[two], :, at[two]].float()) / 2
+    want = want.to(dtype)[None, :, None].expand(rows, 2, group, dim).reshape(q.shape)
+    assert torch.equal(got, want)
+    # the same behind the rows' own keys: the last row alone sees the largest
+    m[-1] = 2 * top
+    k[0, pg, :, at] = (m.double() / 1024).to(dtype)[:, None, None].expand(-1, 2, dim)
+    got = attended(k, v, table, [rows], [ctx], q, None, scale=scale)
+    assert torch.equal(got[:-1], want[:-1])
+    last = v[0, pg[-1], :, at[-1]][:, None].expand(2, group, dim).reshape(-1, dim)
+    assert torch.equal(got[-1], last)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,gap", [(2, 14.5), (2, 18.5), (40, 14.5), (40, 18.5)])
+def test_attend_small_weights_beside_a_huge_row(dtype, rows, gap):
+    """As test_attend_many_small_weights, every second row's scores past 2^20: the
+    rows between them keep what only counts together."""
+    n_ctx = 20000
+    counts, lens = [rows], [n_ctx]
+    g, k, v, table, cu, q = batch(counts, lens, dtype, 1, 1, 64, 256, 8)
+    v, q, k = v.abs(), torch.ones_like(q), torch.zeros_like(k)
+    q[1::2] = 60000
+    pg, row = R.slots(table, 0, 256, n_ctx + rows)
+    k[0, pg[123], :, row[123]] = gap / 64
+    v[0, pg[123], :, row[123]] = 0
+    seen = [[list(range(i + 1)) for i in range(rows)]]
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, 256, 1, 1.0)
+    got = attended(k, v, table, counts, lens, q, None, scale=1.0)
+    near(got[::2], want[::2], tol[::2], "small weights")
+    assert not got[1::2].any()
