@@ -279,6 +279,7 @@ class Rows:
 
     def __init__(self, cu, len, rows: int, max_rows: int):
         torch = _t()
+        _c_int(rows), _c_int(max_rows)
         if cu.dtype != torch.int32 or len.dtype != torch.int32:
             raise TypeError("cu and len are int32")
         if cu.dim() != 1 or len.dim() != 1 or cu.numel() != len.numel() + 1 or cu.device != len.device:
@@ -434,8 +435,8 @@ def qkv_append(cache, layer: int, q, k, v, q_norm, k_norm, pos, slot, q_out, eps
                               w.numel() != dim or not w.is_contiguous()):
             raise ValueError(f"a norm's weights are [{dim}], of the cache's type and device")
         norms.append(None if w is None else w.data_ptr())
-    _call(cache, paged_lib().exl3p_qkv_append, "qkv_append", cache._ref, layer, n, heads, qp, qs, kp,
-          ks, vp, vs, norms[0], norms[1], _ints(pos, "pos", cache, n),
+    _call(cache, paged_lib().exl3p_qkv_append, "qkv_append", cache._ref, _c_int(layer), n,
+          heads, qp, qs, kp, ks, vp, vs, norms[0], norms[1], _ints(pos, "pos", cache, n),
           _ints(slot, "slot", cache, n), op, os_, eps, theta, _stream(cache, stream))
 
 
@@ -465,9 +466,9 @@ def attend(cache, layer: int, rows, q, out=None, mask=None, scale: float | None 
                 scratch = torch.empty(need, dtype=torch.uint8, device=cache.device)
     elif scratch.get_device() != cache.index or not scratch.is_contiguous():
         raise ValueError(f"scratch is dense, on {cache.device}")
-    _call(cache, L.exl3p_attend, "attend", cache._ref, layer, rows._ref, heads, qp, qs, mp, words,
-          1.0 / math.sqrt(dim) if scale is None else scale, op, os_, scratch.data_ptr(),
-          scratch.numel() * scratch.element_size(), _stream(cache, stream))
+    _call(cache, L.exl3p_attend, "attend", cache._ref, _c_int(layer), rows._ref, heads,
+          qp, qs, mp, words, 1.0 / math.sqrt(dim) if scale is None else scale, op, os_,
+          scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream(cache, stream))
     return out
 
 

@@ -391,6 +391,26 @@ def test_a_norm_refuses_an_eps_that_is_none(eps):
     assert v.code == X.UNSUPPORTED and "PagedEps" in v.reason, v
 
 
+def test_operators_take_no_number_for_another():
+    """Layer 2^32 is not layer 0, 2^32 + 1 rows are not one."""
+    import types
+    torch = pytest.importorskip("torch")
+    P._t()
+    i = torch.zeros(2, dtype=torch.int32)
+    for rows, most in ((1 << 32, 1), (1, (1 << 32) + 1), (-(1 << 32), 0)):
+        with pytest.raises(OverflowError):
+            P.Rows(i, i[:1], rows, most)
+    c = types.SimpleNamespace(index=-1, device="cpu", dtype=torch.float16, head_dim=64, kv_heads=1,
+                              _ref=None)
+    r = types.SimpleNamespace(rows=2, max_rows=2, seqs=1, index=-1, _ref=None)
+    x, b = torch.zeros(2, 64, dtype=torch.float16), torch.zeros(64, dtype=torch.uint8)
+    for layer in (1 << 32, 1 << 31, -(1 << 32) - 1):
+        with pytest.raises(OverflowError):
+            P.qkv_append(c, layer, x, x, x, None, None, i, i, x)
+        with pytest.raises(OverflowError):
+            P.attend(c, layer, r, x, x, scratch=b)
+
+
 # ------------------------------------------------- memory that two tensors share
 
 def bytes_of(base, rows, width, stride):
