@@ -136,10 +136,15 @@ class Book:
                            room=self.pages if room is None else room)
 
     def table(self):
-        """A numpy view [seqs][max_pages] of the book's own table."""
+        """A numpy view [seqs][max_pages] of the book's own table, which keeps the
+        book open (but for close())."""
         import numpy as np
-        p = ctypes.cast(paged_lib().exl3p_book_table(self._b), POINTER(c_int32))
-        return np.ctypeslib.as_array(p, (self.seqs, self.max_pages))
+        p = paged_lib().exl3p_book_table(self._b)
+        if p is None:
+            raise ValueError("the book is closed")
+        t = (c_int32 * self.max_pages * self.seqs).from_address(p)
+        t.book = self
+        return np.ctypeslib.as_array(t)
 
     def free_pages(self) -> int:
         return paged_lib().exl3p_book_free_pages(self._b)

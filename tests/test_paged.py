@@ -170,6 +170,27 @@ def test_a_rollback_after_a_fork():
     assert all("shared" in d for d in (P.PagedCache.reserve.__doc__, P.Book.reserve.__doc__))
 
 
+def test_the_table_keeps_its_book():
+    """The view is of the book's memory: it lasts as long as any view does."""
+    import gc
+    import weakref
+    b = P.Book(4, 16, 2, 3)
+    b.reserve(0, 0, 20)
+    t, ref = b.table()[:1], weakref.ref(b)
+    del b
+    gc.collect()
+    assert ref() is not None and t.tolist() == [[0, 1, -1]]
+    ref().reserve(0, 20, 40)
+    assert t.tolist() == [[0, 1, 2]]
+    del t
+    gc.collect()
+    assert ref() is None
+    b = P.Book(4, 16, 2, 3)
+    b.close()
+    with pytest.raises(ValueError):
+        b.table()
+
+
 class HostCache(P.PagedCache):
     """A cache whose device is lists: pages of the text they hold, the table, and
     copies that fail when told to (some of a call's pairs done, as where one of
