@@ -320,6 +320,8 @@ class _on:
     def __init__(self, cache, stream):
         torch = _t()
         self.held = []
+        if stream is not None:
+            _stream(cache, stream)
         if cache.index != torch.cuda.current_device():
             self.held.append(torch.cuda.device(cache.index))
         if stream is not None:
@@ -363,6 +365,9 @@ def _ints(t, what: str, cache, n: int):
 
 def _stream(cache, stream):
     if stream is not None:
+        if stream.device_index != cache.index:
+            raise ValueError(f"the stream is on device {stream.device_index}, "
+                             f"the cache on {cache.device}")
         return stream.cuda_stream
     return _raw_stream(cache.index)
 

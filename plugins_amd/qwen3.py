@@ -316,7 +316,7 @@ class PagedDecoder:
         line)."""
         torch, P, m, c, cache = self.torch, self.P, self.m, self.cfg, self.cache
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with P._on(cache, stream):
                 return self.forward(rows, ids, parent, only)
         T = rows.rows
         P._ints(ids, "ids", cache, T)  # embed reads as many as there are rows
@@ -348,7 +348,7 @@ class PagedDecoder:
         them are the caller's to trim once the lengths are on the host."""
         torch, P = self.torch, self.P
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with P._on(self.cache, stream):
                 return self.verify(rows, ids, parent, most)
         target = self.forward(rows, ids, parent).float().argmax(-1).int()
         i32 = {"dtype": torch.int32, "device": ids.device}

@@ -606,3 +606,24 @@ def test_decoder_refuses_ids_that_are_not_one_a_row(make, why):
     for call in (d.forward, d.verify):
         with pytest.raises(why, match="ids"):
             call(rows, make(torch))
+
+
+def test_streams_of_other_devices_are_refused():
+    """A launch goes to the cache's device: another one's stream is none of its."""
+    import types
+    torch, d, rows = decoder_without_a_gpu()
+    other = types.SimpleNamespace(cuda_stream=5, device_index=1)
+    ids = torch.zeros(4, dtype=torch.int32)
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    c = d.cache
+    c.head_dim, c.kv_heads, c._ref, rows._ref = 64, 1, None, None
+    calls = (lambda s: P.plan(c, rows, stream=s), lambda s: P.copy_pages(c, [0], [1], stream=s),
+             lambda s: P.attend(c, 0, rows, x, x, scratch=x, stream=s),
+             lambda s: P.tree_plan(c, rows, None, ids, ids, stream=s),
+             lambda s: P.qkv_append(c, 0, x, x, x, None, None, ids, ids, x, stream=s),
+             lambda s: P.commit(c, rows, None, ids, ids, ids[:1][None], ids[:1], ids[:1], ids[:1],
+                                stream=s),
+             lambda s: d.forward(rows, ids, stream=s), lambda s: d.verify(rows, ids, stream=s))
+    for call in calls:
+        with pytest.raises(ValueError, match="the stream is on device 1"):
+            call(other)
