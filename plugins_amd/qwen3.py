@@ -320,6 +320,9 @@ class PagedDecoder:
                 return self.forward(rows, ids, parent, only)
         T = rows.rows
         P._ints(ids, "ids", cache, T)  # embed reads as many as there are rows
+        if cache.index != P._device():  # the linears and norms go to the current one
+            with torch.cuda.device(cache.index):
+                return self.forward(rows, ids, parent, only)
         f16 = {"dtype": torch.float16, "device": ids.device}
         if T == 0:
             if only is not None and only.numel() > 0:

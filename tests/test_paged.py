@@ -627,3 +627,31 @@ def test_streams_of_other_devices_are_refused():
     for call in calls:
         with pytest.raises(ValueError, match="the stream is on device 1"):
             call(other)
+
+
+def test_decoder_runs_on_its_caches_device(monkeypatch):
+    """With another device current, the whole step is done under the cache's: the
+    linears and norms go by the current one."""
+    torch, d, rows = decoder_without_a_gpu()
+    now = [1]
+
+    class guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            now.append(self.index)
+
+        def __exit__(self, *e):
+            now.pop()
+
+    def plan(*a):
+        raise StopIteration(now[-1])
+
+    monkeypatch.setattr(P, "_device", lambda: now[-1])
+    monkeypatch.setattr(P, "plan", plan)
+    monkeypatch.setattr(torch.cuda, "device", guard)
+    for call in (d.forward, d.verify):
+        with pytest.raises(StopIteration) as e:
+            call(rows, torch.zeros(4, dtype=torch.int32))
+        assert e.value.value == d.cache.index and now == [1]
