@@ -355,7 +355,7 @@ class PagedDecoder:
                 return self.verify(rows, ids, parent, most)
         target = self.forward(rows, ids, parent).float().argmax(-1).int()
         i32 = {"dtype": torch.int32, "device": ids.device}
-        path = torch.empty(rows.seqs, most or max(1, rows.max_rows), **i32)
+        path = torch.empty(rows.seqs, max(1, rows.max_rows) if most is None else most, **i32)
         count, after, new_len = (torch.empty(rows.seqs, **i32) for _ in range(3))
         P.commit(self.cache, rows, parent, ids, target, path, count, after, new_len)
         return path, count, after, new_len

@@ -5,6 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from plugins_amd import exl3 as X  # noqa: E402
 from plugins_amd import paged as P  # noqa: E402
 from plugins_amd import qwen3 as Q  # noqa: E402
 
@@ -222,3 +223,14 @@ def test_more_rows_than_a_grid_has_in_one_dimension(model):
     d.cache.reserve(2, 0, 600)
     alone = d.forward(P.Rows.of([0, 0, 600], [0] * 3, DEV), ids[65000:])
     assert rel(got, alone) < 1e-2
+
+
+def test_a_path_of_no_rows_is_refused(model):
+    """most=0 is no default; of 1 the certain token alone is accepted."""
+    d = paged(model)
+    d.cache.reserve(0, 0, 3)
+    rows, ids = P.Rows.of([3], [0], DEV), tokens(3, 50)
+    with pytest.raises(X.Exl3Error, match="PagedPath"):
+        d.verify(rows, ids, most=0)
+    path, count, _, new_len = d.verify(rows, ids, most=1)
+    assert path.tolist() == [[0]] and count.tolist() == [1] and new_len.tolist() == [1]
