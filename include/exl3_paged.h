@@ -30,7 +30,7 @@
  *    NaN rows, a row not moved;
  *  - cu must ascend from 0 to at most `rows`; rows behind cu[seqs], and a
  *    sequence's rows behind max_rows, get slot -1 and are left as they were by
- *    every other entry.
+ *    every other entry.  Where cu goes back, exl3p_attend writes no row.
  */
 #ifndef EXL3_PAGED_H
 #define EXL3_PAGED_H

@@ -98,16 +98,18 @@ struct Step {
 // The rows of a sequence, kept inside the step's tensors: first row, count.
 struct Span {
   int row, n, len;
-  bool bad;  // its keys do not fit its table
+  bool bad;   // its keys do not fit its table
+  bool back;  // cu goes back here: sequences may share rows, and have more than all
 };
 __device__ __forceinline__ Span span_of(const Step &st, int s, int64_t room) {
   const int a = min(max(st.cu[s], 0), st.rows);
-  const int b = min(max(st.cu[s + 1], a), st.rows);
+  const int to = min(max(st.cu[s + 1], 0), st.rows), b = max(to, a);
   Span sp;
   sp.row = a;
   sp.n = min(b - a, st.max_rows);
   sp.len = st.len[s];
   sp.bad = sp.len < 0 || (int64_t)sp.len + sp.n > room;
+  sp.back = to < a;
   if (sp.bad) sp.len = 0;
   return sp;
 }
@@ -333,8 +335,9 @@ __device__ __forceinline__ int scan(int v) {
 // than through LDS, with 64-bit divisions.)
 __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64_t room, int x) {
   const int lane = threadIdx.x & 63;
-  Span sp{0, 0, 0, false};
+  Span sp{0, 0, 0, false, false};
   float units = 0.0f, all = 0.0f, longest = 0.0f;
+  bool back = false;
   auto units_of = [](const Span &v) { return (uint32_t)(v.len + v.n + 63) >> 6; };
   for (int s = lane; s < st.seqs; s += 64) {
     sp = span_of(st, s, room);
@@ -342,7 +345,14 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
     units += t * (float)units_of(sp);
     all += t;
     longest = fmaxf(longest, t > 0.0f ? (float)units_of(sp) : 0.0f);
+    back |= sp.back;
   }
+  // The launch and the scratch are sized for no more rows than the step has: a
+  // step whose sequences share rows does nothing.
+  Work w;
+  w.s = -1;
+  w.total = 0;
+  if (__ballot(back) != 0) return w;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     units += exl3::xor_lanes(units, m);
@@ -372,8 +382,6 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
                              : ceilf(units * (1.0f + 0x1p-12f) / target);
   const uint32_t chunk = __builtin_amdgcn_readfirstlane(
       (int)fminf(fmaxf(chunk_of, least), (float)(1 << 25)));
-  Work w;
-  w.s = -1;
   int items = 0, tiles = 0;  // of the sequences before
   for (int s0 = 0; s0 < st.seqs; s0 += 64) {
     const int s = s0 + lane;
@@ -402,7 +410,7 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
       // four prompts of up to 300 rows over up to 4000 keys 62.8 against 60.5).
       const int j = (x - before) / n_t, u = (x - before) - j * n_t;
       w.s = s0 + l;
-      w.sp = Span{of(sp.row), of(sp.n), of(sp.len), (bool)of(sp.bad)};
+      w.sp = Span{of(sp.row), of(sp.n), of(sp.len), (bool)of(sp.bad), false};
       w.r0 = (n_t - 1 - u) << sl.tile;
       w.first = before + u * n_s;
       w.place = w.first + j;

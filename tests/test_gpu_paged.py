@@ -769,3 +769,34 @@ def test_attend_small_weights_beside_a_huge_row(dtype, rows, gap):
     got = attended(k, v, table, counts, lens, q, None, scale=1.0)
     near(got[::2], want[::2], tol[::2], "small weights")
     assert not got[1::2].any()
+
+
+@pytest.mark.parametrize("seqs,n,lens", [
+    (40, 300, [0] * 38 + [60000, 0]),  # more items than the launch has, the last ones split
+    (80, 8, [100, 0] * 40), (3, 5, [7, 7, 7])])
+def test_a_cu_that_goes_back_is_not_begun(seqs, n, lens):
+    """Sequences that share rows: the launch and the scratch are sized for the rows
+    that there are.  No row is written, and what lies around the scratch stays."""
+    page, kv, group, dim = 256, 8, 4, 64
+    pages = 240
+    table = torch.arange(pages, dtype=torch.int32).repeat(seqs, 1)
+    k = torch.zeros(1, pages, kv, page, dim, dtype=torch.float16, device=DEV)
+    cache = P.PagedCache.over(k, k.clone(), table.to(DEV))
+    cu = [0] + [n, 0] * (seqs // 2) + [n] * (seqs % 2)
+    rows = P.Rows(torch.tensor(cu, dtype=torch.int32, device=DEV),
+                  torch.tensor(lens, dtype=torch.int32, device=DEV), n, n)
+    q = torch.ones(n, kv * group * dim, dtype=torch.float16, device=DEV)
+    out = torch.full_like(q, 7.0)
+    need = P.attend_scratch_bytes(cache, rows, kv * group)
+    room = torch.full((need + 8192,), 85, dtype=torch.uint8, device=DEV)
+    scratch = room[4096:4096 + need]
+    for _ in range(2):
+        P.attend(cache, 0, rows, q, out, scratch=scratch)
+        torch.cuda.synchronize()
+        assert bool((out == 7.0).all())
+        assert bool((room[:4096] == 85).all()) and bool((room[4096 + need:] == 85).all())
+    # the same scratch, a step as it should be
+    rows.cu.copy_(torch.tensor([0] + [n] * seqs, dtype=torch.int32))
+    P.attend(cache, 0, rows, q, out, scratch=scratch)
+    torch.cuda.synchronize()
+    assert not out.any()

@@ -102,3 +102,13 @@ def test_items_of_the_largest_batches():
     check(1, 1, [1], [(1 << 30) - 1])
     check(2, 4, [1 << 20], [(1 << 30) - (1 << 20)])
     check(1, 8, [1] * 63 + [1024], [1 << 24] * 64)
+
+
+def test_sequences_that_share_rows_pass_the_bounds():
+    """Why a step whose cu goes back is not begun: 300 rows taken 20 times over
+    are more items than the launch has, and the joins of the last ones are never
+    filled in."""
+    sl = split_of(8, 4, 300, 40, 300)
+    for items, split in items_of(sl, [300, 0] * 20, [0] * 38 + [60000, 0]):
+        at = [i for i, x in enumerate(items) if x[0] == 38]
+        assert split > 0 and len(at) > 1 and at[0] >= sl["items"]
