@@ -105,7 +105,8 @@ exl3_verdict exl3p_qkv_append(const exl3p_cache *c, int32_t layer, int32_t rows,
  * h / (heads / kv_heads).  scale, and scale times log2(e), are finite.  A row that
  * sees nothing is zeros; what a row does not see cannot touch it, NaN or not.
  * scratch: exl3p_attend_scratch_bytes() of the same device, written and read within
- * the call (calls that may overlap need their own).
+ * the call (calls that may overlap need their own); its size goes by the device and
+ * the heads, a little by the sequences, and not by the rows once they are many.
  * out may be q, rows of the same stride; apart from that out and the scratch lie
  * over nothing that is read, nor over each other.
  * The sums' order goes by the sizes and lengths alone: results repeat. */

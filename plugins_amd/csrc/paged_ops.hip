@@ -282,9 +282,9 @@ struct Work {
   int s;       // -1: nothing
   int r0;      // first pair
   int k0, k1;
+  int splits;  // items of the tile; where there are several:
   int first;   // the place of the tile's first item in the scratch
   int place;   // of this one: items of a tile lie side by side
-  int splits;  // items of the tile
   int index;   // of the tile among those that are split
   int total;   // of those, where asked for
   Span sp;
@@ -382,7 +382,7 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
                              : ceilf(units * (1.0f + 0x1p-12f) / target);
   const uint32_t chunk = __builtin_amdgcn_readfirstlane(
       (int)fminf(fmaxf(chunk_of, least), (float)(1 << 25)));
-  int items = 0, tiles = 0;  // of the sequences before
+  int items = 0, tiles = 0, parts = 0;  // of the sequences before: all, and split ones'
   for (int s0 = 0; s0 < st.seqs; s0 += 64) {
     const int s = s0 + lane;
     int nt = 0, ns = 0;
@@ -396,8 +396,8 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
         each = (u + ns - 1) / ns;  // the last items may be empty
       }
     }
-    const int mi = nt * ns, mt = ns > 1 ? nt : 0;
-    const int it = scan(mi), ti = scan(mt);
+    const int mi = nt * ns, mt = ns > 1 ? nt : 0, mp = ns > 1 ? mi : 0;
+    const int it = scan(mi), ti = scan(mt), pi = scan(mp);
     const uint64_t past = __ballot(items + it > x);
     if (w.s < 0 && past != 0) {
       const int l = __builtin_ctzll(past);
@@ -412,7 +412,7 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
       w.s = s0 + l;
       w.sp = Span{of(sp.row), of(sp.n), of(sp.len), (bool)of(sp.bad), false};
       w.r0 = (n_t - 1 - u) << sl.tile;
-      w.first = before + u * n_s;
+      w.first = parts + of(pi - mp) + u * n_s;
       w.place = w.first + j;
       w.splits = n_s;
       w.index = tiles + of(ti - mt) + u;
@@ -423,6 +423,7 @@ __device__ __forceinline__ Work find_work(const Step &st, const Split &sl, int64
     }
     items += __builtin_amdgcn_readlane(it, 63);
     tiles += __builtin_amdgcn_readlane(ti, 63);
+    parts += __builtin_amdgcn_readlane(pi, 63);
   }
   w.total = tiles;
   return w;
@@ -442,8 +443,8 @@ struct AttnArgs {
   int64_t os;
   Joint *joint;  // [0].row: how many; [1 + i]: the split tiles
   int joints;    // that joint holds
-  float *part;   // [items * kv][tile][D] sums, then [items * kv][tile][2] (max, sum)
-  int slots;     // items * kv that part holds
+  float *part;   // [parts * kv][tile][D] sums, then [parts * kv][tile][2] (max, sum)
+  int slots;     // parts * kv that part holds: items of split tiles
 };
 
 // The scratch's head, from the workgroups that find it.
@@ -800,8 +801,8 @@ __global__ __launch_bounds__(64 * AW, NT == 1 ? 3 : 2) void attend_few_kernel(At
       for (int m = 0; m < VH; m += 2)
         b[m >> 1] = l == 0.0f ? 0u : pack2<E>(o[m] * inv, o[m + 1] * inv);
       *reinterpret_cast<VV *>(dst) = b;
-    } else if ((int)blockIdx.x < a.slots) {
-      const size_t to = (size_t)blockIdx.x * ROWS + 16 * n + row;
+    } else if (w.place * a.pool.kv + head < a.slots) {
+      const size_t to = ((size_t)w.place * a.pool.kv + head) * ROWS + 16 * n + row;
       float *dst = a.part + to * D + VH * c;
 #pragma unroll
       for (int m = 0; m < VH; m += 4)
@@ -1514,6 +1515,12 @@ int64_t most_split(const exl3p_rows *r, const Split &sl) {
   const int64_t target = (float)tiles <= sl.few ? (int64_t)sl.round : (int64_t)sl.most;
   return tiles < target ? tiles : target;
 }
+// Items of those: only they leave sums for the join, so that the scratch does not
+// grow with the rows (131072 rows of 32 over 8 heads: 102 MB, for all items 2.2 GB).
+int64_t most_parts(const exl3p_rows *r, const Split &sl) {
+  return (float)most_tiles(r, sl) <= sl.few ? (int64_t)sl.round
+                                            : (int64_t)sl.most + most_split(r, sl);
+}
 
 template <typename F>
 exl3_verdict by_type(const exl3p_cache *c, F &&f) {
@@ -1624,7 +1631,7 @@ size_t exl3p_attend_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int
     return 0;
   const Split sl = split_of(c, r, heads);
   return (size_t)(1 + most_split(r, sl)) * sizeof(Joint) +
-         (size_t)most_items(r, sl) * c->kv_heads * ((size_t)1 << sl.tile) * (c->dim + 2) * sizeof(float);
+         (size_t)most_parts(r, sl) * c->kv_heads * ((size_t)1 << sl.tile) * (c->dim + 2) * sizeof(float);
 }
 
 exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
@@ -1670,17 +1677,18 @@ exl3_verdict exl3p_attend(const exl3p_cache *c, int32_t layer, const exl3p_rows 
   a.out = static_cast<uint16_t *>(out), a.os = out_stride;
   a.joint = static_cast<Joint *>(scratch), a.joints = (int)most_split(r, sl);
   a.part = reinterpret_cast<float *>(a.joint + 1 + most_split(r, sl));
-  a.slots = (int)(most_items(r, sl) * c->kv_heads);
+  a.slots = (int)(most_parts(r, sl) * c->kv_heads);
+  const dim3 items((unsigned)(most_items(r, sl) * c->kv_heads));
   const hipStream_t st = static_cast<hipStream_t>(s);
   return by_type(c, [&](auto e, auto d) {
     if (sl.tile == 4)
-      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d, 1>), dim3((unsigned)a.slots),
+      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d, 1>), items,
                          dim3(64 * AW), 0, st, a);
     else if (sl.tile == 5)
-      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d, 2>), dim3((unsigned)a.slots),
+      hipLaunchKernelGGL((attend_few_kernel<decltype(e), d, 2>), items,
                          dim3(64 * AW), 0, st, a);
     else
-      hipLaunchKernelGGL((attend_many_kernel<decltype(e), d>), dim3((unsigned)a.slots),
+      hipLaunchKernelGGL((attend_many_kernel<decltype(e), d>), items,
                          dim3(64 * AW), 0, st, a);
     hipLaunchKernelGGL((attend_join_kernel<decltype(e), d>),
                        dim3((unsigned)(most_split(r, sl) * c->kv_heads << (sl.tile - 4))), dim3(256),

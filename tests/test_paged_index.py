@@ -112,3 +112,63 @@ def test_sequences_that_share_rows_pass_the_bounds():
     for items, split in items_of(sl, [300, 0] * 20, [0] * 38 + [60000, 0]):
         at = [i for i, x in enumerate(items) if x[0] == 38]
         assert split > 0 and len(at) > 1 and at[0] >= sl["items"]
+
+
+def parts_of(sl):
+    """Items of split tiles that the scratch has places for, of a kv head."""
+    few = sl["items"] == sl["round"]
+    return sl["round"] if few else sl["most"] + sl["split"]
+
+
+def check_parts(kv, group, counts, lens):
+    sl = split_of(kv, group, sum(counts), len(counts), max(counts))
+    for items, split in items_of(sl, counts, lens):
+        of = {}
+        for s, tile, _, _ in items:
+            of[s, tile] = of.get((s, tile), 0) + 1
+        assert sum(n for n in of.values() if n > 1) <= parts_of(sl)
+        assert sum(n > 1 for n in of.values()) == split
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_parts_of_split_tiles_fit_the_scratch(seed):
+    rng = random.Random(1000 + seed)
+    seqs = rng.choice([1, 1, 2, 5, 17, 63, 64, 65, 130, 500])
+    most = rng.choice([1, 1, 2, 4, 8, 33, 64, 300, 2000])
+    ctx = rng.choice([0, 100, 5000, 200000, 3000000])
+    counts = [rng.randint(0, most) for _ in range(seqs)]
+    counts[rng.randrange(seqs)] = most
+    lens = [rng.randint(0, ctx) if rng.random() < 0.8 else 0 for _ in range(seqs)]
+    check_parts(rng.choice([1, 2, 3, 8, 16, 200, 600]), rng.choice([1, 2, 3, 4, 5, 8, 16]), counts, lens)
+
+
+def test_parts_of_the_largest_batches():
+    check_parts(8, 4, [1] * 60000, [7] * 60000)
+    check_parts(1, 1, [1], [(1 << 30) - 1])
+    check_parts(2, 4, [1 << 20], [(1 << 30) - (1 << 20)])
+    check_parts(1, 8, [1] * 63 + [1024], [1 << 24] * 64)
+    check_parts(8, 4, [2000] * 20, [0] * 19 + [3000000])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kv,group", [(1, 8), (8, 4), (64, 1)])
+def test_scratch_does_not_grow_with_the_rows(kv, group, dim):
+    """Whole tiles leave nothing behind: a prompt of any length, or any number of
+    sequences, takes what split tiles can."""
+    import ctypes
+
+    from plugins_amd import exl3 as X
+    from plugins_amd import paged as P
+    c = P.CacheDesc(ctypes.sizeof(P.CacheDesc), X.DT_F16, 4096, 8192, 1, 1 << 20, kv, 16, dim, 60000,
+                    1 << 20, 64)
+
+    def need(seqs, rows, most):
+        r = P.RowsDesc(ctypes.sizeof(P.RowsDesc), seqs, rows, most, 64, 64)
+        return P.paged_lib().exl3p_attend_scratch_bytes(ctypes.byref(c), ctypes.byref(r), kv * group)
+
+    for seqs, rows, most in ((1, 7, 7), (1, 300, 300), (1, 131072, 131072), (4, 8000, 2000),
+                             (64, 64, 1), (60000, 60000, 1), (1, 1 << 24, 1 << 24), (500, 4000, 8)):
+        sl = split_of(kv, group, rows, seqs, most)
+        assert need(seqs, rows, most) == 32 * (1 + sl["split"]) + \
+            parts_of(sl) * kv * (1 << sl["tile"]) * (dim + 2) * 4
+        assert need(seqs, rows, most) < 128 << 20
