@@ -832,9 +832,10 @@ __device__ __forceinline__ void lds_barrier() {
 // large product's rate; without the softmax 221, without the loads 212, without
 // both 184 (times only): what is left lies between the pipes.  16 trees of up to
 // 64 rows over up to 8192 keys 66 us, 3.4 TB/s: a tile's loads are one tile ahead,
-// and the longest item is 1.6 times the mean.
+// and the longest item is 1.6 times the mean.  Heads of 64 have LDS and, held to 128,
+// registers for four (prompts 157.3 us -> 156.1, 16 trees 46.3 -> 46.0).
 template <typename E, int D>
-__global__ __launch_bounds__(64 * AW, 2) void attend_many_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * AW, D == 64 ? 4 : 2) void attend_many_kernel(AttnArgs a) {
   constexpr int KK = D / 16, ND = D / 32;
   constexpr int ROW = D * 2;          // bytes of a key
   constexpr int ARR = 64 * ROW;       // of a tile's keys, or values
