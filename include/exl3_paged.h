@@ -26,8 +26,9 @@
  * arrays:
  *  - a sequence whose len is negative, or whose len + rows pass max_pages *
  *    page, has slots of -1 and attends to NaN; exl3p_commit gives it count 0;
- *  - a page number outside [0, pages) among a sequence's keys likewise: slot -1,
- *    NaN rows, a row not moved;
+ *  - a page number outside [0, pages) among a sequence's keys likewise: slot -1, a
+ *    row not moved, and NaN for every row that sees a key of it (and for others of
+ *    the sequence that are worked on with such a row);
  *  - cu must ascend from 0 to at most `rows`; rows behind cu[seqs], and a
  *    sequence's rows behind max_rows, get slot -1 and are left as they were by
  *    every other entry.  Where cu goes back, exl3p_attend writes no row.

@@ -120,8 +120,19 @@ def walk(parent, ids, target, most):
 
 
 def random_tree(n, g):
-    """Parents of n rows; every third tree of them has several roots."""
+    """Parents of n rows under one root."""
     return [-1] + [int(torch.randint(0, i, (1,), generator=g)) for i in range(1, n)]
+
+
+def random_forest(n, g):
+    """Parents of n rows, about a third of them roots, and some that are parents of
+    nothing that comes behind: the row itself, a later one, a negative number."""
+    out = random_tree(n, g) if n else []
+    for i in range(n):
+        x = int(torch.randint(0, 12, (1,), generator=g))
+        if x < 6:
+            out[i] = {0: i, 1: i + 1, 2: -7}.get(x, -1)
+    return out
 
 
 def random_table(counts, lens, page, extra, g, max_pages=None):

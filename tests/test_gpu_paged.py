@@ -800,3 +800,155 @@ def test_a_cu_that_goes_back_is_not_begun(seqs, n, lens):
     P.attend(cache, 0, rows, q, out, scratch=scratch)
     torch.cuda.synchronize()
     assert not out.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("n,ctx,group", [(3, 37, 4), (3, 4000, 4), (7, 50, 4), (40, 37, 4), (40, 6000, 4),
+                                         (70, 20, 3)])
+def test_attend_values_that_are_not_finite(n, ctx, group, tree, dim, dtype):
+    """Drafted rows whose keys are finite and some elements of whose values are not:
+    the rows that see them are infinite or NaN in just those elements, in both
+    kv heads' own, and right in the others; rows that do not see them are right
+    everywhere."""
+    counts, lens, page = [n, 2], [ctx, 50], 16
+    g, k, v, table, cu, q = batch(counts, lens, dtype, 2, group, dim, page, 61)
+    parents = [[-1] + [max(0, i - 2) for i in range(1, n)], [-1, 0]]
+    seen = [R.ancestors(p) if tree else [list(range(i + 1)) for i in range(len(p))] for p in parents]
+    mask = R.masks([js for s in seen for js in s], -(-n // 64)) if tree else None
+    pg, row = R.slots(table, 0, page, ctx + n)
+    odd = torch.zeros(n, 2, dim)  # what is put where, 0 elsewhere
+    odd[1, 0, 3], odd[1, 0, dim - 1], odd[1, 1, 17] = math.inf, -math.inf, math.nan
+    odd[2, 0, 3], odd[2, 1, 40], odd[n - 1, 1, 16] = -math.inf, math.inf, -math.inf
+    if n > 66:  # rows of another 64-key tile
+        odd[65, 0, 5], odd[66, 0, 5] = math.inf, math.inf
+    where = odd != 0
+    values = v[0, pg[ctx:], :, row[ctx:]]
+    v[0, pg[ctx:], :, row[ctx:]] = torch.where(where, torch.zeros(()).to(dtype), values)
+    want, tol = R.attention(q, k, v, table, cu, lens, seen, page, group, dim ** -0.5)
+    v[0, pg[ctx:], :, row[ctx:]] = torch.where(where, odd.to(dtype), values)
+    got = attended(k, v, table, counts, lens, q, mask)
+    near(got[n:], want[n:], tol[n:], "the other sequence")
+    for i in range(n):
+        add = torch.stack([odd[j] for j in seen[0][i]]).sum(0).repeat_interleave(group, 0)
+        fine = torch.stack([~where[j] for j in seen[0][i]]).all(0).repeat_interleave(group, 0)
+        near(got[i][fine], want[i][fine], tol[i][fine], ("right elements", i))
+        a, b = got[i].float()[~fine], add[~fine]
+        assert torch.equal(torch.isnan(a), torch.isnan(b)), i
+        assert torch.equal(a[~torch.isnan(b)], b[~torch.isnan(b)]), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts,lens,group", [
+    ([40, 40, 40, 40, 40], [30, 30, 30, 30, 30], 4),       # tiles of 128 pairs, whole
+    ([40, 40, 40, 40, 40], [9000, 9000, 700, 60, 60], 4),  # split: one item of several is bad
+    ([2, 2, 2, 2, 2], [9000, 9000, 700, 60, 60], 4), ([5, 5, 5, 5, 5], [30, 5000, 4000, 60, 60], 4)])
+def test_attend_bad_pages_and_lengths_of_split_tiles(counts, lens, group, dtype):
+    """As test_attend_bad_pages_and_lengths_are_nan, tiles of 128 pairs and joined
+    ones among them: a page that is none anywhere in the context makes every row
+    of its sequence NaN, and no other."""
+    g, k, v, table, cu, q = batch(counts, lens, dtype, 1, group, 64, 16, 10)
+    seen = [[list(range(i + 1)) for i in range(n)] if s in (0, 2) else [[]] * n
+            for s, n in enumerate(counts)]
+    want, tol = R.attention(q, k, v, table, cu, [c if s in (0, 2) else 0 for s, c in enumerate(lens)],
+                            seen, 16, group, 0.125)
+    most = 16 * table.shape[1]
+    for page, name in ((0, -1), (lens[1] // 32, k.shape[1]), (lens[1] // 16 - 1, 2 ** 31 - 1)):
+        bad = table.clone()
+        bad[1, page] = name
+        rows = P.Rows.of(counts, lens[:3] + [-1, most - counts[4] + 1], DEV)
+        got = attended(k, v, bad, counts, lens, q, None, rows=rows)
+        seqs = [got[cu[s]:cu[s + 1]] for s in range(5)]
+        assert all(torch.isnan(seqs[s]).all() for s in (1, 3, 4)), (page, name)
+        for s in (0, 2):
+            of = slice(cu[s], cu[s + 1])
+            near(got[of], want[of], tol[of], (page, name, s))
+
+
+def test_pages_beyond_32_bits_of_trees_and_commits():
+    """As test_attend_beyond_32_bits: tiles of 128 pairs, whole and split, and the
+    moves of accepted rows among pages past 2^32 bytes and elements of a layer."""
+    kv, page, dim, group = 8, 256, 128, 4
+    per = kv * page * dim
+    pages = (1 << 32) // per + 9
+    if torch.cuda.mem_get_info()[0] < 4 * 2 * per * pages:
+        pytest.skip("not enough memory")
+    k = torch.empty(2, pages, kv, page, dim, dtype=torch.float16, device=DEV)
+    v = torch.empty_like(k)
+    g = torch.Generator().manual_seed(12)
+    at = [pages - 1, pages - 5, pages - 3, pages - 7]
+    small = [torch.randn(2, 4, kv, page, dim, generator=g).half() for _ in range(2)]
+    for x, p in enumerate(at):
+        k[:, p], v[:, p] = small[0][:, x].to(DEV), small[1][:, x].to(DEV)
+    cache = P.PagedCache.over(k, v, torch.tensor([at], dtype=torch.int32, device=DEV))
+    n, tab = 20, torch.tensor([[0, 1, 2, 3]], dtype=torch.int32)
+    parent = R.random_tree(n, g)
+    q = torch.randn(n, kv * group, dim, generator=g).half()
+    for ctx in (40, 900):
+        rows = P.Rows.of([n], [ctx], DEV)
+        _, slot, mask = P.plan(cache, rows, torch.tensor(parent, dtype=torch.int32, device=DEV))
+        pg, row = R.slots(tab, 0, page, ctx + n)
+        assert slot.tolist() == [at[int(p)] * page + int(r) for p, r in zip(pg[ctx:], row[ctx:])]
+        got = P.attend(cache, 1, rows, q.to(DEV), mask=mask).cpu().view(q.shape)
+        want, tol = R.attention(q, *small, tab, [0, n], [ctx], [R.ancestors(parent)], page, group,
+                                1 / math.sqrt(dim), layer=1)
+        near(got, want, tol, ("far pages", ctx))
+    # a line from row 0 to every third row behind it
+    rows = P.Rows.of([n], [500], DEV)  # from the second page into the third
+    line = [max(0, (i - 1) // 3 * 3) if i % 3 == 0 else -1 for i in range(n)]
+    ids = torch.arange(n, dtype=torch.int32)
+    target = ids + 3
+    i32 = {"dtype": torch.int32, "device": DEV}
+    path, (count, nxt, new) = torch.empty(1, n, **i32), (torch.empty(1, **i32) for _ in range(3))
+    P.commit(cache, rows, torch.tensor(line, **i32), ids.to(DEV), target.to(DEV), path, count, nxt, new)
+    way, after = R.walk(line, ids.tolist(), target.tolist(), n)
+    assert way == list(range(0, n, 3)) and path[0].tolist() == way + [-1] * (n - len(way))
+    assert (count.item(), nxt.item(), new.item()) == (len(way), after, 500 + len(way))
+    pg, row = R.slots(tab, 0, page, 500 + n)
+    src, dst = [500 + i for i in way], list(range(500, 500 + len(way)))
+    for x, pool in zip(small, (k, v)):
+        x[:, pg[dst], :, row[dst]] = x[:, pg[src], :, row[src]].clone()
+        for y, p in enumerate(at):
+            assert torch.equal(pool[:, p].cpu(), x[:, y])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("counts,lens,group", [
+    ([5, 8, 3], [40, 0, 300], 4), ([60, 9, 1], [0, 70, 500], 4), ([70, 33], [900, 0], 2), ([7], [4000], 1)])
+def test_forests_planned_attended_and_committed(counts, lens, group, dtype):
+    """Trees with several roots, and parents that are none, through plan,
+    attention and commit: rows under another root than row 0 see their own
+    ancestors, and are never accepted."""
+    kv, dim, page = 2, 64, 16
+    g, k, v, table, cu, q = batch(counts, lens, dtype, kv, group, dim, page, 71 + counts[0])
+    trees = [R.random_forest(n, g) for n in counts]
+    assert any(sum(not 0 <= p < i for i, p in enumerate(t)) > 1 for t in trees)
+    anc = [R.ancestors(t) for t in trees]
+    i32 = {"dtype": torch.int32, "device": DEV}
+    kd, vd = k.to(DEV), v.to(DEV)
+    cache = P.PagedCache.over(kd, vd, table.to(DEV))
+    rows = P.Rows.of(counts, lens, DEV)
+    parent = torch.tensor([p for t in trees for p in t], **i32)
+    pos, slot, mask = P.plan(cache, rows, parent)
+    assert torch.equal(mask.cpu(), R.masks([a for t in anc for a in t], mask.shape[1]))
+    assert pos.tolist() == [c + len(a) - 1 for t, c in zip(anc, lens) for a in t]
+    want, tol = R.attention(q, k, v, table, cu, lens, anc, page, group, 0.2)
+    near(P.attend(cache, 0, rows, q.to(DEV), mask=mask, scale=0.2).cpu().view(q.shape), want, tol,
+         "forests")
+    # one token everywhere: whatever child there is, is accepted
+    ids = torch.full((cu[-1],), 5, **i32)
+    S, most = len(counts), max(counts)
+    path, (count, nxt, new) = torch.empty(S, most, **i32), (torch.empty(S, **i32) for _ in range(3))
+    P.commit(cache, rows, parent, ids, ids.clone(), path, count, nxt, new)
+    torch.cuda.synchronize()
+    for s, n in enumerate(counts):
+        way, _ = R.walk([p if 0 <= p < i else -1 for i, p in enumerate(trees[s])], [5] * n, [5] * n, most)
+        assert path[s].tolist() == way + [-1] * (most - len(way)) and count[s].item() == len(way)
+        assert all(anc[s][i][0] == 0 for i in way)
+        pg, row = R.slots(table, s, page, lens[s] + n)
+        src, dst = [lens[s] + i for i in way], list(range(lens[s], lens[s] + len(way)))
+        for pool in (k, v):
+            pool[:, pg[dst], :, row[dst]] = pool[:, pg[src], :, row[src]].clone()
+    for pool, now in ((k, kd), (v, vd)):
+        assert torch.equal(now.cpu().view(torch.int16), pool.view(torch.int16))
