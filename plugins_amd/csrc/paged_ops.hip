@@ -195,7 +195,7 @@ struct Rates {
 // turns together lies in one lane, the squares are summed over the head's lanes,
 // and a row's angles, in 64 bits until they are less than a turn, are formed once
 // for the heads that a wave takes.  Bound by bytes: 4428 rows of 48 heads of 128
-// 21.4 us, 5.1 TB/s read and written.
+// 21.9 us, 5.0 TB/s read and written.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void qkv_append_kernel(
     Pool pool, int rows, int nq, const uint16_t *q, int64_t qs,
@@ -550,8 +550,14 @@ __device__ __forceinline__ int clear_of(const AttnArgs &a, const Work &w, int la
 // P^T, wants its right operand if V's keys are taken in the same order: the
 // weights never leave their lane, and no load passes through LDS (16 bytes a lane,
 // the next step's keys on their way while the weights form).  Bound by bytes: trees
-// of 8 rows over 4 contexts of up to 65536 keys 133 us, 5.7 TB/s (a read alone of 2
-// GiB: 6.3); one token over 2048 keys 6.4 us, its chain of loads.
+// of 8 rows over 4 contexts of up to 65536 keys 138 us, 5.5 TB/s (a read alone of 2
+// GiB: 6.3); one token over 2048 keys 7.4 us, its chain of loads.
+//
+// Weights are rounded to the cache's type, since the second product takes both
+// operands in it (in 32 bits it would run at a sixteenth of the rate), and summed
+// as rounded, so that they add up to one: a value is off by half a step of its
+// type, at most, beside the output's own half: 1.2 to 1.4 times the error of 32-bit
+// weights.  References, sums and joins are of 32 bits.
 template <typename E, int D, int NT>
 __global__ __launch_bounds__(64 * AW, NT == 1 ? 3 : 2) void attend_few_kernel(AttnArgs a) {
   constexpr int KK = D / 32;  // products of 32 dims a score
@@ -828,11 +834,11 @@ __device__ __forceinline__ void lds_barrier() {
 // choose their pieces so): pieces of one number of 16 rows of keys lie in 16
 // places of the 64 banks, and so do the 4 rows by 64 bytes of values that 32
 // lanes of a transposing read take.  Two workgroups a CU, each one's products
-// beside the other's softmax.  Prompts of 2048 rows (222 GFLOP) 250 us, 0.72 of a
-// large product's rate; without the softmax 221, without the loads 212, without
-// both 184 (times only): what is left lies between the pipes.  16 trees of up to
-// 64 rows over up to 8192 keys 66 us, 3.4 TB/s: a tile's loads are one tile ahead,
-// and the longest item is 1.6 times the mean.  Heads of 64 have LDS and, held to 128,
+// beside the other's softmax.  Prompts of 2048 rows (222 GFLOP) 239 us, 0.75 of a
+// large product's rate; of an earlier 250, 221 without the softmax, 212 without the
+// loads, 184 without both (times only): what is left lies between the pipes.  16
+// trees of up to 64 rows over up to 8192 keys 68 us, 3.3 TB/s: a tile's loads are one
+// tile ahead, and the longest item is 1.23 times the mean.  Heads of 64 have LDS and, held to 128,
 // registers for four (prompts 157.3 us -> 156.1, 16 trees 46.3 -> 46.0).
 template <typename E, int D>
 __global__ __launch_bounds__(64 * AW, D == 64 ? 4 : 2) void attend_many_kernel(AttnArgs a) {
