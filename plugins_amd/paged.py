@@ -365,9 +365,9 @@ def _ints(t, what: str, cache, n: int):
 
 def _stream(cache, stream):
     if stream is not None:
-        if stream.device_index != cache.index:
-            raise ValueError(f"the stream is on device {stream.device_index}, "
-                             f"the cache on {cache.device}")
+        on = getattr(stream, "device_index", cache.index)  # (others' streams may not say)
+        if on != cache.index:
+            raise ValueError(f"the stream is on device {on}, the cache on {cache.device}")
         return stream.cuda_stream
     return _raw_stream(cache.index)
 

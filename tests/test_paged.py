@@ -627,6 +627,8 @@ def test_streams_of_other_devices_are_refused():
     for call in calls:
         with pytest.raises(ValueError, match="the stream is on device 1"):
             call(other)
+    # one that says nothing but its handle is taken for the cache's
+    assert P._stream(c, types.SimpleNamespace(cuda_stream=7)) == 7
 
 
 def test_decoder_runs_on_its_caches_device(monkeypatch):
