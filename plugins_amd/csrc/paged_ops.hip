@@ -838,8 +838,9 @@ __device__ __forceinline__ void lds_barrier() {
 // large product's rate; of an earlier 250, 221 without the softmax, 212 without the
 // loads, 184 without both (times only): what is left lies between the pipes.  16
 // trees of up to 64 rows over up to 8192 keys 68 us, 3.3 TB/s: a tile's loads are one
-// tile ahead, and the longest item is 1.23 times the mean.  Heads of 64 have LDS and, held to 128,
-// registers for four (prompts 157.3 us -> 156.1, 16 trees 46.3 -> 46.0).
+// tile ahead, and the longest item is 1.23 times the mean.  Heads of 64 have LDS and,
+// held to 128, registers for four workgroups (prompts 157.3 us -> 156.1, 16 trees 46.3
+// -> 46.0).
 template <typename E, int D>
 __global__ __launch_bounds__(64 * AW, D == 64 ? 4 : 2) void attend_many_kernel(AttnArgs a) {
   constexpr int KK = D / 16, ND = D / 32;
