@@ -15,6 +15,10 @@
  *   exl3p_attend      attention over the cache and the rows      (a layer)
  *   exl3p_commit      which rows the model's own tokens accept, and their keys
  *                     and values moved behind the context, all layers (a step)
+ *   exl3p_verify      the tokens that sampling accepts or gives, from the
+ *                     target's logits and given random numbers    (a step)
+ *   exl3p_weigh       the attention weight of every cached key    (a layer)
+ *   exl3p_evict       the keys of most weight stay, up to a budget (as needed)
  *   exl3p_copy_pages  pages copied in all layers (forks, compaction)
  *   exl3p_book_*      which pages are whose: host bookkeeping, no device work
  *
@@ -131,6 +135,81 @@ exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32
                           const int32_t *ids, const int32_t *target, int32_t *path,
                           int32_t max_path, int32_t *count, int32_t *next, int32_t *new_len,
                           exl3_stream s);
+
+/* Sampled verification: target[t] is the token that follows row t on each
+ * sequence's walk, -1 for rows that are not on it, so that exl3p_commit with these
+ * targets walks the same way.  Row t's logits are the model's after row t; its
+ * probabilities p are their softmax at the sequence's temperature.  The walk
+ * begins at row 0.  A row's children, in their order, are drafted tokens that
+ * were drawn from draft[t], the probabilities q that the draft had after row t:
+ * one is accepted with probability min(1, p~ / q~) of its token (u[child] * q~ <
+ * p~), and after a refusal p~ is max(p~ - q~, 0), normalized.  q~ is q, or, with
+ * `distinct` not 0 (siblings drawn without replacement), q without the refused
+ * ones, normalized.  draft NULL: drafted tokens are certain (q~ is 1 at each), as
+ * where a draft's most likely ones were taken.  Where no child is accepted the
+ * token is sampled from what p~ is then: the first of positive probability whose
+ * cumulative sum, in 64 bits and in the vocabulary's order, passes u[row 0]
+ * times the whole.  So the tokens have the distribution that sampling without
+ * drafts has; a step of single rows is the sampler itself.
+ *   temperature [seqs], NULL: 1.  0: the largest logit, the first of equals.
+ *   u [rows], in [0, 1).  A number that is none (NaN) accepts nothing and samples
+ *   the last token of positive probability.
+ * logits [rows][vocab] and draft (logits_dtype, draft_dtype: EXL3_DT_F32, F16 or
+ * BF16; strides in elements, rows apart), -inf: never.  A token outside the
+ * vocabulary is refused as any other.  Where a row's logits have a NaN, no finite
+ * one, or +inf (temperature 0 takes it), or the temperature is negative or not
+ * finite, the walk ends there with target -1.  parent as in exl3p_tree_plan; at
+ * most EXL3P_TREE_MAX rows of a sequence; vocab up to 2^24.  r->len is not read.
+ * scratch: exl3p_verify_scratch_bytes(), written and read within the call.  target
+ * and the scratch lie over nothing that is read, nor over each other. */
+size_t exl3p_verify_scratch_bytes(const exl3p_rows *r, int32_t vocab);
+exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int32_t *ids,
+                          int32_t vocab, const void *logits, int32_t logits_dtype,
+                          int64_t logits_stride, const void *draft, int32_t draft_dtype,
+                          int64_t draft_stride, int32_t distinct, const float *temperature,
+                          const double *u, int32_t *target, void *scratch, size_t scratch_bytes,
+                          exl3_stream s);
+
+/* score[s][h][x] = had + the sum, over the rows of sequence s that count and the
+ * query heads of kv head h, of the softmax weight that each gives key number x:
+ * exl3p_attend's weights, of the same q, mask and scale.  had is decay * score[s][h][x]
+ * for x < base[s] (base NULL: r->len, the keys cached before the step) and 0 for
+ * the others, whose scores begin here.  The last `window` rows of a sequence count,
+ * 0: all.  score [seqs][kv_heads][room] of 32-bit floats, one layer's; keys behind
+ * the sequence's, and sequences without rows, stay as they are, and so does one
+ * whose keys are more than `room`, or do not fit its table.  A sequence with a
+ * page number outside the cache among its keys has scores of NaN.  decay is
+ * finite.  Sums are of 32 bits, in an order that goes by the sizes and lengths alone:
+ * results repeat.  q as in exl3p_attend; values are not read.
+ * scratch: exl3p_weigh_scratch_bytes(), as in exl3p_attend.  score and the scratch lie over
+ * nothing else that is read, nor over each other. */
+size_t exl3p_weigh_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int32_t heads,
+                                 int32_t window, int32_t room);
+exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
+                         const void *q, int64_t q_stride, const uint64_t *mask, int32_t words,
+                         float scale, int32_t window, float decay, const int32_t *base,
+                         float *score, int32_t room, void *scratch, size_t scratch_bytes,
+                         exl3_stream s);
+
+/* Eviction: a sequence of more keys than its budget, min(keep[s], most) (keep
+ * NULL: most), keeps that many in every layer and kv head: its first `first` keys,
+ * its last `last` ones (as far as the budget goes, the first before the last), and
+ * the others of the highest score, of equals the earlier; a NaN is below all
+ * numbers.  The kept keys and values move together, in their order, to key numbers
+ * 0, 1, ..., in the sequence's own pages.  len [seqs]: keys cached; new_len the
+ * same after it.  score [layers][seqs][kv_heads][room]; kept [layers][seqs]
+ * [kv_heads][most]: the numbers that the kept keys had, -1 behind them; new_score,
+ * laid out as score, gets the kept keys' scores (behind them it stays as it is).
+ * new_score may be score itself.  A sequence within its budget, with keep[s]
+ * below 0, more keys than `room` or its table, or a page number outside the cache
+ * among them, stays as it is: kept is -1 throughout, new_len its len.
+ * Pages that a sequence which loses keys holds are its alone (exl3p_book_shared), its
+ * key numbers below new_len are written.  No output lies over an input (but
+ * new_score), another output or the cache. */
+exl3_verdict exl3p_evict(const exl3p_cache *c, int32_t seqs, const int32_t *len,
+                         const float *score, int32_t room, const int32_t *keep, int32_t most,
+                         int32_t first, int32_t last, int32_t *kept, float *new_score,
+                         int32_t *new_len, exl3_stream s);
 
 /* Page dst[i] = page src[i] in every layer, keys and values.  src and dst are
  * HOST arrays, read before the call returns.  Refused: a page outside the

@@ -42,6 +42,8 @@ SOURCES = [
       for k in range(9)],
     ("decoder_ops.hip", "decoder_ops", DEVICE_FLAGS),
     ("paged_ops.hip", "paged_ops", DEVICE_FLAGS),
+    ("paged_verify.hip", "paged_verify", DEVICE_FLAGS),
+    ("paged_budget.hip", "paged_budget", DEVICE_FLAGS),
     ("exl3_noalloc.hip", "exl3_noalloc", DEVICE_FLAGS),
     ("exl3_host.cpp", "exl3_host", HOST_FLAGS),
     ("exl3_json.cpp", "exl3_json", HOST_FLAGS),

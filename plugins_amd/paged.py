@@ -68,6 +68,13 @@ _SIGS = {
     "exl3p_attend": (_V, [_P, c_int32, _P, c_int32, _P, c_int64, _P, c_int32, c_float, _P, c_int64,
                           _P, c_size_t, _P]),
     "exl3p_commit": (_V, [_P, _P, _P, _P, _P, _P, c_int32, _P, _P, _P, _P]),
+    "exl3p_verify_scratch_bytes": (c_size_t, [_P, c_int32]),
+    "exl3p_verify": (_V, [_P, _P, _P, c_int32, _P, c_int32, c_int64, _P, c_int32, c_int64, c_int32, _P,
+                          _P, _P, _P, c_size_t, _P]),
+    "exl3p_weigh_scratch_bytes": (c_size_t, [_P, _P, c_int32, c_int32, c_int32]),
+    "exl3p_weigh": (_V, [_P, c_int32, _P, c_int32, _P, c_int64, _P, c_int32, c_float, c_int32, c_float,
+                         _P, _P, c_int32, _P, c_size_t, _P]),
+    "exl3p_evict": (_V, [_P, c_int32, _P, _P, c_int32, _P, c_int32, c_int32, c_int32, _P, _P, _P, _P]),
     "exl3p_copy_pages": (_V, [_P, _P, _P, c_int32, _P]),
     "exl3p_book_open": (_P, [c_int32, c_int32, c_int32, c_int32, POINTER(_V)]),
     "exl3p_book_close": (None, [_P]),
@@ -513,3 +520,134 @@ def copy_pages(cache, src, dst, stream=None) -> None:
     src, dst = map(_c_int, src), map(_c_int, dst)
     _call(cache, paged_lib().exl3p_copy_pages, "copy_pages", cache._ref, arr(*src), arr(*dst), n,
           _stream(cache, stream))
+
+
+def _floats(t, what: str, on, shape):
+    """A dense float32 tensor of the shape, on the device of `on` (a cache, rows)."""
+    if t.dtype is not _torch.float32:
+        raise TypeError(f"{what} is float32")
+    if tuple(t.shape) != tuple(shape) or t.get_device() != on.index or not t.is_contiguous():
+        raise ValueError(f"{what}: dense {list(shape)} on {on.device}, not {list(t.shape)}")
+    return t.data_ptr()
+
+
+def _bytes(scratch, need: int, on, stream):
+    """The scratch given, or one from torch's allocator for this call."""
+    if scratch is None:
+        if stream is None:
+            return _torch.empty(need, dtype=_torch.uint8, device=on.device)
+        with _on(on, stream):
+            return _torch.empty(need, dtype=_torch.uint8, device=on.device)
+    if scratch.get_device() != on.index or not scratch.is_contiguous():
+        raise ValueError(f"scratch is dense, on {on.device}")
+    return scratch
+
+
+_NUMBERS = None
+
+
+def _probabilities(t, what: str, rows, vocab: int):
+    """Base, type and row stride of [rows, vocab] float32, float16 or bfloat16."""
+    global _NUMBERS
+    if _NUMBERS is None:
+        _NUMBERS = (_torch.float32, _torch.float16, _torch.bfloat16)
+    if t.dtype not in _NUMBERS:
+        raise TypeError(f"{what} is float32, float16 or bfloat16")
+    if t.get_device() != rows.index:
+        raise ValueError(f"{what} is on {t.device}, the rows on {rows.device}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows.rows or shape[1] != vocab or (vocab > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: [{rows.rows}, {vocab}], elements side by side, not {list(shape)} "
+                         f"with strides {t.stride()}")
+    return t.data_ptr(), X.dtype_of(t), t.stride(0) if rows.rows > 1 else vocab
+
+
+def verify(rows, parent, ids, logits, u, target, draft=None, temperature=None,
+           distinct: bool = False, scratch=None, stream=None) -> None:
+    """exl3p_verify: target int32 [rows] from logits [rows, vocab], random numbers u
+    float64 [rows] in [0, 1), the drafts' probabilities draft [rows, vocab] (None:
+    drafted tokens are certain) and temperature float32 [sequences] (None: 1).
+    distinct: siblings were drawn without replacement."""
+    n = rows.rows
+    if logits.dim() != 2:
+        raise ValueError("logits: [rows, vocab]")
+    vocab = _c_int(logits.shape[1])
+    lp, lt, ls = _probabilities(logits, "logits", rows, vocab)
+    dp, dt, ds = (None, 0, 0) if draft is None else _probabilities(draft, "draft", rows, vocab)
+    if u.dtype is not _torch.float64:
+        raise TypeError("u is float64")
+    if u.numel() != n or u.get_device() != rows.index or not u.is_contiguous():
+        raise ValueError(f"u: {n} dense elements on {rows.device}")
+    L = paged_lib()
+    scratch = _bytes(scratch, L.exl3p_verify_scratch_bytes(rows._ref, vocab), rows, stream)
+    _call(rows, L.exl3p_verify, "verify", rows._ref,
+          None if parent is None else _ints(parent, "parent", rows, n), _ints(ids, "ids", rows, n),
+          vocab, lp, lt, ls, dp, dt, ds, bool(distinct),
+          None if temperature is None else _floats(temperature, "temperature", rows, (rows.seqs,)),
+          u.data_ptr(), _ints(target, "target", rows, n), scratch.data_ptr(),
+          scratch.numel() * scratch.element_size(), _stream(rows, stream))
+
+
+def weigh(cache, layer: int, rows, q, score, mask=None, scale: float | None = None,
+          window: int = 0, decay: float = 1.0, base=None, scratch=None, stream=None) -> None:
+    """exl3p_weigh: to score float32 [sequences, kv heads, room] of the layer the weight
+    that each key gets from the rows (the last `window` of each sequence, 0: all),
+    decay times what it had; keys from base int32 [sequences] on (None: rows.len)
+    begin anew.  q as attend's."""
+    _of(cache, rows)
+    n, dim = rows.rows, cache.head_dim
+    heads = _heads(q, cache)
+    qp, qs = _matrix(q, "q", cache, n, heads * dim)
+    mp, words = _mask(mask, cache, rows)
+    if score.dim() != 3:
+        raise ValueError("score: [sequences, kv heads, room]")
+    room = _c_int(score.shape[2])
+    sp = _floats(score, "score", cache, (rows.seqs, cache.kv_heads, room))
+    L = paged_lib()
+    window = _c_int(window)
+    need = _sized(cache, L.exl3p_weigh_scratch_bytes, cache._ref, rows._ref, heads, window, room)
+    scratch = _bytes(scratch, need, cache, stream)
+    _call(cache, L.exl3p_weigh, "weigh", cache._ref, _c_int(layer), rows._ref, heads, qp, qs, mp, words,
+          1.0 / math.sqrt(dim) if scale is None else scale, window, decay,
+          None if base is None else _ints(base, "base", cache, rows.seqs), sp, room,
+          scratch.data_ptr(), scratch.numel() * scratch.element_size(), _stream(cache, stream))
+
+
+def _sized(cache, fn, *args) -> int:
+    """A scratch's size on the cache's device."""
+    if cache.index == _device():
+        return fn(*args)
+    with _torch.cuda.device(cache.index):
+        return fn(*args)
+
+
+def weigh_scratch_bytes(cache, rows, heads: int, window: int = 0, room: int = 0) -> int:
+    """exl3p_weigh_scratch_bytes on the cache's device."""
+    return _sized(cache, paged_lib().exl3p_weigh_scratch_bytes, cache._ref, rows._ref, heads,
+                  _c_int(window), _c_int(room))
+
+
+def verify_scratch_bytes(rows, vocab: int) -> int:
+    """exl3p_verify_scratch_bytes."""
+    return paged_lib().exl3p_verify_scratch_bytes(rows._ref, _c_int(vocab))
+
+
+def evict(cache, lens, score, kept, new_score, new_len, keep=None, first: int = 0, last: int = 0,
+          stream=None) -> None:
+    """exl3p_evict: of the sequences' lens int32 [sequences] keys those of highest score
+    float32 [layers, sequences, kv heads, room] stay, up to kept.shape[-1] or keep int32
+    [sequences] of them, in every layer and kv head; kept int32 [layers, sequences, kv
+    heads, most], new_score (may be score itself), new_len int32 [sequences].  The pages
+    of a sequence that loses keys are its alone."""
+    if score.dim() != 4 or kept.dim() != 4:
+        raise ValueError("score and kept: [layers, sequences, kv heads, ...]")
+    seqs, room, most = lens.numel(), _c_int(score.shape[3]), _c_int(kept.shape[3])
+    shape = (cache.layers, seqs, cache.kv_heads)
+    if tuple(kept.shape[:3]) != shape:
+        raise ValueError(f"kept: {[*shape, 'most']}, not {list(kept.shape)}")
+    _call(cache, paged_lib().exl3p_evict, "evict", cache._ref, _c_int(seqs),
+          _ints(lens, "lens", cache, seqs), _floats(score, "score", cache, (*shape, room)), room,
+          None if keep is None else _ints(keep, "keep", cache, seqs), most, _c_int(first),
+          _c_int(last), _ints(kept, "kept", cache, kept.numel()),
+          _floats(new_score, "new_score", cache, (*shape, room)),
+          _ints(new_len, "new_len", cache, seqs), _stream(cache, stream))
