@@ -21,13 +21,17 @@ struct WeighArgs {
   float *score;
   int room;
   float target;  // items of a kv head
+  float least;   // 64-key units of one, at least
   int slots;     // items * kv that part holds
   f32x2 *part;   // [items * kv][TILE]: an item's reference and sum of each pair
   f32x2 *ref;    // [kv][rows * group]: a pair's reference, and one over its sum
+  float *t;      // few pairs: [seqs][kv][most][wide] scores, in place of ref
+  int most, wide;
 };
 
 constexpr int WW = 4;       // waves of a workgroup
 constexpr int TILE = 128;   // pairs of a row and a query head that an item has
+constexpr int FEW = 16;     // or, where no sequence has more, this many
 constexpr int KEYS = 128;   // keys that a workgroup adds up weights for
 constexpr float SLACK = 4.0f;  // a reference follows its maximum in steps of more (powers of two)
 
@@ -90,7 +94,7 @@ __device__ __forceinline__ Find find(const WeighArgs &a, int x) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) units += exl3::xor_lanes(units, m);
   const int chunk = __builtin_amdgcn_readfirstlane(
-      (int)fminf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / a.target), 4.0f), (float)(1 << 25)));
+      (int)fminf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / a.target), a.least), (float)(1 << 25)));
   int before = 0, items = 0;
   for (int s0 = 0; s0 < a.st.seqs; s0 += 64) {
     const int s = s0 + lane;
@@ -154,6 +158,23 @@ __device__ __forceinline__ void lds_dma16_at(const void *p, uint32_t lds) {
 template <int D>
 __device__ __forceinline__ int swizzle(int row) {
   return D == 128 ? row & 15 : (row >> 1) & 7;
+}
+
+// A score that a row does not see, where scores are kept: its weight is none, also
+// where the row's sum is NaN.
+constexpr float UNSEEN = -0x1.fffffep127f;
+
+// Two parts of a pair's keys: the reference and the sum of weights of both.
+__device__ __forceinline__ void join(float &ref, float &sum, float other, float more) {
+  const float now = __builtin_elementwise_maximum(ref, other), from = now == -INFINITY ? 0.0f : now;
+  sum = sum * __builtin_amdgcn_exp2f(ref - from) + more * __builtin_amdgcn_exp2f(other - from);
+  ref = now;
+}
+// What the second pass wants of them: a pair that sees nothing has no weights, a NaN
+// stays in the factor.
+__device__ __forceinline__ f32x2 ended(float ref, float sum) {
+  return f32x2{ref == -INFINITY || ref != ref ? 0.0f : ref,
+               sum == 0.0f ? 0.0f : ref != ref ? ref : 1.0f / sum};
 }
 
 // The first pass: each pair's reference (its largest score, or less by SLACK at
@@ -278,12 +299,10 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_sums_kernel(WeighArgs a) {
   if (bad) sbad = 1;
   __syncthreads();
   // the two halves of a pair's keys
-  const float other = exl3::xor_lanes(ref, 32), more = exl3::xor_lanes(sum, 32);
-  const float now = __builtin_elementwise_maximum(ref, other), from = now == -INFINITY ? 0.0f : now;
-  sum = sum * __builtin_amdgcn_exp2f(ref - from) + more * __builtin_amdgcn_exp2f(other - from);
+  join(ref, sum, exl3::xor_lanes(ref, 32), exl3::xor_lanes(sum, 32));
   if (sbad) sum = __builtin_nanf("");
   const int64_t slot = (int64_t)(f.first + f.j) * a.pool.kv + head;
-  if (h == 0 && r0 + col < w.pairs && slot < a.slots) a.part[slot * TILE + 32 * wave + col] = f32x2{now, sum};
+  if (h == 0 && r0 + col < w.pairs && slot < a.slots) a.part[slot * TILE + 32 * wave + col] = f32x2{ref, sum};
 }
 
 // A tile's items joined, a pair a thread.
@@ -297,14 +316,9 @@ __global__ __launch_bounds__(TILE) void weigh_join_kernel(WeighArgs a) {
     const int64_t slot = (int64_t)(f.first + j) * a.pool.kv + head;
     if (slot >= a.slots) break;
     const f32x2 v = a.part[slot * TILE + threadIdx.x];
-    const float now = __builtin_elementwise_maximum(ref, v[0]), from = now == -INFINITY ? 0.0f : now;
-    sum = sum * __builtin_amdgcn_exp2f(ref - from) + v[1] * __builtin_amdgcn_exp2f(v[0] - from);
-    ref = now;
+    join(ref, sum, v[0], v[1]);
   }
-  const int64_t to = (int64_t)head * a.st.rows * a.group + (int64_t)(f.w.row + f.w.lo) * a.group + pair;
-  // a pair that sees nothing has no weights; NaN stays in the second
-  a.ref[to] = f32x2{ref == -INFINITY || ref != ref ? 0.0f : ref,
-                    sum == 0.0f ? 0.0f : ref != ref ? ref : 1.0f / sum};
+  a.ref[(int64_t)head * a.st.rows * a.group + (int64_t)(f.w.row + f.w.lo) * a.group + pair] = ended(ref, sum);
 }
 
 // The second pass: KEYS keys a workgroup, 32 a wave in registers; the pairs pass
@@ -405,6 +419,167 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
   }
 }
 
+// Few pairs (single tokens): their scores are kept in 32 bits from the first pass
+// to the second, 4 bytes a pair beside a key's 2 D, so that keys are read
+// once.  The first pass: 16 x 16 products, a lane has 4 keys' scores of one pair; a wave
+// takes 32 keys in turn, the next ones on their way while the sums form.
+template <typename E, int D>
+__global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a) {
+  constexpr int KK = D / 32;
+  typedef typename E::V8 V8;
+  __shared__ f32x2 so[WW][FEW];
+  __shared__ int sbad;
+  const int head = blockIdx.x % a.pool.kv;
+  const Find f = find<ITEM>(a, blockIdx.x / a.pool.kv);
+  if (f.s < 0) return;
+  const Watch &w = f.w;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int pair = min(col, w.pairs - 1), i = w.lo + pair / a.group, hq = head * a.group + pair % a.group;
+  const int k0 = (int)min((int64_t)f.j * f.each * 64, (int64_t)w.keys);
+  const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
+  const int steps = (k1 - k0 + 31) / 32;
+  // keys below this every row that counts sees
+  const int clear = a.mask == nullptr ? w.len + w.lo + 1 : w.len;
+  if (threadIdx.x == 0) sbad = 0;
+  const int *trow = a.pool.table + (size_t)f.s * a.pool.max_pages;
+  const uint16_t *pk = reinterpret_cast<const uint16_t *>(a.pool.k) + col * D + 8 * g;
+  bool bad = false;
+  uint32_t ids[2];
+  u32x4 kf[2][KK];
+  // blocks behind the last key stand for the last key's
+  auto key_of = [&](int step, int t) { return min(k0 + step * 32 + 16 * t, (k1 - 1) & ~15); };
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) ids[t] = (uint32_t)trow[key_of(step, t) >> a.pool.lp];
+  };
+  auto load = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t page = __builtin_amdgcn_readfirstlane(ids[t]);
+      if (page >= (uint32_t)a.pool.pages) bad = true, page = 0;
+      const size_t at = ((((size_t)page * a.pool.kv + head) << a.pool.lp) +
+                         (key_of(step, t) & ((1 << a.pool.lp) - 1))) * D;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        kf[t][kk] = *reinterpret_cast<const u32x4 *>(pk + at + 32 * kk);
+    }
+  };
+  if (wave < steps) fetch(wave);
+  u32x4 qf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk)
+    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + hq * D + 32 * kk + 8 * g);
+  if (wave < steps) {
+    load(wave);
+    fetch(min(wave + WW, steps - 1));
+  }
+  float *to = a.t + (((int64_t)f.s * a.pool.kv + head) * a.most + col) * a.wide + 4 * g;
+  float ref = -INFINITY, sum = 0.0f;
+  for (int step = wave; step < steps; step += WW) {
+    const int kb = k0 + step * 32;
+    f32x4 t[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      t[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        t[b] = E::mma(__builtin_bit_cast(V8, kf[b][kk]), __builtin_bit_cast(V8, qf[kk]), t[b]);
+    }
+    if (step + WW < steps) {
+      load(step + WW);
+      fetch(min(step + 2 * WW, steps - 1));
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) t[b] *= a.scale;
+    f32x4 kept[2] = {t[0], t[1]};
+    if (kb + 32 > clear || kb + 32 > k1) {
+      uint32_t seen = (uint32_t)seen64(a, w, i, kb);
+      if (k1 - kb < 32) seen &= ~0u >> (32 - (k1 - kb));
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!(seen >> (16 * b + 4 * g + r) & 1)) t[b][r] = -INFINITY, kept[b][r] = UNSEEN;
+    }
+    if (col < w.pairs) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        if (kb + 16 * b < k1) *reinterpret_cast<f32x4 *>(to + kb + 16 * b) = kept[b];
+    }
+    float hi = t[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) hi = __builtin_elementwise_maximum(hi, t[e >> 2][e & 3]);
+    if (__ballot(!(hi - ref <= SLACK)) != 0) {
+      const float now = __builtin_elementwise_maximum(ref, hi);
+      sum *= __builtin_amdgcn_exp2f(ref - (now == -INFINITY ? 0.0f : now));
+      ref = now;
+    }
+    const float from = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += __builtin_amdgcn_exp2f(t[e >> 2][e & 3] - from);
+  }
+#pragma unroll
+  for (int m = 16; m < 64; m <<= 1) join(ref, sum, exl3::xor_lanes(ref, m), exl3::xor_lanes(sum, m));
+  __syncthreads();
+  if (bad) sbad = 1;
+  if (g == 0) so[wave][col] = f32x2{ref, sum};
+  __syncthreads();
+  const int64_t slot = (int64_t)(f.first + f.j) * a.pool.kv + head;
+  if (threadIdx.x < FEW && slot < a.slots) {
+    ref = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < WW; ++x) join(ref, sum, so[x][threadIdx.x][0], so[x][threadIdx.x][1]);
+    if (sbad) sum = __builtin_nanf("");
+    a.part[slot * FEW + threadIdx.x] = f32x2{ref, sum};
+  }
+}
+
+// The second pass: the same keys' scores again, 4 keys a thread, once the
+// items of the sequence are joined.
+__global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
+  __shared__ f32x2 so[16][FEW];
+  const int head = blockIdx.x % a.pool.kv;
+  const Find f = find<ITEM>(a, blockIdx.x / a.pool.kv);
+  if (f.s < 0) return;
+  const Watch &w = f.w;
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
+  float ref = -INFINITY, sum = 0.0f;
+  for (int j = row; j < f.parts; j += 16) {
+    const int64_t slot = (int64_t)(f.first + j) * a.pool.kv + head;
+    if (slot >= a.slots) break;
+    const f32x2 v = a.part[slot * FEW + col];
+    join(ref, sum, v[0], v[1]);
+  }
+  so[row][col] = f32x2{ref, sum};
+  __syncthreads();
+  if (threadIdx.x < FEW) {
+    for (int x = 1; x < 16; ++x) join(ref, sum, so[x][col][0], so[x][col][1]);
+    so[0][col] = ended(ref, sum);
+  }
+  __syncthreads();
+  const int k0 = (int)min((int64_t)f.j * f.each * 64, (int64_t)w.keys);
+  const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
+  const float *from = a.t + ((int64_t)f.s * a.pool.kv + head) * a.most * a.wide;
+  float *score = a.score + ((int64_t)f.s * a.pool.kv + head) * a.room;
+  const int base = a.base ? a.base[f.s] : w.len;
+  for (int k = k0 + 4 * (int)threadIdx.x; k < k1; k += 256 * WW) {
+    f32x4 acc{0, 0, 0, 0};
+    for (int p = 0; p < w.pairs; ++p) {
+      const f32x4 t = *reinterpret_cast<const f32x4 *>(from + (int64_t)p * a.wide + k);
+      const f32x2 r = so[0][p];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = fmaf(__builtin_amdgcn_exp2f(t[e] - r[0]), r[1], acc[e]);
+        if (t[e] != UNSEEN) acc[e] = x;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k + e < k1) score[k + e] = k + e < base ? a.decay * score[k + e] + acc[e] : acc[e];
+  }
+}
+
 // ------------------------------------------------------------------- eviction
 
 struct EvictArgs {
@@ -423,6 +598,8 @@ struct EvictArgs {
 
 constexpr int PICK = 1024;   // threads that pick a head's keys
 constexpr int BINS = 2048;
+constexpr int HELD = 32768;  // scores of a head in LDS
+constexpr int FEWEST = 512;  // keys whose border is found by rank
 
 // Keys that a sequence keeps, or -1: it stays as it is.
 __device__ __forceinline__ int budget_of(const EvictArgs &a, int s, int len) {
@@ -464,17 +641,20 @@ __device__ __forceinline__ uint32_t before(uint32_t v, uint32_t (&waves)[PICK / 
 
 // A workgroup a sequence, layer and kv head.  The budget's border is found by
 // counting: the range of the scores in BINS bins, then the bin that holds the
-// border in BINS again, three rounds at most (32 bits of order).  Bins divide
-// the range that the scores have, so that few of them fall into one and the
-// counters in LDS are rarely fought over.  Then the keys above the border, and as
-// many of those on it as are left, earliest first, get their places by counting
-// again.  Up to E * 1024 scores stay in registers; more are read again.
-template <int E>
-__global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a) {
+// border in BINS again, three rounds at most (32 bits of order), or, once a bin
+// holds few keys, by each one's rank among them.  Bins divide the range that
+// the scores have, so that few of them fall into one and the counters in LDS are
+// rarely fought over.  Then the keys above the border, and as many of those on
+// it as are left, earliest first, get their places by counting again.  Scores
+// stay in LDS, HELD of them; where there are more they are read again.
+__global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a, int held) {
+  extern __shared__ float scores[];
   __shared__ uint32_t bins[BINS], waves[PICK / 64];
   __shared__ uint32_t lows[PICK / 64], highs[PICK / 64];
-  __shared__ uint32_t rows[E * PICK / 64];
-  __shared__ int chosen, above;
+  __shared__ uint32_t rows[HELD / 64];
+  __shared__ int chosen, above, holds, count, found_ties;
+  __shared__ uint32_t found;
+  uint32_t *const cand = bins;  // FEWEST keys, then their numbers
   const int heads = a.layers * a.pool.kv;
   const int s = blockIdx.x / heads, lh = blockIdx.x - s * heads;
   const int layer = lh / a.pool.kv, h = lh - layer * a.pool.kv;
@@ -485,6 +665,15 @@ __global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a) {
   const float *score = a.score + at * a.room;
   float *to_score = a.new_score + at * a.room;
   int32_t *kept = a.kept + at * a.most;
+  // a thread reads what it has written: keys tid, tid + PICK, ... of a block
+  const int blocks = b < 0 ? 0 : (len + held - 1) / held;
+  auto read = [&](int blk) {
+    const int n = min(held, len - blk * held);
+#pragma unroll 8
+    for (int i = tid; i < n; i += PICK) scores[i] = score[blk * held + i];
+    return n;
+  };
+  if (blocks == 1) read(0);
   bool bad = b < 0;
   if (!bad)
     for (int x = tid; x < (len + (1 << a.pool.lp) - 1) >> a.pool.lp; x += PICK)
@@ -496,51 +685,36 @@ __global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a) {
   const int head = min(a.first, b), tail = min(a.last, b - head);  // those that stay anyway
   const int lo = head, hi = len - tail;                            // the others
   int need = b - head - tail;
-  float x[E];
-  const int blocks = (len + E * PICK - 1) / (E * PICK);
-  auto read = [&](int blk) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = (blk * E + e) * PICK + tid;
-      x[e] = i < len ? score[i] : 0.0f;
+  // f(key, its number) for the thread's keys among the others
+  auto each = [&](auto &&f) {
+    for (int blk = 0; blk < blocks; ++blk) {
+      const int n = blocks > 1 ? read(blk) : len, from = blk * held;
+#pragma unroll 4
+      for (int i = tid; i < n; i += PICK)
+        if (from + i >= lo && from + i < hi) f(ordered(scores[i]), from + i);
     }
   };
-  auto among = [&](int blk, int e) {
-    const int i = (blk * E + e) * PICK + tid;
-    return i >= lo && i < hi;
-  };
-  if (blocks == 1) read(0);
   // the border: keys of more than `border` stay, and the first `ties` on it
   uint32_t border = ~0u;
   int ties = 0;
   if (need > 0) {
     uint32_t low = ~0u, high = 0;
-    for (int blk = 0; blk < blocks; ++blk) {
-      if (blocks > 1) read(blk);
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (among(blk, e)) low = min(low, ordered(x[e])), high = max(high, ordered(x[e]));
-    }
+    each([&](uint32_t k, int) { low = min(low, k), high = max(high, k); });
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1)
       low = min(low, (uint32_t)__shfl_xor((int)low, m)), high = max(high, (uint32_t)__shfl_xor((int)high, m));
     if (lane == 0) lows[wave] = low, highs[wave] = high;
+    for (int i = tid; i < BINS; i += PICK) bins[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < PICK / 64; ++w) low = min(low, lows[w]), high = max(high, highs[w]);
     uint32_t width = high - low;  // the range: low .. low + width
     for (;;) {
       const int shift = max(0, 32 - (width ? __builtin_clz(width) : 32) - 11);
-      for (int i = tid; i < BINS; i += PICK) bins[i] = 0;
-      __syncthreads();
-      for (int blk = 0; blk < blocks; ++blk) {
-        if (blocks > 1) read(blk);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t d = ordered(x[e]) - low;
-          if (among(blk, e) && d <= width) atomicAdd(&bins[d >> shift], 1u);
-        }
-      }
+      each([&](uint32_t k, int) {
+        if (k - low <= width) atomicAdd(&bins[(k - low) >> shift], 1u);
+      });
+      if (tid == 0) count = 0;
       __syncthreads();
       // a thread's two bins, the highest first
       const int top = BINS - 1 - 2 * tid;
@@ -551,48 +725,73 @@ __global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a) {
         const bool second = over + n1 < (uint32_t)need;
         chosen = top - second;
         above = (int)(over + (second ? n1 : 0));
+        holds = (int)(second ? n0 : n1);
       }
       __syncthreads();
-      const int bin = chosen;
+      const int bin = chosen, n = holds;
       need -= above;
       low += (uint32_t)bin << shift;
       width = min((1u << shift) - 1, width - ((uint32_t)bin << shift));
+      border = low, ties = need;
       if (shift == 0) break;
+      if (n <= FEWEST) {
+        each([&](uint32_t k, int i) {
+          if (k - low > width) return;
+          const int c = atomicAdd(&count, 1);
+          cand[c] = k, cand[FEWEST + c] = i;
+        });
+        __syncthreads();
+        if (tid < n) {
+          const uint32_t k = cand[tid], i = cand[FEWEST + tid];
+          int more = 0, same = 0;  // before this one: of higher keys, of the same and an earlier number
+          for (int c = 0; c < n; ++c) {
+            more += cand[c] > k;
+            same += cand[c] == k && cand[FEWEST + c] < i;
+          }
+          if (more + same == need - 1) found = k, found_ties = need - more;
+        }
+        __syncthreads();
+        border = found, ties = found_ties;
+        break;
+      }
+      for (int i = tid; i < BINS; i += PICK) bins[i] = 0;
+      __syncthreads();
     }
-    border = low, ties = need;
   }
   // places: what stays whatever the ties are, and the ties, before each key
   uint32_t sure0 = 0, tie0 = 0;  // of the blocks before
   for (int blk = 0; blk < blocks; ++blk) {
-    if (blocks > 1) read(blk);
-    uint32_t mine = 0;  // a bit an e: sure
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = (blk * E + e) * PICK + tid;
-      const bool sure = i < len && (i < lo || i >= hi || ordered(x[e]) > border);
-      const bool tie = among(blk, e) && ordered(x[e]) == border;
-      mine |= (uint32_t)sure << e;
-      const uint64_t bs = __ballot(sure), bt = __ballot(tie);
+    const int n = blocks > 1 ? read(blk) : len, from = blk * held;
+    const int turns = (n + PICK - 1) / PICK;
+    auto kind = [&](int e, uint64_t &bs, uint64_t &bt) {
+      const int i = e * PICK + tid, key = from + i;
+      const uint32_t k = i < n ? ordered(scores[i]) : 0;
+      const bool other = key >= lo && key < hi;
+      bs = __ballot(i < n && (!other || k > border));
+      bt = __ballot(i < n && other && k == border);
+    };
+    for (int e = 0; e < turns; ++e) {
+      uint64_t bs, bt;
+      kind(e, bs, bt);
       if (lane == 0) rows[e * (PICK / 64) + wave] = (uint32_t)__popcll(bs) | (uint32_t)__popcll(bt) << 16;
     }
     __syncthreads();
     uint32_t whole;
-    const uint32_t v = tid < E * PICK / 64 ? rows[tid] : 0;
-    const uint32_t pre = before(v, waves, whole);
-    if (tid < E * PICK / 64) rows[tid] = pre;
+    const bool has = tid < turns * (PICK / 64);
+    const uint32_t pre = before(has ? rows[tid] : 0, waves, whole);
+    if (has) rows[tid] = pre;
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = (blk * E + e) * PICK + tid;
-      const bool sure = mine >> e & 1, tie = among(blk, e) && ordered(x[e]) == border;
-      const uint64_t bs = __ballot(sure), bt = __ballot(tie), under = (1ull << lane) - 1;
+    for (int e = 0; e < turns; ++e) {
+      uint64_t bs, bt;
+      kind(e, bs, bt);
+      const uint64_t under = (1ull << lane) - 1;
       const uint32_t r = rows[e * (PICK / 64) + wave];
       const uint32_t ns = sure0 + (r & 0xFFFFu) + __popcll(bs & under);
       const uint32_t nt = tie0 + (r >> 16) + __popcll(bt & under);
-      if (sure || (tie && nt < (uint32_t)ties)) {
+      if (bs >> lane & 1 || (bt >> lane & 1 && nt < (uint32_t)ties)) {
         const uint32_t place = ns + min(nt, (uint32_t)ties);
-        kept[place] = i;
-        to_score[place] = x[e];
+        kept[place] = from + e * PICK + tid;
+        to_score[place] = scores[e * PICK + tid];
       }
     }
     sure0 += whole & 0xFFFFu;
@@ -688,6 +887,32 @@ size_t refs_bytes(const exl3p_cache *c, const exl3p_rows *r, int group) {
   return up16((size_t)r->rows * group * c->kv_heads * sizeof(f32x2));
 }
 
+// How the weights are formed, by what the host knows.  Pairs whose scores are
+// kept read the keys once and the scores (4 bytes a pair and key) twice; others
+// read the keys twice.
+struct Plan {
+  int group;
+  int64_t tiles, items;  // at most
+  int few;               // pairs whose scores are kept, 0: none
+  int wide;              // of a row of them
+  size_t parts, rest;    // bytes
+};
+constexpr size_t KEPT_MAX = (size_t)1 << 30;
+Plan plan_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads, int32_t window, int32_t room) {
+  Plan p;
+  p.group = heads / c->kv_heads;
+  const int64_t rows = window > 0 && window < r->max_rows ? window : r->max_rows;
+  p.wide = (room + 15) & ~15;
+  p.tiles = most_tiles(r, p.group, window);
+  p.items = target_of(c) + p.tiles;
+  p.few = rows * p.group <= FEW ? (int)(rows * p.group) : 0;
+  p.rest = (size_t)r->seqs * c->kv_heads * p.few * p.wide * sizeof(float);
+  if (p.rest > KEPT_MAX) p.few = 0;
+  if (p.few == 0) p.rest = refs_bytes(c, r, p.group);
+  p.parts = (size_t)p.items * c->kv_heads * (p.few ? FEW : TILE) * sizeof(f32x2);
+  return p;
+}
+
 exl3_verdict check_score(const void *p, int32_t room) {
   if (p == nullptr) return refuse(EXL3_FAILED, "PagedScore: a missing array");
   if (!aligned(p, 4)) return refuse(EXL3_UNSUPPORTED, "PagedScore: elements on their own boundaries");
@@ -704,9 +929,8 @@ size_t exl3p_weigh_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int3
   if (check_cache(c).code != EXL3_OK || check_rows(c, r).code != EXL3_OK ||
       check_heads(c, heads).code != EXL3_OK || window < 0 || room <= 0)
     return 0;
-  const int group = heads / c->kv_heads;
-  return (size_t)(target_of(c) + most_tiles(r, group, window)) * c->kv_heads * TILE * sizeof(f32x2) +
-         refs_bytes(c, r, group);
+  const Plan p = plan_of(c, r, heads, window, room);
+  return p.parts + p.rest;
 }
 
 exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
@@ -726,9 +950,8 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
   if (r->rows == 0 || r->seqs == 0 || r->max_rows == 0) return OK;
   EXL3P_TRY(check_score(score, room));
   EXL3P_TRY(check_matrix(q, q_stride, (int64_t)heads * c->dim));
-  const int group = heads / c->kv_heads;
-  const int64_t tiles = most_tiles(r, group, window), items = target_of(c) + tiles;
-  if ((int64_t)r->rows * group > INT32_MAX / 2 || items * c->kv_heads > GRID_MAX)
+  const Plan p = plan_of(c, r, heads, window, room);
+  if ((int64_t)r->rows * p.group > INT32_MAX / 2 || p.items * c->kv_heads > GRID_MAX)
     return refuse(EXL3_TOO_LARGE, "PagedWeigh: too many rows and heads for one call");
   const size_t need = exl3p_weigh_scratch_bytes(c, r, heads, window, room);
   if (scratch == nullptr || !aligned(scratch, 16) || scratch_bytes < need)
@@ -740,17 +963,24 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
                          array(r->cu, 4 * ((int64_t)r->seqs + 1)), array(r->len, 4 * (int64_t)r->seqs),
                          array(base, 4 * (int64_t)r->seqs), table_of(c)}));
   WeighArgs a;
-  a.pool = pool, a.st = step_of(r), a.group = group, a.window = window;
+  a.pool = pool, a.st = step_of(r), a.group = p.group, a.window = window;
   a.q = static_cast<const uint16_t *>(q), a.qs = q_stride, a.mask = mask, a.words = words;
   a.scale = scale * LOG2E, a.decay = decay, a.base = base, a.score = score, a.room = room;
-  a.target = (float)target_of(c), a.slots = (int)(items * c->kv_heads);
-  a.ref = static_cast<f32x2 *>(scratch);
-  a.part = reinterpret_cast<f32x2 *>(static_cast<char *>(scratch) + refs_bytes(c, r, group));
+  a.target = (float)target_of(c), a.slots = (int)(p.items * c->kv_heads);
+  a.least = p.few ? 2.0f : 4.0f;
+  a.part = static_cast<f32x2 *>(scratch);
+  a.ref = reinterpret_cast<f32x2 *>(static_cast<char *>(scratch) + p.parts);
+  a.t = reinterpret_cast<float *>(a.ref), a.most = p.few, a.wide = p.wide;
   const hipStream_t st = static_cast<hipStream_t>(s);
+  const dim3 items((unsigned)(p.items * c->kv_heads));
   return by_type(c, [&](auto e, auto d) {
-    hipLaunchKernelGGL((weigh_sums_kernel<decltype(e), d>), dim3((unsigned)(items * c->kv_heads)),
-                       dim3(64 * WW), 0, st, a);
-    hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)(tiles * c->kv_heads)), dim3(TILE), 0, st, a);
+    if (p.few) {
+      hipLaunchKernelGGL((weigh_few_sums_kernel<decltype(e), d>), items, dim3(64 * WW), 0, st, a);
+      hipLaunchKernelGGL(weigh_few_keys_kernel, items, dim3(64 * WW), 0, st, a);
+      return;
+    }
+    hipLaunchKernelGGL((weigh_sums_kernel<decltype(e), d>), items, dim3(64 * WW), 0, st, a);
+    hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)(p.tiles * c->kv_heads)), dim3(TILE), 0, st, a);
     hipLaunchKernelGGL((weigh_keys_kernel<decltype(e), d>), dim3((unsigned)(2 * target_of(c) * c->kv_heads)),
                        dim3(64 * WW), 0, st, a);
   });
@@ -789,10 +1019,8 @@ exl3_verdict exl3p_evict(const exl3p_cache *c, int32_t seqs, const int32_t *len,
   a.len = len, a.score = score, a.room = room, a.keep = keep, a.most = most;
   a.first = first, a.last = last, a.kept = kept, a.new_score = new_score, a.new_len = new_len;
   const hipStream_t st = static_cast<hipStream_t>(s);
-  if (room <= 8 * PICK)
-    hipLaunchKernelGGL(evict_pick_kernel<8>, dim3((unsigned)n), dim3(PICK), 0, st, a);
-  else
-    hipLaunchKernelGGL(evict_pick_kernel<32>, dim3((unsigned)n), dim3(PICK), 0, st, a);
+  const int held = room < HELD ? (room + PICK - 1) / PICK * PICK : HELD;
+  hipLaunchKernelGGL(evict_pick_kernel, dim3((unsigned)n), dim3(PICK), held * sizeof(float), st, a, held);
   if (c->dim == 64)
     hipLaunchKernelGGL(evict_move_kernel<64>, dim3((unsigned)(n * parts)), dim3(MV), 0, st, a);
   else
