@@ -19,7 +19,8 @@ struct Vec {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(typename E::T) == 4) {
-        x[i] = __builtin_bit_cast(float, raw[i]);
+        const uint32_t v = raw[i];  // (a bit cast of an element itself takes the first)
+        x[i] = __builtin_bit_cast(float, v);
       } else {
         x[2 * i] = to_f32<E>(raw[i] & 0xFFFFu);
         x[2 * i + 1] = to_f32<E>(raw[i] >> 16);
@@ -267,7 +268,7 @@ __device__ __forceinline__ void row_stats(const VerifyArgs &a, Walk<N, DRAFT> &w
   if (threadIdx.x == 0) {
     for (int x = 1; x < waves; ++x) mass += w.sums[x], best = min(best, w.bests[x]);
     const bool whole = heat == 0.0f ? all > -INFINITY : all > -INFINITY && all < INFINITY && mass > 0.0 && mass < INFINITY;
-    w.top[i] = all, w.best[i] = best, w.mass[i] = whole ? mass : -1.0;
+    w.top[i] = all, w.best[i] = best, w.mass[i] = !whole ? -1.0 : heat == 0.0f ? 1.0 : mass;
   }
   __syncthreads();
 }
@@ -333,7 +334,7 @@ __device__ __forceinline__ Tip walk(const VerifyArgs &a, Walk<N, DRAFT> &w, int 
       for (int x = 1; x < 16; x <<= 1) m += __shfl_xor(m, x, 16), best = min(best, __shfl_xor(best, x, 16));
       if (g == 0) {
         const bool whole = fit && (greedy ? all > -INFINITY : all > -INFINITY && all < INFINITY && m > 0.0 && m < INFINITY);
-        w.top[i] = all, w.best[i] = best, w.mass[i] = whole ? m : -1.0;
+        w.top[i] = all, w.best[i] = best, w.mass[i] = !whole ? -1.0 : greedy ? 1.0 : m;
       }
     }
   }
