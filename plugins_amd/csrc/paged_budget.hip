@@ -15,7 +15,8 @@ struct WeighArgs {
   int64_t qs;
   const uint64_t *mask;
   int words;
-  float scale;  // log2(e) times the scale: weights are powers of two
+  float scale;    // |scale| log2(e): weights are powers of two
+  uint32_t flip;  // 0x80008000 where the scale is negative: q's sign bits
   float decay;
   const int32_t *base;
   float *score;
@@ -23,17 +24,25 @@ struct WeighArgs {
   float target;  // items of a kv head
   float least;   // 64-key units of one, at least
   int slots;     // items * kv that part holds
-  f32x2 *part;   // [items * kv][TILE]: an item's reference and sum of each pair
-  f32x2 *ref;    // [kv][rows * group]: a pair's reference, and one over its sum
-  float *t;      // few pairs: [seqs][kv][most][wide] scores, in place of ref
+  int tile;      // pairs of an item
+  f32x2 *part;   // [items * kv][tile]: an item's reference and sum of each pair
+  float *lse;    // [kv][rows * group]: the power of two that a pair's weights sum to
+  float *t;      // few pairs: [seqs][kv][most][wide] scores, in place of lse
   int most, wide;
+  int deal;      // pairs that an item of the second pass adds up, whole tiles
+  int deals;     // such items of a key, at most; where there are several:
+  float *sums;   // [seqs][kv][deals][room]: their sums
 };
 
 constexpr int WW = 4;       // waves of a workgroup
-constexpr int TILE = 128;   // pairs of a row and a query head that an item has
-constexpr int FEW = 16;     // or, where no sequence has more, this many
-constexpr int KEYS = 128;   // keys that a workgroup adds up weights for
+constexpr int TILE = 128;   // pairs of a row and a query head that an item has,
+constexpr int FEW = 16;     // pairs of a row and a query head that a tile has where scores are kept
+constexpr int PART = 4096;  // keys of an item of the second pass, at most
 constexpr float SLACK = 4.0f;  // a reference follows its maximum in steps of more (powers of two)
+// Up to references of FAR a weight's exponent is one multiply-add of score, scale
+// and reference; beyond, the reference's rounding is whole powers of two, and
+// scores are multiplied first.
+constexpr float FAR = 0x1p20f;
 
 // A sequence's rows that count and its keys.
 struct Watch {
@@ -54,82 +63,86 @@ __device__ __forceinline__ Watch watch_of(const WeighArgs &a, int s) {
   return w;
 }
 
-// Sum over the lanes up to and with this one.
-__device__ __forceinline__ int scan(int v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int y = __shfl_up(v, m);
-    if ((int)(threadIdx.x & 63) >= m) v += y;
-  }
-  return v;
-}
-
-enum Kind { ITEM, PAIRS, SPAN };  // (tile, part of the keys); tile; KEYS keys
+enum Kind { ITEM, PAIRS, DEAL };  // part of a tile's keys; a tile; part of a deal's keys
 struct Find {
   int s;       // -1: nothing
-  int u, j;    // tile of pairs, part of the keys
+  int u, j;    // tile or deal of pairs, part of the keys
   int first;   // the tile's first item
-  int parts;   // items of a tile
+  int parts;   // items of a tile or deal
   int each;    // 64-key units of one
+  int tiles;   // tiles or deals of the sequence
   Watch w;
 };
 
-// Number x among the sequences' items, tiles or spans of keys.  A tile of u units of
-// 64 keys has ceil(u / c) items, c the units of all tiles over the target, and
-// what a 32-bit sum may be short of: items are never more than target + tiles.
+// Numbers among the sequences' items.  A tile (or deal of tiles) of u units of 64 keys
+// has ceil(u / c) items, c the units of all over the target, and what a 32-bit sum may
+// be short of: items are never more than target + tiles (deals: where their parts are
+// not cut short at PART).  A lane keeps a sequence, of up to 64.
 template <Kind KIND>
-__device__ __forceinline__ Find find(const WeighArgs &a, int x) {
-  const int lane = threadIdx.x & 63;
-  Find f;
-  f.s = -1;
+struct Finder {
+  const WeighArgs &a;
   Watch w{};
-  float units = 0.0f;
-  bool back = false;
-  for (int s = lane; s < a.st.seqs; s += 64) {
-    w = watch_of(a, s);
-    back |= w.back;
-    units += (float)((w.pairs + TILE - 1) / TILE) * (float)((w.keys + 63) >> 6);
+  int chunk = 1;
+  bool none = false;
+  __device__ __forceinline__ int tiles_of(const Watch &v) const {
+    const int t = KIND == DEAL ? a.deal : a.tile;
+    return (v.pairs + t - 1) / t;
   }
-  if (__ballot(back) != 0) return f;
+  __device__ __forceinline__ explicit Finder(const WeighArgs &args) : a(args) {
+    float units = 0.0f;
+    bool back = false;
+    for (int s = threadIdx.x & 63; s < a.st.seqs; s += 64) {
+      w = watch_of(a, s);
+      back |= w.back;
+      units += (float)tiles_of(w) * (float)((w.keys + 63) >> 6);
+    }
+    none = __ballot(back) != 0;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) units += exl3::xor_lanes(units, m);
-  const int chunk = __builtin_amdgcn_readfirstlane(
-      (int)fminf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / a.target), a.least), (float)(1 << 25)));
-  int before = 0, items = 0;
-  for (int s0 = 0; s0 < a.st.seqs; s0 += 64) {
-    const int s = s0 + lane;
-    int tiles = 0, ns = 0, each = 1, count = 0;
-    if (s < a.st.seqs) {
-      if (a.st.seqs > 64) w = watch_of(a, s);
-      if (w.pairs > 0) {
-        const int u = (w.keys + 63) >> 6;
-        tiles = (w.pairs + TILE - 1) / TILE;
-        ns = (u + chunk - 1) / chunk;
-        each = (u + ns - 1) / ns;  // the last items may be empty
-        count = KIND == ITEM ? tiles * ns : KIND == PAIRS ? tiles : (w.keys + KEYS - 1) / KEYS;
-      }
-    }
-    const int ct = scan(count), it = KIND == SPAN ? 0 : scan(tiles * ns);
-    const uint64_t past = __ballot(before + ct > x);
-    if (past != 0) {
-      const int l = __builtin_ctzll(past);
-      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      const int y = x - before - of(ct - count), nt = of(tiles), n_s = of(ns);
-      f.s = s0 + l;
-      f.w = Watch{of(w.row), of(w.n), of(w.len), of(w.lo), of(w.pairs), of(w.keys), false};
-      f.parts = n_s;
-      f.each = of(each);
-      // tiles that read the same keys side by side
-      f.j = KIND == ITEM ? y / nt : 0;
-      f.u = KIND == ITEM ? y - f.j * nt : y;
-      f.first = items + of(it - tiles * ns) + f.u * n_s;
-      return f;
-    }
-    before += __builtin_amdgcn_readlane(ct, 63);
-    if (KIND != SPAN) items += __builtin_amdgcn_readlane(it, 63);
+    for (int m = 1; m < 64; m <<= 1) units += exl3::xor_lanes(units, m);
+    chunk = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / a.target), a.least),
+                                                      KIND == DEAL ? (float)(PART / 64) : (float)(1 << 25)));
   }
-  return f;
-}
+  __device__ __forceinline__ Find at(int x) {
+    Find f;
+    f.s = -1;
+    if (none) return f;
+    int before = 0, items = 0;
+    for (int s0 = 0; s0 < a.st.seqs; s0 += 64) {
+      const int s = s0 + (int)(threadIdx.x & 63);
+      int tiles = 0, ns = 0, each = 1, count = 0;
+      if (s < a.st.seqs) {
+        if (a.st.seqs > 64) w = watch_of(a, s);
+        if (w.pairs > 0) {
+          const int u = (w.keys + 63) >> 6;
+          tiles = tiles_of(w);
+          ns = (u + chunk - 1) / chunk;
+          each = (u + ns - 1) / ns;  // the last items may be empty
+          count = KIND == PAIRS ? tiles : tiles * ns;
+        }
+      }
+      const int ct = scan(count), it = KIND == PAIRS ? scan(tiles * ns) : ct;
+      const uint64_t past = __ballot(before + ct > x);
+      if (past != 0) {
+        const int l = __builtin_ctzll(past);
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+        const int y = x - before - of(ct - count), nt = of(tiles), n_s = of(ns);
+        f.s = s0 + l;
+        f.w = Watch{of(w.row), of(w.n), of(w.len), of(w.lo), of(w.pairs), of(w.keys), false};
+        f.parts = n_s;
+        f.each = of(each);
+        f.tiles = nt;
+        // tiles that read the same keys side by side, the last, whose rows see most, first
+        f.j = KIND == PAIRS ? 0 : y / nt;
+        f.u = nt - 1 - (y - f.j * nt);
+        f.first = items + of(it - tiles * ns) + f.u * n_s;
+        return f;
+      }
+      before += __builtin_amdgcn_readlane(ct, 63);
+      items += __builtin_amdgcn_readlane(it, 63);
+    }
+    return f;
+  }
+};
 
 // Which of keys kb .. kb + 63 row i of a sequence sees, a bit a key.
 __device__ __forceinline__ uint64_t seen64(const WeighArgs &a, const Watch &w, int i, int kb) {
@@ -147,12 +160,6 @@ __device__ __forceinline__ uint64_t seen64(const WeighArgs &a, const Watch &w, i
   return v;
 }
 
-// 16 bytes a lane from its own address to LDS at `lds` + 16 * lane.
-__device__ __forceinline__ void lds_dma16_at(const void *p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p)
-               : "memory");
-}
-
 // The places of a row's 16-byte pieces in LDS: those of one number of 16 rows lie in
 // 16 places of the banks.
 template <int D>
@@ -160,13 +167,16 @@ __device__ __forceinline__ int swizzle(int row) {
   return D == 128 ? row & 15 : (row >> 1) & 7;
 }
 
+// The larger, NaN if either is.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // A score that a row does not see, where scores are kept: its weight is none, also
 // where the row's sum is NaN.
 constexpr float UNSEEN = -0x1.fffffep127f;
 
 // Two parts of a pair's keys: the reference and the sum of weights of both.
 __device__ __forceinline__ void join(float &ref, float &sum, float other, float more) {
-  const float now = __builtin_elementwise_maximum(ref, other), from = now == -INFINITY ? 0.0f : now;
+  const float now = larger(ref, other), from = now == -INFINITY ? 0.0f : now;
   sum = sum * __builtin_amdgcn_exp2f(ref - from) + more * __builtin_amdgcn_exp2f(other - from);
   ref = now;
 }
@@ -177,20 +187,69 @@ __device__ __forceinline__ f32x2 ended(float ref, float sum) {
                sum == 0.0f ? 0.0f : ref != ref ? ref : 1.0f / sum};
 }
 
+// An item's keys, tiles of 64 of which pass through LDS, the next loaded while one is
+// used: 16 a wave, by direct loads.
+template <typename E, int D>
+struct Keys {
+  static constexpr int ROW = D * 2, ARR = 64 * ROW;
+  static constexpr int LOADS = 16 * ROW / 1024, LR = 1024 / ROW;  // loads a wave, rows a load
+  typedef typename E::V8 V8;
+  const WeighArgs &a;
+  int k0, last, wave, head;
+  const int *trow;
+  const char *lds;
+  uint32_t lbase, ka, id = 0, voff[LOADS];
+  bool bad = false;
+  __device__ __forceinline__ Keys(const WeighArgs &args, const char *to, int s, int head_, int from, int end)
+      : a(args), k0(from), last(end), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), head(head_),
+        trow(args.pool.table + (size_t)s * args.pool.max_pages), lds(to),
+        lbase(__builtin_amdgcn_readfirstlane(
+            (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)to)) {
+    const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+    ka = col * ROW + 16 * (h ^ swizzle<D>(col));
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+      const int row = LR * u + lane / (ROW / 16), place = lane % (ROW / 16);
+      voff[u] = row * ROW + (place ^ swizzle<D>(row)) * 16;
+    }
+  }
+  // blocks behind the last key stand for the last key's
+  __device__ __forceinline__ int key_of(int step) const {
+    return min(k0 + step * 64 + 16 * wave, (last - 1) & ~15);
+  }
+  __device__ __forceinline__ void fetch(int step) { id = (uint32_t)trow[key_of(step) >> a.pool.lp]; }
+  __device__ __forceinline__ void load(int step, int buffer) {
+    uint32_t page = __builtin_amdgcn_readfirstlane(id);
+    if (page >= (uint32_t)a.pool.pages) bad = true, page = 0;
+    const size_t at = ((((size_t)page * a.pool.kv + head) << a.pool.lp) +
+                       (key_of(step) & ((1 << a.pool.lp) - 1))) * ROW;
+    const uint32_t to = lbase + buffer * ARR + 16 * wave * ROW;
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) exl3::lds_dma16(a.pool.k + at, voff[u], to + u * 1024);
+  }
+  // This wave's loads of the tile are in LDS, and so are, behind the barrier, the
+  // others'; all have read the tile before, whose place is loaded next.
+  __device__ __forceinline__ void arrive() const {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  // 8 elements of key 32 b + column, from element 16 kk + 8 h on
+  __device__ __forceinline__ V8 piece(int buffer, int b, int kk) {
+    return *reinterpret_cast<const V8 *>(lds + buffer * ARR + (ka ^ (32 * kk)) + b * 32 * ROW);
+  }
+  __device__ __forceinline__ void anew() { asm volatile("" : "+v"(ka)); }
+};
+
 // The first pass: each pair's reference (its largest score, or less by SLACK at
-// most) and the sum of its weights over an item's keys.  128 pairs a workgroup, 32
-// a wave; tiles of 64 keys pass through LDS, the next loaded while one is used.
-// Scores are S^T = K q^T (rows keys, columns pairs): a lane holds 32 keys' scores
+// most) and the sum of its weights over an item's keys.  128 pairs a workgroup, 32 a
+// wave; scores are S^T = K q^T (rows keys, columns pairs): a lane holds 32 keys' scores
 // of one pair.
 template <typename E, int D>
 __global__ __launch_bounds__(64 * WW, 2) void weigh_sums_kernel(WeighArgs a) {
-  constexpr int KK = D / 16, ROW = D * 2, ARR = 64 * ROW;
-  constexpr int LOADS = 16 * ROW / 1024, LR = 1024 / ROW;
+  constexpr int KK = D / 16;
   typedef typename E::V8 V8;
-  __shared__ __align__(1024) char lds[2 * ARR];
-  __shared__ int sbad;
+  __shared__ __align__(1024) char lds[2 * Keys<E, D>::ARR];
   const int head = blockIdx.x % a.pool.kv;
-  const Find f = find<ITEM>(a, blockIdx.x / a.pool.kv);
+  const Find f = Finder<ITEM>(a).at(blockIdx.x / a.pool.kv);
   if (f.s < 0) return;
   const Watch &w = f.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -203,59 +262,34 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_sums_kernel(WeighArgs a) {
   // the last key that the workgroup's, and the wave's, rows see
   int last = k1, mine = k1;
   if (a.mask == nullptr) {
-    last = min(last, w.len + w.lo + (min(f.u * TILE + TILE, w.pairs) - 1) / G + 1);
+    last = min(last, w.len + w.lo + (min((f.u + 1) * TILE, w.pairs) - 1) / G + 1);
     mine = min(last, w.len + w.lo + (min(r0 + 32, w.pairs) - 1) / G + 1);
   }
   if (r0 >= w.pairs) mine = k0;
   // keys below this every row of the wave sees
-  const int clear = a.mask == nullptr ? w.len + w.lo + r0 / G + 1 : w.len;
-  if (threadIdx.x == 0) sbad = 0;
+  const int clear = min(last, a.mask == nullptr ? w.len + w.lo + r0 / G + 1 : w.len);
   const int steps = last > k0 ? (last - k0 + 63) / 64 : 0;
-  const int *trow = a.pool.table + (size_t)f.s * a.pool.max_pages;
-  const uint32_t lbase = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
-  uint32_t voff[LOADS];
-#pragma unroll
-  for (int u = 0; u < LOADS; ++u) {
-    const int row = LR * u + lane / (ROW / 16), place = lane % (ROW / 16);
-    voff[u] = row * ROW + (place ^ swizzle<D>(row)) * 16;
-  }
-  bool bad = false;
-  auto key_of = [&](int step) { return min(k0 + step * 64 + 16 * wave, (last - 1) & ~15); };
-  uint32_t id = 0;
-  auto fetch = [&](int step) { id = (uint32_t)trow[key_of(step) >> a.pool.lp]; };
-  auto load = [&](int step) {
-    uint32_t page = __builtin_amdgcn_readfirstlane(id);
-    if (page >= (uint32_t)a.pool.pages) bad = true, page = 0;
-    const size_t at = ((((size_t)page * a.pool.kv + head) << a.pool.lp) +
-                       (key_of(step) & ((1 << a.pool.lp) - 1))) * ROW;
-    const uint32_t to = lbase + (step & 1) * ARR + 16 * wave * ROW;
-#pragma unroll
-    for (int u = 0; u < LOADS; ++u) exl3::lds_dma16(a.pool.k + at, voff[u], to + u * 1024);
-  };
+  Keys<E, D> keys(a, lds, f.s, head, k0, last);
   if (steps > 0) {
-    fetch(0);
-    load(0);
-    if (steps > 1) fetch(1);
+    keys.fetch(0);
+    keys.load(0, 0);
+    if (steps > 1) keys.fetch(1);
   }
   u32x4 qf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk)
-    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + hq * D + 16 * kk + 8 * h);
-  uint32_t ka = col * ROW + 16 * (h ^ swizzle<D>(col));
-  float ref = -INFINITY, sum = 0.0f;
-  for (int step = 0; step < steps; ++step) {
-    // this wave's loads of the tile are in LDS, and so are, behind the barrier, the
-    // others'; all have read the tile before, whose buffer is loaded next
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + hq * D + 16 * kk + 8 * h) ^ a.flip;
+  float ref = -INFINITY, sum = 0.0f, scale = a.scale;
+  bool far = false;  // of the wave: its scores are multiplied first, and scale is 1
+  auto turn = [&](int step, auto TAIL) {
+    keys.arrive();
     if (step + 1 < steps) {
-      load(step + 1);
-      if (step + 2 < steps) fetch(step + 2);
+      keys.load(step + 1, (step + 1) & 1);
+      if (step + 2 < steps) keys.fetch(step + 2);
     }
     const int kb = k0 + step * 64;
-    if (kb >= mine) continue;
-    const char *tk = lds + (step & 1) * ARR;
-    asm volatile("" : "+v"(ka));
+    if (kb >= mine) return;
+    keys.anew();
     f32x16 t[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -263,12 +297,9 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_sums_kernel(WeighArgs a) {
       for (int r = 0; r < 16; ++r) t[b][r] = 0.0f;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
-        t[b] = E::mma(*reinterpret_cast<const V8 *>(tk + (ka ^ (32 * kk)) + b * 32 * ROW),
-                      __builtin_bit_cast(V8, qf[kk]), t[b]);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) t[b][r] *= a.scale;
+        t[b] = E::mma(keys.piece(step & 1, b, kk), __builtin_bit_cast(V8, qf[kk]), t[b]);
     }
-    if (kb + 64 > clear || kb + 64 > last) {
+    if constexpr (decltype(TAIL)::value) {
       // element r of block b: key 32 b + 8 (r / 4) + 4 h + r % 4
       uint64_t my = seen64(a, w, i, kb);
       if (last - kb < 64) my &= ~0ull >> (64 - (last - kb));
@@ -279,144 +310,239 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_sums_kernel(WeighArgs a) {
         for (int r = 0; r < 16; ++r)
           if (!((uint32_t)(my >> (32 * b)) >> (8 * (r >> 2) + (r & 3)) & 1)) t[b][r] = -INFINITY;
     }
-    float hi = t[0][0];
+    auto multiply = [&] {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) hi = __builtin_elementwise_maximum(hi, t[b][r]);
+        for (int r = 0; r < 16; ++r) t[b][r] *= a.scale;
+    };
+    if (far) multiply();
+    float hi = larger(t[0][0], t[1][0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) hi = larger(larger(hi, t[0][r]), t[1][r]);
+    hi *= scale;
     if (__ballot(!(hi - ref <= SLACK)) != 0) {
-      const float now = __builtin_elementwise_maximum(ref, hi);
+      const float now = larger(ref, hi);
       sum *= __builtin_amdgcn_exp2f(ref - (now == -INFINITY ? 0.0f : now));
       ref = now;
+      if (!far && __ballot(fabsf(now) > FAR && now != -INFINITY) != 0) {
+        far = true, scale = 1.0f;
+        multiply();
+      }
     }
     const float from = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(t[b][r] - from);
-  }
+      for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(t[b][r], scale, -from));
+  };
+  // tiles that every row of the wave sees whole, then the others
+  const int whole = min(max(clear - k0, 0) / 64, steps);
+  int step = 0;
+  for (; step < whole; ++step) turn(step, std::false_type{});
+  for (; step < steps; ++step) turn(step, std::true_type{});
   __syncthreads();
-  if (bad) sbad = 1;
+  // (no more LDS than the tiles' own: five workgroups a CU)
+  int *const sbad = reinterpret_cast<int *>(lds);
+  if (threadIdx.x == 0) *sbad = 0;
+  __syncthreads();
+  if (keys.bad) *sbad = 1;
   __syncthreads();
   // the two halves of a pair's keys
   join(ref, sum, exl3::xor_lanes(ref, 32), exl3::xor_lanes(sum, 32));
-  if (sbad) sum = __builtin_nanf("");
+  if (*sbad) sum = __builtin_nanf("");
   const int64_t slot = (int64_t)(f.first + f.j) * a.pool.kv + head;
   if (h == 0 && r0 + col < w.pairs && slot < a.slots) a.part[slot * TILE + 32 * wave + col] = f32x2{ref, sum};
 }
 
-// A tile's items joined, a pair a thread.
-__global__ __launch_bounds__(TILE) void weigh_join_kernel(WeighArgs a) {
-  const int head = blockIdx.x % a.pool.kv;
-  const Find f = find<PAIRS>(a, blockIdx.x / a.pool.kv);
-  const int pair = f.u * TILE + (int)threadIdx.x;
-  if (f.s < 0 || pair >= f.w.pairs) return;
+// A tile's items joined, 256 / SHARE pairs a workgroup, whose items are shared out to SHARE
+// threads each.
+template <int SHARE>
+__global__ __launch_bounds__(256) void weigh_join_kernel(WeighArgs a) {
+  constexpr int OF = 256 / SHARE;
+  __shared__ f32x2 so[SHARE][OF];
+  const int head = blockIdx.x % a.pool.kv, rest = blockIdx.x / a.pool.kv;
+  const Find f = Finder<PAIRS>(a).at(rest / (a.tile / OF));
+  const int col = threadIdx.x % OF, row = threadIdx.x / OF;
+  const int in = rest % (a.tile / OF) * OF + col;
+  if (f.s < 0 || f.u * a.tile + in - col >= f.w.pairs) return;
   float ref = -INFINITY, sum = 0.0f;
-  for (int j = 0; j < f.parts; ++j) {
+  for (int j = row; j < f.parts; j += SHARE) {
     const int64_t slot = (int64_t)(f.first + j) * a.pool.kv + head;
     if (slot >= a.slots) break;
-    const f32x2 v = a.part[slot * TILE + threadIdx.x];
+    const f32x2 v = a.part[slot * a.tile + in];
     join(ref, sum, v[0], v[1]);
   }
-  a.ref[(int64_t)head * a.st.rows * a.group + (int64_t)(f.w.row + f.w.lo) * a.group + pair] = ended(ref, sum);
+  so[row][col] = f32x2{ref, sum};
+  __syncthreads();
+  const int pair = f.u * a.tile + in;
+  if (row > 0 || pair >= f.w.pairs) return;
+  for (int x = 1; x < SHARE; ++x) join(ref, sum, so[x][col][0], so[x][col][1]);
+  // (rounded as a score of its size is; a pair that sees nothing has no weights)
+  a.lse[(int64_t)head * a.st.rows * a.group + (int64_t)(f.w.row + f.w.lo) * a.group + pair] =
+      sum == 0.0f ? INFINITY : ref + __builtin_amdgcn_logf(sum);
 }
 
-// The second pass: KEYS keys a workgroup, 32 a wave in registers; the pairs pass
-// through LDS 32 at a time, the next loaded while one tile is used.  A lane adds
-// up the weights of 16 keys over the pairs of its column; the columns join at the end.
+// A key's score: what it had, and the weights of this step.
+__device__ __forceinline__ void add_score(const WeighArgs &a, const Find &f, int head, int key, float more) {
+  float *score = a.score + ((int64_t)f.s * a.pool.kv + head) * a.room + key;
+  const int base = a.base ? a.base[f.s] : f.w.len;
+  *score = key < base ? a.decay * *score + more : more;
+}
+
+// The second pass: each key's weights over a deal of pairs.  The deal's tiles take
+// their turns, each in registers (32 pairs a wave) while the item's keys pass
+// through LDS as in the first pass.  Scores are S = q K^T here (rows pairs, columns
+// keys), so that a lane adds up its key's weights over 16 pairs of a product by
+// itself; the waves' sums join through LDS, one tile of keys behind.  Several deals of a
+// key (many pairs) leave their sums for the next kernel.
 template <typename E, int D>
 __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
-  constexpr int KK = D / 16, ROW = D * 2, ARR = 32 * ROW;
-  constexpr int LOADS = 8 * ROW / 1024, LR = 1024 / ROW;
+  constexpr int KK = D / 16;
   typedef typename E::V8 V8;
-  __shared__ __align__(1024) char lds[2 * ARR];
+  __shared__ __align__(1024) char lds[2 * Keys<E, D>::ARR];
+  __shared__ float joint[2][WW][64];
+  __shared__ float total[PART];
   const int head = blockIdx.x % a.pool.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
   const int G = a.group;
-  const uint32_t lbase = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
-  uint32_t qa = col * ROW + 16 * (h ^ swizzle<D>(col));
+  Finder<DEAL> finder(a);
   for (int x = blockIdx.x / a.pool.kv;; x += gridDim.x / a.pool.kv) {
-    const Find f = find<SPAN>(a, x);
+    const Find f = finder.at(x);
     if (f.s < 0) return;
     const Watch &w = f.w;
-    const int kb0 = f.u * KEYS, kb = kb0 + 32 * wave;
-    // pairs before this one see no key of the span
-    const int p0 = a.mask == nullptr ? max(0, kb0 - w.len - w.lo) * G & ~31 : 0;
-    const int steps = (w.pairs - p0 + 31) / 32;
-    auto load = [&](int step) {
-      const uint32_t to = lbase + (step & 1) * ARR + 8 * wave * ROW;
+    const int k0 = (int)min((int64_t)f.j * f.each * 64, (int64_t)w.keys);
+    const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
+    const int p1 = min((f.u + 1) * a.deal, w.pairs);
+    for (int k = threadIdx.x; k < k1 - k0; k += 64 * WW) total[k] = 0.0f;
+    const float *lses = a.lse + (int64_t)head * a.st.rows * G + (int64_t)(w.row + w.lo) * G;
+    int count = 0;  // tiles of keys done: their places in LDS
+    auto finish = [&](int step) {
+      if (wave > 0) return;
+      float v = 0.0f;
 #pragma unroll
-      for (int u = 0; u < LOADS; ++u) {
-        const int row = 8 * wave + LR * u + lane / (ROW / 16), place = lane % (ROW / 16);
-        const int pair = min(p0 + step * 32 + row, w.pairs - 1), i = pair / G;
-        lds_dma16_at(a.q + (w.row + w.lo + i) * a.qs + (head * G + pair - i * G) * D +
-                         (place ^ swizzle<D>(row)) * 8,
-                     to + u * 1024);
-      }
+      for (int y = 0; y < WW; ++y) v += joint[(count - 1) & 1][y][lane];
+      total[step * 64 + lane] += v;
     };
-    if (steps > 0) load(0);
-    // (a key behind the last, or of no page, stands for one that is there: its
-    // weights are not kept, or are NaN)
-    const int key = min(kb + col, w.keys - 1);
-    const int sl = max(slot_of(a.pool, f.s, key), 0);
-    const char *kp = a.pool.k + ((((size_t)(sl >> a.pool.lp) * a.pool.kv + head) << a.pool.lp) +
-                                 (sl & ((1 << a.pool.lp) - 1))) * ROW + 16 * h;
-    u32x4 kf[KK];
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) kf[kk] = *reinterpret_cast<const u32x4 *>(kp + 32 * kk);
-    const f32x2 *refs = a.ref + (int64_t)head * a.st.rows * G + (int64_t)(w.row + w.lo) * G;
-    float acc[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-    for (int step = 0; step < steps; ++step) {
-      const int p = p0 + step * 32, pair = min(p + col, w.pairs - 1);
-      const f32x2 ref = refs[pair];
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (step + 1 < steps) load(step + 1);
-      const char *tq = lds + (step & 1) * ARR;
-      asm volatile("" : "+v"(qa));
-      f32x16 t;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) t[r] = 0.0f;
+    for (int p0 = f.u * a.deal; p0 < p1; p0 += TILE) {
+      // keys that the tile's rows see
+      const int last = a.mask != nullptr ? k1 : min(k1, w.len + w.lo + (min(p0 + TILE, w.pairs) - 1) / G + 1);
+      if (last <= k0) continue;
+      const int steps = (last - k0 + 63) / 64;
+      const int r0 = p0 + 32 * wave;
+      const bool any = r0 < w.pairs, full = r0 + 32 <= w.pairs;
+      const int clear = min(last, a.mask == nullptr ? w.len + w.lo + r0 / G + 1 : w.len);
+      Keys<E, D> keys(a, lds, f.s, head, k0, last);
+      keys.fetch(0);
+      __syncthreads();  // the tile before is read, and its last sums are joined below
+      keys.load(0, count & 1);
+      if (steps > 1) keys.fetch(1);
+      const int pair = min(r0 + col, w.pairs - 1), i = w.lo + pair / G;
+      u32x4 qf[KK];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
-        t = E::mma(__builtin_bit_cast(V8, kf[kk]),
-                   *reinterpret_cast<const V8 *>(tq + (qa ^ (32 * kk))), t);
-      const bool whole = p + 32 <= w.pairs &&
-                         kb + 32 <= (a.mask == nullptr ? w.len + w.lo + p / G + 1 : w.len);
-      if (whole) {
+        qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + (head * G + pair % G) * D + 16 * kk +
+                                                  8 * h) ^ a.flip;
+      // element r: pair 8 (r / 4) + 4 h + r % 4
+      float lse[16];
+      bool far = false;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          acc[r] = fmaf(__builtin_amdgcn_exp2f(t[r] * a.scale - ref[0]), ref[1], acc[r]);
-      } else {
-        // element r: key 8 (r / 4) + 4 h + r % 4.  What a row does not see it
-        // leaves alone, NaN or not.
-        const uint32_t seen = p + col < w.pairs ? (uint32_t)seen64(a, w, w.lo + pair / G, kb) >> (4 * h) : 0;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float e = fmaf(__builtin_amdgcn_exp2f(t[r] * a.scale - ref[0]), ref[1], acc[r]);
-          if (seen >> (8 * (r >> 2) + (r & 3)) & 1) acc[r] = e;
-        }
+      for (int r = 0; r < 16; ++r) {
+        lse[r] = lses[min(r0 + 8 * (r >> 2) + 4 * h + (r & 3), w.pairs - 1)];
+        far |= fabsf(lse[r]) > FAR;
       }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next span's tiles
-    float mine = 0.0f;  // column r's lane keeps element r
+      far = __ballot(far) != 0;
+      const float scale = far ? 1.0f : a.scale;
+      for (int step = 0; step < steps; ++step, ++count) {
+        keys.arrive();
+        if (step > 0) finish(step - 1);
+        if (step + 1 < steps) {
+          keys.load(step + 1, (count + 1) & 1);
+          if (step + 2 < steps) keys.fetch(step + 2);
+        }
+        const int kb = k0 + step * 64;
+        float v[2] = {0.0f, 0.0f};
+        if (any) {
+          keys.anew();
+          f32x16 t[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float v = acc[r];
+          for (int b = 0; b < 2; ++b) {
 #pragma unroll
-      for (int m = 1; m < 32; m <<= 1) v += exl3::xor_lanes(v, m);
-      if (col == r) mine = v;
+            for (int r = 0; r < 16; ++r) t[b][r] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+              t[b] = E::mma(__builtin_bit_cast(V8, qf[kk]), keys.piece(count & 1, b, kk), t[b]);
+          }
+          if (far) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) t[b][r] *= a.scale;
+          }
+          if (full && kb + 64 <= clear) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) v[b] += __builtin_amdgcn_exp2f(fmaf(t[b][r], scale, -lse[r]));
+          } else {
+            // what each of the wave's pairs sees, a pair a lane.  What a row does not see it
+            // leaves alone, NaN or not.
+            const uint64_t seen = r0 + col < w.pairs ? seen64(a, w, i, kb) : 0;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const uint32_t of = __shfl((int)(uint32_t)(seen >> (32 * b)), 8 * (r >> 2) + 4 * h + (r & 3));
+                const float e = __builtin_amdgcn_exp2f(fmaf(t[b][r], scale, -lse[r]));
+                if (of >> col & 1) v[b] += e;
+              }
+          }
+#pragma unroll
+          for (int b = 0; b < 2; ++b) v[b] += exl3::xor_lanes(v[b], 32);
+        }
+        joint[count & 1][wave][lane] = h ? v[1] : v[0];
+      }
+      __syncthreads();
+      finish(steps - 1);
     }
-    const int to = kb + 8 * (col >> 2) + 4 * h + (col & 3);
-    if (col < 16 && to < w.keys) {
-      float *score = a.score + ((int64_t)f.s * a.pool.kv + head) * a.room + to;
-      const int base = a.base ? a.base[f.s] : w.len;
-      *score = to < base ? a.decay * *score + mine : mine;
+    __syncthreads();
+    float *to = a.sums + (((int64_t)f.s * a.pool.kv + head) * a.deals + f.u) * a.room;
+    for (int k = threadIdx.x; k < k1 - k0; k += 64 * WW) {
+      if (f.tiles == 1)
+        add_score(a, f, head, k0 + k, total[k]);
+      else if (f.u < a.deals)
+        to[k0 + k] = total[k];
     }
+    __syncthreads();
   }
+}
+
+// The deals of a key added up, 64 keys a workgroup, a share of the deals a wave.
+__global__ __launch_bounds__(64 * WW) void weigh_deals_kernel(WeighArgs a) {
+  __shared__ float joint[WW][64];
+  const int spans = (a.room + 63) / 64;
+  const int head = blockIdx.x % a.pool.kv, rest = blockIdx.x / a.pool.kv;
+  Find f;
+  f.s = rest / spans;
+  f.w = watch_of(a, f.s);
+  const int tiles = min((f.w.pairs + a.deal - 1) / a.deal, a.deals);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, key = rest % spans * 64 + lane;
+  if (tiles < 2 || key - lane >= f.w.keys) return;
+  bool back = false;  // (of a step whose cu goes back nothing is done)
+  for (int s = lane; s < a.st.seqs; s += 64) back |= watch_of(a, s).back;
+  if (__ballot(back) != 0) return;
+  const float *from = a.sums + ((int64_t)f.s * a.pool.kv + head) * a.deals * a.room + min(key, f.w.keys - 1);
+  const int each = (tiles + WW - 1) / WW;
+  float v = 0.0f;
+#pragma unroll 8
+  for (int j = wave * each; j < min(tiles, (wave + 1) * each); ++j) v += from[(int64_t)j * a.room];
+  joint[wave][lane] = v;
+  __syncthreads();
+  if (wave > 0 || key >= f.w.keys) return;
+#pragma unroll
+  for (int y = 1; y < WW; ++y) v += joint[y][lane];
+  add_score(a, f, head, key, v);
 }
 
 // Few pairs (single tokens): their scores are kept in 32 bits from the first pass
@@ -430,7 +556,7 @@ __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a)
   __shared__ f32x2 so[WW][FEW];
   __shared__ int sbad;
   const int head = blockIdx.x % a.pool.kv;
-  const Find f = find<ITEM>(a, blockIdx.x / a.pool.kv);
+  const Find f = Finder<ITEM>(a).at(blockIdx.x / a.pool.kv);
   if (f.s < 0) return;
   const Watch &w = f.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -469,7 +595,7 @@ __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a)
   u32x4 qf[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk)
-    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + hq * D + 32 * kk + 8 * g);
+    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + hq * D + 32 * kk + 8 * g) ^ a.flip;
   if (wave < steps) {
     load(wave);
     fetch(min(wave + WW, steps - 1));
@@ -509,9 +635,9 @@ __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a)
     }
     float hi = t[0][0];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) hi = __builtin_elementwise_maximum(hi, t[e >> 2][e & 3]);
+    for (int e = 1; e < 8; ++e) hi = larger(hi, t[e >> 2][e & 3]);
     if (__ballot(!(hi - ref <= SLACK)) != 0) {
-      const float now = __builtin_elementwise_maximum(ref, hi);
+      const float now = larger(ref, hi);
       sum *= __builtin_amdgcn_exp2f(ref - (now == -INFINITY ? 0.0f : now));
       ref = now;
     }
@@ -540,7 +666,7 @@ __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a)
 __global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
   __shared__ f32x2 so[16][FEW];
   const int head = blockIdx.x % a.pool.kv;
-  const Find f = find<ITEM>(a, blockIdx.x / a.pool.kv);
+  const Find f = Finder<ITEM>(a).at(blockIdx.x / a.pool.kv);
   if (f.s < 0) return;
   const Watch &w = f.w;
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
@@ -561,8 +687,6 @@ __global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
   const int k0 = (int)min((int64_t)f.j * f.each * 64, (int64_t)w.keys);
   const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
   const float *from = a.t + ((int64_t)f.s * a.pool.kv + head) * a.most * a.wide;
-  float *score = a.score + ((int64_t)f.s * a.pool.kv + head) * a.room;
-  const int base = a.base ? a.base[f.s] : w.len;
   for (int k = k0 + 4 * (int)threadIdx.x; k < k1; k += 256 * WW) {
     f32x4 acc{0, 0, 0, 0};
     for (int p = 0; p < w.pairs; ++p) {
@@ -576,7 +700,7 @@ __global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (k + e < k1) score[k + e] = k + e < base ? a.decay * score[k + e] + acc[e] : acc[e];
+      if (k + e < k1) add_score(a, f, head, k + e, acc[e]);
   }
 }
 
@@ -880,11 +1004,8 @@ int64_t rows_watched(const exl3p_rows *r, int32_t window) {
 }
 // Workgroups of a kv head that fill the CUs: four of the first pass each.
 int64_t target_of(const exl3p_cache *c) { return (4 * device_cus() + c->kv_heads - 1) / c->kv_heads; }
-int64_t most_tiles(const exl3p_rows *r, int group, int32_t window) {
-  return rows_watched(r, window) * group / TILE + r->seqs;
-}
-size_t refs_bytes(const exl3p_cache *c, const exl3p_rows *r, int group) {
-  return up16((size_t)r->rows * group * c->kv_heads * sizeof(f32x2));
+size_t lse_bytes(const exl3p_cache *c, const exl3p_rows *r, int group) {
+  return up16((size_t)r->rows * group * c->kv_heads * sizeof(float));
 }
 
 // How the weights are formed, by what the host knows.  Pairs whose scores are
@@ -892,24 +1013,35 @@ size_t refs_bytes(const exl3p_cache *c, const exl3p_rows *r, int group) {
 // read the keys twice.
 struct Plan {
   int group;
+  int tile;              // pairs
   int64_t tiles, items;  // at most
   int few;               // pairs whose scores are kept, 0: none
   int wide;              // of a row of them
-  size_t parts, rest;    // bytes
+  int deal, deals;       // pairs of an item of the second pass, such items of a key at most
+  size_t parts, rest, sums;  // bytes
 };
 constexpr size_t KEPT_MAX = (size_t)1 << 30;
+// A deal is a tile, so that its pairs stay in registers, until the deals' sums would
+// take more than this.
+constexpr size_t SUMS_MAX = (size_t)1 << 28;
 Plan plan_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads, int32_t window, int32_t room) {
   Plan p;
   p.group = heads / c->kv_heads;
-  const int64_t rows = window > 0 && window < r->max_rows ? window : r->max_rows;
+  const int64_t rows = window > 0 && window < r->max_rows ? window : r->max_rows, pairs = rows * p.group;
   p.wide = (room + 15) & ~15;
-  p.tiles = most_tiles(r, p.group, window);
-  p.items = target_of(c) + p.tiles;
-  p.few = rows * p.group <= FEW ? (int)(rows * p.group) : 0;
+  p.few = pairs <= FEW ? (int)pairs : 0;
   p.rest = (size_t)r->seqs * c->kv_heads * p.few * p.wide * sizeof(float);
   if (p.rest > KEPT_MAX) p.few = 0;
-  if (p.few == 0) p.rest = refs_bytes(c, r, p.group);
-  p.parts = (size_t)p.items * c->kv_heads * (p.few ? FEW : TILE) * sizeof(f32x2);
+  if (p.few == 0) p.rest = lse_bytes(c, r, p.group);
+  p.tile = p.few ? FEW : TILE;
+  p.tiles = rows_watched(r, window) * p.group / p.tile + r->seqs;
+  p.items = target_of(c) * (p.few ? 1 : 3) + p.tiles;
+  for (p.deal = p.tile;; p.deal *= 2) {
+    p.deals = p.few ? 1 : (int)((pairs + p.deal - 1) / p.deal);
+    p.sums = p.deals > 1 ? up16((size_t)r->seqs * c->kv_heads * p.deals * room * sizeof(float)) : 0;
+    if (p.sums <= SUMS_MAX || p.deals == 2) break;
+  }
+  p.parts = (size_t)p.items * c->kv_heads * p.tile * sizeof(f32x2);
   return p;
 }
 
@@ -930,7 +1062,7 @@ size_t exl3p_weigh_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int3
       check_heads(c, heads).code != EXL3_OK || window < 0 || room <= 0)
     return 0;
   const Plan p = plan_of(c, r, heads, window, room);
-  return p.parts + p.rest;
+  return p.parts + p.rest + p.sums;
 }
 
 exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
@@ -951,7 +1083,11 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
   EXL3P_TRY(check_score(score, room));
   EXL3P_TRY(check_matrix(q, q_stride, (int64_t)heads * c->dim));
   const Plan p = plan_of(c, r, heads, window, room);
-  if ((int64_t)r->rows * p.group > INT32_MAX / 2 || p.items * c->kv_heads > GRID_MAX)
+  // items of a deal and a part of the keys are counted in 32 bits, spans of 64 keys are a grid
+  const int64_t spans = r->seqs * (((int64_t)room + 63) / 64);
+  if ((int64_t)r->rows * p.group > INT32_MAX / 2 || p.items * c->kv_heads * (p.tile / 16) > GRID_MAX ||
+      (r->seqs * ((int64_t)room / PART + 1) + p.items) * p.deals > INT32_MAX / 2 ||
+      (p.deals > 1 && spans * c->kv_heads > GRID_MAX))
     return refuse(EXL3_TOO_LARGE, "PagedWeigh: too many rows and heads for one call");
   const size_t need = exl3p_weigh_scratch_bytes(c, r, heads, window, room);
   if (scratch == nullptr || !aligned(scratch, 16) || scratch_bytes < need)
@@ -965,12 +1101,16 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
   WeighArgs a;
   a.pool = pool, a.st = step_of(r), a.group = p.group, a.window = window;
   a.q = static_cast<const uint16_t *>(q), a.qs = q_stride, a.mask = mask, a.words = words;
-  a.scale = scale * LOG2E, a.decay = decay, a.base = base, a.score = score, a.room = room;
-  a.target = (float)target_of(c), a.slots = (int)(p.items * c->kv_heads);
+  // at least f32's smallest, so that a hidden key's -inf times it stays -inf
+  a.scale = fmaxf(fabsf(scale) * LOG2E, 1.17549435e-38f), a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.decay = decay, a.base = base, a.score = score, a.room = room;
+  a.target = (float)(p.items - p.tiles), a.slots = (int)(p.items * c->kv_heads);
   a.least = p.few ? 2.0f : 4.0f;
   a.part = static_cast<f32x2 *>(scratch);
-  a.ref = reinterpret_cast<f32x2 *>(static_cast<char *>(scratch) + p.parts);
-  a.t = reinterpret_cast<float *>(a.ref), a.most = p.few, a.wide = p.wide;
+  a.lse = reinterpret_cast<float *>(static_cast<char *>(scratch) + p.parts);
+  a.t = a.lse, a.most = p.few, a.wide = p.wide;
+  a.sums = reinterpret_cast<float *>(static_cast<char *>(scratch) + p.parts + p.rest);
+  a.tile = p.tile, a.deal = p.deal, a.deals = p.deals;
   const hipStream_t st = static_cast<hipStream_t>(s);
   const dim3 items((unsigned)(p.items * c->kv_heads));
   return by_type(c, [&](auto e, auto d) {
@@ -979,10 +1119,20 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
       hipLaunchKernelGGL(weigh_few_keys_kernel, items, dim3(64 * WW), 0, st, a);
       return;
     }
+    // the second pass' items: as many as its target may make, or round again
+    const dim3 parts((unsigned)((target_of(c) * 3 + p.tiles) * c->kv_heads));
+
     hipLaunchKernelGGL((weigh_sums_kernel<decltype(e), d>), items, dim3(64 * WW), 0, st, a);
-    hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)(p.tiles * c->kv_heads)), dim3(TILE), 0, st, a);
-    hipLaunchKernelGGL((weigh_keys_kernel<decltype(e), d>), dim3((unsigned)(2 * target_of(c) * c->kv_heads)),
-                       dim3(64 * WW), 0, st, a);
+    // few tiles have many items each
+    if (p.tiles * 8 <= p.items)
+      hipLaunchKernelGGL(weigh_join_kernel<16>, dim3((unsigned)(p.tiles * c->kv_heads * (p.tile / 16))),
+                         dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL(weigh_join_kernel<2>, dim3((unsigned)(p.tiles * c->kv_heads * (p.tile / 128))),
+                         dim3(256), 0, st, a);
+    hipLaunchKernelGGL((weigh_keys_kernel<decltype(e), d>), parts, dim3(64 * WW), 0, st, a);
+    if (p.deals > 1)
+      hipLaunchKernelGGL(weigh_deals_kernel, dim3((unsigned)(spans * c->kv_heads)), dim3(64 * WW), 0, st, a);
   });
 }
 

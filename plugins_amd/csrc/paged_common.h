@@ -112,6 +112,17 @@ __device__ __forceinline__ int slot_of(const Pool &p, int s, int key) {
   return page < (uint32_t)p.pages ? (int)((page << p.lp) | (key & ((1 << p.lp) - 1))) : -1;
 }
 
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ int scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // 1, 2, 4, 8 lanes down a row
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // a row's last lane to the next
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // the second row's to both after
+  return v;
+}
+
 // ----------------------------------------------------------------- host checks
 
 constexpr exl3_verdict OK{EXL3_OK, ""};

@@ -213,17 +213,6 @@ __device__ __forceinline__ int tiles_of(const Span &sp, const Split &sl) {
   return (int)((uint32_t)(sp.n * sl.group + (1 << sl.tile) - 1) >> sl.tile);
 }
 
-// Sum over the lanes up to and with this one.
-__device__ __forceinline__ int scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // 1, 2, 4, 8 lanes down a row
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // a row's last lane to the next
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // the second row's to both after
-  return v;
-}
-
 // Item number x among the sequences' ones.  Every workgroup finds its own: no
 // plan on the device or the host depends on the lengths, so a captured call
 // follows them.  A tile of u units has ceil(u / c) items, c the units of all tiles
