@@ -720,7 +720,7 @@ struct EvictArgs {
   int32_t *new_len;
 };
 
-constexpr int PICK = 1024;   // threads that pick a head's keys
+constexpr int PICK = 1024;   // the most threads that pick a head's keys
 constexpr int BINS = 2048;
 constexpr int HELD = 32768;  // scores of a head in LDS
 constexpr int FEWEST = 512;  // keys whose border is found by rank
@@ -742,40 +742,38 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 
 // Sum over the workgroup's threads before this one, and over all.
-__device__ __forceinline__ uint32_t before(uint32_t v, uint32_t (&waves)[PICK / 64], uint32_t &whole) {
+template <int P>
+__device__ __forceinline__ uint32_t before(uint32_t v, uint32_t (&waves)[P / 64], uint32_t &whole) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t x = v;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint32_t y = __shfl_up(x, m);
-    if (lane >= m) x += y;
-  }
+  const uint32_t x = (uint32_t)scan((int)v);
   __syncthreads();
   if (lane == 63) waves[wave] = x;
   __syncthreads();
   uint32_t base = 0;
   whole = 0;
 #pragma unroll
-  for (int w = 0; w < PICK / 64; ++w) {
+  for (int w = 0; w < P / 64; ++w) {
     if (w < wave) base += waves[w];
     whole += waves[w];
   }
   return base + x - v;
 }
 
-// A workgroup a sequence, layer and kv head.  The budget's border is found by
+// P threads a sequence, layer and kv head.  The budget's border is found by
 // counting: the range of the scores in BINS bins, then the bin that holds the
 // border in BINS again, three rounds at most (32 bits of order), or, once a bin
 // holds few keys, by each one's rank among them.  Bins divide the range that
 // the scores have, so that few of them fall into one and the counters in LDS are
 // rarely fought over.  Then the keys above the border, and as many of those on
 // it as are left, earliest first, get their places by counting again.  Scores
-// stay in LDS, HELD of them; where there are more they are read again.
-__global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a, int held) {
+// stay in LDS, `held` of them; where there are more they are read again.  Bound by
+// the chain of passes and barriers, not by bytes.
+template <int P>
+__global__ __launch_bounds__(P) void evict_pick_kernel(EvictArgs a, int held) {
   extern __shared__ float scores[];
-  __shared__ uint32_t bins[BINS], waves[PICK / 64];
-  __shared__ uint32_t lows[PICK / 64], highs[PICK / 64];
-  __shared__ uint32_t rows[HELD / 64];
+  __shared__ uint32_t bins[BINS], waves[P / 64];
+  __shared__ uint32_t lows[P / 64], highs[P / 64];
+  __shared__ uint32_t rows[32 * P / 64];  // of 32 turns
   __shared__ int chosen, above, holds, count, found_ties;
   __shared__ uint32_t found;
   uint32_t *const cand = bins;  // FEWEST keys, then their numbers
@@ -789,49 +787,50 @@ __global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a, int held)
   const float *score = a.score + at * a.room;
   float *to_score = a.new_score + at * a.room;
   int32_t *kept = a.kept + at * a.most;
-  // a thread reads what it has written: keys tid, tid + PICK, ... of a block
+  const int head = min(a.first, max(b, 0)), tail = min(a.last, max(b, 0) - head);  // those that stay anyway
+  const int lo = head, hi = len - tail;                                            // the others
+  // a thread reads what it has written: keys tid, tid + P, ... of a block
   const int blocks = b < 0 ? 0 : (len + held - 1) / held;
+  uint32_t low = ~0u, high = 0;  // the others' range
   auto read = [&](int blk) {
     const int n = min(held, len - blk * held);
-#pragma unroll 8
-    for (int i = tid; i < n; i += PICK) scores[i] = score[blk * held + i];
+#pragma unroll 16
+    for (int i = tid; i < n; i += P) scores[i] = score[blk * held + i];
     return n;
   };
-  if (blocks == 1) read(0);
-  bool bad = b < 0;
-  if (!bad)
-    for (int x = tid; x < (len + (1 << a.pool.lp) - 1) >> a.pool.lp; x += PICK)
-      bad |= (uint32_t)a.pool.table[(size_t)s * a.pool.max_pages + x] >= (uint32_t)a.pool.pages;
-  bad = __syncthreads_or(bad);
-  if (tid == 0 && lh == 0) a.new_len[s] = bad ? len : b;
-  for (int x = (bad ? 0 : b) + tid; x < a.most; x += PICK) kept[x] = -1;
-  if (bad || b == 0) return;
-  const int head = min(a.first, b), tail = min(a.last, b - head);  // those that stay anyway
-  const int lo = head, hi = len - tail;                            // the others
-  int need = b - head - tail;
   // f(key, its number) for the thread's keys among the others
   auto each = [&](auto &&f) {
     for (int blk = 0; blk < blocks; ++blk) {
       const int n = blocks > 1 ? read(blk) : len, from = blk * held;
 #pragma unroll 4
-      for (int i = tid; i < n; i += PICK)
+      for (int i = tid; i < n; i += P)
         if (from + i >= lo && from + i < hi) f(ordered(scores[i]), from + i);
     }
   };
+  if (blocks == 1) read(0);
+  bool bad = b < 0;
+  if (!bad) {
+#pragma unroll 4
+    for (int x = tid; x < (len + (1 << a.pool.lp) - 1) >> a.pool.lp; x += P)
+      bad |= (uint32_t)a.pool.table[(size_t)s * a.pool.max_pages + x] >= (uint32_t)a.pool.pages;
+    each([&](uint32_t k, int) { low = min(low, k), high = max(high, k); });
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1)
+    low = min(low, (uint32_t)__shfl_xor((int)low, m)), high = max(high, (uint32_t)__shfl_xor((int)high, m));
+  if (lane == 0) lows[wave] = low, highs[wave] = high;
+  for (int i = tid; i < BINS; i += P) bins[i] = 0;
+  bad = __syncthreads_or(bad);
+  if (tid == 0 && lh == 0) a.new_len[s] = bad ? len : b;
+  for (int x = (bad ? 0 : b) + tid; x < a.most; x += P) kept[x] = -1;
+  if (bad || b == 0) return;
+  int need = b - head - tail;
   // the border: keys of more than `border` stay, and the first `ties` on it
   uint32_t border = ~0u;
   int ties = 0;
   if (need > 0) {
-    uint32_t low = ~0u, high = 0;
-    each([&](uint32_t k, int) { low = min(low, k), high = max(high, k); });
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1)
-      low = min(low, (uint32_t)__shfl_xor((int)low, m)), high = max(high, (uint32_t)__shfl_xor((int)high, m));
-    if (lane == 0) lows[wave] = low, highs[wave] = high;
-    for (int i = tid; i < BINS; i += PICK) bins[i] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < PICK / 64; ++w) low = min(low, lows[w]), high = max(high, highs[w]);
+    for (int w = 0; w < P / 64; ++w) low = min(low, lows[w]), high = max(high, highs[w]);
     uint32_t width = high - low;  // the range: low .. low + width
     for (;;) {
       const int shift = max(0, 32 - (width ? __builtin_clz(width) : 32) - 11);
@@ -840,16 +839,19 @@ __global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a, int held)
       });
       if (tid == 0) count = 0;
       __syncthreads();
-      // a thread's two bins, the highest first
-      const int top = BINS - 1 - 2 * tid;
-      const uint32_t n1 = bins[top], n0 = bins[top - 1];
-      uint32_t whole;
-      const uint32_t over = before(n1 + n0, waves, whole);
-      if (over < (uint32_t)need && over + n1 + n0 >= (uint32_t)need) {
-        const bool second = over + n1 < (uint32_t)need;
-        chosen = top - second;
-        above = (int)(over + (second ? n1 : 0));
-        holds = (int)(second ? n0 : n1);
+      // a thread's bins, the highest first
+      constexpr int N = BINS / P;
+      uint32_t own[N], all = 0, whole;
+#pragma unroll
+      for (int e = 0; e < N; ++e) all += own[e] = bins[BINS - 1 - N * tid - e];
+      uint32_t over = before<P>(all, waves, whole);
+      if (over < (uint32_t)need && over + all >= (uint32_t)need) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (over < (uint32_t)need && over + own[e] >= (uint32_t)need)
+            chosen = BINS - 1 - N * tid - e, above = (int)over, holds = (int)own[e];
+          over += own[e];
+        }
       }
       __syncthreads();
       const int bin = chosen, n = holds;
@@ -865,8 +867,8 @@ __global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a, int held)
           cand[c] = k, cand[FEWEST + c] = i;
         });
         __syncthreads();
-        if (tid < n) {
-          const uint32_t k = cand[tid], i = cand[FEWEST + tid];
+        for (int y = tid; y < n; y += P) {
+          const uint32_t k = cand[y], i = cand[FEWEST + y];
           int more = 0, same = 0;  // before this one: of higher keys, of the same and an earlier number
           for (int c = 0; c < n; ++c) {
             more += cand[c] > k;
@@ -878,49 +880,51 @@ __global__ __launch_bounds__(PICK) void evict_pick_kernel(EvictArgs a, int held)
         border = found, ties = found_ties;
         break;
       }
-      for (int i = tid; i < BINS; i += PICK) bins[i] = 0;
+      for (int i = tid; i < BINS; i += P) bins[i] = 0;
       __syncthreads();
     }
   }
-  // places: what stays whatever the ties are, and the ties, before each key
-  uint32_t sure0 = 0, tie0 = 0;  // of the blocks before
+  // places: what stays whatever the ties are, and the ties, before each key; 32 turns
+  // of the threads at once
+  uint32_t sure0 = 0, tie0 = 0;  // of the keys before
   for (int blk = 0; blk < blocks; ++blk) {
-    const int n = blocks > 1 ? read(blk) : len, from = blk * held;
-    const int turns = (n + PICK - 1) / PICK;
-    auto kind = [&](int e, uint64_t &bs, uint64_t &bt) {
-      const int i = e * PICK + tid, key = from + i;
-      const uint32_t k = i < n ? ordered(scores[i]) : 0;
-      const bool other = key >= lo && key < hi;
-      bs = __ballot(i < n && (!other || k > border));
-      bt = __ballot(i < n && other && k == border);
-    };
-    for (int e = 0; e < turns; ++e) {
-      uint64_t bs, bt;
-      kind(e, bs, bt);
-      if (lane == 0) rows[e * (PICK / 64) + wave] = (uint32_t)__popcll(bs) | (uint32_t)__popcll(bt) << 16;
-    }
-    __syncthreads();
-    uint32_t whole;
-    const bool has = tid < turns * (PICK / 64);
-    const uint32_t pre = before(has ? rows[tid] : 0, waves, whole);
-    if (has) rows[tid] = pre;
-    __syncthreads();
-    for (int e = 0; e < turns; ++e) {
-      uint64_t bs, bt;
-      kind(e, bs, bt);
-      const uint64_t under = (1ull << lane) - 1;
-      const uint32_t r = rows[e * (PICK / 64) + wave];
-      const uint32_t ns = sure0 + (r & 0xFFFFu) + __popcll(bs & under);
-      const uint32_t nt = tie0 + (r >> 16) + __popcll(bt & under);
-      if (bs >> lane & 1 || (bt >> lane & 1 && nt < (uint32_t)ties)) {
-        const uint32_t place = ns + min(nt, (uint32_t)ties);
-        kept[place] = from + e * PICK + tid;
-        to_score[place] = scores[e * PICK + tid];
+    const int n = blocks > 1 ? read(blk) : len;
+    for (int i0 = 0; i0 < n; i0 += 32 * P) {
+      const int from = blk * held + i0, turns = min(32, (n - i0 + P - 1) / P);
+      uint32_t stays = 0, on = 0;  // a bit a turn
+      for (int e = 0; e < turns; ++e) {
+        const int i = e * P + tid, key = from + i;
+        const bool there = i0 + i < n, other = key >= lo && key < hi;
+        const uint32_t k = there ? ordered(scores[i0 + i]) : 0;
+        const bool sure = there && (!other || k > border), tie = there && other && k == border;
+        stays |= (uint32_t)sure << e, on |= (uint32_t)tie << e;
+        const uint64_t bs = __ballot(sure), bt = __ballot(tie);
+        if (lane == 0) rows[e * (P / 64) + wave] = (uint32_t)__popcll(bs) | (uint32_t)__popcll(bt) << 16;
       }
+      __syncthreads();
+      // (32 turns' counts for P / 2 threads at most)
+      uint32_t whole;
+      const bool has = tid < turns * (P / 64);
+      const uint32_t pre = before<P>(has ? rows[tid] : 0, waves, whole);
+      if (has) rows[tid] = pre;
+      __syncthreads();
+      const uint64_t under = (1ull << lane) - 1;
+      for (int e = 0; e < turns; ++e) {
+        const bool sure = stays >> e & 1, tie = on >> e & 1;
+        const uint64_t bs = __ballot(sure), bt = __ballot(tie);
+        const uint32_t r = rows[e * (P / 64) + wave];
+        const uint32_t ns = sure0 + (r & 0xFFFFu) + __popcll(bs & under);
+        const uint32_t nt = tie0 + (r >> 16) + __popcll(bt & under);
+        if (sure || (tie && nt < (uint32_t)ties)) {
+          const uint32_t place = ns + min(nt, (uint32_t)ties);
+          kept[place] = from + e * P + tid;
+          to_score[place] = scores[i0 + e * P + tid];
+        }
+      }
+      sure0 += whole & 0xFFFFu;
+      tie0 += whole >> 16;
+      __syncthreads();
     }
-    sure0 += whole & 0xFFFFu;
-    tie0 += whole >> 16;
-    __syncthreads();
   }
 }
 
@@ -1169,8 +1173,13 @@ exl3_verdict exl3p_evict(const exl3p_cache *c, int32_t seqs, const int32_t *len,
   a.len = len, a.score = score, a.room = room, a.keep = keep, a.most = most;
   a.first = first, a.last = last, a.kept = kept, a.new_score = new_score, a.new_len = new_len;
   const hipStream_t st = static_cast<hipStream_t>(s);
-  const int held = room < HELD ? (room + PICK - 1) / PICK * PICK : HELD;
-  hipLaunchKernelGGL(evict_pick_kernel, dim3((unsigned)n), dim3(PICK), held * sizeof(float), st, a, held);
+  if (room <= 16 * 256) {
+    const int held = (room + 255) / 256 * 256;
+    hipLaunchKernelGGL(evict_pick_kernel<256>, dim3((unsigned)n), dim3(256), held * sizeof(float), st, a, held);
+  } else {
+    const int held = room < HELD ? (room + PICK - 1) / PICK * PICK : HELD;
+    hipLaunchKernelGGL(evict_pick_kernel<PICK>, dim3((unsigned)n), dim3(PICK), held * sizeof(float), st, a, held);
+  }
   if (c->dim == 64)
     hipLaunchKernelGGL(evict_move_kernel<64>, dim3((unsigned)(n * parts)), dim3(MV), 0, st, a);
   else

@@ -115,20 +115,25 @@ __device__ __forceinline__ double wave_sum(double v) {
 // ------------------------------------------------------------ rows' statistics
 
 // A workgroup takes PIECE logits of a row into registers: the largest, then the
-// weights' sum (f32 over 8 of a thread, 64 bits beyond).  Bound by bytes.
-template <typename E>
+// weights' sum (f32 over 8 of a thread, 64 bits beyond).  Bound by bytes.  ROOTS:
+// each sequence's first row alone.
+template <typename E, bool ROOTS>
 __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
   constexpr int N = Vec<E>::N, U = PIECE / ST / N;
   __shared__ float tops[ST / 64];
   __shared__ double masses[ST / 64];
   __shared__ int bests[ST / 64];
-  const int t = blockIdx.x / a.pieces, piece = blockIdx.x - t * a.pieces;
+  const int item = blockIdx.x / a.pieces, piece = blockIdx.x - item * a.pieces;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // the row's sequence: how many end at it or before
-  int s = 0;
-  for (int s0 = 0; s0 < a.st.seqs; s0 += 64)
-    s += __popcll(__ballot(s0 + lane < a.st.seqs && a.st.cu[min(s0 + lane, a.st.seqs - 1) + 1] <= t));
-  if (s >= a.st.seqs) return;
+  int t = item, s = 0;
+  if (ROOTS) {
+    s = item, t = max(a.st.cu[s], 0);
+    if (t >= min(a.st.cu[s + 1], a.st.rows)) return;
+  } else {  // the row's sequence: how many end at it or before
+    for (int s0 = 0; s0 < a.st.seqs; s0 += 64)
+      s += __popcll(__ballot(s0 + lane < a.st.seqs && a.st.cu[min(s0 + lane, a.st.seqs - 1) + 1] <= t));
+    if (s >= a.st.seqs) return;
+  }
   if (piece == 0 && threadIdx.x == 0 && t == max(a.st.cu[s], 0)) a.arrived[s] = 0;
   const char *row = static_cast<const char *>(a.logits) + (int64_t)t * a.ls * sizeof(typename E::T);
   const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::T));
@@ -149,7 +154,7 @@ __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
 #pragma unroll
   for (int w = 0; w < ST / 64; ++w) top = __builtin_elementwise_maximum(top, tops[w]);
   const float heat = a.temperature ? a.temperature[s] : 1.0f;
-  Part *part = a.part + (size_t)t * a.pieces + piece;
+  Part *part = a.part + (size_t)item * a.pieces + piece;
   if (heat == 0.0f) {  // the first place of the largest is what counts
     int best = a.vocab;
 #pragma unroll
@@ -207,46 +212,49 @@ enum More { DONE, REST, ROW };  // a walk's next: nothing, what p~ has left, a r
 // their way: each thread's own reference, moved once a sweep.
 template <typename E, int N, bool DRAFT>
 __device__ __forceinline__ void row_stats(const VerifyArgs &a, Walk<N, DRAFT> &w, int t, int i, float heat) {
-  constexpr int V = Vec<E>::N, U = 8;
+  constexpr int V = Vec<E>::N, U = 32 / V;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x / 64;
   const float rate = rate_of(heat);
   const char *row = static_cast<const char *>(a.logits) + (int64_t)t * a.ls * sizeof(typename E::T);
   const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::T));
+  const int sweep = U * V * (int)blockDim.x;
   float top = -INFINITY;
   double mass = 0.0;
   int best = INT32_MAX;
-  for (int e0 = (int)threadIdx.x * V - off; e0 < a.vocab; e0 += U * V * blockDim.x) {
-    u32x4 raw[U];
+  u32x4 raw[U];
+  auto fetch = [&](int e0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = block_of<E>(row, e0 + u * V * (int)blockDim.x, a.vocab);
+  };
+  int e0 = (int)threadIdx.x * V - off;
+  fetch(e0);
+  for (; e0 < a.vocab; e0 += sweep) {
+    float x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec<E>::unpack(raw[u], x[u]);
+    fetch(e0 + sweep);  // (-inf behind the last)
     float now = top;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[V];
-      Vec<E>::unpack(raw[u], x);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int k = 0; k < V; ++k) now = __builtin_elementwise_maximum(now, x[k]);
-    }
+      for (int k = 0; k < V; ++k) now = __builtin_elementwise_maximum(now, x[u][k]);
     if (heat == 0.0f) {
       if (now > top) {
 #pragma unroll
-        for (int u = U - 1; u >= 0; --u) {
-          float x[V];
-          Vec<E>::unpack(raw[u], x);
+        for (int u = U - 1; u >= 0; --u)
 #pragma unroll
           for (int k = V - 1; k >= 0; --k)
-            if (x[k] == now) best = e0 + u * V * (int)blockDim.x + k;
-        }
+            if (x[u][k] == now) best = e0 + u * V * (int)blockDim.x + k;
       }
     } else {
       const float ref = now == -INFINITY ? 0.0f : now;
       mass *= (double)__builtin_amdgcn_exp2f((top - ref) * rate);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[V], y = 0.0f;
-        Vec<E>::unpack(raw[u], x);
+      for (int u = 0; u < U * V / 8; ++u) {
+        float y = 0.0f;
 #pragma unroll
-        for (int k = 0; k < V; ++k) y += __builtin_amdgcn_exp2f((x[k] - ref) * rate);
+        for (int k = 0; k < 8; ++k)
+          y += __builtin_amdgcn_exp2f((x[(8 * u + k) / V][(8 * u + k) % V] - ref) * rate);
         mass += (double)y;
       }
     }
@@ -304,11 +312,11 @@ __device__ __forceinline__ Tip walk(const VerifyArgs &a, Walk<N, DRAFT> &w, int 
     if constexpr (DRAFT) w.q[i] = 0.0f;
     w.next[i] = -1;
   }
-  if constexpr (!LAZY) {
-    // 16 lanes a row
+  // their statistics; of lazy walks only the first row's are there: 16 lanes a row
+  {
     const int g = threadIdx.x & 15;
-    for (int i = threadIdx.x >> 4; i < n; i += blockDim.x / 16) {
-      const Part *part = a.part + (size_t)(begin + i) * a.pieces;
+    for (int i = threadIdx.x >> 4; i < (LAZY ? 1 : n); i += blockDim.x / 16) {
+      const Part *part = a.part + (size_t)(LAZY ? s : begin + i) * a.pieces;
       float hi = -INFINITY;
       int best = INT32_MAX;
       double m = 0.0;
@@ -340,7 +348,6 @@ __device__ __forceinline__ Tip walk(const VerifyArgs &a, Walk<N, DRAFT> &w, int 
   }
   if (threadIdx.x == 0) {
     w.at = 0, w.seen = 0, w.left = 1.0, w.drawn = 1.0, w.share = 0.0, w.more = ROW;
-    if (LAZY && !fit) w.mass[0] = -1.0, w.more = DONE;
   }
   __syncthreads();
   // the children of `of` (-1: of any row) get their probabilities
@@ -355,9 +362,9 @@ __device__ __forceinline__ Tip walk(const VerifyArgs &a, Walk<N, DRAFT> &w, int 
     __syncthreads();
   };
   int what = w.more;  // read between barriers: one wave writes it
-  if constexpr (!LAZY) weigh_children(-1);
+  weigh_children(LAZY ? 0 : -1);
   while (what != DONE) {
-    if (LAZY && what == ROW) {
+    if (LAZY && what == ROW && w.at > 0) {
       row_stats<E>(a, w, begin + w.at, w.at, heat);
       weigh_children(w.at);
     }
@@ -598,7 +605,7 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
   constexpr int N = Vec<E>::N;
   __shared__ Walk<OWN ? SHORT : 1, DRAFT> walked;
   __shared__ uint32_t gone[DRAW / 32];
-  __shared__ double waves[ST / 64], base;
+  __shared__ double waves[ST / 64], whole_waves[ST / 64], base;
   __shared__ int least[2][ST / 64], order;
   const int s = blockIdx.x / a.draws, own_piece = blockIdx.x - s * a.draws;
   Tip tip;
@@ -621,19 +628,12 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
       for (int i = 0; i < N; ++i) all += p[i], left += r[i];
     }
     all = wave_sum(all), left = wave_sum(left);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = left;
-    __syncthreads();
-    double v = 0.0;
-#pragma unroll
-    for (int w = 0; w < ST / 64; ++w) v += waves[w];
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = all;
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = left, whole_waves[threadIdx.x >> 6] = all;
     __syncthreads();
     if (threadIdx.x == 0) {
-      all = 0.0;
 #pragma unroll
-      for (int w = 0; w < ST / 64; ++w) all += waves[w];
-      __hip_atomic_store(&sums[2 * own_piece], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int w = 1; w < ST / 64; ++w) left += waves[w], all += whole_waves[w];
+      __hip_atomic_store(&sums[2 * own_piece], left, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __hip_atomic_store(&sums[2 * own_piece + 1], all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // both are there before the count
       order = __hip_atomic_fetch_add(&a.arrived[s], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -812,8 +812,11 @@ exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int3
   };
   by_dtype(logits_dtype, [&](auto e) {
     if (!lazy)
-      hipLaunchKernelGGL((verify_stats_kernel<decltype(e)>), dim3((unsigned)(r->rows * pieces)), dim3(ST),
-                         0, st, a);
+      hipLaunchKernelGGL((verify_stats_kernel<decltype(e), false>), dim3((unsigned)(r->rows * pieces)),
+                         dim3(ST), 0, st, a);
+    else
+      hipLaunchKernelGGL((verify_stats_kernel<decltype(e), true>), dim3((unsigned)(r->seqs * pieces)),
+                         dim3(ST), 0, st, a);
     if (draft == nullptr)
       after(e, e, std::false_type{});
     else
