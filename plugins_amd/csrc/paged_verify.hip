@@ -54,17 +54,31 @@ __device__ __forceinline__ u32x4 block_of(const char *row, int e, int vocab) {
   }
   return raw;
 }
+// Drafts' probabilities of tokens e .., 0 outside the vocabulary; of any alignment.
+template <typename Q, int N>
+__device__ __forceinline__ void drafts_of(const typename Q::T *q, int e, int vocab, float (&y)[N]) {
+  if (e >= 0 && e + N <= vocab) {
+    typename Q::T t[N];
+    __builtin_memcpy(t, q + e, sizeof(t));
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[k] = (float)t[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[k] = e + k >= 0 && e + k < vocab ? (float)q[e + k] : 0.0f;
+  }
+}
 template <typename E>
 __device__ __forceinline__ float one_of(const void *p, size_t i) {
   return (float)static_cast<const typename E::T *>(p)[i];
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int ST = 256;       // threads of a statistics or sampling workgroup,
-constexpr int PIECE = 8192;   // elements of a row that the first takes,
-constexpr int DRAW = 4096;    // and the second
-constexpr int WALK = 1024;    // the most threads of a walk
+constexpr int ST = 256;       // threads of most workgroups,
+constexpr int PIECE = 8192;   // elements of a row that one takes,
+constexpr int DRAW = 4096;    // and of a row that is sampled
+constexpr int ALONE = 1024;   // threads of a workgroup that walks alone
 constexpr int SHORT = 32;     // rows of a sequence that the sampling walks by itself
+constexpr int MIDDLE = 128;   // rows of a sequence whose walk takes little LDS
 
 // A piece's largest logit, the first place of it, and the sum of its weights
 // 2^((logit - top) log2(e) / T).
@@ -72,6 +86,20 @@ struct Part {
   float top;
   int32_t best;
   double mass;
+};
+
+// What a walk waits for: nothing, it has ended; what p~ has left after a refusal; a
+// row's statistics.
+enum Need : int32_t { END, REST, STATS };
+
+// A walk: the row that it is at (among its sequence's), the last child looked at, and
+// of p~ and q~ there: what p~ has left, what is left of q (siblings drawn without
+// replacement), the share of q that p has lost; the row's statistics.
+struct State {
+  int32_t at, seen, need, best;
+  double left, drawn, share;
+  double mass;  // -1: the row has no distribution
+  float top, pad;
 };
 
 // Where a sequence's walk ended: what the sampling needs.
@@ -95,7 +123,10 @@ struct VerifyArgs {
   const double *u;
   int32_t *target;
   int distinct;
+  int lazy;       // rows' statistics are formed when a walk gets there
   Part *part;     // [rows][pieces]
+  State *state;   // [2][seqs]: a round reads one and leaves the other
+  double *rest;   // [2][seqs][pieces]: what p~ has left, likewise
   Tip *tip;       // [seqs]
   double *sums;   // [seqs][draws][2]: of what p has left, of p
   int *arrived;   // [seqs]: sampling workgroups that are done
@@ -111,33 +142,53 @@ __device__ __forceinline__ double wave_sum(double v) {
   for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
   return v;
 }
+__device__ __forceinline__ float larger(float a, float b) {  // NaN if either is
+  return __builtin_elementwise_maximum(a, b);
+}
+
+// A sequence's rows and temperature.
+struct Seq {
+  int begin, n;
+  float heat, rate;
+  double inv;
+  bool fit, greedy;
+};
+__device__ __forceinline__ Seq seq_of(const VerifyArgs &a, int s) {
+  Seq q;
+  q.begin = min(max(a.st.cu[s], 0), a.st.rows);
+  q.n = min(min(max(a.st.cu[s + 1], q.begin), a.st.rows) - q.begin, min(a.st.max_rows, EXL3P_TREE_MAX));
+  q.heat = a.temperature ? a.temperature[s] : 1.0f;
+  q.rate = rate_of(q.heat);
+  q.inv = 1.0 / (double)q.heat;
+  q.fit = q.heat >= 0.0f && q.heat < INFINITY;
+  q.greedy = q.heat == 0.0f;
+  return q;
+}
 
 // ------------------------------------------------------------ rows' statistics
 
+// A row's first element of a piece: the piece's blocks of 16 bytes lie on their
+// boundaries, the row may not.
+template <typename E>
+__device__ __forceinline__ const char *row_of(const VerifyArgs &a, int t) {
+  return static_cast<const char *>(a.logits) + (int64_t)t * a.ls * (int)sizeof(typename E::T);
+}
+template <typename E>
+__device__ __forceinline__ int first_of(const char *row, int piece, int size) {
+  return piece * size - (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::T));
+}
+
 // A workgroup takes PIECE logits of a row into registers: the largest, then the
-// weights' sum (f32 over 8 of a thread, 64 bits beyond).  Bound by bytes.  ROOTS:
-// each sequence's first row alone.
-template <typename E, bool ROOTS>
-__global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
+// weights' sum (f32 over 8 of a thread, 64 bits beyond).
+template <typename E>
+__device__ __forceinline__ void piece_stats(const VerifyArgs &a, int t, int piece, float heat, Part *to) {
   constexpr int N = Vec<E>::N, U = PIECE / ST / N;
   __shared__ float tops[ST / 64];
   __shared__ double masses[ST / 64];
   __shared__ int bests[ST / 64];
-  const int item = blockIdx.x / a.pieces, piece = blockIdx.x - item * a.pieces;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int t = item, s = 0;
-  if (ROOTS) {
-    s = item, t = max(a.st.cu[s], 0);
-    if (t >= min(a.st.cu[s + 1], a.st.rows)) return;
-  } else {  // the row's sequence: how many end at it or before
-    for (int s0 = 0; s0 < a.st.seqs; s0 += 64)
-      s += __popcll(__ballot(s0 + lane < a.st.seqs && a.st.cu[min(s0 + lane, a.st.seqs - 1) + 1] <= t));
-    if (s >= a.st.seqs) return;
-  }
-  if (piece == 0 && threadIdx.x == 0 && t == max(a.st.cu[s], 0)) a.arrived[s] = 0;
-  const char *row = static_cast<const char *>(a.logits) + (int64_t)t * a.ls * sizeof(typename E::T);
-  const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::T));
-  const int first = piece * PIECE - off;  // the first block's first element
+  const char *row = row_of<E>(a, t);
+  const int first = first_of<E>(row, piece, PIECE);
   float x[U][N];
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -146,17 +197,15 @@ __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = __builtin_elementwise_maximum(top, x[u][i]);  // NaN stays
+    for (int i = 0; i < N; ++i) top = larger(top, x[u][i]);
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) top = __builtin_elementwise_maximum(top, exl3::xor_lanes(top, m));
+  for (int m = 1; m < 64; m <<= 1) top = larger(top, exl3::xor_lanes(top, m));
   if (lane == 0) tops[wave] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < ST / 64; ++w) top = __builtin_elementwise_maximum(top, tops[w]);
-  const float heat = a.temperature ? a.temperature[s] : 1.0f;
-  Part *part = a.part + (size_t)item * a.pieces + piece;
+  for (int w = 0; w < ST / 64; ++w) top = larger(top, tops[w]);
   if (heat == 0.0f) {  // the first place of the largest is what counts
-    int best = a.vocab;
+    int best = INT32_MAX;
 #pragma unroll
     for (int u = U - 1; u >= 0; --u)
 #pragma unroll
@@ -169,7 +218,7 @@ __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
     if (threadIdx.x == 0) {
 #pragma unroll
       for (int w = 1; w < ST / 64; ++w) best = min(best, bests[w]);
-      *part = Part{top, best, 0.0};
+      *to = Part{top, best, 0.0};
     }
     return;
   }
@@ -189,72 +238,340 @@ __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int w = 1; w < ST / 64; ++w) mass += masses[w];
-    *part = Part{top, 0, mass};
+    *to = Part{top, 0, mass};
   }
+}
+
+// All rows' statistics, a piece a workgroup.  Bound by bytes.
+template <typename E>
+__global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
+  const int t = blockIdx.x / a.pieces, piece = blockIdx.x - t * a.pieces;
+  const int lane = threadIdx.x & 63;
+  // the row's sequence: how many end at it or before
+  int s = 0;
+  for (int s0 = 0; s0 < a.st.seqs; s0 += 64)
+    s += __popcll(__ballot(s0 + lane < a.st.seqs && a.st.cu[min(s0 + lane, a.st.seqs - 1) + 1] <= t));
+  if (s >= a.st.seqs) return;
+  if (piece == 0 && threadIdx.x == 0 && t == max(a.st.cu[s], 0)) a.arrived[s] = 0;
+  piece_stats<E>(a, t, piece, a.temperature ? a.temperature[s] : 1.0f, a.part + (size_t)t * a.pieces + piece);
 }
 
 // ------------------------------------------------------------------- the walk
 
-// A wave's sequences of a walk in LDS: N rows at most.
+// A walk in LDS: N rows at most.
 template <int N, bool DRAFT>
 struct Walk {
-  double mass[N], p[N], us[N];  // mass -1: a row without a distribution
-  float q[DRAFT ? N : 1], top[N];
-  int up[N], tok[N], best[N], next[N];
-  double left, drawn, share, sums[WALK / 64];
-  float tops[WALK / 64];
-  int bests[WALK / 64];
-  int at, seen, more;
+  State st;
+  double p[N], us[N];
+  Part stat[N];  // rows' statistics, mass -1: none; not of lazy walks
+  float q[DRAFT ? N : 1];
+  int up[N], tok[N], next[N];
+  double sums[ALONE / 64];
+  float tops[ALONE / 64];
+  int bests[ALONE / 64];
 };
-enum More { DONE, REST, ROW };  // a walk's next: nothing, what p~ has left, a row's statistics
 
-// A row's statistics by one workgroup, for walks that look only at the rows on
-// their way: each thread's own reference, moved once a sweep.
+template <int N, bool DRAFT>
+__device__ __forceinline__ void load_rows(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q) {
+  for (int i = threadIdx.x; i < min(q.n, N); i += blockDim.x) {
+    const int t = q.begin + i, x = a.parent ? a.parent[t] : i - 1;
+    w.up[i] = x >= 0 && x < i ? x : -1;
+    w.tok[i] = a.ids[t];
+    w.us[i] = a.u[t];
+    w.next[i] = -1;
+  }
+}
+
+// A row's statistics, mass -1 where it has no distribution.
+__device__ __forceinline__ Part stats_of(const Seq &q, float top, int best, double mass) {
+  const bool whole = q.fit && (q.greedy ? top > -INFINITY : top > -INFINITY && top < INFINITY && mass > 0.0 && mass < INFINITY);
+  return Part{top, best, !whole ? -1.0 : q.greedy ? 1.0 : mass};
+}
+__device__ __forceinline__ void enter(State &st, const Part &x) {
+  st.top = x.top, st.best = x.best, st.mass = x.mass;
+}
+// A row's parts joined, by 16 lanes.
+__device__ __forceinline__ Part join_parts(const VerifyArgs &a, const Seq &q, int row) {
+  const Part *part = a.part + (size_t)(q.begin + row) * a.pieces;
+  float hi = -INFINITY;
+  int best = INT32_MAX;
+  double m = 0.0;
+  for (int k = threadIdx.x & 15; k < a.pieces; k += 16) {
+    const Part y = part[k];
+    const float now = larger(hi, y.top), ref = now == -INFINITY ? 0.0f : now;
+    if (y.top > hi) best = y.best;
+    if (!q.greedy)
+      m = m * (double)__builtin_amdgcn_exp2f((hi - ref) * q.rate) +
+          y.mass * (double)__builtin_amdgcn_exp2f((y.top - ref) * q.rate);
+    hi = now;
+  }
+  float all = hi;
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) all = larger(all, __shfl_xor(all, x, 16));
+  const float ref = all == -INFINITY ? 0.0f : all;
+  if (!q.greedy) m *= (double)__builtin_amdgcn_exp2f((hi - ref) * q.rate);
+  best = hi == all ? best : INT32_MAX;
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) m += __shfl_xor(m, x, 16), best = min(best, __shfl_xor(best, x, 16));
+  return stats_of(q, all, best, m);
+}
+// The statistics of the rows (of lazy walks: of the one that the walk is at) and what
+// they give the tokens of their children.  Behind a barrier, and before one.
+template <typename E, typename Q, bool DRAFT, int N>
+__device__ __forceinline__ void take_rows(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q, bool joined) {
+  const int n = min(q.n, N), at = w.st.at;
+  if (!joined) {
+    if (!a.lazy) {
+      for (int i = threadIdx.x >> 4; i < n; i += blockDim.x / 16) {
+        const Part x = join_parts(a, q, i);
+        if ((threadIdx.x & 15) == 0) {
+          w.stat[i] = x;
+          if (i == at) enter(w.st, x);
+        }
+      }
+    } else if (threadIdx.x < 16) {
+      const Part x = join_parts(a, q, at);
+      if (threadIdx.x == 0) enter(w.st, x);
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x + 1; i < n; i += blockDim.x) {
+    const int j = w.up[i];
+    double p = 0.0;
+    float d = 0.0f;
+    if (j >= 0 && (j == at || !a.lazy) && !q.greedy && (uint32_t)w.tok[i] < (uint32_t)a.vocab) {
+      const double mass = a.lazy ? w.st.mass : w.stat[j].mass;
+      const float top = a.lazy ? w.st.top : w.stat[j].top;
+      const size_t t = (size_t)(q.begin + j);
+      if (mass > 0.0) {
+        p = exp(((double)one_of<E>(a.logits, t * a.ls + w.tok[i]) - (double)top) * q.inv) / mass;
+        if constexpr (DRAFT) d = one_of<Q>(a.draft, t * a.ds + w.tok[i]);
+      }
+    }
+    w.p[i] = p;
+    if constexpr (DRAFT) w.q[i] = d;
+  }
+  __syncthreads();
+}
+
+// The walk goes on from the row that it is at to its end or to what it needs next, by
+// the first wave: the next child of a row is found among 64 rows a ballot.
+//
+// The refused tokens' probabilities, q given: p~ after refusals is max(p -
+// share q, 0), share the sum of A_j / B_j over the refusals, A_j the sum of p~
+// and B_j that of q~ (1, or what the refused ones leave of it).  A refused token
+// has none left: u A_j / B_j q >= p~ says that p~ is below what is taken.
+template <bool DRAFT, int N>
+__device__ __forceinline__ int walk_on(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q) {
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x, n = min(q.n, N);
+    State st = w.st;
+    st.need = END;
+    // the next child of the row behind row `from`
+    auto next = [&](int from) {
+      for (int b = (from + 1) & ~63; b < n; b += 64) {
+        const int i = b + lane;
+        const uint64_t f = __ballot(i > from && i < n && w.up[min(i, n - 1)] == st.at);
+        if (f != 0) return b + __builtin_ctzll(f);
+      }
+      return n;
+    };
+    int c = st.mass >= 0.0 ? next(max(st.seen, st.at)) : n;
+    while (c < n) {
+      bool hit;
+      double less = 0.0, step = 0.0;
+      if (q.greedy) {
+        hit = w.tok[c] == st.best;
+      } else if constexpr (DRAFT) {
+        step = st.left / fmax(st.drawn, 0x1p-53);
+        hit = w.us[c] * step * (double)w.q[c] < fmax(w.p[c] - st.share * (double)w.q[c], 0.0);
+      } else {
+        // a token that a sibling before it had is not there any more
+        less = w.p[c];
+        for (int b = 0; b < c; b += 64) {
+          const int i = b + lane;
+          if (__ballot(i > 0 && i < c && w.up[i] == st.at && w.tok[i] == w.tok[c]) != 0) less = 0.0;
+        }
+        hit = w.us[c] * st.left < less;
+      }
+      const int from = st.seen = c;
+      if (hit) {
+        if (lane == 0) w.next[st.at] = w.tok[c];
+        st.at = c, st.left = 1.0, st.drawn = 1.0, st.share = 0.0;
+        if (a.lazy) {
+          st.need = STATS;
+          break;
+        }
+        enter(st, w.stat[c]);
+        c = st.mass >= 0.0 ? next(c) : n;
+        continue;
+      }
+      c = next(from);
+      if (q.greedy) continue;
+      if constexpr (DRAFT) {
+        st.share += step;
+        if (a.distinct) st.drawn -= (double)w.q[from];
+        if (c < n) {
+          st.need = REST;
+          break;
+        }
+      } else {
+        st.left -= less;
+      }
+    }
+    if (lane == 0) w.st = st;
+  }
+  __syncthreads();
+  return w.st.need;
+}
+
+// What p~ has left at the row that the walk is at: of 8 elements, f32 but for the sum.
+template <typename E, typename Q>
+__device__ __forceinline__ double rest_of(const VerifyArgs &a, const State &st, const Seq &q, int begin, int end,
+                                          int by) {
+  constexpr int N = Vec<E>::N;
+  const char *row = row_of<E>(a, q.begin + st.at);
+  const typename Q::T *d = static_cast<const typename Q::T *>(a.draft) + (size_t)(q.begin + st.at) * a.ds;
+  const float inv = (float)(1.0 / st.mass), lost = (float)st.share;
+  double sum = 0.0;
+#pragma unroll 4
+  for (int e = begin; e < end; e += by) {
+    float x[N], y[N], v = 0.0f;
+    Vec<E>::unpack(block_of<E>(row, e, a.vocab), x);
+    drafts_of<Q, N>(d, e, a.vocab, y);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      v += fmaxf(__builtin_amdgcn_exp2f((x[k] - st.top) * q.rate) * inv - lost * y[k], 0.0f);
+    sum += (double)v;
+  }
+  return sum;
+}
+
+// A walk's end: the tokens of its rows (the last one's is the sampling's, where there is one:
+// another workgroup's to write) and what the sampling needs.
+template <int N, bool DRAFT>
+__device__ __forceinline__ Tip tip_of(const Walk<N, DRAFT> &w, const Seq &q) {
+  const int row = w.st.at;
+  if (!(w.st.mass >= 0.0) || q.greedy) return Tip{-1, row, 0.0f, 1.0f, 0.0, 0.0};
+  return Tip{q.begin + row, row, w.st.top, q.heat, w.st.share * w.st.mass, w.us[0]};
+}
+// first: of this sequence nothing has been written yet.
+template <int N, bool DRAFT>
+__device__ __forceinline__ void write_rows(const VerifyArgs &a, const Walk<N, DRAFT> &w, const Seq &q, bool first,
+                                           bool ended, const Tip &tip) {
+  for (int i = threadIdx.x; i < min(q.n, N); i += blockDim.x) {
+    int v = w.next[i];
+    if (ended && i == w.st.at) {
+      if (tip.row >= 0) continue;
+      if (q.greedy && w.st.mass >= 0.0) v = w.st.best;
+    }
+    if (first || v >= 0) a.target[q.begin + i] = v;
+  }
+}
+
+// A round: every workgroup of a sequence takes what the last round's have found, walks on,
+// all alike, and forms its piece of what the walk needs next.  Rounds are launches, so
+// nothing waits; a sequence whose walk has ended is left alone.  A chain of loads (state,
+// parts, rows, children's logits, a piece): 6 us a round.
+template <typename E, typename Q, bool DRAFT, int N>
+__global__ __launch_bounds__(ST) void verify_round_kernel(VerifyArgs a, int round) {
+  __shared__ Walk<N, DRAFT> w;
+  const int s = blockIdx.x / a.pieces, piece = blockIdx.x - s * a.pieces;
+  const Seq q = seq_of(a, s);
+  if (round == 0 && piece == 0 && threadIdx.x == 0) {
+    a.arrived[s] = 0, a.tip[s].row = -1;
+    if (q.n <= 0) a.state[a.st.seqs + s].need = END;
+  }
+  if (q.n <= 0) return;
+  const State had = round == 0 ? State{0, 0, STATS, 0, 1.0, 1.0, 0.0, -1.0, 0.0f, 0.0f}
+                               : a.state[(size_t)(round & 1) * a.st.seqs + s];
+  if (had.need == END) {
+    if (piece == 0 && threadIdx.x == 0) a.state[(size_t)(~round & 1) * a.st.seqs + s].need = END;
+    return;
+  }
+  // walks that need nothing are one workgroup's
+  if (piece > 0 && !a.lazy && !(DRAFT && a.parent != nullptr && a.st.max_rows > 2)) return;
+  load_rows(a, w, q);
+  if (threadIdx.x == 0) w.st = had;
+  __syncthreads();
+  int need = STATS;
+  if (round > 0 || !a.lazy) {
+    if (had.need == REST) {
+      if (threadIdx.x < 64) {
+        const double *rest = a.rest + ((size_t)(round & 1) * a.st.seqs + s) * a.pieces;
+        double left = 0.0;
+        for (int k = threadIdx.x; k < a.pieces; k += 64) left += rest[k];
+        left = wave_sum(left);
+        if (threadIdx.x == 0) w.st.left = left;
+      }
+    }
+    take_rows<E, Q>(a, w, q, a.lazy && had.need == REST);
+    need = walk_on(a, w, q);
+  }
+  if (piece == 0) {
+    const Tip tip = tip_of(w, q);
+    write_rows(a, w, q, round == 0, need == END, tip);
+    if (threadIdx.x == 0) {
+      a.state[(size_t)(~round & 1) * a.st.seqs + s] = w.st;
+      if (need == END) a.tip[s] = tip;
+    }
+  }
+  if (need == STATS) {
+    const int t = q.begin + w.st.at;
+    piece_stats<E>(a, t, piece, q.fit ? q.heat : 1.0f, a.part + (size_t)t * a.pieces + piece);
+  }
+  if constexpr (DRAFT) {
+    if (need == REST) {
+      const int from = first_of<E>(row_of<E>(a, q.begin + w.st.at), piece, PIECE);
+      constexpr int V = Vec<E>::N;
+      const double sum = wave_sum(rest_of<E, Q>(a, w.st, q, from + (int)threadIdx.x * V, from + PIECE, ST * V));
+      if ((threadIdx.x & 63) == 0) w.sums[threadIdx.x >> 6] = sum;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        double all = w.sums[0];
+#pragma unroll
+        for (int x = 1; x < ST / 64; ++x) all += w.sums[x];
+        a.rest[((size_t)(~round & 1) * a.st.seqs + s) * a.pieces + piece] = all;
+      }
+    }
+  }
+}
+
+// A row's statistics by one workgroup: each thread's own reference, moved once a sweep.
 template <typename E, int N, bool DRAFT>
-__device__ __forceinline__ void row_stats(const VerifyArgs &a, Walk<N, DRAFT> &w, int t, int i, float heat) {
+__device__ __forceinline__ void row_stats(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q) {
   constexpr int V = Vec<E>::N, U = 32 / V;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x / 64;
-  const float rate = rate_of(heat);
-  const char *row = static_cast<const char *>(a.logits) + (int64_t)t * a.ls * sizeof(typename E::T);
-  const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::T));
-  const int sweep = U * V * (int)blockDim.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const char *row = row_of<E>(a, q.begin + w.st.at);
+  constexpr int SWEEP = U * V * ALONE;
   float top = -INFINITY;
   double mass = 0.0;
   int best = INT32_MAX;
-  u32x4 raw[U];
-  auto fetch = [&](int e0) {
+  for (int e0 = first_of<E>(row, 0, 0) + (int)threadIdx.x * V; e0 < a.vocab; e0 += SWEEP) {
+    float x[U][V], now = top;
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = block_of<E>(row, e0 + u * V * (int)blockDim.x, a.vocab);
-  };
-  int e0 = (int)threadIdx.x * V - off;
-  fetch(e0);
-  for (; e0 < a.vocab; e0 += sweep) {
-    float x[U][V];
-#pragma unroll
-    for (int u = 0; u < U; ++u) Vec<E>::unpack(raw[u], x[u]);
-    fetch(e0 + sweep);  // (-inf behind the last)
-    float now = top;
+    for (int u = 0; u < U; ++u) Vec<E>::unpack(block_of<E>(row, e0 + u * V * ALONE, a.vocab), x[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int k = 0; k < V; ++k) now = __builtin_elementwise_maximum(now, x[u][k]);
-    if (heat == 0.0f) {
+      for (int k = 0; k < V; ++k) now = larger(now, x[u][k]);
+    if (q.greedy) {
       if (now > top) {
 #pragma unroll
         for (int u = U - 1; u >= 0; --u)
 #pragma unroll
           for (int k = V - 1; k >= 0; --k)
-            if (x[u][k] == now) best = e0 + u * V * (int)blockDim.x + k;
+            if (x[u][k] == now) best = e0 + u * V * ALONE + k;
       }
     } else {
       const float ref = now == -INFINITY ? 0.0f : now;
-      mass *= (double)__builtin_amdgcn_exp2f((top - ref) * rate);
+      mass *= (double)__builtin_amdgcn_exp2f((top - ref) * q.rate);
 #pragma unroll
       for (int u = 0; u < U * V / 8; ++u) {
         float y = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          y += __builtin_amdgcn_exp2f((x[(8 * u + k) / V][(8 * u + k) % V] - ref) * rate);
+          y += __builtin_amdgcn_exp2f((x[(8 * u + k) / V][(8 * u + k) % V] - ref) * q.rate);
         mass += (double)y;
       }
     }
@@ -262,225 +579,72 @@ __device__ __forceinline__ void row_stats(const VerifyArgs &a, Walk<N, DRAFT> &w
   }
   float all = top;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) all = __builtin_elementwise_maximum(all, exl3::xor_lanes(all, m));
+  for (int m = 1; m < 64; m <<= 1) all = larger(all, exl3::xor_lanes(all, m));
   if (lane == 0) w.tops[wave] = all;
   __syncthreads();
-  for (int x = 0; x < waves; ++x) all = __builtin_elementwise_maximum(all, w.tops[x]);
+  for (int x = 0; x < ALONE / 64; ++x) all = larger(all, w.tops[x]);
   const float ref = all == -INFINITY ? 0.0f : all;
-  mass = wave_sum(mass * (double)__builtin_amdgcn_exp2f((top - ref) * rate));
+  mass = wave_sum(mass * (double)__builtin_amdgcn_exp2f((top - ref) * q.rate));
   best = top == all ? best : INT32_MAX;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) best = min(best, __shfl_xor(best, m));
   if (lane == 0) w.sums[wave] = mass, w.bests[wave] = best;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int x = 1; x < waves; ++x) mass += w.sums[x], best = min(best, w.bests[x]);
-    const bool whole = heat == 0.0f ? all > -INFINITY : all > -INFINITY && all < INFINITY && mass > 0.0 && mass < INFINITY;
-    w.top[i] = all, w.best[i] = best, w.mass[i] = !whole ? -1.0 : heat == 0.0f ? 1.0 : mass;
+    for (int x = 1; x < ALONE / 64; ++x) mass += w.sums[x], best = min(best, w.bests[x]);
+    enter(w.st, stats_of(q, all, best, mass));
   }
   __syncthreads();
 }
 
-// A sequence's walk, by a workgroup.  Each row's pieces are joined, or (LAZY) a
-// row's logits looked at when the walk gets there; the tokens of rows get their
-// probabilities under their parents, all at once; then one wave walks: the
-// next child of a row is found among 64 rows a ballot.  Where a drafted sibling is
-// left after a refusal, all threads sum max(p - share q, 0).
-//
-// The refused tokens' probabilities, q given: p~ after refusals is max(p -
-// share q, 0), share the sum of A_j / B_j over the refusals, A_j the sum of p~
-// and B_j that of q~ (1, or what the refused ones leave of it).  A refused token
-// has none left: u A_j / B_j q >= p~ says that p~ is below what is taken.
-template <typename E, typename Q, bool DRAFT, bool LAZY, int N>
-__device__ __forceinline__ Tip walk(const VerifyArgs &a, Walk<N, DRAFT> &w, int s, bool writes) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int begin = min(max(a.st.cu[s], 0), a.st.rows), end = min(max(a.st.cu[s + 1], begin), a.st.rows);
-  const int n = min(end - begin, min(a.st.max_rows, N));
-  Tip tip{-1, 0, 0.0f, 1.0f, 0.0, 0.0};
-  if (n <= 0) return tip;
-  const float heat = a.temperature ? a.temperature[s] : 1.0f;
-  const bool fit = heat >= 0.0f && heat < INFINITY, greedy = heat == 0.0f;
-  const float rate = rate_of(heat);
-  const double inv = 1.0 / (double)heat;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int t = begin + i;
-    const int x = a.parent ? a.parent[t] : i - 1;
-    w.up[i] = x >= 0 && x < i ? x : -1;
-    w.tok[i] = a.ids[t];
-    w.us[i] = a.u[t];
-    w.p[i] = 0.0;
-    if constexpr (DRAFT) w.q[i] = 0.0f;
-    w.next[i] = -1;
-  }
-  // their statistics; of lazy walks only the first row's are there: 16 lanes a row
-  {
-    const int g = threadIdx.x & 15;
-    for (int i = threadIdx.x >> 4; i < (LAZY ? 1 : n); i += blockDim.x / 16) {
-      const Part *part = a.part + (size_t)(LAZY ? s : begin + i) * a.pieces;
-      float hi = -INFINITY;
-      int best = INT32_MAX;
-      double m = 0.0;
-      for (int k = g; k < a.pieces; k += 16) {
-        const Part y = part[k];
-        if (greedy) {
-          if (y.top > hi) best = y.best;
-          hi = __builtin_elementwise_maximum(hi, y.top);
-        } else {
-          const float now = __builtin_elementwise_maximum(hi, y.top), ref = now == -INFINITY ? 0.0f : now;
-          m = m * (double)__builtin_amdgcn_exp2f((hi - ref) * rate) +
-              y.mass * (double)__builtin_amdgcn_exp2f((y.top - ref) * rate);
-          hi = now;
-        }
-      }
-      float all = hi;
-#pragma unroll
-      for (int x = 1; x < 16; x <<= 1) all = __builtin_elementwise_maximum(all, __shfl_xor(all, x, 16));
-      const float ref = all == -INFINITY ? 0.0f : all;
-      m *= (double)__builtin_amdgcn_exp2f((hi - ref) * rate);
-      best = hi == all ? best : INT32_MAX;
-#pragma unroll
-      for (int x = 1; x < 16; x <<= 1) m += __shfl_xor(m, x, 16), best = min(best, __shfl_xor(best, x, 16));
-      if (g == 0) {
-        const bool whole = fit && (greedy ? all > -INFINITY : all > -INFINITY && all < INFINITY && m > 0.0 && m < INFINITY);
-        w.top[i] = all, w.best[i] = best, w.mass[i] = !whole ? -1.0 : greedy ? 1.0 : m;
-      }
-    }
-  }
-  if (threadIdx.x == 0) {
-    w.at = 0, w.seen = 0, w.left = 1.0, w.drawn = 1.0, w.share = 0.0, w.more = ROW;
-  }
-  __syncthreads();
-  // the children of `of` (-1: of any row) get their probabilities
-  auto weigh_children = [&](int of) {
-    for (int i = threadIdx.x + 1; i < n; i += blockDim.x) {
-      const int j = w.up[i];
-      if (j < 0 || (of >= 0 && j != of) || greedy || !(w.mass[j] > 0.0) || (uint32_t)w.tok[i] >= (uint32_t)a.vocab)
-        continue;
-      w.p[i] = exp(((double)one_of<E>(a.logits, (int64_t)(begin + j) * a.ls + w.tok[i]) - (double)w.top[j]) * inv) / w.mass[j];
-      if constexpr (DRAFT) w.q[i] = one_of<Q>(a.draft, (int64_t)(begin + j) * a.ds + w.tok[i]);
-    }
-    __syncthreads();
-  };
-  int what = w.more;  // read between barriers: one wave writes it
-  weigh_children(LAZY ? 0 : -1);
-  while (what != DONE) {
-    if (LAZY && what == ROW && w.at > 0) {
-      row_stats<E>(a, w, begin + w.at, w.at, heat);
-      weigh_children(w.at);
-    }
-    if (wave == 0) {
-      // the next child of `row` behind row `from`
-      auto next = [&](int row, int from) {
-        for (int b = (from + 1) & ~63; b < n; b += 64) {
-          const int i = b + lane;
-          const uint64_t f = __ballot(i > from && i < n && w.up[min(i, n - 1)] == row);
-          if (f != 0) return b + __builtin_ctzll(f);
-        }
-        return n;
-      };
-      int row = w.at, from = w.seen, then = DONE;
-      double A = w.left, B = w.drawn, L = w.share;
-      int c = w.mass[row] >= 0.0 ? next(row, from) : n;
-      while (c < n) {
-        bool hit;
-        double less = 0.0, step = 0.0;
-        if (greedy) {
-          hit = w.tok[c] == w.best[row];
-        } else if constexpr (DRAFT) {
-          step = A / fmax(B, 0x1p-53);
-          hit = w.us[c] * step * (double)w.q[c] < fmax(w.p[c] - L * (double)w.q[c], 0.0);
-        } else {
-          // a token that a sibling before it had is not there any more
-          less = w.p[c];
-          for (int b = 0; b < c; b += 64) {
-            const int i = b + lane;
-            if (__ballot(i > 0 && i < c && w.up[i] == row && w.tok[i] == w.tok[c]) != 0) less = 0.0;
-          }
-          hit = w.us[c] * A < less;
-        }
-        from = c;
-        if (hit) {
-          if (lane == 0) w.next[row] = w.tok[c];
-          row = c, A = 1.0, B = 1.0, L = 0.0;
-          if (LAZY) {
-            then = ROW;
-            break;
-          }
-          c = w.mass[row] >= 0.0 ? next(row, from) : n;
-          continue;
-        }
-        c = next(row, from);
-        if (greedy) continue;
-        if constexpr (DRAFT) {
-          L += step;
-          if (a.distinct) B -= (double)w.q[from];
-          if (c < n) {
-            then = REST;
-            break;
-          }
-        } else {
-          A -= less;
-        }
-      }
-      if (lane == 0) w.at = row, w.seen = from, w.more = then, w.left = A, w.drawn = B, w.share = L;
-    }
-    __syncthreads();
-    what = w.more;
-    if constexpr (DRAFT) {
-      if (what == REST) {  // what p~ has left
-        const int row = w.at;
-        const float hi = w.top[row], by = (float)(1.0 / w.mass[row]), lost = (float)w.share;
-        const size_t z = (size_t)(begin + row) * a.ls, d = (size_t)(begin + row) * a.ds;
-        double sum = 0.0;
-        for (int e0 = threadIdx.x; e0 < a.vocab; e0 += 16 * blockDim.x) {
-          float x[16], y[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int e = e0 + k * blockDim.x;
-            x[k] = -INFINITY, y[k] = 0.0f;
-            if (e < a.vocab) x[k] = one_of<E>(a.logits, z + e), y[k] = one_of<Q>(a.draft, d + e);
-          }
-          float v = 0.0f;
-#pragma unroll
-          for (int k = 0; k < 16; ++k)
-            v += fmaxf(__builtin_amdgcn_exp2f((x[k] - hi) * rate) * by - lost * y[k], 0.0f);
-          sum += (double)v;
-        }
-        sum = wave_sum(sum);
-        if (lane == 0) w.sums[wave] = sum;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          for (int x = 1; x < (int)blockDim.x / 64; ++x) sum += w.sums[x];
-          w.left = sum;
-        }
-        __syncthreads();
-      }
-    }
-  }
-  const int row = w.at;
-  const bool whole = w.mass[row] >= 0.0;
-  tip.at = row;
-  if (whole && !greedy) tip = Tip{begin + row, row, w.top[row], heat, w.share * w.mass[row], w.us[0]};
-  // (the last row's is another workgroup's to write where it is sampled)
-  if (writes)
-    for (int i = threadIdx.x; i < n; i += blockDim.x)
-      if (i != row || tip.row < 0) a.target[begin + i] = i == row && whole ? w.best[row] : w.next[i];
-  return tip;
-}
-
-template <typename E, typename Q, bool DRAFT, bool LAZY>
-__global__ __launch_bounds__(WALK) void verify_walk_kernel(VerifyArgs a) {
+// What the rounds have left of the walks, a workgroup a sequence: 10 to 13 us a row or a
+// refusal at 152 thousand tokens, its exponentials.
+template <typename E, typename Q, bool DRAFT>
+__global__ __launch_bounds__(ALONE) void verify_alone_kernel(VerifyArgs a, int round) {
   __shared__ Walk<EXL3P_TREE_MAX, DRAFT> w;
-  const Tip tip = walk<E, Q, DRAFT, LAZY>(a, w, blockIdx.x, true);
-  if (threadIdx.x == 0) a.tip[blockIdx.x] = tip, a.arrived[blockIdx.x] = 0;
+  const int s = blockIdx.x;
+  const Seq q = seq_of(a, s);
+  const State had = a.state[(size_t)(round & 1) * a.st.seqs + s];
+  if (q.n <= 0 || had.need == END) return;
+  load_rows(a, w, q);
+  if (threadIdx.x == 0) w.st = had;
+  __syncthreads();
+  // (the last round has formed the first row's parts)
+  for (int need = had.need, first = 1; need != END; first = 0) {
+    const bool joined = need == REST ? a.lazy : !first;
+    if (need == STATS && !first) {
+      row_stats<E>(a, w, q);
+    } else if (DRAFT && need == REST) {
+     if constexpr (DRAFT) {
+      constexpr int V = Vec<E>::N;
+      const int from = first_of<E>(row_of<E>(a, q.begin + w.st.at), 0, 0);
+      const double sum = wave_sum(rest_of<E, Q>(a, w.st, q, from + (int)threadIdx.x * V, a.vocab, ALONE * V));
+      if ((threadIdx.x & 63) == 0) w.sums[threadIdx.x >> 6] = sum;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        double all = w.sums[0];
+        for (int x = 1; x < ALONE / 64; ++x) all += w.sums[x];
+        w.st.left = all;
+      }
+      __syncthreads();
+     }
+    }
+    take_rows<E, Q>(a, w, q, joined);
+    need = walk_on(a, w, q);
+    __syncthreads();  // all have read it
+  }
+  const Tip tip = tip_of(w, q);
+  write_rows(a, w, q, false, true, tip);
+  if (threadIdx.x == 0) a.tip[s] = tip;
 }
 
 // ------------------------------------------------------------------- sampling
 
 // e^x for x <= 0 in 64 bits: a power of two times the series of e^f, |f| <= ln(2) / 2,
 // whose 14th term is below 2^-57 of the sum.
-__device__ __forceinline__ double exp_of(double x) {
-  if (!(x > -746.0)) return x != x ? x : 0.0;  // below the smallest number
+__device__ __forceinline__ double exp_of(double arg) {
+  const bool there = arg > -746.0;  // else below the smallest number
+  const double x = there ? arg : 0.0;
   const double n = __builtin_rint(x * 1.4426950408889634074);
   // ln(2) in two parts, the first with zeros behind its 32nd bit
   double f = fma(n, -0x1.62e42feep-1, x);
@@ -499,7 +663,7 @@ __device__ __forceinline__ double exp_of(double x) {
   y = fma(y, f, 0.5);
   y = fma(y, f, 1.0);
   y = fma(y, f, 1.0);
-  return __builtin_amdgcn_ldexp(y, (int)n);
+  return there ? __builtin_amdgcn_ldexp(y, (int)n) : 0.0;
 }
 
 // What p~ has left of a token, times the row's mass: exponents in 64 bits, since the
@@ -510,34 +674,19 @@ struct Rest {
   const VerifyArgs &a;
   Tip tip;
   double inv;
-  size_t z, d;
+  size_t d;
   __device__ __forceinline__ Rest(const VerifyArgs &args, const Tip &t)
-      : a(args), tip(t), inv(1.0 / (double)t.heat), z((size_t)max(t.row, 0) * args.ls),
-        d((size_t)max(t.row, 0) * args.ds) {}
-  // the first element of a piece: its blocks of 16 bytes lie on their boundaries
+      : a(args), tip(t), inv(1.0 / (double)t.heat), d((size_t)max(t.row, 0) * args.ds) {}
   __device__ __forceinline__ int first(int piece) const {
-    const char *row = static_cast<const char *>(a.logits) + z * sizeof(typename E::T);
-    return piece * DRAW - (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename E::T));
+    return first_of<E>(row_of<E>(a, max(tip.row, 0)), piece, DRAW);
   }
   // of p, and of p~, of the block at e; gone: bits of the piece that begins at `from`
   static constexpr int N = Vec<E>::N;
   __device__ __forceinline__ void of(int e, const uint32_t *gone, int from, double (&p)[N], double (&r)[N]) const {
     float x[N];
-    Vec<E>::unpack(block_of<E>(static_cast<const char *>(a.logits) + z * sizeof(typename E::T), e, a.vocab), x);
+    Vec<E>::unpack(block_of<E>(row_of<E>(a, max(tip.row, 0)), e, a.vocab), x);
     float y[N];
-    if constexpr (DRAFT) {
-      typedef typename Q::T T;
-      const T *q = static_cast<const T *>(a.draft) + d;
-      if (e >= 0 && e + N <= a.vocab) {
-        T t[N];
-        __builtin_memcpy(t, q + e, sizeof(t));
-#pragma unroll
-        for (int k = 0; k < N; ++k) y[k] = (float)t[k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) y[k] = e + k >= 0 && e + k < a.vocab ? (float)q[e + k] : 0.0f;
-      }
-    }
+    if constexpr (DRAFT) drafts_of<Q, N>(static_cast<const typename Q::T *>(a.draft) + d, e, a.vocab, y);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       r[k] = p[k] = exp_of(((double)x[k] - (double)tip.top) * inv);
@@ -609,10 +758,19 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
   __shared__ int least[2][ST / 64], order;
   const int s = blockIdx.x / a.draws, own_piece = blockIdx.x - s * a.draws;
   Tip tip;
-  if constexpr (OWN)
-    tip = walk<E, Q, DRAFT, false>(a, walked, s, own_piece == 0);
-  else
+  if constexpr (OWN) {
+    const Seq q = seq_of(a, s);
+    if (q.n <= 0) return;
+    load_rows(a, walked, q);
+    if (threadIdx.x == 0) walked.st = State{0, 0, STATS, 0, 1.0, 1.0, 0.0, -1.0, 0.0f, 0.0f};
+    __syncthreads();
+    take_rows<E, Q>(a, walked, q, false);
+    walk_on(a, walked, q);
+    tip = tip_of(walked, q);
+    if (own_piece == 0) write_rows(a, walked, q, true, true, tip);
+  } else {
     tip = a.tip[s];
+  }
   if (tip.row < 0) return;
   const Rest<E, Q, DRAFT> rest(a, tip);
   double *sums = a.sums + (size_t)s * a.draws * 2;
@@ -699,6 +857,7 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
 // ------------------------------------------------------------------- host side
 
 constexpr int VOCAB_MAX = 1 << 24;
+constexpr int ROUNDS = 6;
 
 int pieces_of(int32_t vocab) { return (vocab + 7 + PIECE - 1) / PIECE; }
 int draws_of(int32_t vocab) { return (vocab + 7 + DRAW - 1) / DRAW; }
@@ -734,14 +893,25 @@ exl3_verdict check_probabilities(const void *p, int32_t dtype, int64_t stride, i
   return OK;
 }
 
+// Where the scratch's arrays lie: parts, states, rests, tips, sums, counters; its size.
+size_t places(const exl3p_rows *r, int32_t vocab, size_t (&at)[6]) {
+  const size_t seqs = r->seqs, pieces = pieces_of(vocab);
+  const size_t bytes[6] = {(size_t)r->rows * pieces * sizeof(Part), 2 * seqs * sizeof(State),
+                           2 * seqs * pieces * sizeof(double),      seqs * sizeof(Tip),
+                           seqs * draws_of(vocab) * 2 * sizeof(double), seqs * sizeof(int)};
+  size_t end = 0;
+  for (int i = 0; i < 6; ++i) at[i] = end, end += up16(bytes[i]);
+  return end;
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t exl3p_verify_scratch_bytes(const exl3p_rows *r, int32_t vocab) {
   if (check_step(r).code != EXL3_OK || vocab <= 0 || vocab > VOCAB_MAX) return 0;
-  return up16((size_t)r->rows * pieces_of(vocab) * sizeof(Part)) + up16((size_t)r->seqs * sizeof(Tip)) +
-         (size_t)r->seqs * draws_of(vocab) * 2 * sizeof(double) + (size_t)r->seqs * sizeof(int);
+  size_t at[6];
+  return places(r, vocab, at);
 }
 
 exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int32_t *ids,
@@ -782,19 +952,25 @@ exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int3
   a.st = step_of(r), a.vocab = vocab, a.pieces = pieces, a.draws = draws;
   a.parent = parent, a.ids = ids, a.temperature = temperature, a.u = u, a.target = target;
   a.distinct = distinct != 0;
-  char *at = static_cast<char *>(scratch);
-  a.part = reinterpret_cast<Part *>(at);
-  at += up16((size_t)r->rows * pieces * sizeof(Part));
-  a.tip = reinterpret_cast<Tip *>(at);
-  at += up16((size_t)r->seqs * sizeof(Tip));
-  a.sums = reinterpret_cast<double *>(at);
-  a.arrived = reinterpret_cast<int *>(a.sums + (size_t)r->seqs * draws * 2);
+  size_t at[6];
+  places(r, vocab, at);
+  char *const base = static_cast<char *>(scratch);
+  a.part = reinterpret_cast<Part *>(base + at[0]);
+  a.state = reinterpret_cast<State *>(base + at[1]);
+  a.rest = reinterpret_cast<double *>(base + at[2]);
+  a.tip = reinterpret_cast<Tip *>(base + at[3]);
+  a.sums = reinterpret_cast<double *>(base + at[4]);
+  a.arrived = reinterpret_cast<int *>(base + at[5]);
   const hipStream_t st = static_cast<hipStream_t>(s);
-  // rows that drafted siblings may follow: sums over the vocabulary within the walk
-  const bool siblings = draft != nullptr && parent != nullptr;
+  // a refusal with a drafted sibling left wants a sum over the vocabulary
+  const bool siblings = draft != nullptr && parent != nullptr && r->max_rows > 2;
   const bool lazy = r->rows > 500 && r->rows >= 4 * (int64_t)r->seqs;
   const bool own = !lazy && !siblings && r->max_rows <= SHORT;
-  const dim3 all((unsigned)(r->seqs * draws));
+  a.lazy = lazy;
+  // rounds: what walks usually need; the rest is for one workgroup a sequence
+  const int needs = (lazy ? r->max_rows : 0) + (siblings ? r->max_rows - 2 : 0);
+  const int rounds = needs < ROUNDS ? needs : ROUNDS;
+  const dim3 all((unsigned)(r->seqs * draws)), each((unsigned)(r->seqs * pieces));
   auto after = [&](auto e, auto q, auto drafted) {
     typedef decltype(e) E;
     typedef decltype(q) Q;
@@ -803,20 +979,20 @@ exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int3
       hipLaunchKernelGGL((verify_draw_kernel<E, Q, D, true>), all, dim3(ST), 0, st, a);
       return;
     }
-    if (lazy)
-      hipLaunchKernelGGL((verify_walk_kernel<E, Q, D, true>), dim3(r->seqs), dim3(WALK), 0, st, a);
-    else  // the sums after a refusal want many threads, the walk itself few
-      hipLaunchKernelGGL((verify_walk_kernel<E, Q, D, false>), dim3(r->seqs), dim3(siblings ? WALK : ST), 0,
-                         st, a);
+    for (int k = 0; k <= rounds; ++k) {
+      if (r->max_rows <= MIDDLE)
+        hipLaunchKernelGGL((verify_round_kernel<E, Q, D, MIDDLE>), each, dim3(ST), 0, st, a, k);
+      else
+        hipLaunchKernelGGL((verify_round_kernel<E, Q, D, EXL3P_TREE_MAX>), each, dim3(ST), 0, st, a, k);
+    }
+    if (needs > rounds)
+      hipLaunchKernelGGL((verify_alone_kernel<E, Q, D>), dim3(r->seqs), dim3(ALONE), 0, st, a, rounds + 1);
     hipLaunchKernelGGL((verify_draw_kernel<E, Q, D, false>), all, dim3(ST), 0, st, a);
   };
   by_dtype(logits_dtype, [&](auto e) {
     if (!lazy)
-      hipLaunchKernelGGL((verify_stats_kernel<decltype(e), false>), dim3((unsigned)(r->rows * pieces)),
-                         dim3(ST), 0, st, a);
-    else
-      hipLaunchKernelGGL((verify_stats_kernel<decltype(e), true>), dim3((unsigned)(r->seqs * pieces)),
-                         dim3(ST), 0, st, a);
+      hipLaunchKernelGGL((verify_stats_kernel<decltype(e)>), dim3((unsigned)(r->rows * pieces)), dim3(ST), 0,
+                         st, a);
     if (draft == nullptr)
       after(e, e, std::false_type{});
     else
