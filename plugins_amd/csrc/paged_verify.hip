@@ -858,6 +858,7 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
 
 constexpr int VOCAB_MAX = 1 << 24;
 constexpr int ROUNDS = 6;
+constexpr int64_t LAZY = 1 << 25;  // bytes of logits
 
 int pieces_of(int32_t vocab) { return (vocab + 7 + PIECE - 1) / PIECE; }
 int draws_of(int32_t vocab) { return (vocab + 7 + DRAW - 1) / DRAW; }
@@ -964,7 +965,15 @@ exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int3
   const hipStream_t st = static_cast<hipStream_t>(s);
   // a refusal with a drafted sibling left wants a sum over the vocabulary
   const bool siblings = draft != nullptr && parent != nullptr && r->max_rows > 2;
-  const bool lazy = r->rows > 500 && r->rows >= 4 * (int64_t)r->seqs;
+  // Statistics when a walk gets there: of a tree, most of whose rows no walk gets to (a
+  // line's are drafted to be accepted), where all rows' would take longer than the rounds
+  // of the walks.  Measured at bf16, 151936 tokens, 4 to 32 us a call apart: 16 trees of
+  // 16 rows (78 MB) 47 us for all, 60 as the walks go; 16 of 32 (156 MB) 62 and 60; 64 of
+  // 16 (311 MB) 110 and 83.  Drafted trees go in rounds in any case: 4 of 16
+  // rows in f32 (39 MB) 78 and 73, 16 of 16 (78 MB) 96 and 85.  Lines that are accepted
+  // whole lose: 64 of 8 (156 MB) 76 and 121.
+  const int64_t read = (int64_t)r->rows * vocab * size_of(logits_dtype);
+  const bool lazy = parent != nullptr && r->rows >= 4 * (int64_t)r->seqs && read > (siblings ? LAZY : 5 * LAZY);
   const bool own = !lazy && !siblings && r->max_rows <= SHORT;
   a.lazy = lazy;
   // rounds: what walks usually need; the rest is for one workgroup a sequence

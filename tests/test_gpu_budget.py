@@ -105,27 +105,39 @@ def test_verify(counts, vocab, tree, draft, distinct, dtype):
         assert verified(counts, z, q, None, ids, heats, u, distinct) == want
 
 
-@pytest.mark.parametrize("draft", [None, F32])
-@pytest.mark.parametrize("counts,vocab", [([130, 90, 200, 0, 150], 67), ([600], 1501), ([64] * 9, 9001)])
-def test_verify_large_batches(counts, vocab, draft):
+@pytest.mark.parametrize("counts,vocab,dtype,draft", [
+    ([130, 90, 200, 0, 150], 67, BF16, None), ([130, 90, 200, 0, 150], 67, BF16, F32),
+    ([600], 1501, BF16, None), ([64] * 9, 9001, BF16, F32),
+    # read as the walks go
+    ([64] * 9, 30011, BF16, F32), ([300, 0, 150], 20001, F32, F16), ([64] * 9, 151936, BF16, None),
+    ([200, 0, 400], 151936, F16, None), ([9, 4, 1], 3200003, F32, None), ([3, 8, 1, 4], 600007, F32, BF16)])
+def test_verify_large_batches(counts, vocab, dtype, draft):
     """Batches of which the walks look at few rows."""
     seed = 1
     while True:
-        args = drafted(counts, vocab, BF16, draft, draft is not None, seed)
+        args = drafted(counts, vocab, dtype, draft, draft is not None, seed)
         want, margin = expected(counts, *args, draft is not None)
         if margin > MARGIN:
             break
         seed += 1
     got = verified(counts, *args, draft is not None)
     assert got == want
-    # a path that is deep: every row its parent's only child, and certain
-    n = max(counts)
+
+
+@pytest.mark.parametrize("n,vocab,tree,draft", [
+    (600, 67, False, None), (600, 67, True, None), (600, 151936, True, None), (600, 151936, False, None),
+    (300, 60013, True, F16), (200, 1001, True, F16)])
+def test_verify_a_path_that_is_deep(n, vocab, tree, draft):
+    """Every row its parent's only child, and certain."""
     z = torch.zeros(n, vocab)
     ids = [(7 * i) % vocab for i in range(n)]
     for i in range(n - 1):
         z[i, ids[i + 1]] = 60.0
     z[n - 1, 5] = 60.0
-    got = verified([n], z, None, None, ids, [1.0], torch.full((n,), 0.5, dtype=torch.float64), False)
+    z = z.to(F16)
+    q = None if draft is None else torch.full((n, vocab), 1.0 / vocab).to(draft)
+    got = verified([n], z, q, list(range(-1, n - 1)) if tree else None, ids, [1.0],
+                   torch.full((n,), 0.5, dtype=torch.float64), False)
     assert got == ids[1:] + [5]
 
 
@@ -159,11 +171,11 @@ def test_verify_strides_and_rows_behind(off, dtype, draft):
     assert target.tolist() == [77, 77, *want, 77, 77, 77]
 
 
-@pytest.mark.parametrize("rows", [3, 700])
-def test_verify_rows_without_a_distribution(rows):
+@pytest.mark.parametrize("rows,V", [(3, 50), (700, 50), (700, 60011)])
+def test_verify_rows_without_a_distribution(rows, V):
     """NaN, +inf, nothing but -inf; temperatures that are none: the walk ends there
     with -1.  A largest logit of +inf is one at temperature 0."""
-    V, counts = 50, [3] * 9 + ([70] * 10 if rows > 3 else [])
+    counts = [3] * 9 + ([70] * 10 if rows > 3 else [])
     z = torch.zeros(sum(counts), V)
     z[:, 11] = 30.0  # every row says 11
     ids, parent = [11] * sum(counts), []
