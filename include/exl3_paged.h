@@ -203,8 +203,8 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
  * new_score may be score itself.  A sequence within its budget, with keep[s]
  * below 0, more keys than `room` or its table, or a page number outside the cache
  * among them, stays as it is: kept is -1 throughout, new_len its len.
- * Pages that a sequence which loses keys holds are its alone (exl3p_book_shared), its
- * key numbers below new_len are written.  No output lies over an input (but
+ * A sequence that loses keys has its key numbers below new_len written: their pages
+ * are its alone (exl3p_book_shared); those behind them are only read.  No output lies over an input (but
  * new_score), another output or the cache. */
 exl3_verdict exl3p_evict(const exl3p_cache *c, int32_t seqs, const int32_t *len,
                          const float *score, int32_t room, const int32_t *keep, int32_t most,

@@ -638,7 +638,7 @@ def evict(cache, lens, score, kept, new_score, new_len, keep=None, first: int = 
     float32 [layers, sequences, kv heads, room] stay, up to kept.shape[-1] or keep int32
     [sequences] of them, in every layer and kv head; kept int32 [layers, sequences, kv
     heads, most], new_score (may be score itself), new_len int32 [sequences].  The pages
-    of a sequence that loses keys are its alone."""
+    of the kept keys' new numbers are their sequence's alone."""
     if score.dim() != 4 or kept.dim() != 4:
         raise ValueError("score and kept: [layers, sequences, kv heads, ...]")
     seqs, room, most = lens.numel(), _c_int(score.shape[3]), _c_int(kept.shape[3])

@@ -300,29 +300,48 @@ class PagedDecoder:
     (turboexl3_qwen38/src/spec/drafter.zig); its verify rows take the decode
     chain of the quant table, as these linears do up to 16 rows."""
 
-    def __init__(self, model: Qwen3Decoder, seqs: int, pages: int, max_pages: int, page: int = 64):
+    def __init__(self, model: Qwen3Decoder, seqs: int, pages: int, max_pages: int, page: int = 64,
+                 window: int | None = None, decay: float = 1.0):
         from . import paged as P
         self.P, self.m, self.cfg, self.torch = P, model, model.cfg, model.torch
         c = model.cfg
         self.cache = P.PagedCache(c.layers, pages, c.kv_heads, seqs, max_pages, page, HEAD_DIM,
                                   self.torch.float16, model.embed_table.device)
+        self.window, self.decay = window, decay
+        self.score = self.gone = None
+        if window is not None:
+            dev = model.embed_table.device
+            self.score = self.torch.zeros(c.layers, seqs, c.kv_heads, max_pages * page, device=dev)
+            self.gone = self.torch.zeros(seqs, dtype=self.torch.int32, device=dev)
 
-    def forward(self, rows, ids, parent=None, only=None, stream=None):
+    def _row_of(self, cu, n: int):
+        """Of rows 0 .. n - 1 of a step: their sequences (the last one's for rows
+        behind it) and their places in them."""
+        t = self.torch.arange(n, dtype=self.torch.int32, device=cu.device)
+        s = self.torch.searchsorted(cu[1:], t, right=True).clamp(max=cu.numel() - 2)
+        return s, t - cu[s]
+
+    def _weigh(self, layer: int, rows, q, mask) -> None:
+        self.P.weigh(self.cache, layer, rows, q, self.score[layer, :rows.seqs], mask, None, self.window,
+                     self.decay)
+
+    def forward(self, rows, ids, parent=None, only=None, stream=None, queries=None):
         """Logits [rows, vocab] of the step's rows (of the rows numbered by `only`,
         int64, if given), whose keys and values go into the cache behind each
         sequence's `rows.len`; the pages are there (cache.reserve).  ids int32
         [rows], one outside the vocabulary (in rows that pad the step, say) taken
         as the nearest in it; parent: the trees (None: each sequence's rows in a
-        line)."""
+        line).  queries: a list that gets each layer's, whose weights of the keys are
+        then not taken here."""
         torch, P, m, c, cache = self.torch, self.P, self.m, self.cfg, self.cache
         if stream is not None:
             with P._on(cache, stream):
-                return self.forward(rows, ids, parent, only)
+                return self.forward(rows, ids, parent, only, queries=queries)
         T = rows.rows
         P._ints(ids, "ids", cache, T)  # embed reads as many as there are rows
         if cache.index != P._device():  # the linears and norms go to the current one
             with torch.cuda.device(cache.index):
-                return self.forward(rows, ids, parent, only)
+                return self.forward(rows, ids, parent, only, queries=queries)
         f16 = {"dtype": torch.float16, "device": ids.device}
         if T == 0:
             if only is not None and only.numel() > 0:
@@ -331,6 +350,8 @@ class PagedDecoder:
         h = torch.empty(T, c.hidden, dtype=torch.float32, device=ids.device)
         x, att = torch.empty(T, c.hidden, **f16), torch.empty(T, c.q_dim, **f16)
         pos, slot, mask = P.plan(cache, rows, parent)
+        if self.gone is not None and rows.seqs:
+            pos += self.gone[self._row_of(rows.cu, T)[0]]
         embed(ids.clamp(0, c.vocab - 1), m.embed_table, h)
         add = None
         for li, L in enumerate(m.layers):
@@ -338,24 +359,105 @@ class PagedDecoder:
             q, k, v = X.matmul_shared([L["q"].weight, L["k"].weight, L["v"].weight], x)
             P.qkv_append(cache, li, q, k, v, L["q_norm"], L["k_norm"], pos, slot, q, c.eps, c.theta)
             P.attend(cache, li, rows, q, att, mask)
+            if queries is not None:
+                queries.append(q)
+            elif self.score is not None:
+                self._weigh(li, rows, q, mask)
             add_rmsnorm(h, X.matmul(L["o"].weight, att), L["post_norm"], x, c.eps)
             add = X.swiglu(L["gate"].weight, L["up"].weight, L["down"].weight, x)
         add_rmsnorm(h, add, m.final_norm, x, c.eps)
         return X.matmul(m.lm_head.weight, x if only is None else x[only])
 
-    def verify(self, rows, ids, parent=None, most: int | None = None, stream=None):
-        """One greedy verification: the rows' logits, then the walk down each
-        sequence's tree by the model's own tokens (row 0 is a token that is certain
-        already).  Returns path, count, next and new_len (int32 on the device);
-        the cache holds each sequence's first new_len keys, and the pages behind
-        them are the caller's to trim once the lengths are on the host."""
+    def verify(self, rows, ids, parent=None, most: int | None = None, stream=None,
+               temperature=None, draft=None, distinct: bool = False, u=None):
+        """One verification: the rows' logits, then the walk down each sequence's tree
+        (row 0 is a token that is certain already) by the model's most likely tokens,
+        or, with `temperature` float32 [sequences], by ones sampled: draft [rows,
+        vocab] are the probabilities that drafted tokens were drawn with (None: they
+        were chosen), distinct says that siblings were drawn without replacement, u
+        float64 [rows] are the random numbers (None: of torch's generator).  Returns
+        path, count, next and new_len (int32 on the device); the cache holds each
+        sequence's first new_len keys, and the pages behind them are the caller's to
+        trim once the lengths are on the host.  Keys get their weights from the
+        accepted rows alone."""
         torch, P = self.torch, self.P
         if stream is not None:
             with P._on(self.cache, stream):
-                return self.verify(rows, ids, parent, most)
-        target = self.forward(rows, ids, parent).float().argmax(-1).int()
+                return self.verify(rows, ids, parent, most, None, temperature, draft, distinct, u)
+        if temperature is None and (draft is not None or u is not None or distinct):
+            raise ValueError("draft, distinct and u are of a sampled verification: give a temperature")
+        queries = None if self.score is None else []
+        logits = self.forward(rows, ids, parent, queries=queries)
         i32 = {"dtype": torch.int32, "device": ids.device}
+        if temperature is None:
+            target = logits.float().argmax(-1).int()
+        else:
+            target = torch.empty(rows.rows, **i32)
+            if u is None:
+                u = torch.rand(rows.rows, dtype=torch.float64, device=ids.device)
+            P.verify(rows, parent, ids, logits, u, target, draft, temperature, distinct)
         path = torch.empty(rows.seqs, max(1, rows.max_rows) if most is None else most, **i32)
         count, after, new_len = (torch.empty(rows.seqs, **i32) for _ in range(3))
         P.commit(self.cache, rows, parent, ids, target, path, count, after, new_len)
+        if queries:
+            # the accepted rows, now in a line behind the keys they followed
+            cu = torch.zeros_like(rows.cu)
+            torch.cumsum(count, 0, dtype=torch.int32, out=cu[1:])
+            n, longest = rows.rows, min(rows.max_rows, path.shape[1])
+            line = P.Rows(cu, rows.len, n, longest)
+            s, i = self._row_of(cu, n)
+            at = rows.cu[s] + path[s, i.clamp(max=path.shape[1] - 1)].clamp(min=0)
+            at.clamp_(0, n - 1)
+            for li, q in enumerate(queries):
+                self._weigh(li, line, q[at], None)
         return path, count, after, new_len
+
+    def fork(self, src: int, dst: int, keys: int, stream=None) -> None:
+        """Sequence dst starts with src's first `keys` keys, pages shared, and their
+        weights."""
+        with self.P._on(self.cache, stream):
+            self.cache.fork(src, dst, keys)
+            if self.score is not None:
+                self.score[:, dst, :, :keys].copy_(self.score[:, src, :, :keys])
+                self.gone[dst:dst + 1].copy_(self.gone[src:src + 1])
+
+    def restart(self, seq: int, stream=None) -> None:
+        """Gives back a sequence's pages: it holds no keys, and none are gone."""
+        with self.P._on(self.cache, stream):
+            self.cache.trim(seq, 0)
+            if self.gone is not None:
+                self.gone[seq:seq + 1].zero_()
+
+    def evict(self, lens, keep: int, first: int = 0, last: int = 0, stream=None):
+        """Of each sequence's lens[s] keys (a host list, a length for each sequence of
+        the cache) at most `keep` stay, in every layer and kv head: the first `first`,
+        the last `last` and those of the highest weights.  The pages behind them are
+        given back.  Returns the new lengths and `kept` int32 [layers, sequences, kv
+        heads, keep] (the numbers that the kept keys had; -1 throughout where none went)."""
+        torch, P, cache = self.torch, self.P, self.cache
+        if self.score is None:
+            raise RuntimeError("a decoder without `window` keeps no weights")
+        lens = [int(n) for n in lens]
+        if len(lens) != self.score.shape[1] or keep < 1:
+            raise ValueError("a length for each sequence, and at least one key to keep")
+        if stream is not None:
+            with P._on(cache, stream):
+                return self.evict(lens, keep, first, last)
+        book, page = cache._book(), cache.page
+        over = [s for s, n in enumerate(lens) if n > keep]
+        for s in over:
+            if lens[s] > book.held(s) * page:
+                raise ValueError(f"sequence {s} holds pages of {book.held(s) * page} keys, not of {lens[s]}")
+        table = book.table()
+        for s in over:  # the pages that are written: no other sequence's
+            for i in range((keep + page - 1) // page):
+                if book.shared(int(table[s, i])) > 1:
+                    cache.reserve(s, i * page + 1, (i + 1) * page)
+        i32 = {"dtype": torch.int32, "device": self.score.device}
+        before = torch.tensor(lens, **i32)
+        new_len, kept = torch.empty_like(before), torch.empty(*self.score.shape[:3], keep, **i32)
+        P.evict(cache, before, self.score, kept, self.score, new_len, None, first, last)
+        self.gone += before - new_len
+        for s in over:
+            cache.trim(s, keep)
+        return [min(n, keep) for n in lens], kept
