@@ -720,9 +720,7 @@ struct EvictArgs {
   int32_t *new_len;
 };
 
-constexpr int PICK = 1024;   // the most threads that pick a head's keys
 constexpr int BINS = 2048;
-constexpr int HELD = 32768;  // scores of a head in LDS
 constexpr int FEWEST = 512;  // keys whose border is found by rank
 
 // Keys that a sequence keeps, or -1: it stays as it is.
@@ -735,52 +733,60 @@ __device__ __forceinline__ int budget_of(const EvictArgs &a, int s, int len) {
   return len > b && len <= a.room && len <= (int64_t)a.pool.max_pages << a.pool.lp ? b : -1;
 }
 
-// Scores in the order of whole numbers; NaN below all, zeros alike.
+// Scores in the order of whole numbers, between NEVER and ALWAYS; NaN below all, zeros alike.
+constexpr uint32_t NEVER = 0, ALWAYS = ~0u;
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
-  return x != x ? 0u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return x != x ? 1u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
+// Bits of the lanes below this one, and `more`.
+__device__ __forceinline__ uint32_t below(uint64_t bits, uint32_t more) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(bits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bits, more));
+}
+// Of the waves' numbers: the sum of those before this wave, and of all.  (By lanes: P / 64
+// numbers in registers would be too many beside the scores.)
+template <int P>
+__device__ __forceinline__ uint32_t before_wave(const uint32_t (&waves)[P / 64], uint32_t &whole) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t v = lane < P / 64 ? waves[lane] : 0, x = (uint32_t)scan((int)v);
+  whole = __builtin_amdgcn_readlane(x, 63);
+  return __builtin_amdgcn_readlane(x - v, wave);
+}
 // Sum over the workgroup's threads before this one, and over all.
 template <int P>
 __device__ __forceinline__ uint32_t before(uint32_t v, uint32_t (&waves)[P / 64], uint32_t &whole) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t x = (uint32_t)scan((int)v);
   __syncthreads();
-  if (lane == 63) waves[wave] = x;
+  if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = x;
   __syncthreads();
-  uint32_t base = 0;
-  whole = 0;
-#pragma unroll
-  for (int w = 0; w < P / 64; ++w) {
-    if (w < wave) base += waves[w];
-    whole += waves[w];
-  }
-  return base + x - v;
+  return before_wave<P>(waves, whole) + x - v;
 }
 
-// P threads a sequence, layer and kv head.  The budget's border is found by
+// P threads a sequence, layer and kv head, N scores of each in registers (where there
+// are more than P N they are read again in each pass).  The budget's border is found by
 // counting: the range of the scores in BINS bins, then the bin that holds the
 // border in BINS again, three rounds at most (32 bits of order), or, once a bin
 // holds few keys, by each one's rank among them.  Bins divide the range that
 // the scores have, so that few of them fall into one and the counters in LDS are
 // rarely fought over.  Then the keys above the border, and as many of those on
-// it as are left, earliest first, get their places by counting again.  Scores
-// stay in LDS, `held` of them; where there are more they are read again.  Bound by
-// the chain of passes and barriers, not by bytes.
-template <int P>
-__global__ __launch_bounds__(P) void evict_pick_kernel(EvictArgs a, int held) {
-  extern __shared__ float scores[];
-  __shared__ uint32_t bins[BINS], waves[P / 64];
-  __shared__ uint32_t lows[P / 64], highs[P / 64];
-  __shared__ uint32_t rows[32 * P / 64];  // of 32 turns
+// it as are left, earliest first, get their places by counting: a wave's keys lie
+// side by side, so that the waves' counts join once.
+template <int P, int N, bool MANY>
+__global__ __launch_bounds__(P) void evict_pick_kernel(EvictArgs a) {
+  constexpr int HELD = P * N, WAVES = P / 64;
+  // the keys that stay meet in LDS, where a turn's few of a wave cost less than stores
+  constexpr int STAGED = HELD < 4096 ? HELD : 4096;
+  __shared__ int places[STAGED];
+  // few keys: of their order, and the earlier one above the later
+  __shared__ __align__(16) union { uint32_t bins[BINS]; uint64_t cand[FEWEST + 1]; } m;
+  __shared__ uint32_t waves[WAVES], lows[WAVES], highs[WAVES];
   __shared__ int chosen, above, holds, count, found_ties;
   __shared__ uint32_t found;
-  uint32_t *const cand = bins;  // FEWEST keys, then their numbers
   const int heads = a.layers * a.pool.kv;
   const int s = blockIdx.x / heads, lh = blockIdx.x - s * heads;
   const int layer = lh / a.pool.kv, h = lh - layer * a.pool.kv;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int len = a.len[s];
   const int b = budget_of(a, s, len);
   const size_t at = ((size_t)layer * a.seqs + s) * a.pool.kv + h;
@@ -789,67 +795,79 @@ __global__ __launch_bounds__(P) void evict_pick_kernel(EvictArgs a, int held) {
   int32_t *kept = a.kept + at * a.most;
   const int head = min(a.first, max(b, 0)), tail = min(a.last, max(b, 0) - head);  // those that stay anyway
   const int lo = head, hi = len - tail;                                            // the others
-  // a thread reads what it has written: keys tid, tid + P, ... of a block
-  const int blocks = b < 0 ? 0 : (len + held - 1) / held;
-  uint32_t low = ~0u, high = 0;  // the others' range
-  auto read = [&](int blk) {
-    const int n = min(held, len - blk * held);
-#pragma unroll 16
-    for (int i = tid; i < n; i += P) scores[i] = score[blk * held + i];
-    return n;
-  };
-  // f(key, its number) for the thread's keys among the others
-  auto each = [&](auto &&f) {
-    for (int blk = 0; blk < blocks; ++blk) {
-      const int n = blocks > 1 ? read(blk) : len, from = blk * held;
-#pragma unroll 4
-      for (int i = tid; i < n; i += P)
-        if (from + i >= lo && from + i < hi) f(ordered(scores[i]), from + i);
+  const int blocks = b < 0 ? 0 : MANY ? (len + HELD - 1) / HELD : 1;
+  // key number k0 + 64 e in turn e; those that are not among the others ALWAYS, those behind
+  // the wave's keys (in turns that a short sequence does not need) NEVER
+  uint32_t key[N];
+  int k0 = 0;
+  auto read = [&](int blk) __attribute__((always_inline)) {
+    const int each = 64 * ((min(HELD, len - blk * HELD) + P - 1) / P);
+    k0 = blk * HELD + wave * each + lane;
+    const int end = min(blk * HELD + (wave + 1) * each, len);
+    float x[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = score[min(k0 + 64 * e, len - 1)];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int k = k0 + 64 * e;
+      key[e] = k >= end ? NEVER : (uint32_t)(k - lo) < (uint32_t)(hi - lo) ? ordered(x[e]) : ALWAYS;
     }
   };
-  if (blocks == 1) read(0);
+  auto each = [&](auto &&f) __attribute__((always_inline)) {
+    for (int blk = 0; blk < blocks; ++blk) {
+      if (MANY) read(blk);
+      asm volatile("" : "+v"(k0));  // (N numbers of keys are not kept)
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(key[e], k0 + 64 * e);
+    }
+  };
+  if (!MANY && b >= 0) read(0);
+  uint32_t low = ALWAYS, past = 0;  // the others' range: low + 1 .. past - 1
   bool bad = b < 0;
   if (!bad) {
 #pragma unroll 4
-    for (int x = tid; x < (len + (1 << a.pool.lp) - 1) >> a.pool.lp; x += P)
-      bad |= (uint32_t)a.pool.table[(size_t)s * a.pool.max_pages + x] >= (uint32_t)a.pool.pages;
-    each([&](uint32_t k, int) { low = min(low, k), high = max(high, k); });
+    for (int y = tid; y < (len + (1 << a.pool.lp) - 1) >> a.pool.lp; y += P)
+      bad |= (uint32_t)a.pool.table[(size_t)s * a.pool.max_pages + y] >= (uint32_t)a.pool.pages;
+    each([&](uint32_t k, int) { low = min(low, k - 1), past = max(past, k + 1); });
   }
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1)
-    low = min(low, (uint32_t)__shfl_xor((int)low, m)), high = max(high, (uint32_t)__shfl_xor((int)high, m));
-  if (lane == 0) lows[wave] = low, highs[wave] = high;
-  for (int i = tid; i < BINS; i += P) bins[i] = 0;
+  for (int y = 1; y < 64; y <<= 1)
+    low = min(low, (uint32_t)__shfl_xor((int)low, y)), past = max(past, (uint32_t)__shfl_xor((int)past, y));
+  if (lane == 0) lows[wave] = low, highs[wave] = past;
+  for (int i = tid; i < BINS; i += P) m.bins[i] = 0;
   bad = __syncthreads_or(bad);
   if (tid == 0 && lh == 0) a.new_len[s] = bad ? len : b;
-  for (int x = (bad ? 0 : b) + tid; x < a.most; x += P) kept[x] = -1;
+  for (int y = (bad ? 0 : b) + tid; y < a.most; y += P) kept[y] = -1;
   if (bad || b == 0) return;
   int need = b - head - tail;
   // the border: keys of more than `border` stay, and the first `ties` on it
-  uint32_t border = ~0u;
+  uint32_t border = ALWAYS - 1;
   int ties = 0;
   if (need > 0) {
+    low = lows[lane % WAVES], past = highs[lane % WAVES];
 #pragma unroll
-    for (int w = 0; w < P / 64; ++w) low = min(low, lows[w]), high = max(high, highs[w]);
-    uint32_t width = high - low;  // the range: low .. low + width
+    for (int y = 1; y < WAVES; y <<= 1)
+      low = min(low, (uint32_t)__shfl_xor((int)low, y)), past = max(past, (uint32_t)__shfl_xor((int)past, y));
+    uint32_t width = past - 2 - low;  // the range: low .. low + width
+    ++low;
     for (;;) {
       const int shift = max(0, 32 - (width ? __builtin_clz(width) : 32) - 11);
       each([&](uint32_t k, int) {
-        if (k - low <= width) atomicAdd(&bins[(k - low) >> shift], 1u);
+        if (k - low <= width) atomicAdd(&m.bins[(k - low) >> shift], 1u);
       });
       if (tid == 0) count = 0;
       __syncthreads();
       // a thread's bins, the highest first
-      constexpr int N = BINS / P;
-      uint32_t own[N], all = 0, whole;
+      constexpr int B = BINS / P;
+      uint32_t own[B], all = 0, whole;
 #pragma unroll
-      for (int e = 0; e < N; ++e) all += own[e] = bins[BINS - 1 - N * tid - e];
+      for (int e = 0; e < B; ++e) all += own[e] = m.bins[BINS - 1 - B * tid - e];
       uint32_t over = before<P>(all, waves, whole);
       if (over < (uint32_t)need && over + all >= (uint32_t)need) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
+        for (int e = 0; e < B; ++e) {
           if (over < (uint32_t)need && over + own[e] >= (uint32_t)need)
-            chosen = BINS - 1 - N * tid - e, above = (int)over, holds = (int)own[e];
+            chosen = BINS - 1 - B * tid - e, above = (int)over, holds = (int)own[e];
           over += own[e];
         }
       }
@@ -862,68 +880,98 @@ __global__ __launch_bounds__(P) void evict_pick_kernel(EvictArgs a, int held) {
       if (shift == 0) break;
       if (n <= FEWEST) {
         each([&](uint32_t k, int i) {
-          if (k - low > width) return;
-          const int c = atomicAdd(&count, 1);
-          cand[c] = k, cand[FEWEST + c] = i;
+          if (k - low <= width) m.cand[atomicAdd(&count, 1)] = (uint64_t)k << 32 | ~(uint32_t)i;
         });
+        if (tid == 0) m.cand[n] = 0;
         __syncthreads();
         for (int y = tid; y < n; y += P) {
-          const uint32_t k = cand[y], i = cand[FEWEST + y];
-          int more = 0, same = 0;  // before this one: of higher keys, of the same and an earlier number
-          for (int c = 0; c < n; ++c) {
-            more += cand[c] > k;
-            same += cand[c] == k && cand[FEWEST + c] < i;
+          const uint64_t own_key = m.cand[y];
+          int more = 0, higher = 0;  // before this one, and those of them of higher scores
+#pragma unroll 4
+          for (int c = 0; c < n; c += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(m.cand + c);
+            more += (two.x > own_key) + (two.y > own_key);
+            higher += (uint32_t)(two.x >> 32) > (uint32_t)(own_key >> 32);
+            higher += (uint32_t)(two.y >> 32) > (uint32_t)(own_key >> 32);
           }
-          if (more + same == need - 1) found = k, found_ties = need - more;
+          if (more == need - 1) found = (uint32_t)(own_key >> 32), found_ties = need - higher;
         }
         __syncthreads();
         border = found, ties = found_ties;
         break;
       }
-      for (int i = tid; i < BINS; i += P) bins[i] = 0;
+      for (int i = tid; i < BINS; i += P) m.bins[i] = 0;
       __syncthreads();
     }
   }
-  // places: what stays whatever the ties are, and the ties, before each key; 32 turns
-  // of the threads at once
-  uint32_t sure0 = 0, tie0 = 0;  // of the keys before
+  // places: what stays whatever the ties are, and the ties, before each key
+  const bool staged = b <= STAGED;
+  uint32_t sure0 = 0, tie0 = 0;  // of the blocks before
   for (int blk = 0; blk < blocks; ++blk) {
-    const int n = blocks > 1 ? read(blk) : len;
-    for (int i0 = 0; i0 < n; i0 += 32 * P) {
-      const int from = blk * held + i0, turns = min(32, (n - i0 + P - 1) / P);
-      uint32_t stays = 0, on = 0;  // a bit a turn
-      for (int e = 0; e < turns; ++e) {
-        const int i = e * P + tid, key = from + i;
-        const bool there = i0 + i < n, other = key >= lo && key < hi;
-        const uint32_t k = there ? ordered(scores[i0 + i]) : 0;
-        const bool sure = there && (!other || k > border), tie = there && other && k == border;
-        stays |= (uint32_t)sure << e, on |= (uint32_t)tie << e;
-        const uint64_t bs = __ballot(sure), bt = __ballot(tie);
-        if (lane == 0) rows[e * (P / 64) + wave] = (uint32_t)__popcll(bs) | (uint32_t)__popcll(bt) << 16;
-      }
-      __syncthreads();
-      // (32 turns' counts for P / 2 threads at most)
-      uint32_t whole;
-      const bool has = tid < turns * (P / 64);
-      const uint32_t pre = before<P>(has ? rows[tid] : 0, waves, whole);
-      if (has) rows[tid] = pre;
-      __syncthreads();
-      const uint64_t under = (1ull << lane) - 1;
-      for (int e = 0; e < turns; ++e) {
-        const bool sure = stays >> e & 1, tie = on >> e & 1;
-        const uint64_t bs = __ballot(sure), bt = __ballot(tie);
-        const uint32_t r = rows[e * (P / 64) + wave];
-        const uint32_t ns = sure0 + (r & 0xFFFFu) + __popcll(bs & under);
-        const uint32_t nt = tie0 + (r >> 16) + __popcll(bt & under);
-        if (sure || (tie && nt < (uint32_t)ties)) {
-          const uint32_t place = ns + min(nt, (uint32_t)ties);
-          kept[place] = from + e * P + tid;
-          to_score[place] = scores[i0 + e * P + tid];
+    if (MANY) read(blk);
+    uint32_t sure = 0, tie = 0;  // the wave's
+    asm volatile("" : "+v"(k0));
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      sure += __popcll(__ballot(key[e] > border));
+      tie += __popcll(__ballot(key[e] == border));
+    }
+    // (of a wave and of a block, neither is more than 16 bits hold)
+    __syncthreads();
+    if (lane == 0) waves[wave] = sure | tie << 16;
+    __syncthreads();
+    uint32_t whole;
+    const uint32_t both = before_wave<P>(waves, whole);
+    uint32_t ns = sure0 + (both & 0xFFFFu), nt = tie0 + (both >> 16);
+    sure0 += whole & 0xFFFFu, tie0 += whole >> 16;
+    auto place = [&](auto &&put) __attribute__((always_inline)) {
+      if (tie == 0) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          asm volatile("" : "+v"(border), "+v"(k0));  // (compared again, not kept from before)
+          const uint64_t bs = __ballot(key[e] > border);
+          if (key[e] > border) put(below(bs, ns + min(nt, (uint32_t)ties)), e);
+          ns += __popcll(bs);
         }
+        return;
       }
-      sure0 += whole & 0xFFFFu;
-      tie0 += whole >> 16;
-      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        asm volatile("" : "+v"(border), "+v"(k0));
+        const bool on = key[e] == border;
+        const uint64_t bs = __ballot(key[e] > border), bt = __ballot(on);
+        const uint32_t t = below(bt, nt);
+        if (key[e] > border || (on && t < (uint32_t)ties)) put(below(bs, ns) + min(t, (uint32_t)ties), e);
+        ns += __popcll(bs), nt += __popcll(bt);
+      }
+    };
+    if (staged)
+      place([&](uint32_t to, int e) { places[to] = k0 + 64 * e; });
+    else
+      place([&](uint32_t to, int e) { kept[to] = k0 + 64 * e; });
+  }
+  // places ascend and no key moves back: what a turn overwrites only turns up to it read
+  for (int y0 = 0; y0 < b; y0 += 4 * P) {
+    __syncthreads();
+    int from[4];
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int y = min(y0 + P * i + tid, b - 1);
+      from[i] = staged ? places[y] : kept[y];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = score[from[i]];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x[i]));  // in its register
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int y = y0 + P * i + tid;
+      if (y < b) {
+        if (staged) kept[y] = from[i];
+        to_score[y] = x[i];
+      }
     }
   }
 }
@@ -1173,13 +1221,26 @@ exl3_verdict exl3p_evict(const exl3p_cache *c, int32_t seqs, const int32_t *len,
   a.len = len, a.score = score, a.room = room, a.keep = keep, a.most = most;
   a.first = first, a.last = last, a.kept = kept, a.new_score = new_score, a.new_len = new_len;
   const hipStream_t st = static_cast<hipStream_t>(s);
-  if (room <= 16 * 256) {
-    const int held = (room + 255) / 256 * 256;
-    hipLaunchKernelGGL(evict_pick_kernel<256>, dim3((unsigned)n), dim3(256), held * sizeof(float), st, a, held);
-  } else {
-    const int held = room < HELD ? (room + PICK - 1) / PICK * PICK : HELD;
-    hipLaunchKernelGGL(evict_pick_kernel<PICK>, dim3((unsigned)n), dim3(PICK), held * sizeof(float), st, a, held);
-  }
+  auto pick = [&](auto threads, auto each, auto many) {
+    hipLaunchKernelGGL((evict_pick_kernel<decltype(threads)::value, decltype(each)::value, decltype(many)::value>),
+                       dim3((unsigned)n), dim3(decltype(threads)::value), 0, st, a);
+  };
+  typedef std::integral_constant<int, 256> Few;
+  typedef std::integral_constant<int, 1024> Many;
+  // as few turns as the room asks for (a turn is work whether it has keys or not), and
+  // wide workgroups only where 256 threads would have too many: 9.0 us for 1100 keys
+  // with 16 turns of 256, 7.9 with 8; 19 for 4096 keys of 128 heads with 1024 threads, 13
+  // with 256; 35 for 32768 with the scores in LDS, 18 in registers
+  if (room <= 256 * 8)
+    pick(Few{}, std::integral_constant<int, 8>{}, std::false_type{});
+  else if (room <= 256 * 16)
+    pick(Few{}, std::integral_constant<int, 16>{}, std::false_type{});
+  else if (room <= 1024 * 16)
+    pick(Many{}, std::integral_constant<int, 16>{}, std::false_type{});
+  else if (room <= 1024 * 32)
+    pick(Many{}, std::integral_constant<int, 32>{}, std::false_type{});
+  else
+    pick(Many{}, std::integral_constant<int, 32>{}, std::true_type{});
   if (c->dim == 64)
     hipLaunchKernelGGL(evict_move_kernel<64>, dim3((unsigned)(n * parts)), dim3(MV), 0, st, a);
   else
