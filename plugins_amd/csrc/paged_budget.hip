@@ -1204,7 +1204,7 @@ exl3_verdict exl3p_evict(const exl3p_cache *c, int32_t seqs, const int32_t *len,
     return refuse(EXL3_FAILED, "PagedEvict: a missing array");
   const int64_t n = (int64_t)c->layers * seqs * c->kv_heads;
   const int parts = 2 * c->dim / 64;
-  if (n * 4 > GRID_MAX)  // of 1024 threads, and of 256
+  if (n * 4 > GRID_MAX)  // of 1024 threads, and `parts` of 256
     return refuse(EXL3_TOO_LARGE, "PagedEvict: too many layers, sequences and heads for one call");
   const Span2D from = array(score, n * room * 4), to = array(new_score, n * room * 4);
   const int64_t pool = (int64_t)layer_bytes(c) * c->layers;
@@ -1225,22 +1225,23 @@ exl3_verdict exl3p_evict(const exl3p_cache *c, int32_t seqs, const int32_t *len,
     hipLaunchKernelGGL((evict_pick_kernel<decltype(threads)::value, decltype(each)::value, decltype(many)::value>),
                        dim3((unsigned)n), dim3(decltype(threads)::value), 0, st, a);
   };
-  typedef std::integral_constant<int, 256> Few;
-  typedef std::integral_constant<int, 1024> Many;
-  // as few turns as the room asks for (a turn is work whether it has keys or not), and
-  // wide workgroups only where 256 threads would have too many: 9.0 us for 1100 keys
-  // with 16 turns of 256, 7.9 with 8; 19 for 4096 keys of 128 heads with 1024 threads, 13
-  // with 256; 35 for 32768 with the scores in LDS, 18 in registers
+  // as few turns and threads as the room asks for (a turn is work whether it has keys or
+  // not): 9.4 us for 1100 keys of 288 heads with 16 turns of 256 threads, 7.9 with 8; 12.8 for
+  // 4096 of 1024 heads with 16 of 256, 11.2 with 8 of 512, 16.6 with 4 of 1024; 18 for 32768
+  // of 64 heads, 36 with the scores in LDS instead
+  typedef std::integral_constant<int, 8> Few;
+  typedef std::integral_constant<int, 32> Many;
+  typedef std::integral_constant<int, 1024> Wide;
   if (room <= 256 * 8)
-    pick(Few{}, std::integral_constant<int, 8>{}, std::false_type{});
-  else if (room <= 256 * 16)
-    pick(Few{}, std::integral_constant<int, 16>{}, std::false_type{});
-  else if (room <= 1024 * 16)
-    pick(Many{}, std::integral_constant<int, 16>{}, std::false_type{});
+    pick(std::integral_constant<int, 256>{}, Few{}, std::false_type{});
+  else if (room <= 512 * 8)
+    pick(std::integral_constant<int, 512>{}, Few{}, std::false_type{});
+  else if (room <= 1024 * 8)
+    pick(Wide{}, Few{}, std::false_type{});
   else if (room <= 1024 * 32)
-    pick(Many{}, std::integral_constant<int, 32>{}, std::false_type{});
+    pick(Wide{}, Many{}, std::false_type{});
   else
-    pick(Many{}, std::integral_constant<int, 32>{}, std::true_type{});
+    pick(Wide{}, Many{}, std::true_type{});
   if (c->dim == 64)
     hipLaunchKernelGGL(evict_move_kernel<64>, dim3((unsigned)(n * parts)), dim3(MV), 0, st, a);
   else

@@ -618,6 +618,9 @@ EVICT = [
     ([9000], 2, 64, 128, 1, 700, 4, 32, 7),
     ([600, 700], 2, 128, 64, 1, 10, 20, 5, 0),
     ([5000], 1, 128, 64, 2, 4200, 0, 1, 2),
+    ([4096, 2049, 2048], 1, 64, 16, 1, 2048, 4, 0, 0), ([16384, 4097], 1, 64, 64, 1, 8000, 1, 3, 0),
+    ([20000, 9001], 1, 64, 64, 1, 9000, 3, 5, 0), ([70001, 33000], 1, 64, 256, 1, 40000, 7, 100, 3),
+    ([50000], 1, 64, 256, 1, 3000, 0, 40, 0),
 ]
 
 
@@ -635,7 +638,7 @@ def test_evict(lens, kv, dim, page, layers, most, first, last, more, in_place, d
 def test_evict_scores(kind, n):
     """Scores that are alike, of few values, of both signs and zeros, infinities and NaN,
     in order, below the smallest normal number, or next to one another; more of them
-    than LDS holds."""
+    than registers hold."""
     if n > 1000 and kind in ("tiny", "signs"):
         pytest.skip("the small size covers it")
     page = 64
