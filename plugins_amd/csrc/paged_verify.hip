@@ -745,6 +745,66 @@ __device__ __forceinline__ void ends(int &lo, int &hi, int (&waves)[2][ST / 64])
   for (int w = 0; w < ST / 64; ++w) lo = min(lo, waves[0][w]), hi = max(hi, waves[1][w]);
 }
 
+// The token that u says: the piece whose sum passes the border first, then the place in
+// it.  sum_of(x, kind): piece x's sum; at(piece): its first element; of(e, kind, r): the
+// block at e.  Kinds after the first stand in where all before them are 0 throughout.
+template <int N, typename SUM, typename AT, typename OF>
+__device__ __forceinline__ void choose(const VerifyArgs &a, int row, double u, int kinds, SUM &&sum_of, AT &&at,
+                                       OF &&of) {
+  __shared__ double waves[ST / 64], base;
+  __shared__ int least[2][ST / 64];
+  const int each = (a.draws + ST - 1) / ST, x0 = threadIdx.x * each, x1 = min(x0 + each, a.draws);
+  double whole, run;
+  int kind = 0;
+  for (;; ++kind) {
+    double own = 0.0;
+    for (int x = x0; x < x1; ++x) own += sum_of(x, kind);
+    run = before(own, waves, whole);
+    if (whole > 0.0 || kind == kinds - 1) break;
+  }
+  const double border = u * whole;
+  int found = INT32_MAX, last = -1;
+  double under = 0.0;  // what lies before the piece found
+  for (int x = x0; x < x1; ++x) {
+    const double v = sum_of(x, kind);
+    if (v > 0.0) {
+      last = x;
+      if (found == INT32_MAX && run + v > border) found = x, under = run;
+    }
+    run += v;
+  }
+  const int mine = found;
+  ends(found, last, least);
+  const bool passed = found != INT32_MAX;
+  const int piece = passed ? found : max(last, 0);
+  if (passed && mine == found) base = under;
+  const int from = at(piece);
+  __syncthreads();
+  double r[DRAW / ST], own = 0.0;
+#pragma unroll
+  for (int k = 0; k < DRAW / ST / N; ++k) {
+    double v[N];
+    of(from + ((int)threadIdx.x * (DRAW / ST / N) + k) * N, kind, v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) own += r[k * N + i] = v[i];
+  }
+  double sum;
+  run = (passed ? base : -INFINITY) + before(own, waves, sum);
+  found = INT32_MAX, last = -1;
+#pragma unroll
+  for (int k = 0; k < DRAW / ST; ++k) {
+    run += r[k];
+    const int e = from + (int)threadIdx.x * (DRAW / ST) + k;
+    if (r[k] > 0.0) {
+      last = e;
+      if (found == INT32_MAX && run > border) found = e;
+    }
+  }
+  ends(found, last, least);
+  // (sums in another order may end a step short of the border: the last one then)
+  if (threadIdx.x == 0) a.target[row] = found != INT32_MAX ? found : last;
+}
+
 // The sampling: sums of DRAW tokens a workgroup, and by the sequence's last one to
 // arrive the token, the piece whose sum passes the border first, then the place in it.
 // The sums go out and come in past the caches of an XCD.  OWN: the
@@ -754,8 +814,8 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
   constexpr int N = Vec<E>::N;
   __shared__ Walk<OWN ? SHORT : 1, DRAFT> walked;
   __shared__ uint32_t gone[DRAW / 32];
-  __shared__ double waves[ST / 64], whole_waves[ST / 64], base;
-  __shared__ int least[2][ST / 64], order;
+  __shared__ double waves[ST / 64], whole_waves[ST / 64];
+  __shared__ int order;
   const int s = blockIdx.x / a.draws, own_piece = blockIdx.x - s * a.draws;
   Tip tip;
   if constexpr (OWN) {
@@ -799,59 +859,124 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
     __syncthreads();
     if (order != a.draws - 1) return;
   }
-  const int each = (a.draws + ST - 1) / ST, x0 = threadIdx.x * each, x1 = min(x0 + each, a.draws);
+  // two kinds: where nothing is left of p~ (by rounding), p in its place
   auto sum_of = [&](int x, int kind) {
     return __hip_atomic_load(&sums[2 * x + kind], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   };
-  double whole, run;
-  int kind = 0;  // 1: nothing is left of p~ (by rounding), p in its place
-  for (;; kind = 1) {
-    double own = 0.0;
-    for (int x = x0; x < x1; ++x) own += sum_of(x, kind);
-    run = before(own, waves, whole);
-    if (whole > 0.0 || kind == 1) break;
-  }
-  const double border = tip.u * whole;
-  int found = INT32_MAX, last = -1;
-  double under = 0.0;  // what lies before the piece found
-  for (int x = x0; x < x1; ++x) {
-    const double v = sum_of(x, kind);
-    if (v > 0.0) {
-      last = x;
-      if (found == INT32_MAX && run + v > border) found = x, under = run;
-    }
-    run += v;
-  }
-  const int mine = found;
-  ends(found, last, least);
-  const bool passed = found != INT32_MAX;
-  const int piece = passed ? found : max(last, 0), from = rest.first(piece);
-  if (passed && mine == found) base = under;
-  rest.mark(s, from, gone);
-  __syncthreads();
-  double r[DRAW / ST], own = 0.0;
-#pragma unroll
-  for (int k = 0; k < DRAW / ST / N; ++k) {
+  int from = 0;
+  auto at = [&](int piece) {
+    from = rest.first(piece);
+    rest.mark(s, from, gone);
+    return from;
+  };
+  auto of = [&](int e, int kind, double (&v)[N]) {
     double p[N], left[N];
-    rest.of(from + ((int)threadIdx.x * (DRAW / ST / N) + k) * N, gone, from, p, left);
+    rest.of(e, gone, from, p, left);
 #pragma unroll
-    for (int i = 0; i < N; ++i) own += r[k * N + i] = kind == 1 ? p[i] : left[i];
-  }
-  double sum;
-  run = (passed ? base : -INFINITY) + before(own, waves, sum);
-  found = INT32_MAX, last = -1;
+    for (int i = 0; i < N; ++i) v[i] = kind == 1 ? p[i] : left[i];
+  };
+  choose<N>(a, tip.row, tip.u, 2, sum_of, at, of);
+}
+
+// A step of single rows has nothing to walk: each piece's largest logit and the sum of its
+// powers below that one, in 64 bits at once, ...
+template <typename E>
+__global__ __launch_bounds__(ST) void verify_single_kernel(VerifyArgs a) {
+  constexpr int N = Vec<E>::N, U = DRAW / ST / N;
+  __shared__ float tops[ST / 64];
+  __shared__ double waves[ST / 64];
+  const int s = blockIdx.x / a.draws, piece = blockIdx.x - s * a.draws;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Seq q = seq_of(a, s);
+  if (q.n <= 0) return;
+  const char *row = row_of<E>(a, q.begin);
+  const int first = first_of<E>(row, piece, DRAW);
+  float x[U][N];
 #pragma unroll
-  for (int k = 0; k < DRAW / ST; ++k) {
-    run += r[k];
-    const int e = from + (int)threadIdx.x * (DRAW / ST) + k;
-    if (r[k] > 0.0) {
-      last = e;
-      if (found == INT32_MAX && run > border) found = e;
-    }
+  for (int k = 0; k < U; ++k)
+    Vec<E>::unpack(block_of<E>(row, first + (k * ST + (int)threadIdx.x) * N, a.vocab), x[k]);
+  float top = x[0][0];
+#pragma unroll
+  for (int k = 0; k < U; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = larger(top, x[k][i]);
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) top = larger(top, exl3::xor_lanes(top, m));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < ST / 64; ++w) top = larger(top, tops[w]);
+  // (greedy: minus the first place of it, the largest of which is looked for)
+  double all = q.greedy ? -INFINITY : 0.0;
+  if (q.greedy) {
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (x[k][i] == top) all = fmax(all, -(double)(first + (k * ST + (int)threadIdx.x) * N + i));
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) all = fmax(all, __shfl_xor(all, m));
+  } else if (q.fit && top > -INFINITY && top < INFINITY) {
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) all += exp_of(((double)x[k][i] - (double)top) * q.inv);
+    all = wave_sum(all);
   }
-  ends(found, last, least);
-  // (sums in another order may end a step short of the border: the last one then)
-  if (threadIdx.x == 0) a.target[tip.row] = found != INT32_MAX ? found : last;
+  if (lane == 0) waves[wave] = all;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < ST / 64; ++w) all = q.greedy ? fmax(all, waves[w]) : all + waves[w];
+    double *to = a.sums + ((size_t)s * a.draws + piece) * 2;
+    to[0] = all, to[1] = (double)top;
+  }
+}
+// ... and the token, a workgroup a sequence.
+template <typename E>
+__global__ __launch_bounds__(ST) void verify_single_draw_kernel(VerifyArgs a) {
+  constexpr int N = Vec<E>::N;
+  __shared__ float tops[ST / 64];
+  __shared__ int firsts[ST / 64];
+  const int s = blockIdx.x;
+  const Seq q = seq_of(a, s);
+  if (q.n <= 0) return;
+  const double *sums = a.sums + (size_t)s * a.draws * 2;
+  float top = -INFINITY;
+  for (int x = threadIdx.x; x < a.draws; x += ST) top = larger(top, (float)sums[2 * x + 1]);
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) top = larger(top, exl3::xor_lanes(top, m));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < ST / 64; ++w) top = larger(top, tops[w]);
+  if (!q.fit || !(top > -INFINITY) || (!q.greedy && top == INFINITY)) {
+    if (threadIdx.x == 0) a.target[q.begin] = -1;
+    return;
+  }
+  if (q.greedy) {
+    int best = INT32_MAX;
+    for (int x = threadIdx.x; x < a.draws; x += ST)
+      if ((float)sums[2 * x + 1] == top) best = min(best, (int)-sums[2 * x]);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) best = min(best, __shfl_xor(best, m));
+    if ((threadIdx.x & 63) == 0) firsts[threadIdx.x >> 6] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < ST / 64; ++w) best = min(best, firsts[w]);
+    if (threadIdx.x == 0) a.target[q.begin] = best;
+    return;
+  }
+  const char *row = row_of<E>(a, q.begin);
+  auto sum_of = [&](int x, int) { return sums[2 * x] * exp_of((sums[2 * x + 1] - (double)top) * q.inv); };
+  auto at = [&](int piece) { return first_of<E>(row, piece, DRAW); };
+  auto of = [&](int e, int, double (&v)[N]) {
+    float x[N];
+    Vec<E>::unpack(block_of<E>(row, e, a.vocab), x);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = exp_of(((double)x[k] - (double)top) * q.inv);
+  };
+  choose<N>(a, q.begin, a.u[q.begin], 1, sum_of, at, of);
 }
 
 // ------------------------------------------------------------------- host side
@@ -999,6 +1124,11 @@ exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int3
     hipLaunchKernelGGL((verify_draw_kernel<E, Q, D, false>), all, dim3(ST), 0, st, a);
   };
   by_dtype(logits_dtype, [&](auto e) {
+    if (r->max_rows == 1) {
+      hipLaunchKernelGGL((verify_single_kernel<decltype(e)>), all, dim3(ST), 0, st, a);
+      hipLaunchKernelGGL((verify_single_draw_kernel<decltype(e)>), dim3(r->seqs), dim3(ST), 0, st, a);
+      return;
+    }
     if (!lazy)
       hipLaunchKernelGGL((verify_stats_kernel<decltype(e)>), dim3((unsigned)(r->rows * pieces)), dim3(ST), 0,
                          st, a);
