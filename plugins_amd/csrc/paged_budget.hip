@@ -22,7 +22,8 @@ struct WeighArgs {
   float *score;
   int room;
   float target;  // items of a kv head
-  float least;   // 64-key units of one, at least
+  float least;   // 64-key units of one, at least,
+  float fill, some;  // and as many as leave `fill` items of a kv head, up to `some`
   int slots;     // items * kv that part holds
   int tile;      // pairs of an item
   f32x2 *part;   // [items * kv][tile]: an item's reference and sum of each pair
@@ -99,7 +100,8 @@ struct Finder {
     none = __ballot(back) != 0;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) units += exl3::xor_lanes(units, m);
-    chunk = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / a.target), a.least),
+    chunk = __builtin_amdgcn_readfirstlane((int)fminf(fmaxf(fmaxf(ceilf(units * (1.0f + 0x1p-12f) / a.target), a.least),
+                                                            fminf(ceilf(units / a.fill), a.some)),
                                                       KIND == DEAL ? (float)(PART / 64) : (float)(1 << 25)));
   }
   __device__ __forceinline__ Find at(int x) {
@@ -239,6 +241,37 @@ struct Keys {
   __device__ __forceinline__ void anew() { asm volatile("" : "+v"(ka)); }
 };
 
+// A tile's products, of 64 keys and 32 pairs.  Four pieces of keys are on their way from LDS
+// while four are multiplied (the compiler's own order waits for each piece right after it
+// has asked for it: 287 us, not 270, for 3 prompts of up to 2048 rows).  64 pairs a wave,
+// which reads half as much of LDS, leave two waves a SIMD: 286 us.
+template <typename E, int D, typename MMA>
+__device__ __forceinline__ void products(Keys<E, D> &keys, int buffer, f32x16 (&t)[2], MMA &&mma) {
+  constexpr int KK = D / 16, AT = 4, GROUPS = 2 * KK / AT;
+  typename E::V8 kf[2][AT];
+  auto read = [&](int g) {
+#pragma unroll
+    for (int x = 0; x < AT; ++x) kf[g & 1][x] = keys.piece(buffer, (g * AT + x) / KK, (g * AT + x) % KK);
+  };
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[b][r] = 0.0f;
+  read(0);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    if (g + 1 < GROUPS) read(g + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < AT; ++x) {
+      const int b = (g * AT + x) / KK, kk = (g * AT + x) % KK;
+      t[b] = mma(kf[g & 1][x], kk, t[b]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // The first pass: each pair's reference (its largest score, or less by SLACK at
 // most) and the sum of its weights over an item's keys.  128 pairs a workgroup, 32 a
 // wave; scores are S^T = K q^T (rows keys, columns pairs): a lane holds 32 keys' scores
@@ -291,14 +324,8 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_sums_kernel(WeighArgs a) {
     if (kb >= mine) return;
     keys.anew();
     f32x16 t[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) t[b][r] = 0.0f;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        t[b] = E::mma(keys.piece(step & 1, b, kk), __builtin_bit_cast(V8, qf[kk]), t[b]);
-    }
+    products<E, D>(keys, step & 1, t,
+                   [&](V8 kf, int kk, f32x16 c) { return E::mma(kf, __builtin_bit_cast(V8, qf[kk]), c); });
     if constexpr (decltype(TAIL)::value) {
       // element r of block b: key 32 b + 8 (r / 4) + 4 h + r % 4
       uint64_t my = seen64(a, w, i, kb);
@@ -453,6 +480,8 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
         far |= fabsf(lse[r]) > FAR;
       }
       far = __ballot(far) != 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(qf[kk]));  // (the sign is not turned in each tile)
       const float scale = far ? 1.0f : a.scale;
       for (int step = 0; step < steps; ++step, ++count) {
         keys.arrive();
@@ -466,14 +495,8 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
         if (any) {
           keys.anew();
           f32x16 t[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) t[b][r] = 0.0f;
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-              t[b] = E::mma(__builtin_bit_cast(V8, qf[kk]), keys.piece(count & 1, b, kk), t[b]);
-          }
+          products<E, D>(keys, count & 1, t,
+                         [&](V8 kf, int kk, f32x16 c) { return E::mma(__builtin_bit_cast(V8, qf[kk]), kf, c); });
           if (far) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -1076,6 +1099,9 @@ constexpr size_t KEPT_MAX = (size_t)1 << 30;
 // A deal is a tile, so that its pairs stay in registers, until the deals' sums would
 // take more than this.
 constexpr size_t SUMS_MAX = (size_t)1 << 28;
+// Items of many pairs, in first passes' workgroups: 264 us for 3 prompts of up to 2048 rows
+// with 2, 270 with 3, 305 and more with 4; 315 with 1, some of which are long after others.
+constexpr int ROUNDS = 2;
 Plan plan_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads, int32_t window, int32_t room) {
   Plan p;
   p.group = heads / c->kv_heads;
@@ -1087,7 +1113,7 @@ Plan plan_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads, int32_t w
   if (p.few == 0) p.rest = lse_bytes(c, r, p.group);
   p.tile = p.few ? FEW : TILE;
   p.tiles = rows_watched(r, window) * p.group / p.tile + r->seqs;
-  p.items = target_of(c) * (p.few ? 1 : 3) + p.tiles;
+  p.items = target_of(c) * (p.few ? 1 : ROUNDS) + p.tiles;
   for (p.deal = p.tile;; p.deal *= 2) {
     p.deals = p.few ? 1 : (int)((pairs + p.deal - 1) / p.deal);
     p.sums = p.deals > 1 ? up16((size_t)r->seqs * c->kv_heads * p.deals * room * sizeof(float)) : 0;
@@ -1158,6 +1184,11 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
   a.decay = decay, a.base = base, a.score = score, a.room = room;
   a.target = (float)(p.items - p.tiles), a.slots = (int)(p.items * c->kv_heads);
   a.least = p.few ? 2.0f : 4.0f;
+  // An item's start (its place among the items, its pairs' 32 KB of q) costs as much as some tiles
+  // of keys: up to 16 units while half the first pass' workgroups are left.  A window of 128
+  // pairs over 32048 keys and one over 24456: 78.5 us with 4 units at least, 72.7 while all of them are
+  // left, 67.7 so, 66.7 up to 24 units, 77.4 up to 32 and a quarter of them.
+  a.fill = 0.5f * (float)target_of(c), a.some = p.few ? 0.0f : 16.0f;
   a.part = static_cast<f32x2 *>(scratch);
   a.lse = reinterpret_cast<float *>(static_cast<char *>(scratch) + p.parts);
   a.t = a.lse, a.most = p.few, a.wide = p.wide;
@@ -1172,7 +1203,7 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
       return;
     }
     // the second pass' items: as many as its target may make, or round again
-    const dim3 parts((unsigned)((target_of(c) * 3 + p.tiles) * c->kv_heads));
+    const dim3 parts((unsigned)((target_of(c) * ROUNDS + p.tiles) * c->kv_heads));
 
     hipLaunchKernelGGL((weigh_sums_kernel<decltype(e), d>), items, dim3(64 * WW), 0, st, a);
     // few tiles have many items each
