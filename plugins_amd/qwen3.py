@@ -300,6 +300,9 @@ class PagedDecoder:
     (turboexl3_qwen38/src/spec/drafter.zig); its verify rows take the decode
     chain of the quant table, as these linears do up to 16 rows."""
 
+    window, decay = None, 1.0
+    score = gone = None  # with a window: the keys' weights, and how many each sequence has evicted
+
     def __init__(self, model: Qwen3Decoder, seqs: int, pages: int, max_pages: int, page: int = 64,
                  window: int | None = None, decay: float = 1.0):
         from . import paged as P
@@ -307,9 +310,8 @@ class PagedDecoder:
         c = model.cfg
         self.cache = P.PagedCache(c.layers, pages, c.kv_heads, seqs, max_pages, page, HEAD_DIM,
                                   self.torch.float16, model.embed_table.device)
-        self.window, self.decay = window, decay
-        self.score = self.gone = None
         if window is not None:
+            self.window, self.decay = window, decay
             dev = model.embed_table.device
             self.score = self.torch.zeros(c.layers, seqs, c.kv_heads, max_pages * page, device=dev)
             self.gone = self.torch.zeros(seqs, dtype=self.torch.int32, device=dev)
