@@ -137,9 +137,37 @@ __device__ __forceinline__ float rate_of(float heat) {
   return fminf(LOG2E / heat, 3.0e38f);
 }
 
+// v of lane (this lane ^ m) without the LDS crossbar (exl3::xor_lanes).  For m below 16 a row
+// of 16 lanes may take part alone.
+template <typename T>
+__device__ __forceinline__ T across(T v, int m) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, exl3::xor_lanes(__builtin_bit_cast(float, v), m));
+  } else {
+    const u32x2 x = __builtin_bit_cast(u32x2, v);
+    const uint32_t lo = x[0], hi = x[1];
+    return __builtin_bit_cast(T, u32x2{across(lo, m), across(hi, m)});
+  }
+}
+// Sum over the lanes up to and with this one, as scan's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const u32x2 x = __builtin_bit_cast(u32x2, v);
+  return __builtin_bit_cast(double, u32x2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)x[0], CTRL, ROWS, 0xF, false),
+                                          (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x[1], CTRL, ROWS, 0xF, false)});
+}
+__device__ __forceinline__ double scan(double v) {
+  v += moved<0x111, 0xF>(v);
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);
+  v += moved<0x143, 0xC>(v);
+  return v;
+}
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  for (int m = 1; m < 64; m <<= 1) v += across(v, m);
   return v;
 }
 __device__ __forceinline__ float larger(float a, float b) {  // NaN if either is
@@ -212,7 +240,7 @@ __device__ __forceinline__ void piece_stats(const VerifyArgs &a, int t, int piec
       for (int i = N - 1; i >= 0; --i)
         if (x[u][i] == top) best = first + (u * ST + (int)threadIdx.x) * N + i;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) best = min(best, __shfl_xor(best, m));
+    for (int m = 1; m < 64; m <<= 1) best = min(best, across(best, m));
     if (lane == 0) bests[wave] = best;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -307,12 +335,12 @@ __device__ __forceinline__ Part join_parts(const VerifyArgs &a, const Seq &q, in
   }
   float all = hi;
 #pragma unroll
-  for (int x = 1; x < 16; x <<= 1) all = larger(all, __shfl_xor(all, x, 16));
+  for (int x = 1; x < 16; x <<= 1) all = larger(all, across(all, x));
   const float ref = all == -INFINITY ? 0.0f : all;
   if (!q.greedy) m *= (double)__builtin_amdgcn_exp2f((hi - ref) * q.rate);
   best = hi == all ? best : INT32_MAX;
 #pragma unroll
-  for (int x = 1; x < 16; x <<= 1) m += __shfl_xor(m, x, 16), best = min(best, __shfl_xor(best, x, 16));
+  for (int x = 1; x < 16; x <<= 1) m += across(m, x), best = min(best, across(best, x));
   return stats_of(q, all, best, m);
 }
 // The statistics of the rows (of lazy walks: of the one that the walk is at) and what
@@ -587,7 +615,7 @@ __device__ __forceinline__ void row_stats(const VerifyArgs &a, Walk<N, DRAFT> &w
   mass = wave_sum(mass * (double)__builtin_amdgcn_exp2f((top - ref) * q.rate));
   best = top == all ? best : INT32_MAX;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) best = min(best, __shfl_xor(best, m));
+  for (int m = 1; m < 64; m <<= 1) best = min(best, across(best, m));
   if (lane == 0) w.sums[wave] = mass, w.bests[wave] = best;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -716,12 +744,7 @@ struct Rest {
 // Sum over the threads before this one; all threads', in `whole`.
 __device__ __forceinline__ double before(double v, double (&waves)[ST / 64], double &whole) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double y = __shfl_up(x, m);
-    if (lane >= m) x += y;
-  }
+  const double x = scan(v);
   __syncthreads();
   if (lane == 63) waves[wave] = x;
   __syncthreads();
@@ -737,7 +760,7 @@ __device__ __forceinline__ double before(double v, double (&waves)[ST / 64], dou
 // The workgroup's least and largest.
 __device__ __forceinline__ void ends(int &lo, int &hi, int (&waves)[2][ST / 64]) {
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) lo = min(lo, __shfl_xor(lo, m)), hi = max(hi, __shfl_xor(hi, m));
+  for (int m = 1; m < 64; m <<= 1) lo = min(lo, across(lo, m)), hi = max(hi, across(hi, m));
   __syncthreads();
   if ((threadIdx.x & 63) == 0) waves[0][threadIdx.x >> 6] = lo, waves[1][threadIdx.x >> 6] = hi;
   __syncthreads();
@@ -915,7 +938,7 @@ __global__ __launch_bounds__(ST) void verify_single_kernel(VerifyArgs a) {
       for (int i = 0; i < N; ++i)
         if (x[k][i] == top) all = fmax(all, -(double)(first + (k * ST + (int)threadIdx.x) * N + i));
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) all = fmax(all, __shfl_xor(all, m));
+    for (int m = 1; m < 64; m <<= 1) all = fmax(all, across(all, m));
   } else if (q.fit && top > -INFINITY && top < INFINITY) {
 #pragma unroll
     for (int k = 0; k < U; ++k)
@@ -959,7 +982,7 @@ __global__ __launch_bounds__(ST) void verify_single_draw_kernel(VerifyArgs a) {
     for (int x = threadIdx.x; x < a.draws; x += ST)
       if ((float)sums[2 * x + 1] == top) best = min(best, (int)-sums[2 * x]);
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) best = min(best, __shfl_xor(best, m));
+    for (int m = 1; m < 64; m <<= 1) best = min(best, across(best, m));
     if ((threadIdx.x & 63) == 0) firsts[threadIdx.x >> 6] = best;
     __syncthreads();
 #pragma unroll
