@@ -298,7 +298,12 @@ class PagedDecoder:
 
     The reference's counterpart is its drafter and verify step on MLX
     (turboexl3_qwen38/src/spec/drafter.zig); its verify rows take the decode
-    chain of the quant table, as these linears do up to 16 rows."""
+    chain of the quant table, as these linears do up to 16 rows.
+
+    With `window` (0: all rows, else the last ones of each sequence's step) every key
+    keeps the attention weight that it has had, `decay` times what it had a step before,
+    and `evict` brings sequences down to the heaviest; `fork` and `restart` are then the
+    decoder's, not the cache's."""
 
     window, decay = None, 1.0
     score = gone = None  # with a window: the keys' weights, and how many each sequence has evicted
