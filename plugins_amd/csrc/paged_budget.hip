@@ -684,14 +684,33 @@ __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a)
   }
 }
 
-// The second pass: the same keys' scores again, 4 keys a thread, once the
-// items of the sequence are joined.
+// The second pass: the same keys' scores again, 4 keys a thread, once the items of the
+// sequence are joined.  Four pairs' scores are asked for at once, the first ones ahead of the
+// joining, since a load's latency is all that a thread waits for.
 __global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
   __shared__ f32x2 so[16][FEW];
+  constexpr int AT = 4, BY = 256 * WW;
   const int head = blockIdx.x % a.pool.kv;
   const Find f = Finder<ITEM>(a).at(blockIdx.x / a.pool.kv);
   if (f.s < 0) return;
   const Watch &w = f.w;
+  const int k0 = (int)min((int64_t)f.j * f.each * 64, (int64_t)w.keys);
+  const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
+  const float *from = a.t + ((int64_t)f.s * a.pool.kv + head) * a.most * a.wide;
+  float *score = a.score + ((int64_t)f.s * a.pool.kv + head) * a.room;
+  const int base = a.base ? a.base[f.s] : w.len;
+  f32x4 t[AT];
+  float had[4];
+  auto load = [&](int k, int p) {
+#pragma unroll
+    for (int x = 0; x < AT; ++x)
+      if (p + x < w.pairs) t[x] = *reinterpret_cast<const f32x4 *>(from + (int64_t)(p + x) * a.wide + k);
+    if (p > 0) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) had[e] = k + e < min(k1, base) ? score[k + e] : 0.0f;
+  };
+  int k = k0 + 4 * (int)threadIdx.x;
+  if (k < k1) load(k, 0);
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
   float ref = -INFINITY, sum = 0.0f;
   for (int j = row; j < f.parts; j += 16) {
@@ -707,23 +726,27 @@ __global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
     so[0][col] = ended(ref, sum);
   }
   __syncthreads();
-  const int k0 = (int)min((int64_t)f.j * f.each * 64, (int64_t)w.keys);
-  const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
-  const float *from = a.t + ((int64_t)f.s * a.pool.kv + head) * a.most * a.wide;
-  for (int k = k0 + 4 * (int)threadIdx.x; k < k1; k += 256 * WW) {
+  for (; k < k1; k += BY) {
     f32x4 acc{0, 0, 0, 0};
-    for (int p = 0; p < w.pairs; ++p) {
-      const f32x4 t = *reinterpret_cast<const f32x4 *>(from + (int64_t)p * a.wide + k);
-      const f32x2 r = so[0][p];
+    for (int p = 0;;) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = fmaf(__builtin_amdgcn_exp2f(t[e] - r[0]), r[1], acc[e]);
-        if (t[e] != UNSEEN) acc[e] = x;
+      for (int x = 0; x < AT; ++x) {
+        if (p + x >= w.pairs) break;
+        const f32x2 r = so[0][p + x];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = fmaf(__builtin_amdgcn_exp2f(t[x][e] - r[0]), r[1], acc[e]);
+          if (t[x][e] != UNSEEN) acc[e] = y;
+        }
       }
+      p += AT;
+      if (p >= w.pairs) break;
+      load(k, p);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (k + e < k1) add_score(a, f, head, k + e, acc[e]);
+      if (k + e < k1) score[k + e] = k + e < base ? a.decay * had[e] + acc[e] : acc[e];
+    if (k + BY < k1) load(k + BY, 0);
   }
 }
 
