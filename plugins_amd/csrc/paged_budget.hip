@@ -37,7 +37,7 @@ struct WeighArgs {
 
 constexpr int WW = 4;       // waves of a workgroup
 constexpr int TILE = 128;   // pairs of a row and a query head that an item has,
-constexpr int FEW = 16;     // pairs of a row and a query head that a tile has where scores are kept
+constexpr int FEW = 16;     // or where scores are kept, this many or twice as many,
 constexpr int PART = 4096;  // keys of an item of the second pass, at most
 constexpr float SLACK = 4.0f;  // a reference follows its maximum in steps of more (powers of two)
 // Up to references of FAR a weight's exponent is one multiply-add of score, scale
@@ -568,15 +568,15 @@ __global__ __launch_bounds__(64 * WW) void weigh_deals_kernel(WeighArgs a) {
   add_score(a, f, head, key, v);
 }
 
-// Few pairs (single tokens): their scores are kept in 32 bits from the first pass
-// to the second, 4 bytes a pair beside a key's 2 D, so that keys are read
-// once.  The first pass: 16 x 16 products, a lane has 4 keys' scores of one pair; a wave
-// takes 32 keys in turn, the next ones on their way while the sums form.
-template <typename E, int D>
+// Few pairs (single tokens, small trees): their scores are kept in 32 bits from the first
+// pass to the second, 4 bytes a pair beside a key's 2 D, so that keys are read
+// once.  The first pass: 16 x 16 products, a lane has 4 keys' scores of each of NB pairs; a
+// wave takes 32 keys in turn, the next ones on their way while the sums form.
+template <typename E, int D, int NB>
 __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a) {
-  constexpr int KK = D / 32;
+  constexpr int KK = D / 32, TILE = FEW * NB;
   typedef typename E::V8 V8;
-  __shared__ f32x2 so[WW][FEW];
+  __shared__ f32x2 so[WW][TILE];
   __shared__ int sbad;
   const int head = blockIdx.x % a.pool.kv;
   const Find f = Finder<ITEM>(a).at(blockIdx.x / a.pool.kv);
@@ -584,7 +584,6 @@ __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a)
   const Watch &w = f.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int pair = min(col, w.pairs - 1), i = w.lo + pair / a.group, hq = head * a.group + pair % a.group;
   const int k0 = (int)min((int64_t)f.j * f.each * 64, (int64_t)w.keys);
   const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
   const int steps = (k1 - k0 + 31) / 32;
@@ -615,81 +614,109 @@ __global__ __launch_bounds__(64 * WW, 4) void weigh_few_sums_kernel(WeighArgs a)
     }
   };
   if (wave < steps) fetch(wave);
-  u32x4 qf[KK];
+  int i[NB];
+  u32x4 qf[NB][KK];
+  float ref[NB], sum[NB];
 #pragma unroll
-  for (int kk = 0; kk < KK; ++kk)
-    qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + hq * D + 32 * kk + 8 * g) ^ a.flip;
+  for (int p = 0; p < NB; ++p) {
+    const int pair = min(FEW * p + col, w.pairs - 1), hq = head * a.group + pair % a.group;
+    i[p] = w.lo + pair / a.group;
+    ref[p] = -INFINITY, sum[p] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      qf[p][kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i[p]) * a.qs + hq * D + 32 * kk + 8 * g) ^ a.flip;
+  }
   if (wave < steps) {
     load(wave);
     fetch(min(wave + WW, steps - 1));
   }
   float *to = a.t + (((int64_t)f.s * a.pool.kv + head) * a.most + col) * a.wide + 4 * g;
-  float ref = -INFINITY, sum = 0.0f;
   for (int step = wave; step < steps; step += WW) {
     const int kb = k0 + step * 32;
-    f32x4 t[2];
+    f32x4 t[NB][2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      t[b] = f32x4{0, 0, 0, 0};
+    for (int p = 0; p < NB; ++p)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        t[b] = E::mma(__builtin_bit_cast(V8, kf[b][kk]), __builtin_bit_cast(V8, qf[kk]), t[b]);
-    }
+      for (int b = 0; b < 2; ++b) {
+        t[p][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          t[p][b] = E::mma(__builtin_bit_cast(V8, kf[b][kk]), __builtin_bit_cast(V8, qf[p][kk]), t[p][b]);
+      }
     if (step + WW < steps) {
       load(step + WW);
       fetch(min(step + 2 * WW, steps - 1));
     }
+    float hi[NB];
+    bool moves = false;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) t[b] *= a.scale;
-    f32x4 kept[2] = {t[0], t[1]};
-    if (kb + 32 > clear || kb + 32 > k1) {
-      uint32_t seen = (uint32_t)seen64(a, w, i, kb);
-      if (k1 - kb < 32) seen &= ~0u >> (32 - (k1 - kb));
+    for (int p = 0; p < NB; ++p) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b) t[p][b] *= a.scale;
+      f32x4 kept[2] = {t[p][0], t[p][1]};
+      if (kb + 32 > clear || kb + 32 > k1) {
+        uint32_t seen = (uint32_t)seen64(a, w, i[p], kb);
+        if (k1 - kb < 32) seen &= ~0u >> (32 - (k1 - kb));
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!(seen >> (16 * b + 4 * g + r) & 1)) t[b][r] = -INFINITY, kept[b][r] = UNSEEN;
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!(seen >> (16 * b + 4 * g + r) & 1)) t[p][b][r] = -INFINITY, kept[b][r] = UNSEEN;
+      }
+      if (FEW * p + col < w.pairs) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          if (kb + 16 * b < k1)
+            *reinterpret_cast<f32x4 *>(to + (int64_t)FEW * p * a.wide + kb + 16 * b) = kept[b];
+      }
+      hi[p] = t[p][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) hi[p] = larger(hi[p], t[p][e >> 2][e & 3]);
+      moves |= !(hi[p] - ref[p] <= SLACK);
     }
-    if (col < w.pairs) {
+    if (__ballot(moves) != 0) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-        if (kb + 16 * b < k1) *reinterpret_cast<f32x4 *>(to + kb + 16 * b) = kept[b];
+      for (int p = 0; p < NB; ++p) {
+        const float now = larger(ref[p], hi[p]);
+        sum[p] *= __builtin_amdgcn_exp2f(ref[p] - (now == -INFINITY ? 0.0f : now));
+        ref[p] = now;
+      }
     }
-    float hi = t[0][0];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) hi = larger(hi, t[e >> 2][e & 3]);
-    if (__ballot(!(hi - ref <= SLACK)) != 0) {
-      const float now = larger(ref, hi);
-      sum *= __builtin_amdgcn_exp2f(ref - (now == -INFINITY ? 0.0f : now));
-      ref = now;
+    for (int p = 0; p < NB; ++p) {
+      const float from = ref[p] == -INFINITY ? 0.0f : ref[p];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[p] += __builtin_amdgcn_exp2f(t[p][e >> 2][e & 3] - from);
     }
-    const float from = ref == -INFINITY ? 0.0f : ref;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += __builtin_amdgcn_exp2f(t[e >> 2][e & 3] - from);
   }
 #pragma unroll
-  for (int m = 16; m < 64; m <<= 1) join(ref, sum, exl3::xor_lanes(ref, m), exl3::xor_lanes(sum, m));
+  for (int p = 0; p < NB; ++p)
+#pragma unroll
+    for (int m = 16; m < 64; m <<= 1)
+      join(ref[p], sum[p], exl3::xor_lanes(ref[p], m), exl3::xor_lanes(sum[p], m));
   __syncthreads();
   if (bad) sbad = 1;
-  if (g == 0) so[wave][col] = f32x2{ref, sum};
+#pragma unroll
+  for (int p = 0; p < NB; ++p)
+    if (g == 0) so[wave][FEW * p + col] = f32x2{ref[p], sum[p]};
   __syncthreads();
   const int64_t slot = (int64_t)(f.first + f.j) * a.pool.kv + head;
-  if (threadIdx.x < FEW && slot < a.slots) {
-    ref = -INFINITY, sum = 0.0f;
+  if (threadIdx.x < TILE && slot < a.slots) {
+    float all = -INFINITY, whole = 0.0f;
 #pragma unroll
-    for (int x = 0; x < WW; ++x) join(ref, sum, so[x][threadIdx.x][0], so[x][threadIdx.x][1]);
-    if (sbad) sum = __builtin_nanf("");
-    a.part[slot * FEW + threadIdx.x] = f32x2{ref, sum};
+    for (int x = 0; x < WW; ++x) join(all, whole, so[x][threadIdx.x][0], so[x][threadIdx.x][1]);
+    if (sbad) whole = __builtin_nanf("");
+    a.part[slot * TILE + threadIdx.x] = f32x2{all, whole};
   }
 }
 
 // The second pass: the same keys' scores again, 4 keys a thread, once the items of the
 // sequence are joined.  Four pairs' scores are asked for at once, the first ones ahead of the
 // joining, since a load's latency is all that a thread waits for.
+template <int NB>
 __global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
-  __shared__ f32x2 so[16][FEW];
-  constexpr int AT = 4, BY = 256 * WW;
+  constexpr int AT = 4, BY = 256 * WW, TILE = FEW * NB, ROWS = 64 * WW / TILE;
+  __shared__ f32x2 so[ROWS][TILE];
   const int head = blockIdx.x % a.pool.kv;
   const Find f = Finder<ITEM>(a).at(blockIdx.x / a.pool.kv);
   if (f.s < 0) return;
@@ -711,18 +738,18 @@ __global__ __launch_bounds__(64 * WW) void weigh_few_keys_kernel(WeighArgs a) {
   };
   int k = k0 + 4 * (int)threadIdx.x;
   if (k < k1) load(k, 0);
-  const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int col = threadIdx.x % TILE, row = threadIdx.x / TILE;
   float ref = -INFINITY, sum = 0.0f;
-  for (int j = row; j < f.parts; j += 16) {
+  for (int j = row; j < f.parts; j += ROWS) {
     const int64_t slot = (int64_t)(f.first + j) * a.pool.kv + head;
     if (slot >= a.slots) break;
-    const f32x2 v = a.part[slot * FEW + col];
+    const f32x2 v = a.part[slot * TILE + col];
     join(ref, sum, v[0], v[1]);
   }
   so[row][col] = f32x2{ref, sum};
   __syncthreads();
-  if (threadIdx.x < FEW) {
-    for (int x = 1; x < 16; ++x) join(ref, sum, so[x][col][0], so[x][col][1]);
+  if (threadIdx.x < TILE) {
+    for (int x = 1; x < ROWS; ++x) join(ref, sum, so[x][col][0], so[x][col][1]);
     so[0][col] = ended(ref, sum);
   }
   __syncthreads();
@@ -1108,7 +1135,10 @@ size_t lse_bytes(const exl3p_cache *c, const exl3p_rows *r, int group) {
 
 // How the weights are formed, by what the host knows.  Pairs whose scores are
 // kept read the keys once and the scores (4 bytes a pair and key) twice; others
-// read the keys twice.
+// read the keys twice, in a launch or two more.  32 pairs (trees of 8 rows, 4 query heads of
+// 128), kept and not: over 2000 keys 14.7 and 20.6 us, 16 sequences over up to 4000 keys 39 and
+// 56, 48 over up to 3000 57 and 79, but one over 40000 43.7 and 40.6.  64 pairs kept would be 21.9
+// and 21.2 over 2000 keys, 69 and 42 over 40000.
 struct Plan {
   int group;
   int tile;              // pairs
@@ -1130,11 +1160,11 @@ Plan plan_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads, int32_t w
   p.group = heads / c->kv_heads;
   const int64_t rows = window > 0 && window < r->max_rows ? window : r->max_rows, pairs = rows * p.group;
   p.wide = (room + 15) & ~15;
-  p.few = pairs <= FEW ? (int)pairs : 0;
+  p.few = pairs <= 2 * FEW ? (int)pairs : 0;
   p.rest = (size_t)r->seqs * c->kv_heads * p.few * p.wide * sizeof(float);
   if (p.rest > KEPT_MAX) p.few = 0;
   if (p.few == 0) p.rest = lse_bytes(c, r, p.group);
-  p.tile = p.few ? FEW : TILE;
+  p.tile = p.few > FEW ? 2 * FEW : p.few ? FEW : TILE;
   p.tiles = rows_watched(r, window) * p.group / p.tile + r->seqs;
   p.items = target_of(c) * (p.few ? 1 : ROUNDS) + p.tiles;
   for (p.deal = p.tile;; p.deal *= 2) {
@@ -1221,8 +1251,14 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
   const dim3 items((unsigned)(p.items * c->kv_heads));
   return by_type(c, [&](auto e, auto d) {
     if (p.few) {
-      hipLaunchKernelGGL((weigh_few_sums_kernel<decltype(e), d>), items, dim3(64 * WW), 0, st, a);
-      hipLaunchKernelGGL(weigh_few_keys_kernel, items, dim3(64 * WW), 0, st, a);
+      auto blocks = [&](auto nb) {
+        hipLaunchKernelGGL((weigh_few_sums_kernel<decltype(e), d, nb>), items, dim3(64 * WW), 0, st, a);
+        hipLaunchKernelGGL((weigh_few_keys_kernel<nb>), items, dim3(64 * WW), 0, st, a);
+      };
+      if (p.tile == FEW)
+        blocks(std::integral_constant<int, 1>{});
+      else
+        blocks(std::integral_constant<int, 2>{});
       return;
     }
     // the second pass' items: as many as its target may make, or round again

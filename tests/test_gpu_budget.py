@@ -356,6 +356,7 @@ WEIGH = [
     ([1, 1], [4095, 4096], 8, 1, 128, 256, 0),
     ([200], [0], 2, 2, 128, 16, 0),
     ([2, 4], [900, 33], 2, 4, 64, 32, 0),
+    ([8, 3, 1], [2000, 77, 0], 2, 4, 128, 64, 0), ([17], [500], 1, 1, 64, 16, 0),
 ]
 
 
@@ -376,7 +377,7 @@ def test_weigh(counts, lens, kv, group, dim, page, window, dtype, tree):
     assert torch.equal(got, weighed(k, table, counts, lens, q, had, mask, window=window, decay=0.9))
 
 
-@pytest.mark.parametrize("n", [1, 30])
+@pytest.mark.parametrize("n", [1, 8, 30])
 def test_weigh_base_decay_and_what_stays(n):
     """Keys from `base` on begin anew, whatever was there (NaN); keys behind the
     sequence's, sequences without rows and those that do not fit stay as they
@@ -407,7 +408,7 @@ def test_weigh_base_decay_and_what_stays(n):
 
 
 @pytest.mark.parametrize("what", [math.nan, math.inf])
-@pytest.mark.parametrize("n,group", [(3, 4), (40, 4)])
+@pytest.mark.parametrize("n,group", [(3, 4), (8, 4), (40, 4)])
 def test_weigh_keeps_what_is_masked_out(what, n, group):
     """A drafted row whose key overflowed: rows that see it give NaN to what they see, the
     others' weights are as if it were not there: keys that only they see are
@@ -448,7 +449,7 @@ def test_weigh_free_masks_and_empty_rows():
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 3000.0])
-@pytest.mark.parametrize("n", [2, 30])
+@pytest.mark.parametrize("n", [2, 8, 30])
 def test_weigh_scales(scale, n):
     counts, lens = [n], [150]
     g, k, v, table, cu, q = batch(counts, lens, F16, 1, 4, 64, 16, 7)
@@ -484,7 +485,7 @@ def test_weigh_strides_layers_and_rows_behind():
         assert ((score.cpu().double() - want).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("n", [1, 8, 40])
 def test_weigh_bad_pages_and_lengths(n):
     """A page number outside the cache: NaN; a length that does not fit: untouched."""
     counts, lens = [n, n, n], [100, 60, 80]
@@ -504,7 +505,7 @@ def test_weigh_bad_pages_and_lengths(n):
     assert torch.equal(weighed(k, table, counts, lens, q, had, rows=rows), had)
 
 
-@pytest.mark.parametrize("n", [1, 50])
+@pytest.mark.parametrize("n", [1, 7, 50])
 def test_weigh_graph_and_stream(n):
     """Captured twice over the same rows, lengths and q changed between the replays,
     eager calls beside them; another stream."""

@@ -27,7 +27,7 @@ def far_pools(shape, small, table):
     return big[0], big[1], torch.where(table < 0, -1, to[table.clamp(min=0)]).to(torch.int32)
 
 
-@pytest.mark.parametrize("n,window", [(1, 0), (40, 0), (40, 8)])
+@pytest.mark.parametrize("n,window", [(1, 0), (8, 0), (40, 0), (40, 8)])
 def test_weigh_pools_past_32_bits(n, window):
     g = torch.Generator(device=DEV).manual_seed(n)
     shape = (2, 256, 128)
