@@ -458,7 +458,7 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
       if (last <= k0) continue;
       const int steps = (last - k0 + 63) / 64;
       const int r0 = p0 + 32 * wave;
-      const bool any = r0 < w.pairs, full = r0 + 32 <= w.pairs;
+      const bool any = r0 < w.pairs;
       const int clear = min(last, a.mask == nullptr ? w.len + w.lo + r0 / G + 1 : w.len);
       Keys<E, D> keys(a, lds, f.s, head, k0, last);
       keys.fetch(0);
@@ -476,8 +476,11 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
       bool far = false;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        lse[r] = lses[min(r0 + 8 * (r >> 2) + 4 * h + (r & 3), w.pairs - 1)];
+        const int p = r0 + 8 * (r >> 2) + 4 * h + (r & 3);
+        lse[r] = lses[min(p, w.pairs - 1)];
         far |= fabsf(lse[r]) > FAR;
+        // a pair behind the last is that one's copy: no weight, but for a NaN that it gives too
+        if (p >= w.pairs) lse[r] = INFINITY;
       }
       far = __ballot(far) != 0;
 #pragma unroll
@@ -503,7 +506,7 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
 #pragma unroll
               for (int r = 0; r < 16; ++r) t[b][r] *= a.scale;
           }
-          if (full && kb + 64 <= clear) {
+          if (kb + 64 <= clear) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll

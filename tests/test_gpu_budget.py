@@ -408,7 +408,7 @@ def test_weigh_base_decay_and_what_stays(n):
 
 
 @pytest.mark.parametrize("what", [math.nan, math.inf])
-@pytest.mark.parametrize("n,group", [(3, 4), (8, 4), (40, 4)])
+@pytest.mark.parametrize("n,group", [(3, 4), (8, 4), (11, 4), (40, 4)])
 def test_weigh_keeps_what_is_masked_out(what, n, group):
     """A drafted row whose key overflowed: rows that see it give NaN to what they see, the
     others' weights are as if it were not there: keys that only they see are
