@@ -1118,13 +1118,15 @@ exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int3
   const bool siblings = draft != nullptr && parent != nullptr && r->max_rows > 2;
   // Statistics when a walk gets there: of a tree, most of whose rows no walk gets to (a
   // line's are drafted to be accepted), where all rows' would take longer than the rounds
-  // of the walks.  Measured at bf16, 151936 tokens, 4 to 32 us a call apart: 16 trees of
-  // 16 rows (78 MB) 47 us for all, 60 as the walks go; 16 of 32 (156 MB) 62 and 60; 64 of
-  // 16 (311 MB) 110 and 83.  Drafted trees go in rounds in any case: 4 of 16
-  // rows in f32 (39 MB) 78 and 73, 16 of 16 (78 MB) 96 and 85.  Lines that are accepted
-  // whole lose: 64 of 8 (156 MB) 76 and 121.
+  // of the walks.  All and as the walks go, ragged batches, 151936 tokens where no other number
+  // is given: 16 trees of up to 16 rows (bf16, 53 MB of logits) 26.5 and 35.9 us, 64 of 64
+  // (32000 tokens, 139 MB) 46.8 and 44.7, 64 of 16 (167 MB) 60.3 and 59.3, 64 of 24 (259 MB) 74.7 and
+  // 56.6, 16 of 64 (f32, 314 MB) 77.9 and 43.0.  Siblings that were drawn need rounds in any
+  // case: 32 of 16 (88 MB) 66 and 83, 64 of 16 91 and 106, 12 of 64 (f32, 237 MB) 95.7 and
+  // 99.8, 64 of 32 (355 MB) 138 and 134, 32 of 64 (f32, 589 MB) 167 and 122.  Lines that are
+  // accepted whole lose: 64 of 8 (102 MB) 50.6 and 57.0.
   const int64_t read = (int64_t)r->rows * vocab * size_of(logits_dtype);
-  const bool lazy = parent != nullptr && r->rows >= 4 * (int64_t)r->seqs && read > (siblings ? LAZY : 5 * LAZY);
+  const bool lazy = parent != nullptr && r->rows >= 4 * (int64_t)r->seqs && read > (siblings ? 8 : 5) * LAZY;
   const bool own = !lazy && !siblings && r->max_rows <= SHORT;
   a.lazy = lazy;
   // rounds: what walks usually need; the rest is for one workgroup a sequence

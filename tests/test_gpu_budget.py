@@ -110,7 +110,8 @@ def test_verify(counts, vocab, tree, draft, distinct, dtype):
     ([600], 1501, BF16, None), ([64] * 9, 9001, BF16, F32),
     # read as the walks go
     ([64] * 9, 30011, BF16, F32), ([300, 0, 150], 20001, F32, F16), ([64] * 9, 151936, BF16, None),
-    ([200, 0, 400], 151936, F16, None), ([9, 4, 1], 3200003, F32, None), ([3, 8, 1, 4], 600007, F32, BF16)])
+    ([200, 0, 400], 151936, F16, None), ([9, 4, 1], 3200003, F32, None), ([3, 8, 1, 4], 600007, F32, BF16),
+    ([64] * 9, 151936, F32, F16), ([30, 9], 2000003, F32, BF16)])
 def test_verify_large_batches(counts, vocab, dtype, draft):
     """Batches of which the walks look at few rows."""
     seed = 1
@@ -126,7 +127,7 @@ def test_verify_large_batches(counts, vocab, dtype, draft):
 
 @pytest.mark.parametrize("n,vocab,tree,draft", [
     (600, 67, False, None), (600, 67, True, None), (600, 151936, True, None), (600, 151936, False, None),
-    (300, 60013, True, F16), (200, 1001, True, F16)])
+    (300, 60013, True, F16), (200, 1001, True, F16), (900, 151936, True, F16)])
 def test_verify_a_path_that_is_deep(n, vocab, tree, draft):
     """Every row its parent's only child, and certain."""
     z = torch.zeros(n, vocab)
