@@ -155,7 +155,8 @@ exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32
  *   u [rows], in [0, 1).  A number that is none (NaN) accepts nothing and samples
  *   the last token of positive probability.
  * logits [rows][vocab] and draft (logits_dtype, draft_dtype: EXL3_DT_F32, F16 or
- * BF16; strides in elements, rows apart), -inf: never.  A token outside the
+ * BF16; strides in elements, rows apart), -inf: never.  Of the draft, rows without
+ * children are not read, nor what a walk does not need.  A token outside the
  * vocabulary is refused as any other.  Where a row's logits have a NaN, no finite
  * one, or +inf (temperature 0 takes it), or the temperature is negative or not
  * finite, the walk ends there with target -1.  parent as in exl3p_tree_plan; at

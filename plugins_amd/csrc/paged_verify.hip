@@ -703,8 +703,12 @@ struct Rest {
   Tip tip;
   double inv;
   size_t d;
+  // of the workgroup: where no child was refused the draft's row is not read (nobody may have
+  // filled it: a draft is not asked what follows its leaves)
+  bool refused;
   __device__ __forceinline__ Rest(const VerifyArgs &args, const Tip &t)
-      : a(args), tip(t), inv(1.0 / (double)t.heat), d((size_t)max(t.row, 0) * args.ds) {}
+      : a(args), tip(t), inv(1.0 / (double)t.heat), d((size_t)max(t.row, 0) * args.ds),
+        refused(__builtin_amdgcn_readfirstlane(t.share != 0.0)) {}
   __device__ __forceinline__ int first(int piece) const {
     return first_of<E>(row_of<E>(a, max(tip.row, 0)), piece, DRAW);
   }
@@ -714,15 +718,18 @@ struct Rest {
     float x[N];
     Vec<E>::unpack(block_of<E>(row_of<E>(a, max(tip.row, 0)), e, a.vocab), x);
     float y[N];
-    if constexpr (DRAFT) drafts_of<Q, N>(static_cast<const typename Q::T *>(a.draft) + d, e, a.vocab, y);
+    if constexpr (DRAFT)
+      if (refused) drafts_of<Q, N>(static_cast<const typename Q::T *>(a.draft) + d, e, a.vocab, y);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       r[k] = p[k] = exp_of(((double)x[k] - (double)tip.top) * inv);
-      if constexpr (DRAFT)
-        r[k] = fmax(p[k] - tip.share * (double)y[k], 0.0);
-      else if (gone[(e + k - from) >> 5] >> ((e + k - from) & 31) & 1)
-        r[k] = 0.0;
+      if constexpr (!DRAFT)
+        if (gone[(e + k - from) >> 5] >> ((e + k - from) & 31) & 1) r[k] = 0.0;
     }
+    if constexpr (DRAFT)
+      if (refused)
+#pragma unroll
+        for (int k = 0; k < N; ++k) r[k] = fmax(p[k] - tip.share * (double)y[k], 0.0);
   }
   // the tokens of the row's children, all refused
   __device__ __forceinline__ void mark(int s, int from, uint32_t *gone) const {
