@@ -303,10 +303,15 @@ class PagedDecoder:
     With `window` (0: all rows, else the last ones of each sequence's step) every key
     keeps the attention weight that it has had, `decay` times what it had a step before,
     and `evict` brings sequences down to the heaviest; `fork` and `restart` are then the
-    decoder's, not the cache's."""
+    decoder's, not the cache's.  Rows go on behind a sequence's keys, at the place that its
+    text has there: one that is to go on from earlier is forked there, or started again."""
 
     window, decay = None, 1.0
     score = gone = None  # with a window: the keys' weights, and how many each sequence has evicted
+    # ... and of each sequence two key numbers: up to the first its keys are the text's first
+    # ones, from the second on they are the text's `gone` places further.  Those between are
+    # other ones in every layer and head.
+    even = None
 
     def __init__(self, model: Qwen3Decoder, seqs: int, pages: int, max_pages: int, page: int = 64,
                  window: int | None = None, decay: float = 1.0):
@@ -320,6 +325,7 @@ class PagedDecoder:
             dev = model.embed_table.device
             self.score = self.torch.zeros(c.layers, seqs, c.kv_heads, max_pages * page, device=dev)
             self.gone = self.torch.zeros(seqs, dtype=self.torch.int32, device=dev)
+            self.even = [(max_pages * page, 0)] * seqs
 
     def _row_of(self, cu, n: int):
         """Of rows 0 .. n - 1 of a step: their sequences (the last one's for rows
@@ -421,12 +427,25 @@ class PagedDecoder:
 
     def fork(self, src: int, dst: int, keys: int, stream=None) -> None:
         """Sequence dst starts with src's first `keys` keys, pages shared, and their
-        weights."""
+        weights.  Where src has evicted keys these are the first ones of the text, up to the
+        least `first` that evictions had, or reach the last ones that they left; a number between,
+        up to which every head kept other keys of the text, is refused."""
+        whole = True
+        if self.score is not None and 0 <= src < len(self.even):
+            below, behind = self.even[src]
+            whole = keys <= below
+            if not whole and keys < behind:
+                raise ValueError(f"sequence {src} has evicted keys: it forks at up to {below} or from {behind} on, "
+                                 f"not at {keys}")
         with self.P._on(self.cache, stream):
             self.cache.fork(src, dst, keys)
             if self.score is not None:
                 self.score[:, dst, :, :keys].copy_(self.score[:, src, :, :keys])
-                self.gone[dst:dst + 1].copy_(self.gone[src:src + 1])
+                if whole:
+                    self.gone[dst:dst + 1].zero_()
+                else:
+                    self.gone[dst:dst + 1].copy_(self.gone[src:src + 1])
+                self.even[dst] = (self.score.shape[3], 0) if whole else self.even[src]
 
     def restart(self, seq: int, stream=None) -> None:
         """Gives back a sequence's pages: it holds no keys, and none are gone."""
@@ -434,6 +453,7 @@ class PagedDecoder:
             self.cache.trim(seq, 0)
             if self.gone is not None:
                 self.gone[seq:seq + 1].zero_()
+                self.even[seq] = (self.score.shape[3], 0)
 
     def evict(self, lens, keep: int, first: int = 0, last: int = 0, stream=None):
         """Of each sequence's lens[s] keys (a host list, a length for each sequence of
@@ -465,6 +485,10 @@ class PagedDecoder:
         new_len, kept = torch.empty_like(before), torch.empty(*self.score.shape[:3], keep, **i32)
         P.evict(cache, before, self.score, kept, self.score, new_len, None, first, last)
         self.gone += before - new_len
+        head = min(first, keep)
+        tail = min(last, keep - head)
         for s in over:
+            below, behind = self.even[s]
+            self.even[s] = min(below, head), max(keep - tail, behind - (lens[s] - keep))
             cache.trim(s, keep)
         return [min(n, keep) for n in lens], kept
