@@ -27,8 +27,8 @@ struct WeighArgs {
   int slots;     // items * kv that part holds
   int tile;      // pairs of an item
   f32x2 *part;   // [items * kv][tile]: an item's reference and sum of each pair
-  float *lse;    // [kv][rows * group]: the power of two that a pair's weights sum to
-  float *t;      // few pairs: [seqs][kv][most][wide] scores, in place of lse
+  float *ref, *inv;  // [kv][rows * group]: a pair's reference and 1 / sum of its weights below it
+  float *t;      // few pairs: [seqs][kv][most][wide] scores, in place of these
   int most, wide;
   int deal;      // pairs that an item of the second pass adds up, whole tiles
   int deals;     // such items of a key, at most; where there are several:
@@ -405,9 +405,11 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(WeighArgs a) {
   const int pair = f.u * a.tile + in;
   if (row > 0 || pair >= f.w.pairs) return;
   for (int x = 1; x < SHARE; ++x) join(ref, sum, so[x][col][0], so[x][col][1]);
-  // (rounded as a score of its size is; a pair that sees nothing has no weights)
-  a.lse[(int64_t)head * a.st.rows * a.group + (int64_t)(f.w.row + f.w.lo) * a.group + pair] =
-      sum == 0.0f ? INFINITY : ref + __builtin_amdgcn_logf(sum);
+  // (two numbers: the logarithm of what a row's weights sum to would be rounded as a score of
+  // its size is, all of the row's weights by one factor, 1 % at scores of 2^18)
+  const f32x2 both = ended(ref, sum);
+  const int64_t at = (int64_t)head * a.st.rows * a.group + (int64_t)(f.w.row + f.w.lo) * a.group + pair;
+  a.ref[at] = both[0], a.inv[at] = both[1];
 }
 
 // A key's score: what it had, and the weights of this step.
@@ -430,6 +432,7 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
   __shared__ __align__(1024) char lds[2 * Keys<E, D>::ARR];
   __shared__ float joint[2][WW][64];
   __shared__ float total[PART];
+  __shared__ __align__(16) float invs[WW][32];
   const int head = blockIdx.x % a.pool.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
     const int k1 = (int)min((int64_t)k0 + (int64_t)f.each * 64, (int64_t)w.keys);
     const int p1 = min((f.u + 1) * a.deal, w.pairs);
     for (int k = threadIdx.x; k < k1 - k0; k += 64 * WW) total[k] = 0.0f;
-    const float *lses = a.lse + (int64_t)head * a.st.rows * G + (int64_t)(w.row + w.lo) * G;
+    const int64_t pairs0 = (int64_t)head * a.st.rows * G + (int64_t)(w.row + w.lo) * G;
     int count = 0;  // tiles of keys done: their places in LDS
     auto finish = [&](int step) {
       if (wave > 0) return;
@@ -471,18 +474,19 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
       for (int kk = 0; kk < KK; ++kk)
         qf[kk] = *reinterpret_cast<const u32x4 *>(a.q + (w.row + i) * a.qs + (head * G + pair % G) * D + 16 * kk +
                                                   8 * h) ^ a.flip;
-      // element r: pair 8 (r / 4) + 4 h + r % 4
-      float lse[16];
+      // element r: pair 8 (r / 4) + 4 h + r % 4; its 1 / sum is read from LDS where it is needed
+      // (16 more registers would leave two waves a SIMD).  A pair behind the last is that one's
+      // copy: no weight, but for a NaN that it gives too.
+      float ref[16];
       bool far = false;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int p = r0 + 8 * (r >> 2) + 4 * h + (r & 3);
-        lse[r] = lses[min(p, w.pairs - 1)];
-        far |= fabsf(lse[r]) > FAR;
-        // a pair behind the last is that one's copy: no weight, but for a NaN that it gives too
-        if (p >= w.pairs) lse[r] = INFINITY;
+        ref[r] = a.ref[pairs0 + min(r0 + 8 * (r >> 2) + 4 * h + (r & 3), w.pairs - 1)];
+        far |= fabsf(ref[r]) > FAR;
       }
       far = __ballot(far) != 0;
+      if (h == 0) invs[wave][col] = r0 + col < w.pairs ? a.inv[pairs0 + pair] : 0.0f;
+      auto inv4 = [&](int r) { return *reinterpret_cast<const f32x4 *>(&invs[wave][8 * (r >> 2) + 4 * h]); };
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(qf[kk]));  // (the sign is not turned in each tile)
       const float scale = far ? 1.0f : a.scale;
@@ -508,21 +512,30 @@ __global__ __launch_bounds__(64 * WW, 2) void weigh_keys_kernel(WeighArgs a) {
           }
           if (kb + 64 <= clear) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int r4 = 0; r4 < 16; r4 += 4) {
+              const f32x4 inv = inv4(r4);
 #pragma unroll
-              for (int r = 0; r < 16; ++r) v[b] += __builtin_amdgcn_exp2f(fmaf(t[b][r], scale, -lse[r]));
+              for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = r4; r < r4 + 4; ++r)
+                  v[b] = fmaf(__builtin_amdgcn_exp2f(fmaf(t[b][r], scale, -ref[r])), inv[r - r4], v[b]);
+            }
           } else {
             // what each of the wave's pairs sees, a pair a lane.  What a row does not see it
             // leaves alone, NaN or not.
             const uint64_t seen = r0 + col < w.pairs ? seen64(a, w, i, kb) : 0;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int r4 = 0; r4 < 16; r4 += 4) {
+              const f32x4 inv = inv4(r4);
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const uint32_t of = __shfl((int)(uint32_t)(seen >> (32 * b)), 8 * (r >> 2) + 4 * h + (r & 3));
-                const float e = __builtin_amdgcn_exp2f(fmaf(t[b][r], scale, -lse[r]));
-                if (of >> col & 1) v[b] += e;
-              }
+              for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = r4; r < r4 + 4; ++r) {
+                  const uint32_t of = __shfl((int)(uint32_t)(seen >> (32 * b)), 8 * (r >> 2) + 4 * h + (r & 3));
+                  const float y = fmaf(__builtin_amdgcn_exp2f(fmaf(t[b][r], scale, -ref[r])), inv[r - r4], v[b]);
+                  if (of >> col & 1) v[b] = y;
+                }
+            }
           }
 #pragma unroll
           for (int b = 0; b < 2; ++b) v[b] += exl3::xor_lanes(v[b], 32);
@@ -1132,7 +1145,8 @@ int64_t rows_watched(const exl3p_rows *r, int32_t window) {
 }
 // Workgroups of a kv head that fill the CUs: four of the first pass each.
 int64_t target_of(const exl3p_cache *c) { return (4 * device_cus() + c->kv_heads - 1) / c->kv_heads; }
-size_t lse_bytes(const exl3p_cache *c, const exl3p_rows *r, int group) {
+// Of every pair's reference, and as many of its 1 / sum.
+size_t refs_bytes(const exl3p_cache *c, const exl3p_rows *r, int group) {
   return up16((size_t)r->rows * group * c->kv_heads * sizeof(float));
 }
 
@@ -1166,7 +1180,7 @@ Plan plan_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads, int32_t w
   p.few = pairs <= 2 * FEW ? (int)pairs : 0;
   p.rest = (size_t)r->seqs * c->kv_heads * p.few * p.wide * sizeof(float);
   if (p.rest > KEPT_MAX) p.few = 0;
-  if (p.few == 0) p.rest = lse_bytes(c, r, p.group);
+  if (p.few == 0) p.rest = 2 * refs_bytes(c, r, p.group);
   p.tile = p.few > FEW ? 2 * FEW : p.few ? FEW : TILE;
   p.tiles = rows_watched(r, window) * p.group / p.tile + r->seqs;
   p.items = target_of(c) * (p.few ? 1 : ROUNDS) + p.tiles;
@@ -1246,8 +1260,9 @@ exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *
   // left, 67.7 so, 66.7 up to 24 units, 77.4 up to 32 and a quarter of them.
   a.fill = 0.5f * (float)target_of(c), a.some = p.few ? 0.0f : 16.0f;
   a.part = static_cast<f32x2 *>(scratch);
-  a.lse = reinterpret_cast<float *>(static_cast<char *>(scratch) + p.parts);
-  a.t = a.lse, a.most = p.few, a.wide = p.wide;
+  a.t = a.ref = reinterpret_cast<float *>(static_cast<char *>(scratch) + p.parts);
+  a.inv = a.ref + refs_bytes(c, r, p.group) / sizeof(float);
+  a.most = p.few, a.wide = p.wide;
   a.sums = reinterpret_cast<float *>(static_cast<char *>(scratch) + p.parts + p.rest);
   a.tile = p.tile, a.deal = p.deal, a.deals = p.deals;
   const hipStream_t st = static_cast<hipStream_t>(s);
