@@ -146,14 +146,18 @@ exl3_verdict exl3p_commit(const exl3p_cache *c, const exl3p_rows *r, const int32
  * p~), and after a refusal p~ is max(p~ - q~, 0), normalized.  q~ is q, or, with
  * `distinct` not 0 (siblings drawn without replacement), q without the refused
  * ones, normalized.  draft NULL: drafted tokens are certain (q~ is 1 at each), as
- * where a draft's most likely ones were taken.  Where no child is accepted the
+ * where a draft's most likely ones were taken.  A refusal that would leave nothing of
+ * p~ -- the draft's numbers are rounded, and may add up to more than 1 -- is none: its
+ * child is accepted, or p~ stays as it was where it had nothing of the child's token, so
+ * that a token that may follow is always accepted or left.  Where no child is accepted the
  * token is sampled from what p~ is then: the first of positive probability whose
  * cumulative sum, in 64 bits and in the vocabulary's order, passes u[row 0]
  * times the whole.  So the tokens have the distribution that sampling without
  * drafts has; a step of single rows is the sampler itself.
  *   temperature [seqs], NULL: 1.  0: the largest logit, the first of equals.
  *   u [rows], in [0, 1).  A number that is none (NaN) accepts nothing and samples
- *   the last token of positive probability.
+ *   the last token of positive probability (a refused child's, where there are no others:
+ *   the walk of exl3p_commit then ends in a row of target -1).
  * logits [rows][vocab] and draft (logits_dtype, draft_dtype: EXL3_DT_F32, F16 or
  * BF16; strides in elements, rows apart), -inf: never.  Of the draft, rows without
  * children are not read, nor what a walk does not need.  A token outside the

@@ -89,18 +89,27 @@ struct Part {
 };
 
 // What a walk waits for: nothing, it has ended; what p~ has left after a refusal; a
-// row's statistics.
-enum Need : int32_t { END, REST, STATS };
+// row's statistics; whether a refusal has left anything (within a launch alone).
+enum Need : int32_t { END, REST, STATS, DOUBT };
 
 // A walk: the row that it is at (among its sequence's), the last child looked at, and
 // of p~ and q~ there: what p~ has left, what is left of q (siblings drawn without
-// replacement), the share of q that p has lost; the row's statistics.
+// replacement), the share of q that p has lost and what the last refusal adds to it once that
+// is known to leave something; the row's statistics.  (64 bytes: a larger one is not kept in
+// registers, and verify_tree_64 takes 92 us, not 59.)
 struct State {
   int32_t at, seen, need, best;
-  double left, drawn, share;
+  double left, drawn, share, step;
   double mass;  // -1: the row has no distribution
-  float top, pad;
+  float top;
+  int32_t spare;  // what follows where the refusals leave nothing: a child, or
 };
+static_assert(sizeof(State) == 64, "");
+constexpr int AS_BEFORE = -1, NO_MATTER = -2;
+constexpr double SCANT = 0x1p-16;  // what p~ has left is nothing, perhaps: 32-bit sums are off by less
+__device__ __forceinline__ State begun() {
+  return State{0, 0, STATS, 0, 1.0, 1.0, 0.0, 0.0, -1.0, 0.0f, NO_MATTER};
+}
 
 // Where a sequence's walk ended: what the sampling needs.
 struct Tip {
@@ -286,10 +295,44 @@ __global__ __launch_bounds__(ST) void verify_stats_kernel(VerifyArgs a) {
 
 // ------------------------------------------------------------------- the walk
 
+// e^x for x <= 0 in 64 bits: a power of two times the series of e^f, |f| <= ln(2) / 2,
+// whose 14th term is below 2^-57 of the sum.
+__device__ __forceinline__ double exp_of(double arg) {
+  const bool there = arg > -746.0;  // else below the smallest number
+  const double x = there ? arg : 0.0;
+  const double n = __builtin_rint(x * 1.4426950408889634074);
+  // ln(2) in two parts, the first with zeros behind its 32nd bit
+  double f = fma(n, -0x1.62e42feep-1, x);
+  f = fma(n, -0x1.a39ef35793c76p-33, f);
+  double y = 1.0 / 6227020800.0;
+  y = fma(y, f, 1.0 / 479001600.0);
+  y = fma(y, f, 1.0 / 39916800.0);
+  y = fma(y, f, 1.0 / 3628800.0);
+  y = fma(y, f, 1.0 / 362880.0);
+  y = fma(y, f, 1.0 / 40320.0);
+  y = fma(y, f, 1.0 / 5040.0);
+  y = fma(y, f, 1.0 / 720.0);
+  y = fma(y, f, 1.0 / 120.0);
+  y = fma(y, f, 1.0 / 24.0);
+  y = fma(y, f, 1.0 / 6.0);
+  y = fma(y, f, 0.5);
+  y = fma(y, f, 1.0);
+  y = fma(y, f, 1.0);
+  return there ? __builtin_amdgcn_ldexp(y, (int)n) : 0.0;
+}
+
+// p - taken, nothing where that is no more than the roundings of 64 bits: a refused token has
+// none left.
+__device__ __forceinline__ double remains(double p, double taken) {
+  const double d = p - taken;
+  return d > 0x1p-48 * p ? d : 0.0;
+}
+
 // A walk in LDS: N rows at most.
 template <int N, bool DRAFT>
 struct Walk {
   State st;
+  double rest;  // what p~ has left after the last refusal
   double p[N], us[N];
   Part stat[N];  // rows' statistics, mass -1: none; not of lazy walks
   float q[DRAFT ? N : 1];
@@ -389,12 +432,28 @@ __device__ __forceinline__ void take_rows(const VerifyArgs &a, Walk<N, DRAFT> &w
 // share q, 0), share the sum of A_j / B_j over the refusals, A_j the sum of p~
 // and B_j that of q~ (1, or what the refused ones leave of it).  A refused token
 // has none left: u A_j / B_j q >= p~ says that p~ is below what is taken.
-template <bool DRAFT, int N>
-__device__ __forceinline__ int walk_on(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q) {
+//
+// Refusals that leave nothing of p~ at all are roundings' alone: u is below 1, so of tokens that
+// p~ has one is accepted or left.  In 64 bits they are not, but the logits' mass is a sum of
+// powers of 32 bits (no draft: the last child that was there would not be certain), and the
+// draft's numbers are rounded, to a sum above 1 perhaps, so that max(p - q, 0) may be 0
+// throughout.  The sampling then had to say a refused child's token, and whoever goes by the
+// targets would go on to that child.  So the child that such a refusal refused is accepted
+// after all; where p~ had nothing of its token, p~ stays as it was before.  Whether there is
+// nothing is looked for where it can be: without a draft, where SCANT is left; with one, a
+// token's step q is above p~ everywhere, by no more than step (the sum of q - 1) in all, so by
+// no more than that at the child.
+template <typename Q>
+__device__ __forceinline__ double above_one(int vocab) {  // the sum of a rounded q, less 1
+  return sizeof(typename Q::T) == 4 ? SCANT : Q::EXP == F16::EXP ? 0x1p-10 + vocab * 0x1p-25 : 0x1p-7;
+}
+template <typename Q, bool DRAFT, int N>
+__device__ __forceinline__ int walk_on(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q, bool less_now) {
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x, n = min(q.n, N);
     State st = w.st;
     st.need = END;
+    if (DRAFT && less_now) st.share += st.step, st.left = w.rest;  // (not read where the walk ends here)
     // the next child of the row behind row `from`
     auto next = [&](int from) {
       for (int b = (from + 1) & ~63; b < n; b += 64) {
@@ -407,12 +466,13 @@ __device__ __forceinline__ int walk_on(const VerifyArgs &a, Walk<N, DRAFT> &w, c
     int c = st.mass >= 0.0 ? next(max(st.seen, st.at)) : n;
     while (c < n) {
       bool hit;
-      double less = 0.0, step = 0.0;
+      double less = 0.0, step = 0.0, mine = 0.0;
       if (q.greedy) {
         hit = w.tok[c] == st.best;
       } else if constexpr (DRAFT) {
         step = st.left / fmax(st.drawn, 0x1p-53);
-        hit = w.us[c] * step * (double)w.q[c] < fmax(w.p[c] - st.share * (double)w.q[c], 0.0);
+        mine = remains(w.p[c], st.share * (double)w.q[c]);
+        hit = w.us[c] * step * (double)w.q[c] < mine;
       } else {
         // a token that a sibling before it had is not there any more
         less = w.p[c];
@@ -425,7 +485,7 @@ __device__ __forceinline__ int walk_on(const VerifyArgs &a, Walk<N, DRAFT> &w, c
       const int from = st.seen = c;
       if (hit) {
         if (lane == 0) w.next[st.at] = w.tok[c];
-        st.at = c, st.left = 1.0, st.drawn = 1.0, st.share = 0.0;
+        st.at = c, st.left = 1.0, st.drawn = 1.0, st.share = 0.0, st.spare = NO_MATTER;
         if (a.lazy) {
           st.need = STATS;
           break;
@@ -436,21 +496,83 @@ __device__ __forceinline__ int walk_on(const VerifyArgs &a, Walk<N, DRAFT> &w, c
       }
       c = next(from);
       if (q.greedy) continue;
+      const bool real = w.us[from] < 1.0;  // (not of numbers that are none)
       if constexpr (DRAFT) {
-        st.share += step;
+        st.spare = !real ? NO_MATTER : mine > 0.0 ? from : AS_BEFORE;
+        st.step = step;
         if (a.distinct) st.drawn -= (double)w.q[from];
         if (c < n) {
           st.need = REST;
           break;
         }
+        if (real && step * ((double)w.q[from] - above_one<Q>(a.vocab)) <= mine + SCANT)
+          st.need = DOUBT;
+        else
+          st.share += step;
       } else {
         st.left -= less;
+        if (real && less > 0.0) st.spare = from;
+        if (c >= n && st.spare >= 0 && st.left <= SCANT) st.need = DOUBT;
       }
     }
     if (lane == 0) w.st = st;
   }
   __syncthreads();
   return w.st.need;
+}
+
+// Whether refusals have left anything, where that is in doubt: of any token, in the sampling's
+// own numbers (LEFT).  Usually the first elements that are looked at have something.  Where not,
+// the walk is put as said above (PUT), for a row's statistics perhaps (WAITS).
+enum Settled { LEFT, PUT, WAITS };
+template <typename E, typename Q, bool DRAFT, int N>
+__device__ __forceinline__ Settled settle(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q) {
+  constexpr int V = Vec<E>::N;
+  const int at = w.st.at, spare = w.st.spare, n = min(q.n, N);
+  const double top = (double)w.st.top, lost = (w.st.share + w.st.step) * w.st.mass;
+  const char *row = row_of<E>(a, q.begin + at);
+  bool any = false;
+  for (int e = first_of<E>(row, 0, 0) + (int)threadIdx.x * V; e < a.vocab && !any; e += (int)blockDim.x * V) {
+    float x[V], y[V];
+    Vec<E>::unpack(block_of<E>(row, e, a.vocab), x);
+    if constexpr (DRAFT)
+      drafts_of<Q, V>(static_cast<const typename Q::T *>(a.draft) + (size_t)(q.begin + at) * a.ds, e, a.vocab, y);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const double p = exp_of(((double)x[k] - top) * q.inv);
+      if constexpr (DRAFT) {
+        any |= remains(p, lost * (double)y[k]) > 0.0;
+      } else if (p > 0.0) {
+        bool there = true;
+        for (int i = at + 1; i < n; ++i) there &= w.up[i] != at || w.tok[i] != e + k;
+        any |= there;
+      }
+    }
+  }
+  if (__syncthreads_or(any)) return LEFT;
+  if (threadIdx.x == 0 && spare >= 0) {
+    w.next[at] = w.tok[spare];
+    w.st.at = w.st.seen = spare, w.st.left = 1.0, w.st.drawn = 1.0, w.st.share = 0.0, w.st.spare = NO_MATTER;
+    w.st.need = STATS;
+    if (!a.lazy) enter(w.st, w.stat[spare]);
+  }
+  __syncthreads();
+  return a.lazy && spare >= 0 ? WAITS : PUT;
+}
+// The walk from a row whose statistics are there, or (rest) from behind a refusal whose rest is.
+template <typename E, typename Q, bool DRAFT, int N>
+__device__ __forceinline__ int walk_from(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q, bool rest) {
+  bool doubt = rest && w.st.spare != NO_MATTER && w.rest < SCANT;
+  for (;;) {
+    if (doubt) {
+      const Settled how = settle<E, Q>(a, w, q);
+      if (how == WAITS) return STATS;
+      rest = how == LEFT;
+    }
+    const int need = walk_on<Q>(a, w, q, rest);
+    if (need != DOUBT) return need;
+    doubt = true;
+  }
 }
 
 // What p~ has left at the row that the walk is at: of 8 elements, f32 but for the sum.
@@ -460,7 +582,7 @@ __device__ __forceinline__ double rest_of(const VerifyArgs &a, const State &st, 
   constexpr int N = Vec<E>::N;
   const char *row = row_of<E>(a, q.begin + st.at);
   const typename Q::T *d = static_cast<const typename Q::T *>(a.draft) + (size_t)(q.begin + st.at) * a.ds;
-  const float inv = (float)(1.0 / st.mass), lost = (float)st.share;
+  const float inv = (float)(1.0 / st.mass), lost = (float)(st.share + st.step);
   double sum = 0.0;
 #pragma unroll 4
   for (int e = begin; e < end; e += by) {
@@ -511,8 +633,7 @@ __global__ __launch_bounds__(ST) void verify_round_kernel(VerifyArgs a, int roun
     if (q.n <= 0) a.state[a.st.seqs + s].need = END;
   }
   if (q.n <= 0) return;
-  const State had = round == 0 ? State{0, 0, STATS, 0, 1.0, 1.0, 0.0, -1.0, 0.0f, 0.0f}
-                               : a.state[(size_t)(round & 1) * a.st.seqs + s];
+  const State had = round == 0 ? begun() : a.state[(size_t)(round & 1) * a.st.seqs + s];
   if (had.need == END) {
     if (piece == 0 && threadIdx.x == 0) a.state[(size_t)(~round & 1) * a.st.seqs + s].need = END;
     return;
@@ -530,11 +651,11 @@ __global__ __launch_bounds__(ST) void verify_round_kernel(VerifyArgs a, int roun
         double left = 0.0;
         for (int k = threadIdx.x; k < a.pieces; k += 64) left += rest[k];
         left = wave_sum(left);
-        if (threadIdx.x == 0) w.st.left = left;
+        if (threadIdx.x == 0) w.rest = left;
       }
     }
     take_rows<E, Q>(a, w, q, a.lazy && had.need == REST);
-    need = walk_on(a, w, q);
+    need = walk_from<E, Q>(a, w, q, had.need == REST);
   }
   if (piece == 0) {
     const Tip tip = tip_of(w, q);
@@ -652,13 +773,13 @@ __global__ __launch_bounds__(ALONE) void verify_alone_kernel(VerifyArgs a, int r
       if (threadIdx.x == 0) {
         double all = w.sums[0];
         for (int x = 1; x < ALONE / 64; ++x) all += w.sums[x];
-        w.st.left = all;
+        w.rest = all;
       }
       __syncthreads();
      }
     }
     take_rows<E, Q>(a, w, q, joined);
-    need = walk_on(a, w, q);
+    need = walk_from<E, Q>(a, w, q, need == REST);
     __syncthreads();  // all have read it
   }
   const Tip tip = tip_of(w, q);
@@ -667,32 +788,6 @@ __global__ __launch_bounds__(ALONE) void verify_alone_kernel(VerifyArgs a, int r
 }
 
 // ------------------------------------------------------------------- sampling
-
-// e^x for x <= 0 in 64 bits: a power of two times the series of e^f, |f| <= ln(2) / 2,
-// whose 14th term is below 2^-57 of the sum.
-__device__ __forceinline__ double exp_of(double arg) {
-  const bool there = arg > -746.0;  // else below the smallest number
-  const double x = there ? arg : 0.0;
-  const double n = __builtin_rint(x * 1.4426950408889634074);
-  // ln(2) in two parts, the first with zeros behind its 32nd bit
-  double f = fma(n, -0x1.62e42feep-1, x);
-  f = fma(n, -0x1.a39ef35793c76p-33, f);
-  double y = 1.0 / 6227020800.0;
-  y = fma(y, f, 1.0 / 479001600.0);
-  y = fma(y, f, 1.0 / 39916800.0);
-  y = fma(y, f, 1.0 / 3628800.0);
-  y = fma(y, f, 1.0 / 362880.0);
-  y = fma(y, f, 1.0 / 40320.0);
-  y = fma(y, f, 1.0 / 5040.0);
-  y = fma(y, f, 1.0 / 720.0);
-  y = fma(y, f, 1.0 / 120.0);
-  y = fma(y, f, 1.0 / 24.0);
-  y = fma(y, f, 1.0 / 6.0);
-  y = fma(y, f, 0.5);
-  y = fma(y, f, 1.0);
-  y = fma(y, f, 1.0);
-  return there ? __builtin_amdgcn_ldexp(y, (int)n) : 0.0;
-}
 
 // What p~ has left of a token, times the row's mass: exponents in 64 bits, since the
 // cumulative sums lie next to u's border (f32 ones would give another token once in
@@ -729,7 +824,7 @@ struct Rest {
     if constexpr (DRAFT)
       if (refused)
 #pragma unroll
-        for (int k = 0; k < N; ++k) r[k] = fmax(p[k] - tip.share * (double)y[k], 0.0);
+        for (int k = 0; k < N; ++k) r[k] = remains(p[k], tip.share * (double)y[k]);
   }
   // the tokens of the row's children, all refused
   __device__ __forceinline__ void mark(int s, int from, uint32_t *gone) const {
@@ -852,10 +947,10 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
     const Seq q = seq_of(a, s);
     if (q.n <= 0) return;
     load_rows(a, walked, q);
-    if (threadIdx.x == 0) walked.st = State{0, 0, STATS, 0, 1.0, 1.0, 0.0, -1.0, 0.0f, 0.0f};
+    if (threadIdx.x == 0) walked.st = begun();
     __syncthreads();
     take_rows<E, Q>(a, walked, q, false);
-    walk_on(a, walked, q);
+    walk_from<E, Q>(a, walked, q, false);
     tip = tip_of(walked, q);
     if (own_piece == 0) write_rows(a, walked, q, true, true, tip);
   } else {
@@ -889,7 +984,7 @@ __global__ __launch_bounds__(ST) void verify_draw_kernel(VerifyArgs a) {
     __syncthreads();
     if (order != a.draws - 1) return;
   }
-  // two kinds: where nothing is left of p~ (by rounding), p in its place
+  // two kinds: where nothing is left of p~ (numbers that are none refused it), p in its place
   auto sum_of = [&](int x, int kind) {
     return __hip_atomic_load(&sums[2 * x + kind], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   };

@@ -1,0 +1,121 @@
+"""Sampled verification where few tokens may follow at all (a grammar's mask): a draft's
+roundings then leave nothing of the target's probabilities after a refusal, or every token
+that may follow is among the children.  The walk still ends in a token that may follow,
+and exl3p_commit takes the same way to it."""
+import random
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from plugins_amd import paged as P  # noqa: E402
+from tests import _paged as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+I32 = {"dtype": torch.int32, "device": DEV}
+BELOW_ONE = 1 - 2.0 ** -53  # the largest of numbers in [0, 1)
+
+
+def masked(seqs, n, fan, support, vocab, dtype, draft, seed, order):
+    """Trees of n rows of which each has up to `fan` children, among the `support` tokens
+    that its logits leave; draft: the softmax of the same logits, rounded."""
+    rng, g = random.Random(seed), torch.Generator(device=DEV).manual_seed(seed)
+    T = seqs * n
+    one = [-1] + [(i - 1) // fan for i in range(1, n)]
+    tokens = torch.randint(0, vocab // support, (T, support), generator=g, device=DEV) + \
+        torch.arange(support, device=DEV) * (vocab // support)
+    z = torch.full((T, vocab), float("-inf"), dtype=dtype, device=DEV)
+    some = torch.randn(T, support, generator=g, device=DEV).to(dtype)
+    z.scatter_(1, tokens, some)
+    q = None
+    if draft is not None:
+        q = torch.zeros(T, vocab, dtype=draft, device=DEV)
+        q.scatter_(1, tokens, torch.softmax(some.double(), -1).to(draft))
+    may, ids = tokens.tolist(), []
+    for s in range(seqs):
+        taken = {}
+        for i in range(n):
+            up = s * n + max(0, one[i])
+            if up not in taken:
+                taken[up] = list(may[up])
+                if order == "any":
+                    rng.shuffle(taken[up])
+                elif order == "twice":  # drawn with replacement
+                    taken[up] = [rng.choice(may[up]) for _ in range(fan + 1)]
+            ids.append(taken[up].pop(0) if i and taken[up] else may[up][0])
+    u = [BELOW_ONE if rng.random() < 0.6 else rng.random() for _ in range(T)]
+    return z, q, one * seqs, ids, torch.tensor(u, dtype=torch.float64), may
+
+
+@pytest.mark.parametrize("seqs,n,fan,support,vocab,dtype,draft,order", [
+    # one launch: lines, and trees of certain tokens
+    (400, 2, 1, 2, 40, F16, BF16, "any"), (400, 5, 1, 2, 4100, F32, F16, "any"), (300, 3, 1, 3, 60, BF16, F32, "any"),
+    (300, 4, 3, 3, 50, F32, None, "any"), (100, 13, 3, 3, 9000, F16, None, "any"), (200, 2, 1, 1, 30, F16, BF16, "any"),
+    # rounds: drawn siblings
+    (300, 3, 2, 2, 40, F16, BF16, "any"), (300, 3, 2, 2, 40, F16, BF16, "twice"), (100, 7, 2, 2, 5000, BF16, F16, "any"),
+    (100, 13, 3, 3, 300, F32, BF16, "any"), (100, 13, 3, 3, 300, F32, F32, "twice"),
+    # the lone workgroup's
+    (50, 60, 3, 3, 900, F16, BF16, "any"), (60, 40, 5, 5, 9000, F32, F16, "twice"), (8, 300, 4, 4, 2000, BF16, BF16, "any"),
+    # read as the walks go
+    (80, 13, 3, 3, 151936, F16, None, "any"), (90, 13, 3, 3, 151936, F16, BF16, "any"),
+    (90, 13, 3, 3, 151936, BF16, F16, "twice"), (3, 200, 3, 3, 500009, F16, BF16, "any")])
+def test_a_walk_ends_in_a_token_that_may_follow(seqs, n, fan, support, vocab, dtype, draft, order):
+    for seed in range(3):
+        z, q, parent, ids, u, may = masked(seqs, n, fan, support, vocab, dtype, draft, seed, order)
+        target = torch.full((seqs * n,), 77, **I32)
+        P.verify(P.Rows.of([n] * seqs, [0] * seqs, DEV), None if fan == 1 and seed else torch.tensor(parent, **I32),
+                 torch.tensor(ids, **I32), z, u.to(DEV), target, draft=q,
+                 distinct=order == "any" and fan > 1)
+        target = target.tolist()
+        for s in range(seqs):
+            at, got = s * n, target[s * n:s * n + n]
+            path, after = R.walk(parent[at:at + n], ids[at:at + n], got, n)
+            assert [i for i in range(n) if got[i] != -1] == path, (seed, s, path, got[:8])
+            for i in path:
+                assert got[i] in may[at + i], (seed, s, i)
+            assert after == got[path[-1]] != -1
+
+
+@pytest.mark.parametrize("draft", [None, BF16])
+def test_nothing_left_is_accepted_after_all(draft):
+    """Two tokens may follow, of 0.6 and 0.4; the draft's nearest numbers of 8 bits are above
+    both (154 / 256 and 205 / 512): a number next to 1 refuses the first by the rounding alone, and no token
+    has anything left.  Without a draft both are children, and certain."""
+    V, n = 64, 4
+    z = torch.full((n, V), float("-inf"), device=DEV)
+    z[:, 5], z[:, 40] = 0.4054651, 0.0  # ln 1.5
+    q = None
+    if draft is not None:
+        q = torch.zeros(n, V, device=DEV, dtype=draft)
+        q[:, 5], q[:, 40] = 154 / 256, 205 / 512
+    for ids, parent, distinct, path in (([1, 5, 40, 5], [-1, 0, 0, 1], True, None), ([1, 40, 5, 40], [-1, 0, 0, 1], True, None),
+                                        ([1, 5, 40, 5], [-1, 0, 1, 2], False, [0, 1, 2, 3])):
+        if draft is None and path:
+            continue  # (in a line the other token is left)
+        target = torch.empty(n, **I32)
+        u = torch.tensor([0.3] + [BELOW_ONE] * 3, dtype=torch.float64, device=DEV)
+        P.verify(P.Rows.of([n], [0], DEV), torch.tensor(parent, **I32), torch.tensor(ids, **I32), z, u, target, draft=q,
+                 distinct=distinct)
+        got = target.tolist()
+        way, after = R.walk(parent, ids, got, n)
+        assert after in (5, 40) and len(way) >= 2
+        if path:
+            assert way == path and got[:3] == ids[1:]
+
+
+def test_a_token_that_may_not_follow_is_not_accepted_for_want_of_others():
+    """The draft's token has no probability at all and what it leaves of the others is below
+    its own roundings: the others stay as they were."""
+    V = 64
+    z = torch.full((2, V), float("-inf"), device=DEV)
+    z[:, 5], z[:, 40] = 0.4054651, 0.0
+    q = torch.zeros(2, V, device=DEV, dtype=BF16)
+    q[:, 5], q[:, 40], q[:, 9] = 154 / 256, 205 / 512, 1 / 512
+    for token in (9, -3, V):
+        for first, want in ((0.3, 5), (0.7, 40)):
+            target = torch.empty(2, **I32)
+            u = torch.tensor([first, 0.5], dtype=torch.float64, device=DEV)
+            P.verify(P.Rows.of([2], [0], DEV), None, torch.tensor([1, token], **I32), z, u, target, draft=q)
+            assert target.tolist() == [want, -1]
