@@ -122,3 +122,16 @@ def test_draft_rows_behind_leaves_are_not_read(counts, vocab, fan, distinct, dty
     assert verified(counts, *args, distinct) == want
     if fan == 0:
         assert verified(counts, z, q, None, ids, heats, u, distinct) == want
+
+
+@pytest.mark.parametrize("counts,vocab,fan,distinct,dtype,draft,needs", [
+    ([16] * 64, 151936, 4, False, BF16, BF16, 6), ([16] * 64, 151936, 6, True, F16, F32, 6),
+    ([300, 0, 150], 400011, 6, True, F16, F16, 7), ([300, 0, 150], 400011, 4, False, BF16, F32, 7),
+    ([40, 9], 3000017, 5, False, F16, BF16, 6), ([64, 20], 1000003, 6, True, F32, F16, 6)])
+def test_walks_that_read_as_they_go_and_are_refused(counts, vocab, fan, distinct, dtype, draft, needs):
+    """Drawn siblings in more than 268 MB of logits: rows' statistics are formed when a walk
+    gets there, and refusals beyond the launched rounds are the lone workgroup's."""
+    assert sum(counts) * vocab * (4 if dtype is F32 else 2) > 8 << 25
+    args, want = settled(counts, vocab, dtype, draft, distinct, fan, 0.8, needs)
+    assert verified(counts, *args, distinct) == want
+
