@@ -412,7 +412,7 @@ class PagedDecoder:
         path = torch.empty(rows.seqs, max(1, rows.max_rows) if most is None else most, **i32)
         count, after, new_len = (torch.empty(rows.seqs, **i32) for _ in range(3))
         P.commit(self.cache, rows, parent, ids, target, path, count, after, new_len)
-        if queries:
+        if queries and rows.seqs:
             # the accepted rows, now in a line behind the keys they followed
             cu = torch.zeros_like(rows.cu)
             torch.cumsum(count, 0, dtype=torch.int32, out=cu[1:])

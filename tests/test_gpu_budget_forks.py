@@ -1,5 +1,5 @@
 """A decoder's forks of sequences that have evicted keys: the rows that follow are at the
-places that their text has."""
+places that their text has.  Verified steps without sequences."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -95,3 +95,15 @@ def test_forks_without_evictions_and_without_weights(model):  # noqa: F811
     put(plain, 0, 0, tokens(40, 1))
     plain.fork(0, 1, 17)
     assert CFG.layers and plain.gone is None
+
+
+@pytest.mark.parametrize("window", [None, 0, 2])
+def test_a_verified_step_of_no_sequences(model, window):  # noqa: F811
+    """Rows that pad a step whose sequences are all gone."""
+    d = decoder(model, window, seqs=2)
+    i32 = {"dtype": torch.int32, "device": DEV}
+    rows = P.Rows(torch.zeros(1, **i32), torch.empty(0, **i32), 5, 0)
+    for kw in ({}, {"temperature": torch.empty(0, device=DEV)}):
+        path, count, after, new_len = d.verify(rows, tokens(5, 1), None, **kw)
+        assert path.shape == (0, 1) and count.shape == after.shape == new_len.shape == (0,)
+    assert not d.cache.k.any() and (window is None or not d.score.any())
