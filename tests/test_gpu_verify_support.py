@@ -119,3 +119,39 @@ def test_a_token_that_may_not_follow_is_not_accepted_for_want_of_others():
             u = torch.tensor([first, 0.5], dtype=torch.float64, device=DEV)
             P.verify(P.Rows.of([2], [0], DEV), None, torch.tensor([1, token], **I32), z, u, target, draft=q)
             assert target.tolist() == [want, -1]
+
+
+@pytest.mark.parametrize("how", ["line", "siblings", "distinct", "certain"])
+@pytest.mark.parametrize("tokens,near", [(2, 0.0), (3, 0.0), (3, 0.5)])
+def test_tokens_are_as_often_as_the_target_says(tokens, near, how):
+    """The first token behind 196605 roots, whose drafts (of 8 bits) are the target itself or
+    near it.  A share's standard deviation is at most sqrt(1 / 4 / 196605) = 0.00113; six of
+    them, and what the draft's roundings move: half a step, 2^-8 of a share of at most 1."""
+    V, S, n = 48, 65535, {"line": 2, "siblings": 4, "distinct": 1 + tokens, "certain": tokens}[how]
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    may = torch.tensor([5, 40, 21][:tokens], device=DEV)
+    x = torch.tensor([0.41, 0.0, -0.7][:tokens], device=DEV)
+    p = torch.softmax(x.double(), 0)
+    q = torch.softmax(x.double() + near * torch.tensor([1.0, -1.0, 0.3][:tokens], device=DEV), 0).to(BF16)
+    z = torch.full((1, V), float("-inf"), device=DEV)
+    z[0, may] = x
+    draft = torch.zeros(1, V, dtype=BF16, device=DEV)
+    draft[0, may] = q
+    z, draft = z.repeat(S * n, 1), draft.repeat(S * n, 1)
+    parent = torch.tensor(([-1] + [0] * (n - 1)) * S, **I32)
+    seen = torch.zeros(V, dtype=torch.long, device=DEV)
+    for _ in range(3):
+        key = torch.empty(S, n, tokens, device=DEV).exponential_(generator=g)
+        if how in ("distinct", "certain"):
+            pick = (key[:, 0] / q.float()).argsort(-1)
+            ids = torch.cat([pick[:, :1], pick], 1)[:, :n]
+        else:
+            ids = (key / q.float()).argmin(-1)
+        target = torch.empty(S * n, **I32)
+        u = torch.rand(S * n, dtype=torch.float64, generator=g, device=DEV)
+        P.verify(P.Rows.of([n] * S, [0] * S, DEV), parent, may[ids].flatten().int(), z, u, target,
+                 draft=None if how == "certain" else draft, distinct=how == "distinct")
+        seen += torch.bincount(target.view(S, n)[:, 0].clamp(min=0), minlength=V)
+    off = (seen[may].double() / (3 * S) - p).abs()
+    assert int(seen.sum() - seen[may].sum()) == 0
+    assert (off < 6 * 0.00113 + (0 if how == "certain" else 2.0 ** -8)).all(), off.tolist()
