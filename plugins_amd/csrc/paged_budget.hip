@@ -1170,7 +1170,8 @@ constexpr size_t KEPT_MAX = (size_t)1 << 30;
 // take more than this.
 constexpr size_t SUMS_MAX = (size_t)1 << 28;
 // Items of many pairs, in first passes' workgroups: 264 us for 3 prompts of up to 2048 rows
-// with 2, 270 with 3, 305 and more with 4; 315 with 1, some of which are long after others.
+// with 2, 270 with 3, 305 and more with 4; 315 with 1, some of which are long after others (one
+// number a pair between the passes then, 4 us less than two).
 constexpr int ROUNDS = 2;
 Plan plan_of(const exl3p_cache *c, const exl3p_rows *r, int32_t heads, int32_t window, int32_t room) {
   Plan p;

@@ -1108,8 +1108,9 @@ __global__ __launch_bounds__(ST) void verify_single_draw_kernel(VerifyArgs a) {
 // ------------------------------------------------------------------- host side
 
 constexpr int VOCAB_MAX = 1 << 24;
-// Rounds that are launched: 2 us each where no walk needs it, 10 to 13 us for the workgroup
-// alone where one does.  4 trees of 24 rows of f16 and 64 of 64 of bf16 (151936 tokens):
+// Needs of a walk that launches answer, behind a first round that forms the first: 2 us each where
+// no walk has it, 10 to 13 us for the workgroup alone where one does.  4 trees of 24 rows of f16
+// and 64 of 64 of bf16 (151936 tokens, before refusals that leave nothing were looked for):
 // 36.6 and 65.5 us with 2, 40.7 and 61.8 with 4, 44.9 and 66.3 with 6.
 constexpr int ROUNDS = 4;
 constexpr int64_t LAZY = 1 << 25;  // bytes of logits
