@@ -183,13 +183,15 @@ exl3_verdict exl3p_verify(const exl3p_rows *r, const int32_t *parent, const int3
  * 0: all.  score [seqs][kv_heads][room] of 32-bit floats, one layer's; keys behind
  * the sequence's, and sequences without rows, stay as they are, and so does one
  * whose keys are more than `room`, or do not fit its table.  A sequence with a
- * page number outside the cache among its keys has scores of NaN at every key that a
- * row that counts sees.  decay is finite.  Sums are of 32 bits, in an order that goes by the sizes and lengths alone:
- * results repeat.  q as in exl3p_attend; values are not read.
- * scratch: exl3p_weigh_scratch_bytes(), as in exl3p_attend, but by `room` too: up to 32 pairs of
- * a row and a query head keep a number each for every key there is room for, where that is up
- * to 2^30 bytes in all; more pairs two numbers each, and for every such key sums, up to 2^28 bytes
- * of them or two a key and kv head.  score and the scratch lie over nothing else that is read, nor over each other. */
+ * page number outside the cache among its keys has scores of NaN at every key that
+ * a row that counts sees.  decay is finite.  Sums are of 32 bits, in an order that
+ * goes by the sizes and lengths alone: results repeat.  q as in exl3p_attend; values
+ * are not read.
+ * scratch: exl3p_weigh_scratch_bytes(), as in exl3p_attend, but by `room` too: up to
+ * 32 pairs of a row and a query head keep a number each for every key that there is
+ * room for, where that is up to 2^30 bytes in all; more pairs two numbers each, and
+ * for every such key sums, up to 2^28 bytes of them or two a key and kv head.  score
+ * and the scratch lie over nothing else that is read, nor over each other. */
 size_t exl3p_weigh_scratch_bytes(const exl3p_cache *c, const exl3p_rows *r, int32_t heads,
                                  int32_t window, int32_t room);
 exl3_verdict exl3p_weigh(const exl3p_cache *c, int32_t layer, const exl3p_rows *r, int32_t heads,
