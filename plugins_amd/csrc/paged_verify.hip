@@ -436,11 +436,11 @@ __device__ __forceinline__ void take_rows(const VerifyArgs &a, Walk<N, DRAFT> &w
 // a child or leaves something.  But a row's mass is a sum of 32-bit powers (no draft: the last
 // token there is, as a child, is not quite certain), and a draft's numbers are rounded, to a
 // sum above 1 perhaps, so that max(p - q, 0) may be 0 throughout.  The sampling would have to
-// say a refused child's token, and whoever goes by the targets would go on to that child.  So the child that such a refusal refused is accepted
-// after all; where p~ had nothing of its token, p~ stays as it was before.  Whether there is
-// nothing is looked for where it can be: without a draft, where SCANT is left; with one, a
-// token's step q is above p~ everywhere, by no more than step (the sum of q - 1) in all, so by
-// no more than that at the child.
+// say a refused child's token, and whoever goes by the targets would go on to that child.  So
+// the child that such a refusal refused is accepted after all; where p~ had nothing of its
+// token, p~ stays as it was before.  Whether there is nothing is looked for where it can be:
+// without a draft, where SCANT is left; with one, where step q is above p~ for every token, by
+// no more than step (the sum of q - 1) in all, so by no more than that at the child.
 template <typename Q>
 __device__ __forceinline__ double above_one(int vocab) {  // the sum of a rounded q, less 1
   return sizeof(typename Q::T) == 4 ? SCANT : Q::EXP == F16::EXP ? 0x1p-10 + vocab * 0x1p-25 : 0x1p-7;
@@ -451,7 +451,7 @@ __device__ __forceinline__ int walk_on(const VerifyArgs &a, Walk<N, DRAFT> &w, c
     const int lane = threadIdx.x, n = min(q.n, N);
     State st = w.st;
     st.need = END;
-    if (DRAFT && less_now) st.share = lost(st.share, st.step), st.left = w.rest;  // (not read where the walk ends here)
+    if (DRAFT && less_now) st.share = lost(st.share, st.step), st.left = w.rest;  // (not read at a walk's end)
     // the next child of the row behind row `from`
     auto next = [&](int from) {
       for (int b = (from + 1) & ~63; b < n; b += 64) {
@@ -560,7 +560,11 @@ __device__ __forceinline__ Settled settle(const VerifyArgs &a, Walk<N, DRAFT> &w
 // The walk from a row whose statistics are there, or (rest) from behind a refusal whose rest is.
 template <typename E, typename Q, bool DRAFT, int N>
 __device__ __forceinline__ int walk_from(const VerifyArgs &a, Walk<N, DRAFT> &w, const Seq &q, bool rest) {
-  bool doubt = rest && w.st.spare != NO_MATTER && w.rest < SCANT;
+  bool doubt = false;
+  if (rest) {
+    doubt = w.st.spare != NO_MATTER && w.rest < SCANT;
+    __syncthreads();  // all have read it: the walk goes on from there, by one wave
+  }
   for (;;) {
     if (doubt) {
       const Settled how = settle<E, Q>(a, w, q);

@@ -155,3 +155,24 @@ def test_tokens_are_as_often_as_the_target_says(tokens, near, how):
     off = (seen[may].double() / (3 * S) - p).abs()
     assert int(seen.sum() - seen[may].sum()) == 0
     assert (off < 6 * 0.00113 + (0 if how == "certain" else 2.0 ** -8)).all(), off.tolist()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), 1.0, 7.0, -1.0])
+@pytest.mark.parametrize("seqs,n,fan,support,vocab,dtype,draft,order", [
+    (200, 3, 1, 2, 40, F16, BF16, "any"), (200, 3, 2, 2, 40, F16, BF16, "any"), (100, 13, 3, 3, 9000, BF16, F16, "twice"),
+    (40, 60, 3, 3, 900, F32, BF16, "any"), (100, 4, 3, 3, 50, F32, None, "any"), (90, 13, 3, 3, 151936, F16, BF16, "any")])
+def test_numbers_that_are_none_beside_others(seqs, n, fan, support, vocab, dtype, draft, order, bad):
+    """Any of the numbers is NaN, or not in [0, 1): every row of a walk still has a token that may
+    follow, and calls repeat."""
+    z, q, parent, ids, u, may = masked(seqs, n, fan, support, vocab, dtype, draft, 5, order)
+    u[torch.rand(len(u), generator=torch.Generator().manual_seed(2)) < 0.5] = bad
+    out = []
+    for _ in range(3):
+        target = torch.full((seqs * n,), 77, **I32)
+        P.verify(P.Rows.of([n] * seqs, [0] * seqs, DEV), torch.tensor(parent, **I32), torch.tensor(ids, **I32), z, u.to(DEV),
+                 target, draft=q, distinct=order == "any" and fan > 1)
+        out.append(target.tolist())
+    assert out[0] == out[1] == out[2]
+    for t, x in enumerate(out[0]):
+        assert x == -1 or x in may[t] or bad < 0
+        assert t % n or x != -1
