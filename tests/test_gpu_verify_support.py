@@ -2,6 +2,7 @@
 roundings then leave nothing of the target's probabilities after a refusal, or every token
 that may follow is among the children.  The walk still ends in a token that may follow,
 and exl3p_commit takes the same way to it."""
+import math
 import random
 
 import pytest
@@ -176,3 +177,79 @@ def test_numbers_that_are_none_beside_others(seqs, n, fan, support, vocab, dtype
     for t, x in enumerate(out[0]):
         assert x == -1 or x in may[t] or bad < 0
         assert t % n or x != -1
+
+
+def kept_walk(parent, ids, p, u, q, distinct):
+    """(target, margin) of one sequence in 64 bits, as tests._budget.walk, with the rule for
+    refusals that leave nothing; p, q: {token: probability} of each row, what is not there is 0."""
+    n, target, margin, at = len(ids), [-1] * len(ids), math.inf, 0
+    while True:
+        rest, A, B, share, to = dict(p[at]), 1.0, 1.0, 0.0, None
+        for c in (c for c in range(at + 1, n) if parent[c] == at):
+            x = ids[c]
+            mine, drawn = rest.get(x, 0.0), 1.0 if q is None else q[at].get(x, 0.0)
+            step = A if q is None else A / max(B, 2.0 ** -53)
+            need = u[c] * step * drawn
+            if max(need, mine) > 0:
+                margin = min(margin, abs(need - mine) / max(need, mine))
+            if need < mine:
+                to = c
+                break
+            B -= drawn if distinct else 0.0
+            if q is None:
+                less = {k: 0.0 if k == x else v for k, v in rest.items()}
+            else:
+                less = {k: max(v - (share + step) * q[at].get(k, 0.0) * (1 + 2.0 ** -48), 0.0) for k, v in p[at].items()}
+            if any(less.values()):
+                rest, share = less, share + step
+                A = A - mine if q is None else sum(rest.values())
+                margin = min(margin, 1e5 * A)  # (what 32 bits do not see)
+            elif mine > 0:
+                to = c
+                break
+        if to is not None:
+            target[at] = ids[to]
+            at = to
+            continue
+        whole, run = sum(rest.values()), 0.0
+        for k in sorted(rest):
+            run += rest[k]
+            margin = min(margin, 1e7 * abs(run / whole - u[0])) if rest[k] else margin
+            if run > u[0] * whole:
+                target[at] = k
+                return target, margin
+        return target, 0.0
+
+
+@pytest.mark.parametrize("seqs,n,fan,support,vocab,dtype,draft,order", [
+    (500, 2, 1, 2, 40, F16, BF16, "any"), (300, 5, 1, 3, 4100, F32, F16, "any"), (300, 4, 3, 3, 50, F32, None, "any"),
+    (500, 3, 2, 2, 40, F16, BF16, "any"), (400, 5, 4, 2, 40, F16, BF16, "twice"), (200, 13, 3, 3, 300, F32, BF16, "any"),
+    (100, 31, 5, 5, 9000, BF16, BF16, "any"), (60, 60, 6, 4, 900, F32, F16, "twice"), (10, 300, 6, 6, 2000, F16, BF16, "any"),
+    (90, 13, 3, 3, 151936, F16, BF16, "any"), (90, 13, 6, 3, 151936, BF16, BF16, "twice"), (3, 200, 6, 6, 500009, F16, BF16, "any")])
+def test_walks_by_the_rule(seqs, n, fan, support, vocab, dtype, draft, order):
+    """Numbers near 1 and others: the walks are the rule's in 64 bits, but for sequences whose
+    nearest decision is within 1e-5 of its border."""
+    checked = scant = 0
+    for seed in range(3):
+        z, q, parent, ids, _, may = masked(seqs, n, fan, support, vocab, dtype, draft, 50 + seed, order)
+        rng = random.Random(seed)
+        u = [1 - 10 ** rng.uniform(-5, -1) if rng.random() < 0.8 else rng.random() for _ in range(seqs * n)]
+        distinct = order == "any" and fan > 1
+        target = torch.full((seqs * n,), 77, **I32)
+        P.verify(P.Rows.of([n] * seqs, [0] * seqs, DEV), torch.tensor(parent, **I32), torch.tensor(ids, **I32), z,
+                 torch.tensor(u, dtype=torch.float64, device=DEV), target, draft=q, distinct=distinct)
+        got = target.tolist()
+        cols = torch.tensor(may, device=DEV)
+        ps = torch.softmax(z.gather(1, cols).double(), 1).tolist()
+        qs = None if q is None else q.gather(1, cols).double().tolist()
+        for s in range(seqs):
+            at = slice(s * n, s * n + n)
+            p_of = [dict(zip(m, x)) for m, x in zip(may[at], ps[at])]
+            q_of = None if qs is None else [dict(zip(m, x)) for m, x in zip(may[at], qs[at])]
+            want, margin = kept_walk(parent[at], ids[at], p_of, u[at], q_of, distinct)
+            if margin > 1e-5:
+                checked += 1
+                assert got[at] == want, (seed, s)
+            else:
+                scant += 1
+    assert checked > 5 * scant
